@@ -220,6 +220,56 @@ int qmr_supported_bf16_quantization(uint32_t bits, size_t group);
  *     ceil((a+b+c)/16). out holds 4096 u32 slots whose XOR is the XOR of
  *     every 32-bit word read. The read floor of a product's codes and
  *     metadata, for measurement; it computes nothing else.
+ *   "rope_axes"
+ *     Rotary positions with one to four axes (time, height, width, ..), for
+ *     query or key heads. Buffers x [tokens][heads][head_dim], positions int32
+ *     [axes][tokens], freqs FP32 [rotary/2] (radians a position), y; params
+ *     tokens, heads, head_dim, rotary, x stride, y stride, adjacent, dealt,
+ *     axes, four section words. The first `rotary` dimensions turn in pairs,
+ *     (i, i + rotary/2) or, with adjacent = 1, (2i, 2i + 1): (a, b) becomes
+ *     (a cos t - b sin t, b cos t + a sin t), t = position * freqs[i]; the
+ *     others pass. A pair's position is that of its axis: section words n0..n3
+ *     (they add up to rotary/2) give the first n0 pairs to axis 0, the next n1
+ *     to axis 1, and so on; with dealt = 1 pair i goes to axis a = i % axes if
+ *     a > 0 and i < axes * n_a, else to axis 0. Strides are floats from token
+ *     to token. y may be exactly x's view and stride (in place), or rows beside
+ *     x's in one buffer. head_dim even, at most 256.
+ *   "kv_append_rope_bf16", "kv_append_rope_f16"
+ *     What stands between an attention layer's input products and its
+ *     attention: normalises (optional) and rotates new queries and keys, and
+ *     appends keys and values to a paged cache of BF16 or F16. Buffers q, k, v
+ *     (FP32 rows, which may be columns of one buffer), q_norm, k_norm FP32
+ *     [head_dim], positions, freqs, starts u32 [seqs+1], lengths u32 [seqs],
+ *     table u32 [seqs][columns], k_cache, v_cache, q_out; params seqs, tokens,
+ *     q heads, kv heads, head_dim, rotary, strides of q, k, v and q_out,
+ *     adjacent, dealt, axes, four section words, eps as FP32 bits (0: no norm,
+ *     and no norm weights are read), page, pages, columns. Sequence s has the
+ *     tokens starts[s]..starts[s+1]-1; they are the last positions of its
+ *     lengths[s] (new ones counted). Position p is kept in slot p % page of
+ *     page table[s][p / page]; a negative position, one past the columns, or
+ *     one whose page is not below `pages` is dropped, and its queries are
+ *     rotated all the same. q heads may be 0. q_out may be exactly q's view and
+ *     stride. Values round to nearest even, past F16's range to infinity.
+ *     Caches are pages * kv heads * page * head_dim halves, 16-byte aligned, a
+ *     page's head after head as blocks of 32 positions: keys [head_dim/8][32][8],
+ *     position 8a + 4b + c of a block at place 16b + 4a + c; values
+ *     [4][head_dim][8], eight positions of a dimension together. page: a power
+ *     of two, at least 32; head_dim a multiple of 8, at most 256. rotary and
+ *     axes may be 0 together.
+ *   "attn_paged_bf16", "attn_paged_f16"
+ *     Attention of the new tokens over that cache, for single tokens as for
+ *     whole prompts. Buffers q, starts, lengths, table, k_cache, v_cache, out
+ *     (rows beside q's in one buffer at most); params seqs, tokens, q heads,
+ *     kv heads, head_dim, strides of q and out, page, pages, columns, most
+ *     keys, causal, window, scale as FP32 bits. Query head h reads key-value
+ *     head h / (q heads / kv heads). A token at position p sees the positions
+ *     below min(lengths[s], most keys), with causal = 1 those up to p, and with
+ *     a window w > 0 those past p - w; positions of pages not below `pages`
+ *     hold nothing. A row that sees no key is zero. What it does not see does
+ *     not reach it, be it NaN; a key or value that it sees and that is not
+ *     finite makes it not finite. `most keys` bounds the lengths that the
+ *     launch is planned for. Results are near FP32 arithmetic's: no operand is
+ *     rounded below 22 bits.
  *   "matvec_affine_f16meta", "matmul_affine_f16meta", "embed_affine_f16meta"
  *     As the FP32-metadata names, with scales/biases stored as IEEE binary16
  *     (the dtype MLX checkpoints ship). The reference expands F16 metadata

@@ -40,8 +40,10 @@ SOURCES = [
     ("affine_mfma.hip", ["-x", "hip"]),
     ("affine_rows.hip", ["-x", "hip"]),
     ("affine_tile.hip", ["-x", "hip"]),
+    ("attn_paged.hip", ["-x", "hip"]),
     ("dense_mfma.hip", ["-x", "hip"]),
     ("misc_kernels.hip", ["-x", "hip"]),
+    ("rope_append.hip", ["-x", "hip"]),
     ("wide_mfma.hip", ["-x", "hip"]),
 ]
 

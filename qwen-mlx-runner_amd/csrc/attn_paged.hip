@@ -1,0 +1,541 @@
+// Attention of new tokens over a paged key-value cache (layouts:
+// rope_append.hip), for one token a sequence as for whole prompts.
+//
+//   o_r = sum_j p_rj v_j,  p_r = softmax_j(scale q_r . k_j)
+//
+// over the keys j that row r (a token's query head) may see. One pass over the
+// keys with the running maximum m and sum l of each row, in 32 bits, in powers
+// of two (q carries scale * log2 e).
+//
+// Products run on the matrix cores in the cache's own 16-bit type, with no
+// bit of the 32-bit side lost: an FP32 operand is the sum of two f16 terms
+// (22 bits; queries scaled by a power of two a row so that the second term
+// stays normal) or three bf16 terms (24 bits). That is two or three times the
+// matrix work, which a call of few rows has to spare, and an error near 32-bit
+// arithmetic's own, as every product of this library has.
+//
+// Operand placement (v_mfma_f32_16x16x32: A row and B column lane % 16, K
+// chunk lane / 16; D[i][j] in lane j + 16 (i / 4), element i % 4): S^T = K Q^T
+// with the 32 keys of a block dealt to two instructions so that lane (n, g)
+// ends with the scores of row n and keys 8g..8g+7, which is where P^T has to
+// be as the B operand of O^T = V^T P^T. Scores never leave their lane.
+#include <hip/hip_runtime.h>
+
+#include "attn_common.hpp"
+#include "kernels.hpp"
+
+namespace qmr {
+namespace {
+
+using attn::kBlock;
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr uint32_t kNone = 0xFFFFFFFFu;
+
+// Terms of an FP32 operand in the cache's type.
+template <bool BF16>
+constexpr int kTerms = BF16 ? 3 : 2;
+
+template <bool BF16>
+__device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
+    if constexpr (BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+}
+
+__device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) {  // lo >> 16 | hi & 0xFFFF0000
+    return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+}
+
+// Eight FP32 values as kTerms vectors of eight halves that add up to them:
+// truncated terms, each exact in what the ones before leave (the last f16 one
+// rounds at 2^-22).
+template <bool BF16>
+__device__ __forceinline__ void split8(const float (&x)[8], u4 (&t)[kTerms<BF16>]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a = x[2 * i], b = x[2 * i + 1];
+        if constexpr (BF16) {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+                t[k][i] = high_halves(ua, ub);
+                a -= __uint_as_float(ua & 0xFFFF0000u);
+                b -= __uint_as_float(ub & 0xFFFF0000u);
+            }
+        } else {
+            const auto hi = __builtin_amdgcn_cvt_pkrtz(a, b);
+            t[0][i] = __builtin_bit_cast(uint32_t, hi);
+            t[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - float(hi[0]), b - float(hi[1])));
+        }
+    }
+}
+
+// What a workgroup works on: a tile of query rows of one sequence and key
+// head. Row r of the sequence is token r / group, head r % group.
+struct Tile {
+    uint32_t seq, first_token, row0, rows;  // rows: of the whole sequence
+    int length, context;                    // cache length; position of the sequence's first new token
+};
+
+// Tile number `tile` among all sequences' (ceil(rows / R) of each), found by
+// a wave's prefix sum over 64 sequences at a time; false past the last.
+__device__ __forceinline__ bool find_tile(const PagedCache &c, uint32_t group, uint32_t R, uint32_t tile, Tile &t) {
+    const uint32_t l = threadIdx.x % 64;
+    for (uint32_t base = 0; base < c.seqs; base += 64) {
+        const uint32_t s = base + l;
+        uint32_t from = 0, count = 0;
+        if (s < c.seqs) {
+            from = c.starts[s];
+            const uint32_t to = min(c.starts[s + 1], c.tokens);
+            count = to > from ? to - from : 0;
+        }
+        const uint32_t own = (count * group + R - 1) / R;
+        uint32_t sum = own;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t o = __shfl_up(sum, d);
+            if (l >= uint32_t(d)) sum += o;
+        }
+        const uint32_t total = __shfl(sum, 63);
+        if (tile >= total) {
+            tile -= total;
+            continue;
+        }
+        const int at = __ffsll(__ballot(sum > tile)) - 1;
+        t.seq = __builtin_amdgcn_readfirstlane(base + at);
+        t.first_token = __builtin_amdgcn_readfirstlane(__shfl(from, at));
+        t.rows = __builtin_amdgcn_readfirstlane(__shfl(count, at)) * group;
+        t.row0 = __builtin_amdgcn_readfirstlane((tile - __shfl(sum - own, at)) * R);
+        t.length = int(min(c.lengths[t.seq], 0x7FFFFFFFu));
+        t.context = t.length - int(c.starts[t.seq + 1] - t.first_token);
+        return true;
+    }
+    return false;
+}
+
+// Keys [lo, hi) that a new token of the sequence may see.
+__device__ __forceinline__ void visible(const AttendArgs &a, const Tile &t, uint32_t token, int &lo, int &hi) {
+    const int pos = t.context + int(token);
+    hi = a.causal ? min(pos + 1, t.length) : t.length;
+    hi = max(min(hi, int(a.max_keys)), 0);
+    lo = a.window ? max(pos - int(a.window) + 1, 0) : 0;
+}
+
+// Results of key ranges, to be joined: for each (tile, head, range) R rows of
+// DM floats, and their m and l; for each (tile, head) its rows' places in the
+// output (kNone: nothing to join).
+struct Partial {
+    float *o;
+    float2 *ml;
+    uint32_t *place;
+};
+
+__device__ __forceinline__ bool not_finite(u4 v, bool bf16) {
+    const uint32_t e = bf16 ? 0x7F80u : 0x7C00u;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (v[i] & e) == e || ((v[i] >> 16) & e) == e;
+    return bad;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float half_f32(uint16_t h) {
+    if constexpr (BF16) return __uint_as_float(uint32_t(h) << 16);
+    return float(__builtin_bit_cast(_Float16, h));
+}
+
+// Few rows: R = 16 NB rows a workgroup, every wave all of them over its own
+// blocks of the range (block w, w + 4, ..), straight from memory into operand
+// registers: a block is 64 KB/DM-independent whole lines, and nothing is
+// shared but the queries, which wait in LDS as operands. The waves' m, l and O
+// are joined through LDS at the end.
+template <bool BF16, int DM, int NB, bool FULL>
+__global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttendArgs a, AttendPlan pl, Partial ws, bool aligned) {
+    constexpr int R = 16 * NB, T = kTerms<BF16>, KS = DM / 32, VT = DM / 16;
+    // f16 weights are up to 2^15, so that small ones stay normal; the maximum
+    // lags by at most 2^kLag.
+    constexpr float kTop = BF16 ? 0.f : 7.f, kLag = 8.f;
+    constexpr int kPitch = DM + 4;  // LDS pitch of a joined row: 16 rows on different banks
+    extern __shared__ __align__(16) unsigned char lds[];
+    __shared__ float row_scale[R];
+    __shared__ float wave_m[kWaves][16], wave_l[kWaves][16];
+    const PagedCache &c = a.cache;
+    const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t n = l % 16, g = l / 16;
+    const uint32_t split = blockIdx.x % pl.splits, unit = blockIdx.x / pl.splits;  // unit: tile and key head
+    const uint32_t head = unit % c.kv_heads, group = a.heads / c.kv_heads, dim = FULL ? DM : c.dim;
+    Tile t;
+    if (!find_tile(c, group, R, unit / c.kv_heads, t)) {
+        if (pl.splits > 1 && split == 0 && threadIdx.x < R) ws.place[size_t(unit) * R + threadIdx.x] = kNone;
+        return;
+    }
+    const uint32_t in_tile = min(uint32_t(R), t.rows - t.row0);
+
+    // The queries, as operands.
+    u4 *qs = reinterpret_cast<u4 *>(lds);  // [NB][KS][T][64 lanes]
+    {
+        const uint32_t qn = threadIdx.x / 16, p = threadIdx.x % 16;
+        constexpr int CH = (DM / 8 + 15) / 16;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const uint32_t r = nb * 16 + qn;
+            float x[CH][8], most = 0.f;
+            const uint32_t row = t.row0 + min(r, in_tile - 1);
+            const float *q = a.q + size_t(t.first_token + row / group) * a.q_stride +
+                             size_t(head * group + row % group) * dim;
+#pragma unroll
+            for (int k = 0; k < CH; ++k) {
+                const uint32_t ch = p + 16 * k;
+                const bool in = r < in_tile && ch * 8 < dim;
+                if (in && aligned) {
+                    *reinterpret_cast<float4 *>(x[k]) = *reinterpret_cast<const float4 *>(q + ch * 8);
+                    *reinterpret_cast<float4 *>(x[k] + 4) = *reinterpret_cast<const float4 *>(q + ch * 8 + 4);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[k][j] = in ? q[ch * 8 + j] : 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[k][j] *= a.scale * kLog2e;
+                    most = fmaxf(most, fabsf(x[k][j]));
+                }
+            }
+            int e = 0;
+            if constexpr (!BF16) {
+#pragma unroll
+                for (int d = 1; d < 16; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+                if (most > 0.f && most < INFINITY) frexpf(most, &e), e -= 15;
+            }
+            if (p == 0) row_scale[r] = ldexpf(1.f, e);
+#pragma unroll
+            for (int k = 0; k < CH; ++k) {
+                const uint32_t ch = p + 16 * k;
+                if (ch >= DM / 8) continue;
+                if constexpr (!BF16) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[k][j] = ldexpf(x[k][j], -e);
+                }
+                u4 terms[T];
+                split8<BF16>(x[k], terms);
+#pragma unroll
+                for (int i = 0; i < T; ++i) qs[((nb * KS + ch / 4) * T + i) * 64 + (ch % 4) * 16 + qn] = terms[i];
+            }
+        }
+    }
+    __syncthreads();
+
+    // What each row and the whole tile may see.
+    int lo[NB], hi[NB];
+    float rs[NB], m[NB], sum[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const uint32_t r = nb * 16 + n;
+        visible(a, t, (t.row0 + min(r, in_tile - 1)) / group, lo[nb], hi[nb]);
+        rs[nb] = row_scale[r];
+        m[nb] = -INFINITY;
+        sum[nb] = 0.f;
+    }
+    int lo_first, hi_first, lo_last, hi_last;
+    visible(a, t, t.row0 / group, lo_first, hi_first);
+    visible(a, t, (t.row0 + in_tile - 1) / group, lo_last, hi_last);
+    const int base = lo_first / int(kBlock) * int(kBlock);
+    const bool one_range = base + int64_t(pl.keys) >= hi_last;
+    const int64_t from64 = base + int64_t(split) * pl.keys;
+    const int from = from64 < hi_last ? int(from64) : hi_last;
+    const int to = int(min(from64 + int64_t(pl.keys), int64_t(hi_last)));
+
+    f4 o[NB][VT];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int d = 0; d < VT; ++d) o[nb][d] = f4{0.f, 0.f, 0.f, 0.f};
+
+    const uint32_t *table = c.table + size_t(t.seq) * c.columns;
+    for (int key0 = (from / int(kBlock) + int(w)) * int(kBlock); key0 < to; key0 += kWaves * int(kBlock)) {
+        const uint32_t named = __builtin_amdgcn_readfirstlane(table[uint32_t(key0) / c.page]);
+        const bool held = named < c.pages;
+        const size_t at = attn::block_at(c, held ? named : 0, head, uint32_t(key0) % c.page / kBlock);
+        const u4 *kp = reinterpret_cast<const u4 *>(c.k + at);
+        const u4 *vp = reinterpret_cast<const u4 *>(c.v + at);
+        u4 k[KS][2], v[VT];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (FULL || (4 * s + g) * 8 < dim)
+                    k[s][i] = kp[(4 * s + g) * 32 + 16 * i + n];
+                else
+                    k[s][i] = u4{0, 0, 0, 0};
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < VT; ++d) v[d] = vp[g * dim + (FULL ? 16 * d + n : min(16 * d + n, dim - 1))];
+
+        const bool edge = !held || key0 < lo_last || key0 + int(kBlock) > hi_first;
+        bool apart = false;  // a value that some rows see and others do not is not finite
+        if (edge) {
+            // Values that no row sees may be anything: zero them.
+            const int from_key = key0 + 8 * int(g);
+#pragma unroll
+            for (int d = 0; d < VT; ++d) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int key = from_key + e;
+                    if (!held || key < lo_first || key >= hi_last) v[d][e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+                }
+                apart |= not_finite(v[d], BF16);
+            }
+            apart = __ballot(apart) != 0;
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            f4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+#pragma unroll
+                for (int i = 0; i < T; ++i) {
+                    const u4 q = qs[((nb * KS + s) * T + i) * 64 + l];
+                    s0 = mfma16<BF16>(k[s][0], q, s0);
+                    s1 = mfma16<BF16>(k[s][1], q, s1);
+                }
+            }
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = s0[i], p[4 + i] = s1[i];
+            if (edge) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int key = key0 + 8 * int(g) + e;
+                    if (!held || key < lo[nb] || key >= hi[nb]) p[e] = -INFINITY;
+                }
+            }
+            float most = p[0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) most = fmaxf(most, p[e]);
+            most *= rs[nb];
+            if (__ballot(most > m[nb] + kLag) != 0) {
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                const float up = fmaxf(m[nb], most);
+                const float f = up > m[nb] ? exp2f(m[nb] - up) : 1.f;
+                m[nb] = up;
+                sum[nb] *= f;
+#pragma unroll
+                for (int d = 0; d < VT; ++d) o[nb][d] *= f;
+            }
+            const float off = kTop - (m[nb] == -INFINITY ? 0.f : m[nb]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], rs[nb], off));
+                sum[nb] += p[e];
+            }
+            if (apart) {
+                // Row by row: a hidden value must not even meet a zero weight.
+                for (uint32_t j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int key = key0 + 8 * int(j) + e;
+                        const float pj = __shfl(p[e], n + 16 * j);
+                        const bool seen = held && key >= lo[nb] && key < hi[nb];
+#pragma unroll
+                        for (int d = 0; d < VT; ++d) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t at_d = min(uint32_t(16 * d + 4 * g + i), dim - 1);
+                                const uint16_t h = reinterpret_cast<const uint16_t *>(vp)[(j * dim + at_d) * 8 + e];
+                                if (seen) o[nb][d][i] = fmaf(pj, half_f32<BF16>(h), o[nb][d][i]);
+                            }
+                        }
+                    }
+                }
+                continue;
+            }
+            u4 pt[T];
+            split8<BF16>(p, pt);
+#pragma unroll
+            for (int d = 0; d < VT; ++d) {
+#pragma unroll
+                for (int i = 0; i < T; ++i) o[nb][d] = mfma16<BF16>(v[d], pt[i], o[nb][d]);
+            }
+        }
+    }
+
+    // Join the waves, 16 rows at a time.
+    float *os = reinterpret_cast<float *>(lds);  // [kWaves][16][kPitch]
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        float all = sum[nb];
+        all += __shfl_xor(all, 16);
+        all += __shfl_xor(all, 32);
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < VT; ++d) *reinterpret_cast<f4 *>(os + (w * 16 + n) * kPitch + 16 * d + 4 * g) = o[nb][d];
+        if (g == 0) {
+            wave_m[w][n] = m[nb];
+            wave_l[w][n] = all;
+        }
+        __syncthreads();
+        const size_t part = (size_t(unit) * pl.splits + split) * R + nb * 16;
+        for (uint32_t i = threadIdx.x; i < 16 * DM / 4; i += kThreads) {
+            const uint32_t rn = i / (DM / 4), d = i % (DM / 4) * 4, r = nb * 16 + rn;
+            float top = wave_m[0][rn];
+#pragma unroll
+            for (int k = 1; k < kWaves; ++k) top = fmaxf(top, wave_m[k][rn]);
+            float joined = 0.f;
+            f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < kWaves; ++k) {
+                const float f = wave_m[k][rn] == -INFINITY ? (wave_l[k][rn] == 0.f ? 0.f : 1.f) : exp2f(wave_m[k][rn] - top);
+                joined += f * wave_l[k][rn];
+                acc += f * *reinterpret_cast<const f4 *>(os + (k * 16 + rn) * kPitch + d);
+            }
+            const uint32_t row = t.row0 + r;
+            const bool real = r < in_tile;
+            const uint32_t place = (t.first_token + row / group) * a.heads + head * group + row % group;
+            if (one_range) {
+                if (split == 0 && real && d < dim) {
+                    const float f = joined == 0.f ? 0.f : 1.f / joined;
+                    float *y = a.out + size_t(t.first_token + row / group) * a.out_stride +
+                               size_t(head * group + row % group) * dim + d;
+                    acc *= f;
+                    if (aligned) {
+                        *reinterpret_cast<f4 *>(y) = acc;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) y[k] = acc[k];
+                    }
+                }
+            } else {
+                if (joined != 0.f) *reinterpret_cast<f4 *>(ws.o + (part + rn) * DM + d) = acc;
+                if (d == 0) ws.ml[part + rn] = make_float2(top, joined);
+            }
+            if (pl.splits > 1 && split == 0 && d == 0) ws.place[size_t(unit) * R + r] = one_range || !real ? kNone : place;
+        }
+    }
+}
+
+// Adds the ranges of a row up: a workgroup a row, every wave a quarter of the
+// ranges.
+template <int DM>
+__global__ __launch_bounds__(kThreads) void attn_join_kernel(AttendArgs a, AttendPlan pl, Partial ws, bool aligned) {
+    constexpr int E = DM / 64;
+    __shared__ float part_o[kWaves][DM], part_l[kWaves];
+    const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64;
+    const uint32_t place = ws.place[blockIdx.x];
+    if (place == kNone) return;
+    const uint32_t unit = blockIdx.x / pl.rows, r = blockIdx.x % pl.rows;
+    const size_t first = size_t(unit) * pl.splits * pl.rows + r;
+    float top = -INFINITY;
+    for (uint32_t s = l; s < pl.splits; s += 64) top = fmaxf(top, ws.ml[first + size_t(s) * pl.rows].x);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    float acc[E] = {}, all = 0.f;
+    for (uint32_t s = w; s < pl.splits; s += kWaves) {
+        const size_t at = first + size_t(s) * pl.rows;
+        const float2 ml = ws.ml[at];
+        if (ml.y == 0.f) continue;
+        const float f = ml.x == -INFINITY ? 1.f : exp2f(ml.x - top);
+        all += f * ml.y;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += f * ws.o[at * DM + e * 64 + l];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) part_o[w][e * 64 + l] = acc[e];
+    if (l == 0) part_l[w] = all;
+    __syncthreads();
+    all = part_l[0] + part_l[1] + part_l[2] + part_l[3];
+    const float f = all == 0.f ? 0.f : 1.f / all;
+    const uint32_t d = threadIdx.x;
+    if (d < a.cache.dim)
+        a.out[size_t(place / a.heads) * a.out_stride + size_t(place % a.heads) * a.cache.dim + d] =
+            (part_o[0][d] + part_o[1][d] + part_o[2][d] + part_o[3][d]) * f;
+}
+
+uint32_t wide_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+Partial parts(const AttendArgs &a, const AttendPlan &pl, void *ws) {
+    const size_t rows = size_t(pl.tiles) * a.cache.kv_heads * pl.splits * pl.rows;
+    Partial p;
+    p.o = static_cast<float *>(ws);
+    p.ml = reinterpret_cast<float2 *>(p.o + rows * wide_dim(a.cache.dim));
+    p.place = reinterpret_cast<uint32_t *>(p.ml + rows);
+    return p;
+}
+
+size_t workspace_of(const AttendArgs &a, const AttendPlan &pl) {
+    if (pl.splits == 1) return 0;
+    const size_t units = size_t(pl.tiles) * a.cache.kv_heads;
+    return units * pl.rows * (size_t(pl.splits) * (wide_dim(a.cache.dim) + 2) + 1) * 4;
+}
+
+template <bool BF16, int DM, int NB>
+hipError_t launch_rows(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, bool aligned, hipStream_t stream) {
+    const size_t queries = size_t(NB) * (DM / 32) * kTerms<BF16> * 1024;
+    const size_t joined = size_t(kWaves) * 16 * (DM + 4) * 4;
+    const size_t lds = queries > joined ? queries : joined;
+    const auto kernel = a.cache.dim == DM ? attn_rows_kernel<BF16, DM, NB, true> : attn_rows_kernel<BF16, DM, NB, false>;
+    if (lds > 65536 - 2048) {
+        const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
+        if (e != hipSuccess) return e;
+    }
+    kernel<<<pl.tiles * a.cache.kv_heads * pl.splits, kThreads, lds, stream>>>(a, pl, ws, aligned);
+    return hipGetLastError();
+}
+
+template <bool BF16, int DM>
+hipError_t launch_dim(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, bool aligned, hipStream_t stream) {
+    hipError_t e = launch_rows<BF16, DM, 1>(a, pl, ws, aligned, stream);
+    if (e != hipSuccess || pl.splits == 1) return e;
+    attn_join_kernel<DM><<<pl.tiles * a.cache.kv_heads * pl.rows, kThreads, 0, stream>>>(a, pl, ws, aligned);
+    return hipGetLastError();
+}
+
+template <bool BF16>
+hipError_t launch_type(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, bool aligned, hipStream_t stream) {
+    switch (wide_dim(a.cache.dim)) {
+        case 64: return launch_dim<BF16, 64>(a, pl, ws, aligned, stream);
+        case 128: return launch_dim<BF16, 128>(a, pl, ws, aligned, stream);
+        default: return launch_dim<BF16, 256>(a, pl, ws, aligned, stream);
+    }
+}
+
+}  // namespace
+
+AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t workspace_limit) {
+    (void)lim;
+    (void)workspace_limit;
+    const PagedCache &c = a.cache;
+    const uint64_t group = a.heads / c.kv_heads;
+    AttendPlan pl;
+    pl.rows = 16;
+    // Sequences with a row: at most n. Each takes whole tiles.
+    const uint64_t n = c.seqs < c.tokens ? c.seqs : c.tokens;
+    const uint64_t by_rows = n + (c.tokens * group - n) / pl.rows;
+    const uint64_t by_token = c.tokens * ((group + pl.rows - 1) / pl.rows);
+    pl.tiles = uint32_t(by_rows < by_token ? by_rows : by_token);
+    pl.splits = 1;
+    pl.keys = (a.max_keys + kBlock - 1) / kBlock * kBlock;
+    pl.workspace = workspace_of(a, pl);
+    return pl;
+}
+
+const char *attend_kernel_name(const AttendPlan &) { return "attn_rows_kernel"; }
+
+hipError_t launch_attn_paged(const AttendArgs &a, const AttendPlan &pl, void *workspace, hipStream_t stream) {
+    const auto aligned16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const bool aligned = a.q_stride % 4 == 0 && a.out_stride % 4 == 0 && aligned16(a.q) && aligned16(a.out);
+    const Partial ws = pl.splits > 1 ? parts(a, pl, workspace) : Partial{};
+    return a.cache.bf16 ? launch_type<true>(a, pl, ws, aligned, stream) : launch_type<false>(a, pl, ws, aligned, stream);
+}
+
+}  // namespace qmr

@@ -53,6 +53,25 @@ bool is_mlp_name(const std::string &name) {
 
 bool is_fused_name(const std::string &name) { return is_residual_name(name) || is_mlp_name(name); }
 
+bool is_append_name(const std::string &name) { return name == "kv_append_rope_bf16" || name == "kv_append_rope_f16"; }
+
+bool is_attend_name(const std::string &name) { return name == "attn_paged_bf16" || name == "attn_paged_f16"; }
+
+bool is_attention_name(const std::string &name) {
+    return name == "rope_axes" || is_append_name(name) || is_attend_name(name);
+}
+
+RopeWords rope_words(const std::string &name, const uint32_t *p) {
+    const bool append = is_append_name(name);
+    const uint32_t *w = p + (append ? 10 : 6);
+    return {p[append ? 5 : 3], w[0], w[1], w[2], {w[3], w[4], w[5], w[6]}};
+}
+
+bool strided_rows_disjoint(size_t a, size_t a_len, size_t b, size_t b_len, size_t stride) {
+    const size_t from = b >= a ? (b - a) % stride : (stride - (a - b) % stride) % stride;
+    return from >= a_len && from + b_len <= stride;
+}
+
 bool is_affine_matrix_name(const std::string &name) {
     return starts_with(name, "matvec_affine") || starts_with(name, "matmul_affine");
 }
@@ -92,9 +111,105 @@ bool ranges_overlap(size_t a, size_t a_len, size_t b, size_t b_len) {
     return a < b + b_len && b < a + a_len;
 }
 
+namespace {
+
+// Layouts of the attention names (no reference counterpart).
+Layout attention_layout(const std::string &name, const uint32_t *p, size_t np) {
+    const bool append = is_append_name(name), attend = is_attend_name(name);
+    const size_t count = append ? 21 : attend ? 14 : 13;
+    ensure(np == count, name + ": expected " + std::to_string(count) + " parameters");
+    auto bytes = [&](std::initializer_list<size_t> v) -> size_t {
+        size_t size = 1;
+        for (size_t b : v) ensure(!mul_overflow(size, b, &size), "GPU shape overflow");
+        return size;
+    };
+    // FP32 rows of `width`, one every `stride` floats.
+    auto rows = [&](size_t tokens, size_t width, size_t stride) -> size_t {
+        ensure(stride >= width, name + ": a row stride is shorter than its row");
+        return width == 0 ? 0 : bytes({tokens - 1, stride, 4}) + bytes({width, 4});
+    };
+    auto threads = [&](std::initializer_list<size_t> v) -> size_t {
+        const size_t n = bytes(v);
+        ensure(n <= UINT32_MAX, "GPU element index overflow");
+        return n;
+    };
+    Layout out;
+    if (append || attend)
+        ensure(p[4] % 8 == 0 && p[4] <= 256, name + ": head dimensions must be multiples of 8, at most 256");
+    size_t position_bytes = 0, freq_bytes = 0;
+    if (!attend) {
+        const RopeWords r = rope_words(name, p);
+        const size_t tokens = p[append ? 1 : 0], dim = p[append ? 4 : 2], pairs = r.rotary / 2;
+        ensure(r.rotary % 2 == 0 && r.rotary <= dim, name + ": the rotary dimensions must be an even part of the head");
+        ensure(append || r.rotary > 0, name + ": dimensions must be nonzero");
+        ensure(r.adjacent <= 1 && r.dealt <= 1, name + ": the pair and section orders must be 0 or 1");
+        ensure(r.rotary == 0 ? r.axes == 0 : r.axes >= 1 && r.axes <= 4, name + ": positions have one through four axes");
+        size_t sum = 0;
+        for (uint32_t i = 0; i < 4; ++i) {
+            ensure(i < r.axes || r.sections[i] == 0, name + ": a section belongs to no axis");
+            sum += r.sections[i];
+        }
+        ensure(sum == pairs, name + ": the sections must add up to half the rotary dimensions");
+        // Dealt in turn, axis i > 0 takes pairs i, i + axes, ..: all of them there.
+        for (size_t i = 1; r.dealt && i < r.axes; ++i)
+            ensure(r.sections[i] == 0 || i + size_t(r.axes) * (r.sections[i] - 1) < pairs,
+                   name + ": the pairs cannot be dealt to these sections");
+        position_bytes = bytes({r.axes, tokens, 4});
+        freq_bytes = pairs * 4;
+    }
+    if (!append && !attend) {
+        for (size_t i : {0, 1, 2}) ensure(p[i] > 0, name + ": dimensions must be nonzero");
+        ensure(p[2] % 2 == 0 && p[2] <= 256, name + ": head dimensions must be even and at most 256");
+        const size_t width = bytes({p[1], p[2]});
+        out.sizes = {rows(p[0], width, p[4]), position_bytes, freq_bytes, rows(p[0], width, p[5])};
+        out.threads = threads({p[0], p[1], 32});
+        return out;
+    }
+    const size_t seqs = p[0], tokens = p[1], heads = p[2], kv_heads = p[3], dim = p[4];
+    const uint32_t *cache = p + (append ? 18 : 7);
+    const size_t page = cache[0], pages = cache[1], columns = cache[2];
+    ensure(seqs > 0 && tokens > 0 && kv_heads > 0 && dim > 0 && page > 0 && pages > 0 && columns > 0 &&
+               (append || heads > 0),
+           name + ": dimensions must be nonzero");
+    ensure(heads % kv_heads == 0, name + ": query heads must be a multiple of the key-value heads");
+    ensure(page % 32 == 0 && (page & (page - 1)) == 0, name + ": pages must hold a power of two of positions, at least 32");
+    ensure(bytes({columns, page}) <= INT32_MAX, name + ": a sequence's pages hold too many positions");
+    const size_t cache_bytes = bytes({pages, kv_heads, page, dim, 2});
+    const size_t width = bytes({heads, dim}), kv_width = bytes({kv_heads, dim});
+    const std::vector<size_t> where = {bytes({seqs + 1, 4}), bytes({seqs, 4}), bytes({seqs, columns, 4})};
+    auto float_word = [&](size_t i) {
+        float v;
+        std::memcpy(&v, &p[i], 4);
+        return v;
+    };
+    if (append) {
+        const float eps = float_word(17);
+        ensure(p[17] == 0 || (std::isfinite(eps) && eps > 0.f), name + ": epsilon must be finite and positive, or 0 for no norm");
+        const size_t norm = eps > 0.f ? dim * 4 : 0;
+        out.sizes = {rows(tokens, width, p[6]), rows(tokens, kv_width, p[7]), rows(tokens, kv_width, p[8]),
+                     heads > 0 ? norm : 0, norm, position_bytes, freq_bytes, where[0], where[1], where[2],
+                     cache_bytes, cache_bytes, rows(tokens, width, p[9])};
+        out.threads = threads({tokens, heads + 2 * kv_heads, 32});
+        return out;
+    }
+    const float scale = float_word(13);
+    ensure(std::isfinite(scale) && scale > 0.f, name + ": the scale must be finite and positive");
+    ensure(p[10] > 0 && p[10] <= columns * page, name + ": the most keys must be positive and within the table's columns");
+    ensure(p[11] <= 1, name + ": causal must be 0 or 1");
+    ensure(p[12] == 0 || p[11] == 1, name + ": a window needs causal attention");
+    ensure(p[12] <= INT32_MAX, name + ": the window is too long");
+    out.sizes = {rows(tokens, width, p[5]), where[0], where[1], where[2], cache_bytes, cache_bytes,
+                 rows(tokens, width, p[6])};
+    out.threads = threads({tokens, heads, 32});
+    return out;
+}
+
+}  // namespace
+
 // dispatch_layout, matrix part (src/gpu.rs:1041-1172), plus this library's
-// F16-metadata and wide-block names.
+// F16-metadata, wide-block and attention names.
 Layout dispatch_layout(const std::string &name, const uint32_t *p, size_t np) {
+    if (is_attention_name(name)) return attention_layout(name, p, np);
     size_t count;
     if (name == "copy_f32") {
         count = 1;

@@ -90,6 +90,19 @@ bool is_wide_name(const std::string &name);           // matmul_affine_wide*
 bool is_residual_name(const std::string &name);
 bool is_mlp_name(const std::string &name);
 bool is_fused_name(const std::string &name);
+// Attention names with no reference counterpart: rope_axes, and
+// kv_append_rope and attn_paged with their cache's type (_bf16|_f16).
+bool is_append_name(const std::string &name);
+bool is_attend_name(const std::string &name);
+bool is_attention_name(const std::string &name);
+// Where the words of those names stand among their parameters.
+struct RopeWords {
+    uint32_t rotary, adjacent, dealt, axes, sections[4];
+};
+RopeWords rope_words(const std::string &name, const uint32_t *p);
+// Rows of a_len and b_len bytes, one every `stride` bytes from a and from b,
+// of which none of a's shares a byte with one of b's.
+bool strided_rows_disjoint(size_t a, size_t a_len, size_t b, size_t b_len, size_t stride);
 // read_checksum: u32 checksum slots written per launch (the XOR of all of
 // them is the XOR of every 32-bit word read).
 constexpr uint32_t kChecksumSlots = 4096;

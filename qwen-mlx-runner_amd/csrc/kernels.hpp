@@ -1,6 +1,7 @@
 // Launch interface between the host runtime (runtime.cpp) and the HIP
 // kernels (affine_rows.hip, affine_mfma.hip, affine_gemv.hip, affine_tile.hip,
-// dense_mfma.hip, misc_kernels.hip, wide_mfma.hip).
+// dense_mfma.hip, misc_kernels.hip, wide_mfma.hip, rope_append.hip,
+// attn_paged.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -250,6 +251,71 @@ struct WideExtent {
     uint64_t code_end, code_extent, image_end, image_extent, meta_end, meta_extent, meta_short;
 };
 WideExtent wide_address_extent(const AffineArgs &a, WidePlan pl);
+
+// Rotary positions: the first `rotary` dimensions of a head turn in pairs, pair
+// i by the position of its axis times freqs[i]. See rope_append.hip.
+struct RopeSpec {
+    const int32_t *positions;  // [axes][tokens]
+    const float *freqs;        // [rotary / 2]
+    uint32_t rotary;           // 0: nothing turns
+    uint32_t adjacent;         // pairs (2i, 2i + 1) instead of (i, i + rotary/2)
+    uint32_t dealt;            // axes dealt to the pairs in turn, not section by section
+    uint32_t axes;
+    uint32_t sections[4];      // pairs of each axis
+};
+struct RopeArgs {
+    const float *x;
+    float *y;
+    uint32_t tokens, heads, dim, x_stride, y_stride;  // strides: floats from token to token
+    RopeSpec rope;
+};
+hipError_t launch_rope_axes(const RopeArgs &a, const DeviceLimits &lim, hipStream_t stream);
+
+// A paged key-value cache and the sequences that read and extend it. Sequence
+// s has the new tokens starts[s]..starts[s+1]-1, the last `new` of its
+// lengths[s] positions; position p is slot p % page of page table[s][p / page].
+// A page past the pool holds nothing. Block layouts: rope_append.hip.
+struct PagedCache {
+    const uint32_t *starts;   // [seqs + 1]
+    const uint32_t *lengths;  // [seqs]
+    const uint32_t *table;    // [seqs][columns]
+    uint16_t *k;              // [pages][kv_heads][page / 32] key blocks
+    uint16_t *v;              // [pages][kv_heads][page / 32] value blocks
+    uint32_t seqs, tokens, kv_heads, dim, page, pages, columns;
+    bool bf16;
+};
+struct AppendArgs {
+    const float *q, *k, *v;       // rows of one token each
+    const float *q_norm, *k_norm; // [dim], used when eps > 0
+    float *q_out;
+    uint32_t heads, q_stride, k_stride, v_stride, out_stride;
+    float eps;                    // 0: no normalisation
+    RopeSpec rope;
+    PagedCache cache;
+};
+hipError_t launch_kv_append_rope(const AppendArgs &a, const DeviceLimits &lim, hipStream_t stream);
+
+// Attention of the new tokens over the cache. See attn_paged.hip.
+struct AttendArgs {
+    const float *q;  // [tokens] rows of heads * dim
+    float *out;
+    uint32_t heads, q_stride, out_stride;
+    uint32_t max_keys;  // no key at or past this position is read
+    uint32_t causal, window;
+    float scale;
+    PagedCache cache;
+};
+// What a launch does, from sizes alone: the lengths are on the device.
+struct AttendPlan {
+    uint32_t rows = 0;      // query rows of one tile
+    uint32_t tiles = 0;     // tiles of all sequences, at most
+    uint32_t splits = 1;    // key ranges of a tile
+    uint32_t keys = 0;      // keys of one range
+    size_t workspace = 0;   // bytes of the ranges' partial results
+};
+AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t workspace_limit);
+hipError_t launch_attn_paged(const AttendArgs &a, const AttendPlan &pl, void *workspace, hipStream_t stream);
+const char *attend_kernel_name(const AttendPlan &pl);
 
 // The plan the GEMV launcher would use (for tests and tuning reports).
 GemvPlan plan_affine_gemv(const AffineArgs &a, GemvPlan forced, const DeviceLimits &lim);

@@ -76,6 +76,9 @@ struct qmr_device {
     // Workspace of the wide-block kernel: the activation images.
     unsigned char *ws_wide = nullptr;
     size_t ws_wide_bytes = 0;
+    // Workspace of the paged attention's key ranges.
+    unsigned char *ws_attend = nullptr;
+    size_t ws_attend_bytes = 0;
     // This GPU's copy of the static scratch (the workspace of
     // qmr_encode_static, which allocates nothing), and how many of its
     // leading bytes may be non-zero (shared by every handle on the GPU).
@@ -839,6 +842,137 @@ hipError_t launch_wide_block(qmr_device *dev, const qmr::AffineArgs &a, unsigned
     return e;
 }
 
+// Views of the attention names, beyond their sizes: caches start on 16 bytes;
+// an output shares no byte with another view, except that rotated rows may be
+// written over their source and may stand beside other rows of one buffer
+// (queries, keys and values as columns of one product).
+void check_attention_views(const std::string &name, qmr_buffer *const *buffers, const size_t *offsets,
+                           const std::vector<size_t> &sizes, const uint32_t *p) {
+    auto off = [&](size_t i) -> size_t { return offsets ? offsets[i] : 0; };
+    // The FP32 rows of a view: its width and stride in bytes, 0 for other views.
+    auto row = [&](size_t i, size_t &width, size_t &stride) {
+        size_t floats = 0, step = 0;
+        if (name == "rope_axes") {
+            if (i == 0 || i == 3) floats = size_t(p[1]) * p[2], step = p[i == 0 ? 4 : 5];
+        } else if (qmr::is_append_name(name)) {
+            if (i == 0 || i == 12) floats = size_t(p[2]) * p[4], step = p[i == 0 ? 6 : 9];
+            if (i == 1 || i == 2) floats = size_t(p[3]) * p[4], step = p[6 + i];
+        } else if (i == 0 || i == 6) {
+            floats = size_t(p[2]) * p[4], step = p[i == 0 ? 5 : 6];
+        }
+        width = floats * 4;
+        stride = step * 4;
+    };
+    auto apart = [&](size_t out, size_t i) {
+        if (buffers[i] != buffers[out] || sizes[i] == 0 || sizes[out] == 0 ||
+            !qmr::ranges_overlap(off(i), sizes[i], off(out), sizes[out]))
+            return;
+        size_t wo, so, wi, si;
+        row(out, wo, so);
+        row(i, wi, si);
+        const bool rows = wo != 0 && wi != 0 && so == si;
+        const bool in_place = rows && i == 0 && !qmr::is_attend_name(name) && off(i) == off(out);
+        ensure(in_place || (rows && qmr::strided_rows_disjoint(off(out), wo, off(i), wi, so)),
+               name + ": output overlaps input buffer " + std::to_string(i));
+    };
+    const size_t last = sizes.size() - 1;
+    if (qmr::is_append_name(name)) {
+        for (size_t out : {size_t(10), size_t(11)}) {
+            ensure(off(out) % 16 == 0, name + ": caches require a 16-byte aligned offset");
+            for (size_t i = 0; i < out; ++i) apart(out, i);
+        }
+    } else if (qmr::is_attend_name(name)) {
+        ensure(off(4) % 16 == 0 && off(5) % 16 == 0, name + ": caches require a 16-byte aligned offset");
+    }
+    for (size_t i = 0; i < last; ++i) apart(last, i);
+}
+
+// rope_axes, kv_append_rope_* and attn_paged_*.
+hipError_t launch_attention(qmr_device *dev, const std::string &name, qmr_buffer *const *buffers, const size_t *offsets,
+                            const uint32_t *p, unsigned char *fixed) {
+    auto ptr = [&](size_t i) -> char * { return static_cast<char *>(buffers[i]->ptr) + (offsets ? offsets[i] : 0); };
+    auto f32 = [&](size_t i) { return reinterpret_cast<float *>(ptr(i)); };
+    auto u32 = [&](size_t i) { return reinterpret_cast<const uint32_t *>(ptr(i)); };
+    auto rope_at = [&](size_t positions) {
+        const qmr::RopeWords w = qmr::rope_words(name, p);
+        qmr::RopeSpec r{};
+        r.positions = reinterpret_cast<const int32_t *>(ptr(positions));
+        r.freqs = f32(positions + 1);
+        r.rotary = w.rotary;
+        r.adjacent = w.adjacent;
+        r.dealt = w.dealt;
+        r.axes = w.axes;
+        std::copy(w.sections, w.sections + 4, r.sections);
+        return r;
+    };
+    auto cache_at = [&](size_t starts, size_t words) {
+        qmr::PagedCache c{};
+        c.starts = u32(starts);
+        c.lengths = u32(starts + 1);
+        c.table = u32(starts + 2);
+        c.k = reinterpret_cast<uint16_t *>(ptr(starts + 3));
+        c.v = reinterpret_cast<uint16_t *>(ptr(starts + 4));
+        c.seqs = p[0];
+        c.tokens = p[1];
+        c.kv_heads = p[3];
+        c.dim = p[4];
+        c.page = p[words];
+        c.pages = p[words + 1];
+        c.columns = p[words + 2];
+        c.bf16 = qmr::ends_with(name, "_bf16");
+        return c;
+    };
+    if (name == "rope_axes") {
+        start_gpu(dev);
+        return qmr::launch_rope_axes({f32(0), f32(3), p[0], p[1], p[2], p[4], p[5], rope_at(1)}, dev->limits, dev->stream);
+    }
+    if (qmr::is_append_name(name)) {
+        qmr::AppendArgs a{};
+        a.q = f32(0);
+        a.k = f32(1);
+        a.v = f32(2);
+        a.q_norm = f32(3);
+        a.k_norm = f32(4);
+        a.q_out = f32(12);
+        a.heads = p[2];
+        a.q_stride = p[6];
+        a.k_stride = p[7];
+        a.v_stride = p[8];
+        a.out_stride = p[9];
+        std::memcpy(&a.eps, &p[17], 4);
+        a.rope = rope_at(5);
+        a.cache = cache_at(7, 18);
+        start_gpu(dev);
+        return qmr::launch_kv_append_rope(a, dev->limits, dev->stream);
+    }
+    qmr::AttendArgs a{};
+    a.q = f32(0);
+    a.out = f32(6);
+    a.heads = p[2];
+    a.q_stride = p[5];
+    a.out_stride = p[6];
+    a.max_keys = p[10];
+    a.causal = p[11];
+    a.window = p[12];
+    std::memcpy(&a.scale, &p[13], 4);
+    a.cache = cache_at(1, 7);
+    const qmr::AttendPlan pl = qmr::plan_attend(a, dev->limits, fixed ? QMR_STATIC_SCRATCH_BYTES : SIZE_MAX);
+    if (fixed) {
+        check_static_scratch(pl.workspace, "attention's key ranges");
+        if (pl.workspace) mark_static_dirty(dev, pl.workspace);
+    } else if (pl.workspace > dev->ws_attend_bytes) {
+        check_hip(hipStreamSynchronize(dev->stream), "hipStreamSynchronize");
+        if (dev->ws_attend) hipFree(dev->ws_attend);
+        dev->ws_attend = nullptr;
+        dev->ws_attend_bytes = 0;
+        check_hip(hipMalloc(&dev->ws_attend, pl.workspace), "hipMalloc (attention workspace)");
+        dev->ws_attend_bytes = pl.workspace;
+    }
+    dev->last_hip = qmr::attend_kernel_name(pl);
+    start_gpu(dev);
+    return qmr::launch_attn_paged(a, pl, fixed ? fixed : dev->ws_attend, dev->stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -919,6 +1053,7 @@ void qmr_device_close(qmr_device *device) {
         hipStreamDestroy(device->stream);
     }
     if (device->ws_wide) hipFree(device->ws_wide);
+    if (device->ws_attend) hipFree(device->ws_attend);
     if (device->ws_slots) hipFree(device->ws_slots);
     if (device->ws_counters) hipFree(device->ws_counters);
     if (device->status_host) hipHostFree(device->status_host);
@@ -1259,6 +1394,9 @@ static int encode_command(qmr_command *command, const char *cname, qmr_buffer *c
         // (the in-place x += W a of a decoder layer).
         const bool fused = qmr::is_fused_name(name);
         ensure(!dev->reference || !fused, "Fused dispatch is unavailable in reference mode");
+        const bool attention = qmr::is_attention_name(name);
+        ensure(!dev->reference || !attention, "Attention dispatch is unavailable in reference mode");
+        if (attention) check_attention_views(name, buffers, offsets, layout.sizes, params);
         if (qmr::starts_with(name, "matmul_") || name == "copy_f32" || name == "read_checksum" || fused) {
             const size_t out = nbuffers - 1;
             for (size_t i = 0; i < out; ++i) {
@@ -1322,8 +1460,10 @@ static int encode_command(qmr_command *command, const char *cname, qmr_buffer *c
         hipError_t e = hipSuccess;
         // Families that launch without workspace start the frame's GPU time
         // here; the others start it after their workspace is in place.
-        if (!qmr::starts_with(name, "mat") && !fused) start_gpu(dev);
-        if (qmr::starts_with(name, "embed_affine")) {
+        if (!qmr::starts_with(name, "mat") && !fused && !attention) start_gpu(dev);
+        if (attention) {
+            e = launch_attention(dev, name, buffers, offsets, params, fixed);
+        } else if (qmr::starts_with(name, "embed_affine")) {
             e = qmr::launch_embed_affine(reinterpret_cast<const uint32_t *>(ptr(0)), ptr(1), ptr(2),
                                          meta, params[0], params[1], params[2], params[3],
                                          reinterpret_cast<float *>(ptr(3)), dev->stream);
@@ -1645,7 +1785,7 @@ int qmr_gemv_plan(const qmr_device *device, uint32_t rows, uint32_t cols, uint32
 size_t qmr_device_workspace_bytes(const qmr_device *device) {
     if (!device) return 0;
     return device->ws_slots_bytes + device->ws_counter_count * sizeof(uint32_t) +
-           device->ws_wide_bytes;
+           device->ws_wide_bytes + device->ws_attend_bytes;
 }
 
 size_t qmr_device_max_lds(const qmr_device *device) {
