@@ -251,8 +251,9 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttendArgs a, Atten
     const int base = lo_first / int(kBlock) * int(kBlock);
     const bool one_range = base + int64_t(pl.keys) >= hi_last;
     const int64_t from64 = base + int64_t(split) * pl.keys;
-    const int from = from64 < hi_last ? int(from64) : hi_last;
-    const int to = int(min(from64 + int64_t(pl.keys), int64_t(hi_last)));
+    const bool some = from64 < hi_last;
+    const int from = some ? int(from64) : 0;
+    const int to = some ? int(min(from64 + int64_t(pl.keys), int64_t(hi_last))) : 0;
 
     f4 o[NB][VT];
 #pragma unroll
@@ -512,8 +513,6 @@ hipError_t launch_type(const AttendArgs &a, const AttendPlan &pl, const Partial 
 }  // namespace
 
 AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t workspace_limit) {
-    (void)lim;
-    (void)workspace_limit;
     const PagedCache &c = a.cache;
     const uint64_t group = a.heads / c.kv_heads;
     AttendPlan pl;
@@ -523,9 +522,23 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
     const uint64_t by_rows = n + (c.tokens * group - n) / pl.rows;
     const uint64_t by_token = c.tokens * ((group + pl.rows - 1) / pl.rows);
     pl.tiles = uint32_t(by_rows < by_token ? by_rows : by_token);
-    pl.splits = 1;
-    pl.keys = (a.max_keys + kBlock - 1) / kBlock * kBlock;
+    // The keys that a tile's rows see, at most: with a window those of its
+    // first row to those of its last.
+    const uint64_t across = (pl.rows + group - 1) / group + kBlock;
+    const uint64_t keys = a.window && a.window + across < a.max_keys ? a.window + across : a.max_keys;
+    // Ranges of keys until every CU has two workgroups; a range gives each
+    // wave a block at least.
+    const uint64_t units = uint64_t(pl.tiles) * c.kv_heads, want = 2 * uint64_t(lim.num_cus);
+    const uint64_t step = kWaves * kBlock;
+    uint64_t splits = units < want ? want / units : 1;
+    pl.keys = uint32_t(((keys + splits - 1) / splits + step - 1) / step * step);
+    pl.splits = uint32_t((keys + pl.keys - 1) / pl.keys);
     pl.workspace = workspace_of(a, pl);
+    while (pl.splits > 1 && pl.workspace > workspace_limit) {
+        pl.keys *= 2;
+        pl.splits = uint32_t((keys + pl.keys - 1) / pl.keys);
+        pl.workspace = workspace_of(a, pl);
+    }
     return pl;
 }
 
