@@ -37,6 +37,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr uint32_t kMaxSplits = 512;  // key ranges of a tile, at most
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
 // Terms of an FP32 operand in the cache's type.
@@ -140,18 +141,24 @@ struct Partial {
     uint32_t *place;
 };
 
-__device__ __forceinline__ bool not_finite(u4 v, bool bf16) {
-    const uint32_t e = bf16 ? 0x7F80u : 0x7C00u;
+template <bool BF16>
+__device__ __forceinline__ bool not_finite(u4 v) {
+    constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
     bool bad = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (v[i] & e) == e || ((v[i] >> 16) & e) == e;
+    for (int i = 0; i < 4; ++i) bad |= (v[i] & e) == e || (v[i] & (e << 16)) == e << 16;
     return bad;
 }
 
-template <bool BF16>
-__device__ __forceinline__ float half_f32(uint16_t h) {
-    if constexpr (BF16) return __uint_as_float(uint32_t(h) << 16);
-    return float(__builtin_bit_cast(_Float16, h));
+// Ones in the halves of the keys first..first+7 that lie in [lo, hi).
+__device__ __forceinline__ u4 halves_of(int first, int lo, int hi) {
+    u4 m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int k = first + 2 * i;
+        m[i] = (k >= lo && k < hi ? 0x0000FFFFu : 0u) | (k + 1 >= lo && k + 1 < hi ? 0xFFFF0000u : 0u);
+    }
+    return m;
 }
 
 // Few rows: R = 16 NB rows a workgroup, every wave all of them over its own
@@ -160,7 +167,7 @@ __device__ __forceinline__ float half_f32(uint16_t h) {
 // shared but the queries, which wait in LDS as operands. The waves' m, l and O
 // are joined through LDS at the end.
 template <bool BF16, int DM, int NB, bool FULL>
-__global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttendArgs a, AttendPlan pl, Partial ws, bool aligned) {
+__global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(AttendArgs a, AttendPlan pl, Partial ws, bool aligned) {
     constexpr int R = 16 * NB, T = kTerms<BF16>, KS = DM / 32, VT = DM / 16;
     // f16 weights are up to 2^15, so that small ones stay normal; the maximum
     // lags by at most 2^kLag.
@@ -261,14 +268,19 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttendArgs a, Atten
 #pragma unroll
         for (int d = 0; d < VT; ++d) o[nb][d] = f4{0.f, 0.f, 0.f, 0.f};
 
-    const uint32_t *table = c.table + size_t(t.seq) * c.columns;
-    for (int key0 = (from / int(kBlock) + int(w)) * int(kBlock); key0 < to; key0 += kWaves * int(kBlock)) {
-        const uint32_t named = __builtin_amdgcn_readfirstlane(table[uint32_t(key0) / c.page]);
-        const bool held = named < c.pages;
-        const size_t at = attn::block_at(c, held ? named : 0, head, uint32_t(key0) % c.page / kBlock);
+    // Blocks w, w + 4, .. of the range. A block's keys are loaded while the
+    // block before is worked on, its values while its scores are; the page
+    // after next is named by then. Pages are read as constants (scalar loads),
+    // whose wait does not wait for the blocks in flight.
+    const auto *table = (const __attribute__((address_space(4))) uint32_t *)(c.table + size_t(t.seq) * c.columns);
+    const uint32_t last_column = c.columns - 1, page_shift = __builtin_ctz(c.page);
+    auto page_of = [&](int key0) { return table[min(uint32_t(key0) >> page_shift, last_column)]; };
+    auto block_of = [&](uint32_t named, int key0) {
+        return attn::block_at(c, named < c.pages ? named : 0, head, (uint32_t(key0) & (c.page - 1)) / kBlock);
+    };
+    u4 k[KS][2];
+    auto load_keys = [&](size_t at) {
         const u4 *kp = reinterpret_cast<const u4 *>(c.k + at);
-        const u4 *vp = reinterpret_cast<const u4 *>(c.v + at);
-        u4 k[KS][2], v[VT];
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
 #pragma unroll
@@ -279,6 +291,21 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttendArgs a, Atten
                     k[s][i] = u4{0, 0, 0, 0};
             }
         }
+    };
+    const int step = kWaves * int(kBlock);
+    int key0 = from + int(w) * int(kBlock);
+    uint32_t named = 0, next = 0;
+    size_t at = 0;
+    if (key0 < to) {
+        named = page_of(key0);
+        next = page_of(key0 + step);
+        at = block_of(named, key0);
+        load_keys(at);
+    }
+    for (; key0 < to; key0 += step) {
+        const bool held = named < c.pages;
+        const u4 *vp = reinterpret_cast<const u4 *>(c.v + at);
+        u4 v[VT];
 #pragma unroll
         for (int d = 0; d < VT; ++d) v[d] = vp[g * dim + (FULL ? 16 * d + n : min(16 * d + n, dim - 1))];
 
@@ -286,33 +313,43 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttendArgs a, Atten
         bool apart = false;  // a value that some rows see and others do not is not finite
         if (edge) {
             // Values that no row sees may be anything: zero them.
-            const int from_key = key0 + 8 * int(g);
+            const u4 kept = halves_of(key0 + 8 * int(g), held ? lo_first : hi_last, hi_last);
 #pragma unroll
             for (int d = 0; d < VT; ++d) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int key = from_key + e;
-                    if (!held || key < lo_first || key >= hi_last) v[d][e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
-                }
-                apart |= not_finite(v[d], BF16);
+                v[d] &= kept;
+                apart |= not_finite<BF16>(v[d]);
             }
             apart = __ballot(apart) != 0;
         }
+        // The queries' operands come from LDS for every block where they and
+        // the block do not fit the registers together.
+        uint32_t ql = l;
+        if constexpr (DM == 256 || NB > 1 || !FULL) asm volatile("" : "+v"(ql));
+        f4 scores[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            f4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+            scores[nb][0] = scores[nb][1] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
 #pragma unroll
                 for (int i = 0; i < T; ++i) {
-                    const u4 q = qs[((nb * KS + s) * T + i) * 64 + l];
-                    s0 = mfma16<BF16>(k[s][0], q, s0);
-                    s1 = mfma16<BF16>(k[s][1], q, s1);
+                    const u4 q = qs[((nb * KS + s) * T + i) * 64 + ql];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) scores[nb][j] = mfma16<BF16>(k[s][j], q, scores[nb][j]);
                 }
             }
+        }
+        named = next;
+        if (key0 + step < to) {
+            at = block_of(named, key0 + step);
+            load_keys(at);
+        }
+        next = page_of(key0 + 2 * step);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
             float p[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = s0[i], p[4 + i] = s1[i];
+            for (int i = 0; i < 4; ++i) p[i] = scores[nb][0][i], p[4 + i] = scores[nb][1][i];
             if (edge) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -340,33 +377,28 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttendArgs a, Atten
                 p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], rs[nb], off));
                 sum[nb] += p[e];
             }
-            if (apart) {
-                // Row by row: a hidden value must not even meet a zero weight.
-                for (uint32_t j = 0; j < 4; ++j) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int key = key0 + 8 * int(j) + e;
-                        const float pj = __shfl(p[e], n + 16 * j);
-                        const bool seen = held && key >= lo[nb] && key < hi[nb];
-#pragma unroll
-                        for (int d = 0; d < VT; ++d) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t at_d = min(uint32_t(16 * d + 4 * g + i), dim - 1);
-                                const uint16_t h = reinterpret_cast<const uint16_t *>(vp)[(j * dim + at_d) * 8 + e];
-                                if (seen) o[nb][d][i] = fmaf(pj, half_f32<BF16>(h), o[nb][d][i]);
-                            }
-                        }
-                    }
-                }
-                continue;
-            }
             u4 pt[T];
             split8<BF16>(p, pt);
+            if (!apart) {
 #pragma unroll
-            for (int d = 0; d < VT; ++d) {
+                for (int d = 0; d < VT; ++d) {
 #pragma unroll
-                for (int i = 0; i < T; ++i) o[nb][d] = mfma16<BF16>(v[d], pt[i], o[nb][d]);
+                    for (int i = 0; i < T; ++i) o[nb][d] = mfma16<BF16>(v[d], pt[i], o[nb][d]);
+                }
+            } else {
+                // A hidden value must not even meet a zero weight: row by row,
+                // with the values that the row sees.
+#pragma unroll 1
+                for (uint32_t r = 0; r < 16; ++r) {
+                    const u4 kept = halves_of(key0 + 8 * int(g), __shfl(lo[nb], r), __shfl(hi[nb], r));
+#pragma unroll
+                    for (int d = 0; d < VT; ++d) {
+                        f4 row = o[nb][d];
+#pragma unroll
+                        for (int i = 0; i < T; ++i) row = mfma16<BF16>(v[d] & kept, pt[i], row);
+                        if (n == r) o[nb][d] = row;
+                    }
+                }
             }
         }
     }
@@ -416,7 +448,7 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttendArgs a, Atten
                         for (int k = 0; k < 4; ++k) y[k] = acc[k];
                     }
                 }
-            } else {
+            } else if (real) {
                 if (joined != 0.f) *reinterpret_cast<f4 *>(ws.o + (part + rn) * DM + d) = acc;
                 if (d == 0) ws.ml[part + rn] = make_float2(top, joined);
             }
@@ -426,33 +458,41 @@ __global__ __launch_bounds__(kThreads) void attn_rows_kernel(AttendArgs a, Atten
 }
 
 // Adds the ranges of a row up: a workgroup a row, every wave a quarter of the
-// ranges.
+// ranges, whose loads depend on nothing and are all in flight at once.
 template <int DM>
-__global__ __launch_bounds__(kThreads) void attn_join_kernel(AttendArgs a, AttendPlan pl, Partial ws, bool aligned) {
+__global__ __launch_bounds__(kThreads) void attn_join_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
     constexpr int E = DM / 64;
-    __shared__ float part_o[kWaves][DM], part_l[kWaves];
+    typedef float fe __attribute__((ext_vector_type(E)));
+    __shared__ float weight[kMaxSplits], part_o[kWaves][DM], part_l[kWaves];
     const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64;
     const uint32_t place = ws.place[blockIdx.x];
     if (place == kNone) return;
     const uint32_t unit = blockIdx.x / pl.rows, r = blockIdx.x % pl.rows;
     const size_t first = size_t(unit) * pl.splits * pl.rows + r;
-    float top = -INFINITY;
+    float top = -INFINITY, all = 0.f;
     for (uint32_t s = l; s < pl.splits; s += 64) top = fmaxf(top, ws.ml[first + size_t(s) * pl.rows].x);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    float acc[E] = {}, all = 0.f;
-    for (uint32_t s = w; s < pl.splits; s += kWaves) {
-        const size_t at = first + size_t(s) * pl.rows;
-        const float2 ml = ws.ml[at];
-        if (ml.y == 0.f) continue;
-        const float f = ml.x == -INFINITY ? 1.f : exp2f(ml.x - top);
+    // A range that saw nothing (its sum is 0) left no row.
+    for (uint32_t s = threadIdx.x; s < pl.splits; s += kThreads) {
+        const float2 ml = ws.ml[first + size_t(s) * pl.rows];
+        const float f = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? 1.f : exp2f(ml.x - top);
+        weight[s] = ml.y == 0.f ? -1.f : f;
         all += f * ml.y;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += f * ws.o[at * DM + e * 64 + l];
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) part_o[w][e * 64 + l] = acc[e];
+    for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
     if (l == 0) part_l[w] = all;
+    __syncthreads();
+    fe acc = {};
+    const fe *o = reinterpret_cast<const fe *>(ws.o + first * DM) + l;
+#pragma unroll 8
+    for (uint32_t s = w; s < pl.splits; s += kWaves) {
+        const fe x = o[size_t(s) * pl.rows * (DM / E)];
+        const float f = weight[s];
+        if (f >= 0.f || f != f) acc += f * x;
+    }
+    *reinterpret_cast<fe *>(&part_o[w][l * E]) = acc;
     __syncthreads();
     all = part_l[0] + part_l[1] + part_l[2] + part_l[3];
     const float f = all == 0.f ? 0.f : 1.f / all;
@@ -497,7 +537,7 @@ template <bool BF16, int DM>
 hipError_t launch_dim(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, bool aligned, hipStream_t stream) {
     hipError_t e = launch_rows<BF16, DM, 1>(a, pl, ws, aligned, stream);
     if (e != hipSuccess || pl.splits == 1) return e;
-    attn_join_kernel<DM><<<pl.tiles * a.cache.kv_heads * pl.rows, kThreads, 0, stream>>>(a, pl, ws, aligned);
+    attn_join_kernel<DM><<<pl.tiles * a.cache.kv_heads * pl.rows, kThreads, 0, stream>>>(a, pl, ws);
     return hipGetLastError();
 }
 
@@ -531,6 +571,7 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
     const uint64_t units = uint64_t(pl.tiles) * c.kv_heads, want = 2 * uint64_t(lim.num_cus);
     const uint64_t step = kWaves * kBlock;
     uint64_t splits = units < want ? want / units : 1;
+    if (splits > kMaxSplits) splits = kMaxSplits;
     pl.keys = uint32_t(((keys + splits - 1) / splits + step - 1) / step * step);
     pl.splits = uint32_t((keys + pl.keys - 1) / pl.keys);
     pl.workspace = workspace_of(a, pl);
