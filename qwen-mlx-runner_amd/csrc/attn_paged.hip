@@ -94,12 +94,13 @@ __device__ __forceinline__ bool find_tile(const PagedCache &c, uint32_t group, u
     const uint32_t l = threadIdx.x % 64;
     for (uint32_t base = 0; base < c.seqs; base += 64) {
         const uint32_t s = base + l;
-        uint32_t from = 0, count = 0;
+        uint32_t from = 0, end = 0, length = 0;
         if (s < c.seqs) {
             from = c.starts[s];
-            const uint32_t to = min(c.starts[s + 1], c.tokens);
-            count = to > from ? to - from : 0;
+            end = c.starts[s + 1];
+            length = c.lengths[s];
         }
+        const uint32_t to = min(end, c.tokens), count = to > from ? to - from : 0;
         const uint32_t own = (count * group + R - 1) / R;
         uint32_t sum = own;
 #pragma unroll
@@ -117,8 +118,8 @@ __device__ __forceinline__ bool find_tile(const PagedCache &c, uint32_t group, u
         t.first_token = __builtin_amdgcn_readfirstlane(__shfl(from, at));
         t.rows = __builtin_amdgcn_readfirstlane(__shfl(count, at)) * group;
         t.row0 = __builtin_amdgcn_readfirstlane((tile - __shfl(sum - own, at)) * R);
-        t.length = int(min(c.lengths[t.seq], 0x7FFFFFFFu));
-        t.context = t.length - int(c.starts[t.seq + 1] - t.first_token);
+        t.length = int(min(uint32_t(__builtin_amdgcn_readfirstlane(__shfl(length, at))), 0x7FFFFFFFu));
+        t.context = t.length - int(__builtin_amdgcn_readfirstlane(__shfl(end, at)) - t.first_token);
         return true;
     }
     return false;
@@ -188,70 +189,6 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
     }
     const uint32_t in_tile = min(uint32_t(R), t.rows - t.row0);
 
-    // The queries, as operands.
-    u4 *qs = reinterpret_cast<u4 *>(lds);  // [NB][KS][T][64 lanes]
-    {
-        const uint32_t qn = threadIdx.x / 16, p = threadIdx.x % 16;
-        constexpr int CH = (DM / 8 + 15) / 16;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            const uint32_t r = nb * 16 + qn;
-            float x[CH][8], most = 0.f;
-            const uint32_t row = t.row0 + min(r, in_tile - 1);
-            const float *q = a.q + size_t(t.first_token + row / group) * a.q_stride +
-                             size_t(head * group + row % group) * dim;
-#pragma unroll
-            for (int k = 0; k < CH; ++k) {
-                const uint32_t ch = p + 16 * k;
-                const bool in = r < in_tile && ch * 8 < dim;
-                if (in && aligned) {
-                    *reinterpret_cast<float4 *>(x[k]) = *reinterpret_cast<const float4 *>(q + ch * 8);
-                    *reinterpret_cast<float4 *>(x[k] + 4) = *reinterpret_cast<const float4 *>(q + ch * 8 + 4);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[k][j] = in ? q[ch * 8 + j] : 0.f;
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    x[k][j] *= a.scale * kLog2e;
-                    most = fmaxf(most, fabsf(x[k][j]));
-                }
-            }
-            int e = 0;
-            if constexpr (!BF16) {
-#pragma unroll
-                for (int d = 1; d < 16; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-                if (most > 0.f && most < INFINITY) frexpf(most, &e), e -= 15;
-            }
-            if (p == 0) row_scale[r] = ldexpf(1.f, e);
-#pragma unroll
-            for (int k = 0; k < CH; ++k) {
-                const uint32_t ch = p + 16 * k;
-                if (ch >= DM / 8) continue;
-                if constexpr (!BF16) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[k][j] = ldexpf(x[k][j], -e);
-                }
-                u4 terms[T];
-                split8<BF16>(x[k], terms);
-#pragma unroll
-                for (int i = 0; i < T; ++i) qs[((nb * KS + ch / 4) * T + i) * 64 + (ch % 4) * 16 + qn] = terms[i];
-            }
-        }
-    }
-    __syncthreads();
-
-    // What each row and the whole tile may see.
-    int lo[NB], hi[NB];
-    float rs[NB], m[NB], sum[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const uint32_t r = nb * 16 + n;
-        visible(a, t, (t.row0 + min(r, in_tile - 1)) / group, lo[nb], hi[nb]);
-        rs[nb] = row_scale[r];
-        m[nb] = -INFINITY;
-        sum[nb] = 0.f;
-    }
     int lo_first, hi_first, lo_last, hi_last;
     visible(a, t, t.row0 / group, lo_first, hi_first);
     visible(a, t, (t.row0 + in_tile - 1) / group, lo_last, hi_last);
@@ -262,16 +199,34 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
     const int from = some ? int(from64) : 0;
     const int to = some ? int(min(from64 + int64_t(pl.keys), int64_t(hi_last))) : 0;
 
-    f4 o[NB][VT];
+    // The queries' loads go out first: thread (row % 16, p) has chunks p and
+    // p + 16 of 8 dims.
+    constexpr int CH = (DM / 8 + 15) / 16;
+    const uint32_t qn = threadIdx.x / 16, qp = threadIdx.x % 16;
+    float x[NB][CH][8];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int nb = 0; nb < NB; ++nb) {
+        const uint32_t r = nb * 16 + qn, row = t.row0 + min(r, in_tile - 1);
+        const float *q = a.q + size_t(t.first_token + row / group) * a.q_stride + size_t(head * group + row % group) * dim;
 #pragma unroll
-        for (int d = 0; d < VT; ++d) o[nb][d] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < CH; ++k) {
+            const uint32_t ch = qp + 16 * k;
+            const bool in = r < in_tile && ch * 8 < dim;
+            if (in && aligned) {
+                *reinterpret_cast<float4 *>(x[nb][k]) = *reinterpret_cast<const float4 *>(q + ch * 8);
+                *reinterpret_cast<float4 *>(x[nb][k] + 4) = *reinterpret_cast<const float4 *>(q + ch * 8 + 4);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[nb][k][j] = in ? q[ch * 8 + j] : 0.f;
+            }
+        }
+    }
 
     // Blocks w, w + 4, .. of the range. A block's keys are loaded while the
-    // block before is worked on, its values while its scores are; the page
-    // after next is named by then. Pages are read as constants (scalar loads),
-    // whose wait does not wait for the blocks in flight.
+    // block before is weighed, its values while its scores are worked out, the
+    // first ones while the queries are; the page after next is named by then.
+    // Pages are read as constants (scalar loads), whose wait does not wait for
+    // the blocks in flight.
     const auto *table = (const __attribute__((address_space(4))) uint32_t *)(c.table + size_t(t.seq) * c.columns);
     const uint32_t last_column = c.columns - 1, page_shift = __builtin_ctz(c.page);
     auto page_of = [&](int key0) { return table[min(uint32_t(key0) >> page_shift, last_column)]; };
@@ -292,6 +247,12 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
             }
         }
     };
+    u4 v[VT];
+    auto load_values = [&](size_t at) {
+        const u4 *vp = reinterpret_cast<const u4 *>(c.v + at);
+#pragma unroll
+        for (int d = 0; d < VT; ++d) v[d] = vp[g * dim + (FULL ? 16 * d + n : min(16 * d + n, dim - 1))];
+    };
     const int step = kWaves * int(kBlock);
     int key0 = from + int(w) * int(kBlock);
     uint32_t named = 0, next = 0;
@@ -301,26 +262,66 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
         next = page_of(key0 + step);
         at = block_of(named, key0);
         load_keys(at);
+        load_values(at);
     }
+
+    // The queries, as operands.
+    u4 *qs = reinterpret_cast<u4 *>(lds);  // [NB][KS][T][64 lanes]
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const uint32_t r = nb * 16 + qn;
+        float most = 0.f;
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[nb][k][j] *= a.scale * kLog2e;
+                most = fmaxf(most, fabsf(x[nb][k][j]));
+            }
+        }
+        int e = 0;
+        if constexpr (!BF16) {
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+            if (most > 0.f && most < INFINITY) frexpf(most, &e), e -= 15;
+        }
+        if (qp == 0) row_scale[r] = ldexpf(1.f, e);
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+            const uint32_t ch = qp + 16 * k;
+            if (ch >= DM / 8) continue;
+            if constexpr (!BF16) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[nb][k][j] = ldexpf(x[nb][k][j], -e);
+            }
+            u4 terms[T];
+            split8<BF16>(x[nb][k], terms);
+#pragma unroll
+            for (int i = 0; i < T; ++i) qs[((nb * KS + ch / 4) * T + i) * 64 + (ch % 4) * 16 + qn] = terms[i];
+        }
+    }
+    __syncthreads();
+
+    // What each row may see.
+    int lo[NB], hi[NB];
+    float rs[NB], m[NB], sum[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const uint32_t r = nb * 16 + n;
+        visible(a, t, (t.row0 + min(r, in_tile - 1)) / group, lo[nb], hi[nb]);
+        rs[nb] = row_scale[r];
+        m[nb] = -INFINITY;
+        sum[nb] = 0.f;
+    }
+    f4 o[NB][VT];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int d = 0; d < VT; ++d) o[nb][d] = f4{0.f, 0.f, 0.f, 0.f};
+
     for (; key0 < to; key0 += step) {
         const bool held = named < c.pages;
-        const u4 *vp = reinterpret_cast<const u4 *>(c.v + at);
-        u4 v[VT];
-#pragma unroll
-        for (int d = 0; d < VT; ++d) v[d] = vp[g * dim + (FULL ? 16 * d + n : min(16 * d + n, dim - 1))];
-
         const bool edge = !held || key0 < lo_last || key0 + int(kBlock) > hi_first;
-        bool apart = false;  // a value that some rows see and others do not is not finite
-        if (edge) {
-            // Values that no row sees may be anything: zero them.
-            const u4 kept = halves_of(key0 + 8 * int(g), held ? lo_first : hi_last, hi_last);
-#pragma unroll
-            for (int d = 0; d < VT; ++d) {
-                v[d] &= kept;
-                apart |= not_finite<BF16>(v[d]);
-            }
-            apart = __ballot(apart) != 0;
-        }
         // The queries' operands come from LDS for every block where they and
         // the block do not fit the registers together.
         uint32_t ql = l;
@@ -345,6 +346,17 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
             load_keys(at);
         }
         next = page_of(key0 + 2 * step);
+        bool apart = false;  // a value that some rows see and others do not is not finite
+        if (edge) {
+            // Values that no row sees may be anything: zero them.
+            const u4 kept = halves_of(key0 + 8 * int(g), held ? lo_first : hi_last, hi_last);
+#pragma unroll
+            for (int d = 0; d < VT; ++d) {
+                v[d] &= kept;
+                apart |= not_finite<BF16>(v[d]);
+            }
+            apart = __ballot(apart) != 0;
+        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             float p[8];
@@ -401,6 +413,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
                 }
             }
         }
+        if (key0 + step < to) load_values(at);
     }
 
     // Join the waves, 16 rows at a time.
