@@ -32,6 +32,7 @@ using attn::kBlock;
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
@@ -50,6 +51,15 @@ __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
     } else {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+}
+
+template <bool BF16>
+__device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
+    if constexpr (BF16) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     }
 }
 
@@ -151,6 +161,18 @@ __device__ __forceinline__ bool not_finite(u4 v) {
     return bad;
 }
 
+// Of each half: itself where finite, else zero; and 1.0 where it is not finite.
+template <bool BF16>
+__device__ __forceinline__ void part_finite(u4 v, u4 &finite, u4 &bad) {
+    constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u, one = BF16 ? 0x3F80u : 0x3C00u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t m = ((v[i] & e) == e ? 0xFFFFu : 0u) | ((v[i] & (e << 16)) == e << 16 ? 0xFFFF0000u : 0u);
+        finite[i] = v[i] & ~m;
+        bad[i] = (one | one << 16) & m;
+    }
+}
+
 // Ones in the halves of the keys first..first+7 that lie in [lo, hi).
 __device__ __forceinline__ u4 halves_of(int first, int lo, int hi) {
     u4 m;
@@ -159,6 +181,16 @@ __device__ __forceinline__ u4 halves_of(int first, int lo, int hi) {
         const int k = first + 2 * i;
         m[i] = (k >= lo && k < hi ? 0x0000FFFFu : 0u) | (k + 1 >= lo && k + 1 < hi ? 0xFFFF0000u : 0u);
     }
+    return m;
+}
+
+// 1.0 in those halves.
+template <bool BF16>
+__device__ __forceinline__ u4 ones_of(int first, int lo, int hi) {
+    constexpr uint32_t one = BF16 ? 0x3F803F80u : 0x3C003C00u;
+    u4 m = halves_of(first, lo, hi);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] &= one;
     return m;
 }
 
@@ -398,18 +430,20 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
                     for (int i = 0; i < T; ++i) o[nb][d] = mfma16<BF16>(v[d], pt[i], o[nb][d]);
                 }
             } else {
-                // A hidden value must not even meet a zero weight: row by row,
-                // with the values that the row sees.
-#pragma unroll 1
-                for (uint32_t r = 0; r < 16; ++r) {
-                    const u4 kept = halves_of(key0 + 8 * int(g), __shfl(lo[nb], r), __shfl(hi[nb], r));
+                // A value that is not finite must not even meet a zero weight:
+                // the finite ones are added up, and the rows that see another
+                // (a count of them) become NaN.
+                const u4 seen = ones_of<BF16>(key0 + 8 * int(g), lo[nb], hi[nb]);
 #pragma unroll
-                    for (int d = 0; d < VT; ++d) {
-                        f4 row = o[nb][d];
+                for (int d = 0; d < VT; ++d) {
+                    u4 finite, bad;
+                    part_finite<BF16>(v[d], finite, bad);
 #pragma unroll
-                        for (int i = 0; i < T; ++i) row = mfma16<BF16>(v[d] & kept, pt[i], row);
-                        if (n == r) o[nb][d] = row;
-                    }
+                    for (int i = 0; i < T; ++i) o[nb][d] = mfma16<BF16>(finite, pt[i], o[nb][d]);
+                    const f4 count = mfma16<BF16>(bad, seen, f4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (count[i] > 0.f) o[nb][d][i] = __builtin_nanf("");
                 }
             }
         }
@@ -468,6 +502,294 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
             if (pl.splits > 1 && split == 0 && d == 0) ws.place[size_t(unit) * R + r] = one_range || !real ? kNone : place;
         }
     }
+}
+
+// Many rows: 128 rows a workgroup, 32 a wave, which keeps its queries' operands
+// and its O in registers; blocks of 32 keys come through LDS, each read by all
+// four waves. v_mfma_f32_32x32x16 (A row and B column lane % 32, K chunk
+// lane / 32; D[i][j] in lane j + 32 (i / 4 % 2), element i % 4 + 4 (i / 8)), keys
+// dealt so that lane (n, g) ends with row n's scores of keys 16s + 8g + 0..7, as
+// P^T has to stand for step s of O^T = V^T P^T.
+//
+// The scores of block b + 1 are worked out while block b's are weighed: matrix
+// and vector instructions that do not wait for each other. Blocks are loaded
+// to registers an iteration before they go to LDS, two deep, one barrier a
+// block.
+template <bool BF16, int DM>
+__global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(AttendArgs a, AttendPlan pl, Partial ws,
+                                                                               bool aligned) {
+    constexpr int R = 32 * kWaves, T = kTerms<BF16>, KS = DM / 16, VT = DM / 32;
+    constexpr float kTop = BF16 ? 0.f : 7.f, kLag = 8.f;
+    constexpr int kChunks = DM * 4;             // 16-byte chunks of a block
+    constexpr int kEach = kChunks / kThreads;   // a thread's
+    __shared__ u4 kl[2][kChunks], vl[2][kChunks];
+    __shared__ int apart[2];
+    const PagedCache &c = a.cache;
+    const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t n = l % 32, g = l / 32;
+    const uint32_t split = blockIdx.x % pl.splits, unit = blockIdx.x / pl.splits;
+    const uint32_t head = unit % c.kv_heads, group = a.heads / c.kv_heads, dim = c.dim;
+    Tile t;
+    // The last tiles first: they see the most keys.
+    if (!find_tile(c, group, R, pl.tiles - 1 - unit / c.kv_heads, t)) {
+        if (pl.splits > 1 && split == 0 && threadIdx.x < R) ws.place[size_t(unit) * R + threadIdx.x] = kNone;
+        return;
+    }
+    const uint32_t in_tile = min(uint32_t(R), t.rows - t.row0);
+    // Keys that some row of the tile sees, and that all do.
+    int lo_tile, hi_tile, lo_most, hi_least;
+    visible(a, t, t.row0 / group, lo_tile, hi_least);
+    visible(a, t, (t.row0 + in_tile - 1) / group, lo_most, hi_tile);
+    const int base = lo_tile / int(kBlock) * int(kBlock);
+    const bool one_range = base + int64_t(pl.keys) >= hi_tile;
+    const int64_t from64 = base + int64_t(split) * pl.keys;
+    const bool some = from64 < hi_tile;
+    const int from = some ? int(from64) : 0;
+    const int to = some ? int(min(from64 + int64_t(pl.keys), int64_t(hi_tile))) : 0;
+
+    // This wave's rows.
+    const uint32_t r0 = 32 * w, r = r0 + n;
+    int lo, hi, hi_first, lo_last, skip;
+    visible(a, t, (t.row0 + min(r, in_tile - 1)) / group, lo, hi);
+    visible(a, t, (t.row0 + min(r0, in_tile - 1)) / group, skip, hi_first);
+    visible(a, t, (t.row0 + min(r0 + 31, in_tile - 1)) / group, lo_last, skip);
+    if (threadIdx.x < 2) apart[threadIdx.x] = -1;
+    __syncthreads();
+
+    const auto *table = (const __attribute__((address_space(4))) uint32_t *)(c.table + size_t(t.seq) * c.columns);
+    const uint32_t last_column = c.columns - 1, page_shift = __builtin_ctz(c.page);
+    auto page_of = [&](int key0) { return table[min(uint32_t(key0) >> page_shift, last_column)]; };
+    auto block_of = [&](uint32_t named, int key0) {
+        return attn::block_at(c, named < c.pages ? named : 0, head, (uint32_t(key0) & (c.page - 1)) / kBlock);
+    };
+    u4 kr[kEach], vr[kEach];
+    auto load = [&](u4 (&to_regs)[kEach], const uint16_t *pool, size_t at) {
+        const u4 *p = reinterpret_cast<const u4 *>(pool + at);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const uint32_t ch = threadIdx.x + i * kThreads;
+            if (ch < dim * 4) to_regs[i] = p[ch];
+        }
+    };
+    auto stage = [&](u4 *lds, const u4 (&regs)[kEach]) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) lds[threadIdx.x + i * kThreads] = regs[i];
+    };
+    // Values that no row of the tile sees may be anything: zeros. Of a block
+    // that some rows see in part, `apart` says whether a value is not finite.
+    auto stage_values = [&](uint32_t to_buffer, int key0, uint32_t named) {
+        const bool held = named < c.pages;
+        if (!held || key0 < lo_most || key0 + int(kBlock) > hi_least) {
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int first = key0 + 8 * int((threadIdx.x + i * kThreads) / dim);
+                vr[i] &= halves_of(first, held ? lo_tile : hi_tile, hi_tile);
+                bad |= not_finite<BF16>(vr[i]);
+            }
+            if (bad) apart[to_buffer] = key0;
+        }
+        stage(vl[to_buffer], vr);
+    };
+    // Chunks past the head's own stay zero.
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) kr[i] = vr[i] = u4{0, 0, 0, 0};
+
+    uint32_t named0 = 0, named1 = 0, named2 = 0;
+    if (from < to) {
+        named0 = page_of(from);
+        named1 = page_of(from + int(kBlock));
+        named2 = page_of(from + 2 * int(kBlock));
+        load(kr, c.k, block_of(named0, from));
+        load(vr, c.v, block_of(named0, from));
+    }
+
+    // Queries.
+    u4 q[KS][T];
+    float rs = 1.f;
+    {
+        const uint32_t row = t.row0 + min(r, in_tile - 1);
+        const float *src = a.q + size_t(t.first_token + row / group) * a.q_stride + size_t(head * group + row % group) * dim;
+        auto read = [&](int s, float (&x)[8]) {
+            const uint32_t d = 16 * s + 8 * g;
+            if (d < dim && aligned) {
+                *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(src + d);
+                *reinterpret_cast<float4 *>(x + 4) = *reinterpret_cast<const float4 *>(src + d + 4);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = d < dim ? src[d + j] : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= a.scale * kLog2e;
+        };
+        int e = 0;
+        if constexpr (!BF16) {
+            float most = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                float x[8];
+                read(s, x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+            }
+            most = fmaxf(most, __shfl_xor(most, 32));
+            if (most > 0.f && most < INFINITY) frexpf(most, &e), e -= 15;
+            rs = ldexpf(1.f, e);
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            float x[8];
+            read(s, x);
+            if constexpr (!BF16) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = ldexpf(x[j], -e);
+            }
+            split8<BF16>(x, q[s]);
+        }
+    }
+    f16v o[VT];
+#pragma unroll
+    for (int d = 0; d < VT; ++d) o[d] = f16v{};
+    float m = -INFINITY, sum = 0.f;
+
+    const uint32_t key_at = g * 32 + (n & 7) + 2 * (n & 8) + (n & 16) / 2;  // where A's row n is in a key chunk pair
+    auto scores = [&](const u4 *kb) {
+        f16v s0 = {};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const u4 k = kb[s * 64 + key_at];
+#pragma unroll
+            for (int i = 0; i < T; ++i) s0 = mfma32<BF16>(k, q[s][i], s0);
+        }
+        return s0;
+    };
+
+    f16v next = {};
+    if (from < to) {
+        stage(kl[0], kr);
+        stage_values(0, from, named0);
+        load(kr, c.k, block_of(named1, from + int(kBlock)));
+        __syncthreads();
+        next = scores(kl[0]);
+        stage(kl[1], kr);
+    }
+    uint32_t b = 0;
+    for (int key0 = from; key0 < to; key0 += int(kBlock), b ^= 1) {
+        f16v p = next;
+        __syncthreads();
+        load(kr, c.k, block_of(named2, key0 + 2 * int(kBlock)));
+        load(vr, c.v, block_of(named1, key0 + int(kBlock)));
+        const bool held = named0 < c.pages;
+        named0 = named1;
+        named1 = named2;
+        named2 = page_of(key0 + 3 * int(kBlock));
+
+        const bool edge = !held || key0 < lo_last || key0 + int(kBlock) > hi_first;
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = key0 + 16 * (i / 8) + 8 * int(g) + i % 8;
+                if (!held || key < lo || key >= hi) p[i] = -INFINITY;
+            }
+        }
+        float most = p[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) most = fmaxf(most, p[i]);
+        most *= rs;
+        if (__ballot(most > m + kLag) != 0) {
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const float up = fmaxf(m, most);
+            const float f = up > m ? exp2f(m - up) : 1.f;
+            m = up;
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < VT; ++d) o[d] *= f;
+        }
+        const float off = kTop - (m == -INFINITY ? 0.f : m);
+        next = scores(kl[b ^ 1]);
+        u4 pt[2][T];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = __builtin_amdgcn_exp2f(fmaf(p[8 * s + j], rs, off));
+                sum += x[j];
+            }
+            split8<BF16>(x, pt[s]);
+        }
+        const u4 *vb = vl[b];
+        auto value = [&](int s, int d) { return vb[(2 * s + g) * dim + min(32 * d + n, dim - 1)]; };
+        if (apart[b] != key0) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                for (int d = 0; d < VT; ++d) {
+                    const u4 v = value(s, d);
+#pragma unroll
+                    for (int i = 0; i < T; ++i) o[d] = mfma32<BF16>(v, pt[s][i], o[d]);
+                }
+            }
+        } else {
+            // As in the kernel above: the finite values, and NaN for the rows
+            // that see another.
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const u4 seen = ones_of<BF16>(key0 + 16 * s + 8 * int(g), lo, hi);
+#pragma unroll
+                for (int d = 0; d < VT; ++d) {
+                    u4 finite, bad;
+                    part_finite<BF16>(value(s, d), finite, bad);
+#pragma unroll
+                    for (int i = 0; i < T; ++i) o[d] = mfma32<BF16>(finite, pt[s][i], o[d]);
+                    const f16v count = mfma32<BF16>(bad, seen, f16v{});
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (count[i] > 0.f) o[d][i] = __builtin_nanf("");
+                }
+            }
+        }
+        stage(kl[b], kr);
+        stage_values(b ^ 1, key0 + int(kBlock), named0);
+    }
+
+    float all = sum + __shfl_xor(sum, 32);
+    const bool real = r < in_tile;
+    const uint32_t row = t.row0 + min(r, in_tile - 1), token = t.first_token + row / group, qh = head * group + row % group;
+    if (one_range) {
+        if (split == 0 && real) {
+            const float f = all == 0.f ? 0.f : 1.f / all;
+            float *y = a.out + size_t(token) * a.out_stride + size_t(qh) * dim;
+#pragma unroll
+            for (int d = 0; d < VT; ++d) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t at = 32 * d + 8 * i + 4 * g;
+                    if (at >= dim) continue;
+                    const f4 x = {o[d][4 * i] * f, o[d][4 * i + 1] * f, o[d][4 * i + 2] * f, o[d][4 * i + 3] * f};
+                    if (aligned) {
+                        *reinterpret_cast<f4 *>(y + at) = x;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) y[at + j] = x[j];
+                    }
+                }
+            }
+        }
+    } else if (real) {
+        const size_t part = (size_t(unit) * pl.splits + split) * R + r;
+        if (all != 0.f) {
+#pragma unroll
+            for (int d = 0; d < VT; ++d) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f4 *>(ws.o + part * DM + 32 * d + 8 * i + 4 * g) =
+                        f4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+            }
+        }
+        if (g == 0) ws.ml[part] = make_float2(m, all);
+    }
+    if (pl.splits > 1 && split == 0 && g == 0) ws.place[size_t(unit) * R + r] = one_range || !real ? kNone : token * a.heads + qh;
 }
 
 // Adds the ranges of a row up: a workgroup a row, every wave a quarter of the
@@ -548,7 +870,13 @@ hipError_t launch_rows(const AttendArgs &a, const AttendPlan &pl, const Partial 
 
 template <bool BF16, int DM>
 hipError_t launch_dim(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, bool aligned, hipStream_t stream) {
-    hipError_t e = launch_rows<BF16, DM, 1>(a, pl, ws, aligned, stream);
+    hipError_t e;
+    if (pl.rows == 16) {
+        e = launch_rows<BF16, DM, 1>(a, pl, ws, aligned, stream);
+    } else {
+        attn_tile_kernel<BF16, DM><<<pl.tiles * a.cache.kv_heads * pl.splits, kThreads, 0, stream>>>(a, pl, ws, aligned);
+        e = hipGetLastError();
+    }
     if (e != hipSuccess || pl.splits == 1) return e;
     attn_join_kernel<DM><<<pl.tiles * a.cache.kv_heads * pl.rows, kThreads, 0, stream>>>(a, pl, ws);
     return hipGetLastError();
@@ -569,9 +897,10 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
     const PagedCache &c = a.cache;
     const uint64_t group = a.heads / c.kv_heads;
     AttendPlan pl;
-    pl.rows = 16;
     // Sequences with a row: at most n. Each takes whole tiles.
     const uint64_t n = c.seqs < c.tokens ? c.seqs : c.tokens;
+    const uint64_t each = c.tokens * group / n;  // rows of a sequence, on average
+    pl.rows = each <= 32 ? 16 : 128;
     const uint64_t by_rows = n + (c.tokens * group - n) / pl.rows;
     const uint64_t by_token = c.tokens * ((group + pl.rows - 1) / pl.rows);
     pl.tiles = uint32_t(by_rows < by_token ? by_rows : by_token);
@@ -596,7 +925,7 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
     return pl;
 }
 
-const char *attend_kernel_name(const AttendPlan &) { return "attn_rows_kernel"; }
+const char *attend_kernel_name(const AttendPlan &pl) { return pl.rows == 16 ? "attn_rows_kernel" : "attn_tile_kernel"; }
 
 hipError_t launch_attn_paged(const AttendArgs &a, const AttendPlan &pl, void *workspace, hipStream_t stream) {
     const auto aligned16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
