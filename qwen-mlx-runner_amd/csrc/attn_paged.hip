@@ -21,6 +21,8 @@
 // be as the B operand of O^T = V^T P^T. Scores never leave their lane.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "attn_common.hpp"
 #include "kernels.hpp"
 
@@ -34,11 +36,13 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef f4 f4u __attribute__((aligned(4)));  // rows of FP32 need no more
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kMaxSplits = 512;  // key ranges of a tile, at most
+constexpr uint32_t kRsrcWord3 = 0x00020000u;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
 // Terms of an FP32 operand in the cache's type.
@@ -67,6 +71,18 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) {  // 
     return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
 }
 
+// x - the low (0) or high (1) f16 of h, in one instruction.
+template <int HIGH>
+__device__ __forceinline__ float less_half(float x, uint32_t h) {
+    float r;
+    if constexpr (HIGH) {
+        asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    } else {
+        asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    }
+    return r;
+}
+
 // Eight FP32 values as kTerms vectors of eight halves that add up to them:
 // truncated terms, each exact in what the ones before leave (the last f16 one
 // rounds at 2^-22).
@@ -86,9 +102,26 @@ __device__ __forceinline__ void split8(const float (&x)[8], u4 (&t)[kTerms<BF16>
         } else {
             const auto hi = __builtin_amdgcn_cvt_pkrtz(a, b);
             t[0][i] = __builtin_bit_cast(uint32_t, hi);
-            t[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - float(hi[0]), b - float(hi[1])));
+            t[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(less_half<0>(a, t[0][i]), less_half<1>(b, t[0][i])));
         }
     }
+}
+
+// A block of keys or values as a buffer of its own bytes: loads past it give
+// zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const uint16_t *pool, size_t at, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(pool + at), 0, int(bytes), kRsrcWord3);
+}
+
+__device__ __forceinline__ u4 load16(__amdgpu_buffer_rsrc_t r, uint32_t offset, uint32_t more) {
+    return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, int(offset), int(more), 0));
+}
+
+// The order of a stretch of code: groups of instructions of a kind.
+constexpr int kMatrix = 0x8, kVector = 0x2, kLdsRead = 0x100;
+template <int KIND, int COUNT>
+__device__ __forceinline__ void next_are() {
+    __builtin_amdgcn_sched_group_barrier(KIND, COUNT, 0);
 }
 
 // What a workgroup works on: a tile of query rows of one sequence and key
@@ -118,18 +151,18 @@ __device__ __forceinline__ bool find_tile(const PagedCache &c, uint32_t group, u
             const uint32_t o = __shfl_up(sum, d);
             if (l >= uint32_t(d)) sum += o;
         }
-        const uint32_t total = __shfl(sum, 63);
+        const uint32_t total = __builtin_amdgcn_readlane(sum, 63);
         if (tile >= total) {
             tile -= total;
             continue;
         }
         const int at = __ffsll(__ballot(sum > tile)) - 1;
-        t.seq = __builtin_amdgcn_readfirstlane(base + at);
-        t.first_token = __builtin_amdgcn_readfirstlane(__shfl(from, at));
-        t.rows = __builtin_amdgcn_readfirstlane(__shfl(count, at)) * group;
-        t.row0 = __builtin_amdgcn_readfirstlane((tile - __shfl(sum - own, at)) * R);
-        t.length = int(min(uint32_t(__builtin_amdgcn_readfirstlane(__shfl(length, at))), 0x7FFFFFFFu));
-        t.context = t.length - int(__builtin_amdgcn_readfirstlane(__shfl(end, at)) - t.first_token);
+        t.seq = base + at;
+        t.first_token = __builtin_amdgcn_readlane(from, at);
+        t.rows = __builtin_amdgcn_readlane(count, at) * group;
+        t.row0 = (tile - __builtin_amdgcn_readlane(sum - own, at)) * R;
+        t.length = int(min(uint32_t(__builtin_amdgcn_readlane(length, at)), 0x7FFFFFFFu));
+        t.context = t.length - int(__builtin_amdgcn_readlane(end, at) - t.first_token);
         return true;
     }
     return false;
@@ -143,6 +176,27 @@ __device__ __forceinline__ void visible(const AttendArgs &a, const Tile &t, uint
     lo = a.window ? max(pos - int(a.window) + 1, 0) : 0;
 }
 
+// The order of a range's blocks: those that some row sees in part first (the
+// ones before and after what every row sees), then the others, so that the
+// loop over these has no masks.
+struct Order {
+    int first, lead, whole, after, edges, count;
+    __device__ __forceinline__ Order(int from, int to, int lo_most, int hi_least) {
+        const int b = int(kBlock), end = (to + b - 1) / b;
+        first = from / b;
+        whole = min(max((lo_most + b - 1) / b, first), end);
+        after = min(max(hi_least / b, whole), end);
+        lead = whole - first;
+        edges = lead + end - after;
+        count = end - first;
+    }
+    // First key of the i-th block; of the last one past them.
+    __device__ __forceinline__ int key(int i) const {
+        i = min(i, count - 1);
+        return (i < lead ? first + i : i < edges ? after + i - lead : whole + i - edges) * int(kBlock);
+    }
+};
+
 // Results of key ranges, to be joined: for each (tile, head, range) R rows of
 // DM floats, and their m and l; for each (tile, head) its rows' places in the
 // output (kNone: nothing to join).
@@ -152,25 +206,31 @@ struct Partial {
     uint32_t *place;
 };
 
+typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+typedef int16_t is2 __attribute__((ext_vector_type(2)));
+
+// The exponent of the type's infinity and NaNs, and its 1.0, in both halves.
 template <bool BF16>
-__device__ __forceinline__ bool not_finite(u4 v) {
-    constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (v[i] & e) == e || (v[i] & (e << 16)) == e << 16;
-    return bad;
+constexpr uint32_t kInf = BF16 ? 0x7F807F80u : 0x7C007C00u;
+template <bool BF16>
+constexpr uint32_t kOne = BF16 ? 0x3F803F80u : 0x3C003C00u;
+
+// The halves' sizes, the larger of each.
+__device__ __forceinline__ us2 larger(us2 a, uint32_t v) {
+    return __builtin_elementwise_max(a, __builtin_bit_cast(us2, v & 0x7FFF7FFFu));
 }
 
-// Of each half: itself where finite, else zero; and 1.0 where it is not finite.
 template <bool BF16>
-__device__ __forceinline__ void part_finite(u4 v, u4 &finite, u4 &bad) {
-    constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u, one = BF16 ? 0x3F80u : 0x3C00u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t m = ((v[i] & e) == e ? 0xFFFFu : 0u) | ((v[i] & (e << 16)) == e << 16 ? 0xFFFF0000u : 0u);
-        finite[i] = v[i] & ~m;
-        bad[i] = (one | one << 16) & m;
-    }
+__device__ __forceinline__ bool has_not_finite(us2 largest) {
+    constexpr uint16_t inf = kInf<BF16> & 0xFFFF;
+    return largest[0] >= inf || largest[1] >= inf;
+}
+
+// Ones in the halves that are not finite.
+template <bool BF16>
+__device__ __forceinline__ uint32_t not_finite(uint32_t v) {
+    const us2 over = __builtin_bit_cast(us2, v & 0x7FFF7FFFu) + __builtin_bit_cast(us2, 0x80008000u - kInf<BF16>);
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(is2, over) >> 15);
 }
 
 // Ones in the halves of the keys first..first+7 that lie in [lo, hi).
@@ -187,20 +247,16 @@ __device__ __forceinline__ u4 halves_of(int first, int lo, int hi) {
 // 1.0 in those halves.
 template <bool BF16>
 __device__ __forceinline__ u4 ones_of(int first, int lo, int hi) {
-    constexpr uint32_t one = BF16 ? 0x3F803F80u : 0x3C003C00u;
-    u4 m = halves_of(first, lo, hi);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m[i] &= one;
-    return m;
+    return halves_of(first, lo, hi) & kOne<BF16>;
 }
 
 // Few rows: R = 16 NB rows a workgroup, every wave all of them over its own
 // blocks of the range (block w, w + 4, ..), straight from memory into operand
-// registers: a block is 64 KB/DM-independent whole lines, and nothing is
-// shared but the queries, which wait in LDS as operands. The waves' m, l and O
+// registers, whole lines at a time; nothing is shared but the queries, which
+// wait in LDS as operands. The waves' m, l and O
 // are joined through LDS at the end.
-template <bool BF16, int DM, int NB, bool FULL>
-__global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(AttendArgs a, AttendPlan pl, Partial ws, bool aligned) {
+template <bool BF16, int DM, int NB>
+__global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
     constexpr int R = 16 * NB, T = kTerms<BF16>, KS = DM / 32, VT = DM / 16;
     // f16 weights are up to 2^15, so that small ones stay normal; the maximum
     // lags by at most 2^kLag.
@@ -213,7 +269,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
     const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = l % 16, g = l / 16;
     const uint32_t split = blockIdx.x % pl.splits, unit = blockIdx.x / pl.splits;  // unit: tile and key head
-    const uint32_t head = unit % c.kv_heads, group = a.heads / c.kv_heads, dim = FULL ? DM : c.dim;
+    const uint32_t head = unit % c.kv_heads, group = a.heads / c.kv_heads, dim = c.dim;
     Tile t;
     if (!find_tile(c, group, R, unit / c.kv_heads, t)) {
         if (pl.splits > 1 && split == 0 && threadIdx.x < R) ws.place[size_t(unit) * R + threadIdx.x] = kNone;
@@ -243,58 +299,55 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
             const uint32_t ch = qp + 16 * k;
+            const f4 none = {0.f, 0.f, 0.f, 0.f};
             const bool in = r < in_tile && ch * 8 < dim;
-            if (in && aligned) {
-                *reinterpret_cast<float4 *>(x[nb][k]) = *reinterpret_cast<const float4 *>(q + ch * 8);
-                *reinterpret_cast<float4 *>(x[nb][k] + 4) = *reinterpret_cast<const float4 *>(q + ch * 8 + 4);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[nb][k][j] = in ? q[ch * 8 + j] : 0.f;
-            }
+            const float *at = q + (ch * 8 < dim ? ch * 8 : 0);
+            const f4 x0 = *reinterpret_cast<const f4u *>(at), x1 = *reinterpret_cast<const f4u *>(at + 4);
+            *reinterpret_cast<f4 *>(x[nb][k]) = in ? x0 : none;
+            *reinterpret_cast<f4 *>(x[nb][k] + 4) = in ? x1 : none;
         }
     }
 
-    // Blocks w, w + 4, .. of the range. A block's keys are loaded while the
+    // Blocks w, w + 4, .. of the order. A block's keys are loaded while the
     // block before is weighed, its values while its scores are worked out, the
     // first ones while the queries are; the page after next is named by then.
     // Pages are read as constants (scalar loads), whose wait does not wait for
-    // the blocks in flight.
+    // the blocks in flight. A page past the pool, or a block past the last,
+    // reads as zeros: no memory is touched.
+    const Order order(from, to, lo_last, hi_first);
     const auto *table = (const __attribute__((address_space(4))) uint32_t *)(c.table + size_t(t.seq) * c.columns);
-    const uint32_t last_column = c.columns - 1, page_shift = __builtin_ctz(c.page);
-    auto page_of = [&](int key0) { return table[min(uint32_t(key0) >> page_shift, last_column)]; };
-    auto block_of = [&](uint32_t named, int key0) {
-        return attn::block_at(c, named < c.pages ? named : 0, head, (uint32_t(key0) & (c.page - 1)) / kBlock);
+    const uint32_t page_shift = __builtin_ctz(c.page);
+    auto page_of = [&](int key0) { return table[uint32_t(key0) >> page_shift]; };
+    auto rsrc_of = [&](const uint16_t *pool, uint32_t named, int key0, bool real) {
+        const bool held = real && named < c.pages;
+        const size_t at = attn::block_at(c, held ? named : 0, head, (uint32_t(key0) & (c.page - 1)) / kBlock);
+        return block_rsrc(pool, at, held ? dim * kBlock * 2 : 0);
     };
     u4 k[KS][2];
-    auto load_keys = [&](size_t at) {
-        const u4 *kp = reinterpret_cast<const u4 *>(c.k + at);
+    auto load_keys = [&](uint32_t named, int key0, bool real) {
+        const auto r = rsrc_of(c.k, named, key0, real);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (FULL || (4 * s + g) * 8 < dim)
-                    k[s][i] = kp[(4 * s + g) * 32 + 16 * i + n];
-                else
-                    k[s][i] = u4{0, 0, 0, 0};
-            }
+            for (int i = 0; i < 2; ++i) k[s][i] = load16(r, (g * 32 + n) * 16, s * 2048 + i * 256);
         }
     };
+    // Dims past the head's own take other values or zeros, and are not kept.
     u4 v[VT];
-    auto load_values = [&](size_t at) {
-        const u4 *vp = reinterpret_cast<const u4 *>(c.v + at);
+    auto load_values = [&](uint32_t named, int key0, bool real) {
+        const auto r = rsrc_of(c.v, named, key0, real);
 #pragma unroll
-        for (int d = 0; d < VT; ++d) v[d] = vp[g * dim + (FULL ? 16 * d + n : min(16 * d + n, dim - 1))];
+        for (int d = 0; d < VT; ++d) v[d] = load16(r, (g * dim + n) * 16, d * 256);
     };
-    const int step = kWaves * int(kBlock);
-    int key0 = from + int(w) * int(kBlock);
+    int at = int(w), key0 = 0, next_key = 0;
     uint32_t named = 0, next = 0;
-    size_t at = 0;
-    if (key0 < to) {
+    if (at < order.count) {
+        key0 = order.key(at);
+        next_key = order.key(at + kWaves);
         named = page_of(key0);
-        next = page_of(key0 + step);
-        at = block_of(named, key0);
-        load_keys(at);
-        load_values(at);
+        next = page_of(next_key);
+        load_keys(named, key0, true);
+        load_values(named, key0, true);
     }
 
     // The queries, as operands.
@@ -345,19 +398,20 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
         m[nb] = -INFINITY;
         sum[nb] = 0.f;
     }
+    // Of a lane's outputs, those that saw a value that is not finite.
+    uint32_t poison[(NB * VT + 7) / 8] = {};
     f4 o[NB][VT];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int d = 0; d < VT; ++d) o[nb][d] = f4{0.f, 0.f, 0.f, 0.f};
 
-    for (; key0 < to; key0 += step) {
+    auto block = [&](auto edge) {
         const bool held = named < c.pages;
-        const bool edge = !held || key0 < lo_last || key0 + int(kBlock) > hi_first;
         // The queries' operands come from LDS for every block where they and
         // the block do not fit the registers together.
         uint32_t ql = l;
-        if constexpr (DM == 256 || NB > 1 || !FULL) asm volatile("" : "+v"(ql));
+        if constexpr (DM == 256) asm volatile("" : "+v"(ql));
         f4 scores[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -372,39 +426,69 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
                 }
             }
         }
-        named = next;
-        if (key0 + step < to) {
-            at = block_of(named, key0 + step);
-            load_keys(at);
-        }
-        next = page_of(key0 + 2 * step);
-        bool apart = false;  // a value that some rows see and others do not is not finite
-        if (edge) {
+        const bool more = at + kWaves < order.count;
+        load_keys(next, next_key, more);
+        const int key_now = key0;
+        if constexpr (edge()) {
             // Values that no row sees may be anything: zero them.
-            const u4 kept = halves_of(key0 + 8 * int(g), held ? lo_first : hi_last, hi_last);
+            const u4 kept = halves_of(key_now + 8 * int(g), lo_first, hi_last);
 #pragma unroll
-            for (int d = 0; d < VT; ++d) {
-                v[d] &= kept;
-                apart |= not_finite<BF16>(v[d]);
+            for (int d = 0; d < VT; ++d) v[d] &= kept;
+            if (lo_first != lo_last || hi_first != hi_last) {
+                // One that is not finite and that only some rows see must not
+                // even meet the others' zero weights: it is taken out, and the
+                // rows that see it (by a product of its place and what they
+                // see) become NaN.
+                us2 largest = {0, 0};
+#pragma unroll
+                for (int d = 0; d < VT; ++d) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) largest = larger(largest, v[d][i]);
+                }
+                if (__ballot(has_not_finite<BF16>(largest)) != 0) {
+#pragma unroll
+                    for (int d = 0; d < VT; ++d) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[d][i] &= ~not_finite<BF16>(v[d][i]);
+                    }
+                    const auto again = rsrc_of(c.v, named, key_now, true);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const u4 seen = ones_of<BF16>(key_now + 8 * int(g), lo[nb], hi[nb]);
+#pragma unroll
+                        for (int d8 = 0; d8 < VT; d8 += 8) {
+#pragma unroll 1
+                            for (int d = 0; d < 8 && d8 + d < VT; ++d) {
+                                u4 bad = load16(again, (g * dim + n) * 16, (d8 + d) * 256) & kept;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) bad[i] = not_finite<BF16>(bad[i]) & kOne<BF16>;
+                                const f4 count = mfma16<BF16>(bad, seen, f4{0.f, 0.f, 0.f, 0.f});
+                                uint32_t bits = 0;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) bits |= count[i] > 0.f ? 1u << i : 0u;
+                                poison[(nb * VT + d8) / 8] |= bits << (4 * ((nb * VT) % 8 + d));
+                            }
+                        }
+                    }
+                }
             }
-            apart = __ballot(apart) != 0;
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             float p[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) p[i] = scores[nb][0][i], p[4 + i] = scores[nb][1][i];
-            if (edge) {
+            if constexpr (edge()) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int key = key0 + 8 * int(g) + e;
-                    if (!held || key < lo[nb] || key >= hi[nb]) p[e] = -INFINITY;
+                    const int key = key_now + 8 * int(g) + e;
+                    if (key < lo[nb] || key >= hi[nb]) p[e] = -INFINITY;
                 }
             }
             float most = p[0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) most = fmaxf(most, p[e]);
-            most *= rs[nb];
+            most = held ? most * rs[nb] : -INFINITY;
             if (__ballot(most > m[nb] + kLag) != 0) {
                 most = fmaxf(most, __shfl_xor(most, 16));
                 most = fmaxf(most, __shfl_xor(most, 32));
@@ -415,7 +499,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
 #pragma unroll
                 for (int d = 0; d < VT; ++d) o[nb][d] *= f;
             }
-            const float off = kTop - (m[nb] == -INFINITY ? 0.f : m[nb]);
+            const float off = held ? kTop - (m[nb] == -INFINITY ? 0.f : m[nb]) : -INFINITY;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], rs[nb], off));
@@ -423,32 +507,21 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
             }
             u4 pt[T];
             split8<BF16>(p, pt);
-            if (!apart) {
 #pragma unroll
-                for (int d = 0; d < VT; ++d) {
+            for (int d = 0; d < VT; ++d) {
 #pragma unroll
-                    for (int i = 0; i < T; ++i) o[nb][d] = mfma16<BF16>(v[d], pt[i], o[nb][d]);
-                }
-            } else {
-                // A value that is not finite must not even meet a zero weight:
-                // the finite ones are added up, and the rows that see another
-                // (a count of them) become NaN.
-                const u4 seen = ones_of<BF16>(key0 + 8 * int(g), lo[nb], hi[nb]);
-#pragma unroll
-                for (int d = 0; d < VT; ++d) {
-                    u4 finite, bad;
-                    part_finite<BF16>(v[d], finite, bad);
-#pragma unroll
-                    for (int i = 0; i < T; ++i) o[nb][d] = mfma16<BF16>(finite, pt[i], o[nb][d]);
-                    const f4 count = mfma16<BF16>(bad, seen, f4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (count[i] > 0.f) o[nb][d][i] = __builtin_nanf("");
-                }
+                for (int i = 0; i < T; ++i) o[nb][d] = mfma16<BF16>(v[d], pt[i], o[nb][d]);
             }
         }
-        if (key0 + step < to) load_values(at);
-    }
+        load_values(next, next_key, more);
+        at += kWaves;
+        key0 = next_key;
+        named = next;
+        next_key = order.key(at + kWaves);
+        next = page_of(next_key);
+    };
+    while (at < order.edges) block(std::true_type{});
+    while (at < order.count) block(std::false_type{});
 
     // Join the waves, 16 rows at a time.
     float *os = reinterpret_cast<float *>(lds);  // [kWaves][16][kPitch]
@@ -458,6 +531,12 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
         all += __shfl_xor(all, 16);
         all += __shfl_xor(all, 32);
         __syncthreads();
+#pragma unroll
+        for (int d = 0; d < VT; ++d) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (poison[(nb * VT + d) / 8] >> ((nb * VT + d) % 8 * 4 + i) & 1) o[nb][d][i] = __builtin_nanf("");
+        }
 #pragma unroll
         for (int d = 0; d < VT; ++d) *reinterpret_cast<f4 *>(os + (w * 16 + n) * kPitch + 16 * d + 4 * g) = o[nb][d];
         if (g == 0) {
@@ -487,13 +566,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
                     const float f = joined == 0.f ? 0.f : 1.f / joined;
                     float *y = a.out + size_t(t.first_token + row / group) * a.out_stride +
                                size_t(head * group + row % group) * dim + d;
-                    acc *= f;
-                    if (aligned) {
-                        *reinterpret_cast<f4 *>(y) = acc;
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) y[k] = acc[k];
-                    }
+                    *reinterpret_cast<f4u *>(y) = acc * f;
                 }
             } else if (real) {
                 if (joined != 0.f) *reinterpret_cast<f4 *>(ws.o + (part + rn) * DM + d) = acc;
@@ -516,8 +589,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
 // to registers an iteration before they go to LDS, two deep, one barrier a
 // block.
 template <bool BF16, int DM>
-__global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(AttendArgs a, AttendPlan pl, Partial ws,
-                                                                               bool aligned) {
+__global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
     constexpr int R = 32 * kWaves, T = kTerms<BF16>, KS = DM / 16, VT = DM / 32;
     constexpr float kTop = BF16 ? 0.f : 7.f, kLag = 8.f;
     constexpr int kChunks = DM * 4;             // 16-byte chunks of a block
@@ -549,59 +621,55 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 
     // This wave's rows.
     const uint32_t r0 = 32 * w, r = r0 + n;
-    int lo, hi, hi_first, lo_last, skip;
+    int lo, hi;
     visible(a, t, (t.row0 + min(r, in_tile - 1)) / group, lo, hi);
-    visible(a, t, (t.row0 + min(r0, in_tile - 1)) / group, skip, hi_first);
-    visible(a, t, (t.row0 + min(r0 + 31, in_tile - 1)) / group, lo_last, skip);
     if (threadIdx.x < 2) apart[threadIdx.x] = -1;
     __syncthreads();
 
+    const Order order(from, to, lo_most, hi_least);
     const auto *table = (const __attribute__((address_space(4))) uint32_t *)(c.table + size_t(t.seq) * c.columns);
-    const uint32_t last_column = c.columns - 1, page_shift = __builtin_ctz(c.page);
-    auto page_of = [&](int key0) { return table[min(uint32_t(key0) >> page_shift, last_column)]; };
-    auto block_of = [&](uint32_t named, int key0) {
-        return attn::block_at(c, named < c.pages ? named : 0, head, (uint32_t(key0) & (c.page - 1)) / kBlock);
+    const uint32_t page_shift = __builtin_ctz(c.page);
+    auto page_of = [&](int key0) { return table[uint32_t(key0) >> page_shift]; };
+    auto rsrc_of = [&](const uint16_t *pool, uint32_t named, int key0) {
+        const bool held = named < c.pages;
+        const size_t at = attn::block_at(c, held ? named : 0, head, (uint32_t(key0) & (c.page - 1)) / kBlock);
+        return block_rsrc(pool, at, held ? dim * kBlock * 2 : 0);
     };
     u4 kr[kEach], vr[kEach];
-    auto load = [&](u4 (&to_regs)[kEach], const uint16_t *pool, size_t at) {
-        const u4 *p = reinterpret_cast<const u4 *>(pool + at);
+    auto load = [&](u4 (&to_regs)[kEach], __amdgpu_buffer_rsrc_t r) {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const uint32_t ch = threadIdx.x + i * kThreads;
-            if (ch < dim * 4) to_regs[i] = p[ch];
-        }
+        for (int i = 0; i < kEach; ++i) to_regs[i] = load16(r, threadIdx.x * 16, i * kThreads * 16);
     };
     auto stage = [&](u4 *lds, const u4 (&regs)[kEach]) {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) lds[threadIdx.x + i * kThreads] = regs[i];
     };
-    // Values that no row of the tile sees may be anything: zeros. Of a block
-    // that some rows see in part, `apart` says whether a value is not finite.
-    auto stage_values = [&](uint32_t to_buffer, int key0, uint32_t named) {
-        const bool held = named < c.pages;
-        if (!held || key0 < lo_most || key0 + int(kBlock) > hi_least) {
-            bool bad = false;
+    // Values that no row of the tile sees may be anything: zeros. Those that are
+    // not finite in a block that some rows see in part stay out of LDS too, and
+    // `apart` says that there are some.
+    auto clean_values = [&](uint32_t to_buffer, int key0) {
+        uint32_t some_bad = 0;
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int first = key0 + 8 * int((threadIdx.x + i * kThreads) / dim);
-                vr[i] &= halves_of(first, held ? lo_tile : hi_tile, hi_tile);
-                bad |= not_finite<BF16>(vr[i]);
+        for (int i = 0; i < kEach; ++i) {
+            vr[i] &= halves_of(key0 + 8 * int((threadIdx.x + i * kThreads) / dim), lo_tile, hi_tile);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t bad = not_finite<BF16>(vr[i][j]);
+                vr[i][j] &= ~bad;
+                some_bad |= bad;
             }
-            if (bad) apart[to_buffer] = key0;
         }
-        stage(vl[to_buffer], vr);
+        if (some_bad) apart[to_buffer] = key0;
     };
-    // Chunks past the head's own stay zero.
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) kr[i] = vr[i] = u4{0, 0, 0, 0};
 
+    // Blocks, by their place in the order: now, and the three after.
+    int key0 = 0, key1 = 0, key2 = 0;
     uint32_t named0 = 0, named1 = 0, named2 = 0;
-    if (from < to) {
-        named0 = page_of(from);
-        named1 = page_of(from + int(kBlock));
-        named2 = page_of(from + 2 * int(kBlock));
-        load(kr, c.k, block_of(named0, from));
-        load(vr, c.v, block_of(named0, from));
+    if (order.count > 0) {
+        key0 = order.key(0), key1 = order.key(1), key2 = order.key(2);
+        named0 = page_of(key0), named1 = page_of(key1), named2 = page_of(key2);
+        load(kr, rsrc_of(c.k, named0, key0));
+        load(vr, rsrc_of(c.v, named0, key0));
     }
 
     // Queries.
@@ -612,15 +680,11 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         const float *src = a.q + size_t(t.first_token + row / group) * a.q_stride + size_t(head * group + row % group) * dim;
         auto read = [&](int s, float (&x)[8]) {
             const uint32_t d = 16 * s + 8 * g;
-            if (d < dim && aligned) {
-                *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(src + d);
-                *reinterpret_cast<float4 *>(x + 4) = *reinterpret_cast<const float4 *>(src + d + 4);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = d < dim ? src[d + j] : 0.f;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] *= a.scale * kLog2e;
+            const f4 none = {0.f, 0.f, 0.f, 0.f};
+            const float *at = src + (d < dim ? d : 0);
+            const f4 x0 = *reinterpret_cast<const f4u *>(at), x1 = *reinterpret_cast<const f4u *>(at + 4);
+            *reinterpret_cast<f4 *>(x) = d < dim ? x0 * (a.scale * kLog2e) : none;
+            *reinterpret_cast<f4 *>(x + 4) = d < dim ? x1 * (a.scale * kLog2e) : none;
         };
         int e = 0;
         if constexpr (!BF16) {
@@ -651,6 +715,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 #pragma unroll
     for (int d = 0; d < VT; ++d) o[d] = f16v{};
     float m = -INFINITY, sum = 0.f;
+    uint32_t poison[(VT + 1) / 2] = {};  // of a lane's outputs, those that saw a value that is not finite
 
     const uint32_t key_at = g * 32 + (n & 7) + 2 * (n & 8) + (n & 16) / 2;  // where A's row n is in a key chunk pair
     auto scores = [&](const u4 *kb) {
@@ -665,37 +730,36 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     };
 
     f16v next = {};
-    if (from < to) {
+    if (order.count > 0) {
         stage(kl[0], kr);
-        stage_values(0, from, named0);
-        load(kr, c.k, block_of(named1, from + int(kBlock)));
+        if (order.edges > 0) clean_values(0, key0);
+        stage(vl[0], vr);
+        load(kr, rsrc_of(c.k, named1, key1));
         __syncthreads();
         next = scores(kl[0]);
         stage(kl[1], kr);
     }
     uint32_t b = 0;
-    for (int key0 = from; key0 < to; key0 += int(kBlock), b ^= 1) {
+    int at = 0;
+    auto block = [&](auto edge) {
         f16v p = next;
         __syncthreads();
-        load(kr, c.k, block_of(named2, key0 + 2 * int(kBlock)));
-        load(vr, c.v, block_of(named1, key0 + int(kBlock)));
+        load(kr, rsrc_of(c.k, named2, key2));
+        load(vr, rsrc_of(c.v, named1, key1));
+        const int key3 = order.key(at + 3);
+        const uint32_t named3 = page_of(key3);
         const bool held = named0 < c.pages;
-        named0 = named1;
-        named1 = named2;
-        named2 = page_of(key0 + 3 * int(kBlock));
-
-        const bool edge = !held || key0 < lo_last || key0 + int(kBlock) > hi_first;
-        if (edge) {
+        if constexpr (edge()) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int key = key0 + 16 * (i / 8) + 8 * int(g) + i % 8;
-                if (!held || key < lo || key >= hi) p[i] = -INFINITY;
+                if (key < lo || key >= hi) p[i] = -INFINITY;
             }
         }
         float most = p[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) most = fmaxf(most, p[i]);
-        most *= rs;
+        most = held ? most * rs : -INFINITY;
         if (__ballot(most > m + kLag) != 0) {
             most = fmaxf(most, __shfl_xor(most, 32));
             const float up = fmaxf(m, most);
@@ -705,7 +769,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 #pragma unroll
             for (int d = 0; d < VT; ++d) o[d] *= f;
         }
-        const float off = kTop - (m == -INFINITY ? 0.f : m);
+        const float off = held ? kTop - (m == -INFINITY ? 0.f : m) : -INFINITY;
         next = scores(kl[b ^ 1]);
         u4 pt[2][T];
 #pragma unroll
@@ -719,40 +783,72 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
             split8<BF16>(x, pt[s]);
         }
         const u4 *vb = vl[b];
-        auto value = [&](int s, int d) { return vb[(2 * s + g) * dim + min(32 * d + n, dim - 1)]; };
-        if (apart[b] != key0) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < 2; ++s) {
 #pragma unroll
-                for (int d = 0; d < VT; ++d) {
-                    const u4 v = value(s, d);
+            for (int d = 0; d < VT; ++d) {
+                const u4 v = vb[(2 * s + g) * dim + 32 * d + n];
 #pragma unroll
-                    for (int i = 0; i < T; ++i) o[d] = mfma32<BF16>(v, pt[s][i], o[d]);
-                }
+                for (int i = 0; i < T; ++i) o[d] = mfma32<BF16>(v, pt[s][i], o[d]);
             }
-        } else {
-            // As in the kernel above: the finite values, and NaN for the rows
-            // that see another.
+        }
+        // Matrix instructions with the vector ones between them, two LDS reads
+        // ahead of their use.
+        next_are<kLdsRead, 2>();
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const u4 seen = ones_of<BF16>(key0 + 16 * s + 8 * int(g), lo, hi);
+        for (int i = 0; i < KS; ++i) {
+            next_are<kMatrix, T>();
+            next_are<kVector, (BF16 ? 180 : 110) / KS>();
+            next_are<kLdsRead, 1>();
+        }
 #pragma unroll
-                for (int d = 0; d < VT; ++d) {
-                    u4 finite, bad;
-                    part_finite<BF16>(value(s, d), finite, bad);
+        for (int i = 0; i < 2 * VT; ++i) {
+            next_are<kMatrix, T>();
+            next_are<kLdsRead, 1>();
+        }
+        if constexpr (edge()) {
+            if (apart[b] == key0) {
+                // The rows that see one of the values left out become NaN.
+                const auto again = rsrc_of(c.v, named0, key0);
 #pragma unroll
-                    for (int i = 0; i < T; ++i) o[d] = mfma32<BF16>(finite, pt[s][i], o[d]);
-                    const f16v count = mfma32<BF16>(bad, seen, f16v{});
+                for (int d2 = 0; d2 < VT; d2 += 2) {
+#pragma unroll 1
+                    for (int d = 0; d < 2; ++d) {
+                        f16v count = {};
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (count[i] > 0.f) o[d][i] = __builtin_nanf("");
+                        for (int s = 0; s < 2; ++s) {
+                            u4 bad = load16(again, ((2 * s + g) * dim + n) * 16, (d2 + d) * 512);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) bad[i] = not_finite<BF16>(bad[i]) & kOne<BF16>;
+                            count = mfma32<BF16>(bad, ones_of<BF16>(key0 + 16 * s + 8 * int(g), lo, hi), count);
+                        }
+                        uint32_t bits = 0;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) bits |= count[i] > 0.f ? 1u << i : 0u;
+                        poison[d2 / 2] |= bits << (16 * d);
+                    }
                 }
             }
         }
         stage(kl[b], kr);
-        stage_values(b ^ 1, key0 + int(kBlock), named0);
-    }
+        if constexpr (edge()) {
+            if (at + 1 < order.edges) clean_values(b ^ 1, key1);
+        }
+        stage(vl[b ^ 1], vr);
+        key0 = key1, key1 = key2, key2 = key3;
+        named0 = named1, named1 = named2, named2 = named3;
+        b ^= 1;
+        ++at;
+    };
+    while (at < order.edges) block(std::true_type{});
+    while (at < order.count) block(std::false_type{});
 
+#pragma unroll
+    for (int d = 0; d < VT; ++d) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (poison[d / 2] >> (d % 2 * 16 + i) & 1) o[d][i] = __builtin_nanf("");
+    }
     float all = sum + __shfl_xor(sum, 32);
     const bool real = r < in_tile;
     const uint32_t row = t.row0 + min(r, in_tile - 1), token = t.first_token + row / group, qh = head * group + row % group;
@@ -766,13 +862,8 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t at = 32 * d + 8 * i + 4 * g;
                     if (at >= dim) continue;
-                    const f4 x = {o[d][4 * i] * f, o[d][4 * i + 1] * f, o[d][4 * i + 2] * f, o[d][4 * i + 3] * f};
-                    if (aligned) {
-                        *reinterpret_cast<f4 *>(y + at) = x;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) y[at + j] = x[j];
-                    }
+                    const f4 x = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                    *reinterpret_cast<f4u *>(y + at) = x * f;
                 }
             }
         }
@@ -855,26 +946,26 @@ size_t workspace_of(const AttendArgs &a, const AttendPlan &pl) {
 }
 
 template <bool BF16, int DM, int NB>
-hipError_t launch_rows(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, bool aligned, hipStream_t stream) {
+hipError_t launch_rows(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, hipStream_t stream) {
     const size_t queries = size_t(NB) * (DM / 32) * kTerms<BF16> * 1024;
     const size_t joined = size_t(kWaves) * 16 * (DM + 4) * 4;
     const size_t lds = queries > joined ? queries : joined;
-    const auto kernel = a.cache.dim == DM ? attn_rows_kernel<BF16, DM, NB, true> : attn_rows_kernel<BF16, DM, NB, false>;
+    const auto kernel = attn_rows_kernel<BF16, DM, NB>;
     if (lds > 65536 - 2048) {
         const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
         if (e != hipSuccess) return e;
     }
-    kernel<<<pl.tiles * a.cache.kv_heads * pl.splits, kThreads, lds, stream>>>(a, pl, ws, aligned);
+    kernel<<<pl.tiles * a.cache.kv_heads * pl.splits, kThreads, lds, stream>>>(a, pl, ws);
     return hipGetLastError();
 }
 
 template <bool BF16, int DM>
-hipError_t launch_dim(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, bool aligned, hipStream_t stream) {
+hipError_t launch_dim(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, hipStream_t stream) {
     hipError_t e;
     if (pl.rows == 16) {
-        e = launch_rows<BF16, DM, 1>(a, pl, ws, aligned, stream);
+        e = launch_rows<BF16, DM, 1>(a, pl, ws, stream);
     } else {
-        attn_tile_kernel<BF16, DM><<<pl.tiles * a.cache.kv_heads * pl.splits, kThreads, 0, stream>>>(a, pl, ws, aligned);
+        attn_tile_kernel<BF16, DM><<<pl.tiles * a.cache.kv_heads * pl.splits, kThreads, 0, stream>>>(a, pl, ws);
         e = hipGetLastError();
     }
     if (e != hipSuccess || pl.splits == 1) return e;
@@ -883,11 +974,11 @@ hipError_t launch_dim(const AttendArgs &a, const AttendPlan &pl, const Partial &
 }
 
 template <bool BF16>
-hipError_t launch_type(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, bool aligned, hipStream_t stream) {
+hipError_t launch_type(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, hipStream_t stream) {
     switch (wide_dim(a.cache.dim)) {
-        case 64: return launch_dim<BF16, 64>(a, pl, ws, aligned, stream);
-        case 128: return launch_dim<BF16, 128>(a, pl, ws, aligned, stream);
-        default: return launch_dim<BF16, 256>(a, pl, ws, aligned, stream);
+        case 64: return launch_dim<BF16, 64>(a, pl, ws, stream);
+        case 128: return launch_dim<BF16, 128>(a, pl, ws, stream);
+        default: return launch_dim<BF16, 256>(a, pl, ws, stream);
     }
 }
 
@@ -928,10 +1019,8 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
 const char *attend_kernel_name(const AttendPlan &pl) { return pl.rows == 16 ? "attn_rows_kernel" : "attn_tile_kernel"; }
 
 hipError_t launch_attn_paged(const AttendArgs &a, const AttendPlan &pl, void *workspace, hipStream_t stream) {
-    const auto aligned16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    const bool aligned = a.q_stride % 4 == 0 && a.out_stride % 4 == 0 && aligned16(a.q) && aligned16(a.out);
     const Partial ws = pl.splits > 1 ? parts(a, pl, workspace) : Partial{};
-    return a.cache.bf16 ? launch_type<true>(a, pl, ws, aligned, stream) : launch_type<false>(a, pl, ws, aligned, stream);
+    return a.cache.bf16 ? launch_type<true>(a, pl, ws, stream) : launch_type<false>(a, pl, ws, stream);
 }
 
 }  // namespace qmr
