@@ -594,7 +594,12 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     constexpr float kTop = BF16 ? 0.f : 7.f, kLag = 8.f;
     constexpr int kChunks = DM * 4;             // 16-byte chunks of a block
     constexpr int kEach = kChunks / kThreads;   // a thread's
-    __shared__ u4 kl[2][kChunks], vl[2][kChunks];
+    // Of a query's terms two stay in registers; the third of bf16 would not fit
+    // beside O and waits in LDS.
+    extern __shared__ __align__(16) unsigned char lds[];
+    u4(*kl)[kChunks] = reinterpret_cast<u4(*)[kChunks]>(lds);
+    u4(*vl)[kChunks] = kl + 2;
+    u4 *ql = reinterpret_cast<u4 *>(kl + 4) + (threadIdx.x / 64) * (KS * 64);
     __shared__ int apart[2];
     const PagedCache &c = a.cache;
     const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -673,7 +678,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     }
 
     // Queries.
-    u4 q[KS][T];
+    u4 q[KS][2];
     float rs = 1.f;
     {
         const uint32_t row = t.row0 + min(r, in_tile - 1);
@@ -708,7 +713,11 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = ldexpf(x[j], -e);
             }
-            split8<BF16>(x, q[s]);
+            u4 terms[T];
+            split8<BF16>(x, terms);
+            q[s][0] = terms[0];
+            q[s][1] = terms[1];
+            if constexpr (T == 3) ql[s * 64 + l] = terms[2];
         }
     }
     f16v o[VT];
@@ -723,8 +732,9 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const u4 k = kb[s * 64 + key_at];
-#pragma unroll
-            for (int i = 0; i < T; ++i) s0 = mfma32<BF16>(k, q[s][i], s0);
+            s0 = mfma32<BF16>(k, q[s][0], s0);
+            s0 = mfma32<BF16>(k, q[s][1], s0);
+            if constexpr (T == 3) s0 = mfma32<BF16>(k, ql[s * 64 + l], s0);
         }
         return s0;
     };
@@ -794,12 +804,12 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         }
         // Matrix instructions with the vector ones between them, two LDS reads
         // ahead of their use.
-        next_are<kLdsRead, 2>();
+        next_are<kLdsRead, 2 * (T - 1)>();
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             next_are<kMatrix, T>();
             next_are<kVector, (BF16 ? 180 : 110) / KS>();
-            next_are<kLdsRead, 1>();
+            next_are<kLdsRead, T - 1>();
         }
 #pragma unroll
         for (int i = 0; i < 2 * VT; ++i) {
@@ -965,7 +975,14 @@ hipError_t launch_dim(const AttendArgs &a, const AttendPlan &pl, const Partial &
     if (pl.rows == 16) {
         e = launch_rows<BF16, DM, 1>(a, pl, ws, stream);
     } else {
-        attn_tile_kernel<BF16, DM><<<pl.tiles * a.cache.kv_heads * pl.splits, kThreads, 0, stream>>>(a, pl, ws);
+        // Two blocks of keys and of values, and bf16's third query terms.
+        constexpr size_t lds = 4 * DM * 64 + (BF16 ? kWaves * DM * 64 : 0);
+        const auto kernel = attn_tile_kernel<BF16, DM>;
+        if (lds > 65536 - 2048) {
+            e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
+            if (e != hipSuccess) return e;
+        }
+        kernel<<<pl.tiles * a.cache.kv_heads * pl.splits, kThreads, lds, stream>>>(a, pl, ws);
         e = hipGetLastError();
     }
     if (e != hipSuccess || pl.splits == 1) return e;
