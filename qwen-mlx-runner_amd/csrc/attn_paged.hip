@@ -117,6 +117,38 @@ __device__ __forceinline__ u4 load16(__amdgpu_buffer_rsrc_t r, uint32_t offset, 
     return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, int(offset), int(more), 0));
 }
 
+// The same as four words in scalar registers, for dma16.
+__device__ __forceinline__ u4 block_words(const uint16_t *pool, size_t at, uint32_t bytes) {
+    const uint64_t p = reinterpret_cast<uint64_t>(pool + at);
+    return u4{uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(p))),
+              uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(p >> 32) & 0xFFFFu)),
+              uint32_t(__builtin_amdgcn_readfirstlane(bytes)), kRsrcWord3};
+}
+
+// A wave's 64 chunks of 16 bytes from memory straight to LDS, chunk after chunk
+// from byte `to`. The compiler does not see that they are on their way:
+// wait_dma is the wait. The idle cycles are those a load has to keep from a
+// vector instruction that wrote its scalar operands, and from m0's own write.
+__device__ __forceinline__ void dma16(u4 rsrc, uint32_t offset, uint32_t more, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(more))
+                 : "memory");
+}
+
+// Until at most LATER of this wave's loads are on their way.
+template <int LATER>
+__device__ __forceinline__ void wait_dma() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LATER) : "memory");
+}
+
+// A barrier that orders LDS alone: loads stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // The order of a stretch of code: groups of instructions of a kind.
 constexpr int kMatrix = 0x8, kVector = 0x2, kLdsRead = 0x100;
 template <int KIND, int COUNT>
@@ -584,23 +616,24 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
 // dealt so that lane (n, g) ends with row n's scores of keys 16s + 8g + 0..7, as
 // P^T has to stand for step s of O^T = V^T P^T.
 //
-// The scores of block b + 1 are worked out while block b's are weighed: matrix
-// and vector instructions that do not wait for each other. Blocks are loaded
-// to registers an iteration before they go to LDS, two deep, one barrier a
-// block.
+// The scores of block i + 1 are worked out while block i's are weighed: matrix
+// and vector instructions that do not wait for each other. Blocks go from
+// memory straight to a ring of three in LDS, two iterations ahead of their
+// use, with one barrier a block.
 template <bool BF16, int DM>
 __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
     constexpr int R = 32 * kWaves, T = kTerms<BF16>, KS = DM / 16, VT = DM / 32;
     constexpr float kTop = BF16 ? 0.f : 7.f, kLag = 8.f;
     constexpr int kChunks = DM * 4;             // 16-byte chunks of a block
     constexpr int kEach = kChunks / kThreads;   // a thread's
+    constexpr uint32_t kBytes = kChunks * 16;
     // Of a query's terms two stay in registers; the third of bf16 would not fit
-    // beside O and waits in LDS.
-    extern __shared__ __align__(16) unsigned char lds[];
-    u4(*kl)[kChunks] = reinterpret_cast<u4(*)[kChunks]>(lds);
-    u4(*vl)[kChunks] = kl + 2;
-    u4 *ql = reinterpret_cast<u4 *>(kl + 4) + (threadIdx.x / 64) * (KS * 64);
-    __shared__ int apart[2];
+    // beside O and waits in LDS, but for the last steps of the largest heads,
+    // for which LDS is too small.
+    constexpr int kLow = T < 3 ? 0 : DM == 256 ? KS - 2 : KS;
+    extern __shared__ __align__(16) unsigned char lds[];  // three blocks of keys, three of values, kLow steps a wave
+    u4 *ql = reinterpret_cast<u4 *>(lds + 6 * kBytes) + (threadIdx.x / 64) * (kLow * 64);
+    __shared__ int apart;
     const PagedCache &c = a.cache;
     const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = l % 32, g = l / 32;
@@ -628,57 +661,63 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     const uint32_t r0 = 32 * w, r = r0 + n;
     int lo, hi;
     visible(a, t, (t.row0 + min(r, in_tile - 1)) / group, lo, hi);
-    if (threadIdx.x < 2) apart[threadIdx.x] = -1;
-    __syncthreads();
+    if (threadIdx.x == 0) apart = -1;
 
     const Order order(from, to, lo_most, hi_least);
     const auto *table = (const __attribute__((address_space(4))) uint32_t *)(c.table + size_t(t.seq) * c.columns);
     const uint32_t page_shift = __builtin_ctz(c.page);
     auto page_of = [&](int key0) { return table[uint32_t(key0) >> page_shift]; };
-    auto rsrc_of = [&](const uint16_t *pool, uint32_t named, int key0) {
+    const uint32_t lds0 = uint32_t(uintptr_t((__attribute__((address_space(3))) unsigned char *)lds));
+    // Block `key0` of page `named` to the ring's slot at byte `to`. Nothing is
+    // written for a page past the pool, whose scores count as hidden.
+    auto fetch = [&](const uint16_t *pool, uint32_t named, int key0, uint32_t to) {
         const bool held = named < c.pages;
         const size_t at = attn::block_at(c, held ? named : 0, head, (uint32_t(key0) & (c.page - 1)) / kBlock);
-        return block_rsrc(pool, at, held ? dim * kBlock * 2 : 0);
-    };
-    u4 kr[kEach], vr[kEach];
-    auto load = [&](u4 (&to_regs)[kEach], __amdgpu_buffer_rsrc_t r) {
+        const u4 rsrc = block_words(pool, at, held ? dim * kBlock * 2 : 0);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) to_regs[i] = load16(r, threadIdx.x * 16, i * kThreads * 16);
-    };
-    auto stage = [&](u4 *lds, const u4 (&regs)[kEach]) {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) lds[threadIdx.x + i * kThreads] = regs[i];
+        for (int i = 0; i < kEach; ++i) dma16(rsrc, l * 16, (i * kWaves + w) * 1024, lds0 + to + (i * kWaves + w) * 1024);
     };
     // Values that no row of the tile sees may be anything: zeros. Those that are
-    // not finite in a block that some rows see in part stay out of LDS too, and
+    // not finite in a block that some rows see in part are zeros too, and
     // `apart` says that there are some.
-    auto clean_values = [&](uint32_t to_buffer, int key0) {
+    auto clean_values = [&](uint32_t at, int key0) {
+        u4 *vb = reinterpret_cast<u4 *>(lds + at);
         uint32_t some_bad = 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            vr[i] &= halves_of(key0 + 8 * int((threadIdx.x + i * kThreads) / dim), lo_tile, hi_tile);
+            const uint32_t ch = threadIdx.x + i * kThreads;
+            u4 v = vb[ch] & halves_of(key0 + 8 * int(ch / dim), lo_tile, hi_tile);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t bad = not_finite<BF16>(vr[i][j]);
-                vr[i][j] &= ~bad;
+                const uint32_t bad = not_finite<BF16>(v[j]);
+                v[j] &= ~bad;
                 some_bad |= bad;
             }
+            vb[ch] = v;
         }
-        if (some_bad) apart[to_buffer] = key0;
+        if (some_bad) apart = key0;
     };
 
-    // Blocks, by their place in the order: now, and the three after.
-    int key0 = 0, key1 = 0, key2 = 0;
-    uint32_t named0 = 0, named1 = 0, named2 = 0;
+    // Blocks, by their place in the order: this one and the three after; the
+    // ring's slots of keys and of values in the order of their use.
+    int key0 = 0, key1 = 0, key2 = 0, key3 = 0;
+    uint32_t named0 = 0, named1 = 0, named2 = 0, named3 = 0;
+    uint32_t k0 = 0, k1 = kBytes, k2 = 2 * kBytes, v0 = 3 * kBytes, v1 = 4 * kBytes, v2 = 5 * kBytes;
+    // What no load writes (dims past the head's, pages past the pool) is zero.
+    for (uint32_t i = threadIdx.x; i < 6 * kChunks; i += kThreads) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
+    lds_barrier();
     if (order.count > 0) {
-        key0 = order.key(0), key1 = order.key(1), key2 = order.key(2);
-        named0 = page_of(key0), named1 = page_of(key1), named2 = page_of(key2);
-        load(kr, rsrc_of(c.k, named0, key0));
-        load(vr, rsrc_of(c.v, named0, key0));
+        key0 = order.key(0), key1 = order.key(1), key2 = order.key(2), key3 = order.key(3);
+        named0 = page_of(key0), named1 = page_of(key1), named2 = page_of(key2), named3 = page_of(key3);
+        fetch(c.k, named0, key0, k0);
+        fetch(c.k, named1, key1, k1);
+        fetch(c.v, named0, key0, v0);
+        fetch(c.k, named2, key2, k2);
+        fetch(c.v, named1, key1, v1);
     }
 
     // Queries.
-    u4 q[KS][2];
+    u4 q[KS][2], q_last[2];
     float rs = 1.f;
     {
         const uint32_t row = t.row0 + min(r, in_tile - 1);
@@ -717,7 +756,8 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
             split8<BF16>(x, terms);
             q[s][0] = terms[0];
             q[s][1] = terms[1];
-            if constexpr (T == 3) ql[s * 64 + l] = terms[2];
+            if (s < kLow) ql[s * 64 + l] = terms[T - 1];
+            if (T == 3 && s >= kLow) q_last[T == 3 ? s - kLow : 0] = terms[T - 1];
         }
     }
     f16v o[VT];
@@ -727,38 +767,37 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     uint32_t poison[(VT + 1) / 2] = {};  // of a lane's outputs, those that saw a value that is not finite
 
     const uint32_t key_at = g * 32 + (n & 7) + 2 * (n & 8) + (n & 16) / 2;  // where A's row n is in a key chunk pair
-    auto scores = [&](const u4 *kb) {
+    auto scores = [&](uint32_t at) {
+        const u4 *kb = reinterpret_cast<const u4 *>(lds + at);
         f16v s0 = {};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const u4 k = kb[s * 64 + key_at];
             s0 = mfma32<BF16>(k, q[s][0], s0);
             s0 = mfma32<BF16>(k, q[s][1], s0);
-            if constexpr (T == 3) s0 = mfma32<BF16>(k, ql[s * 64 + l], s0);
+            if constexpr (T == 3) s0 = mfma32<BF16>(k, s < kLow ? ql[s * 64 + l] : q_last[s < kLow ? 0 : s - kLow], s0);
         }
         return s0;
     };
 
     f16v next = {};
     if (order.count > 0) {
-        stage(kl[0], kr);
-        if (order.edges > 0) clean_values(0, key0);
-        stage(vl[0], vr);
-        load(kr, rsrc_of(c.k, named1, key1));
-        __syncthreads();
-        next = scores(kl[0]);
-        stage(kl[1], kr);
+        wait_dma<4 * kEach>();
+        lds_barrier();
+        next = scores(k0);
     }
-    uint32_t b = 0;
     int at = 0;
     auto block = [&](auto edge) {
         f16v p = next;
-        __syncthreads();
-        load(kr, rsrc_of(c.k, named2, key2));
-        load(vr, rsrc_of(c.v, named1, key1));
-        const int key3 = order.key(at + 3);
-        const uint32_t named3 = page_of(key3);
+        wait_dma<2 * kEach>();  // the next keys and these values are there
+        lds_barrier();
+        fetch(c.k, named3, key3, k0);
+        fetch(c.v, named2, key2, v2);
+        const int key4 = order.key(at + 4);
+        const uint32_t named4 = page_of(key4);
         const bool held = named0 < c.pages;
+        if (!held) p = f16v{} - INFINITY;
+        if constexpr (edge()) clean_values(v0, key0);
         if constexpr (edge()) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -769,7 +808,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         float most = p[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) most = fmaxf(most, p[i]);
-        most = held ? most * rs : -INFINITY;
+        most *= rs;
         if (__ballot(most > m + kLag) != 0) {
             most = fmaxf(most, __shfl_xor(most, 32));
             const float up = fmaxf(m, most);
@@ -779,8 +818,9 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 #pragma unroll
             for (int d = 0; d < VT; ++d) o[d] *= f;
         }
-        const float off = held ? kTop - (m == -INFINITY ? 0.f : m) : -INFINITY;
-        next = scores(kl[b ^ 1]);
+        const float off = kTop - (m == -INFINITY ? 0.f : m);
+        if constexpr (edge()) lds_barrier();
+        next = scores(k1);
         u4 pt[2][T];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -792,7 +832,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
             }
             split8<BF16>(x, pt[s]);
         }
-        const u4 *vb = vl[b];
+        const u4 *vb = reinterpret_cast<const u4 *>(lds + v0);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
 #pragma unroll
@@ -817,9 +857,10 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
             next_are<kLdsRead, 1>();
         }
         if constexpr (edge()) {
-            if (apart[b] == key0) {
+            if (apart == key0) {
                 // The rows that see one of the values left out become NaN.
-                const auto again = rsrc_of(c.v, named0, key0);
+                const auto again = block_rsrc(
+                    c.v, attn::block_at(c, named0, head, (uint32_t(key0) & (c.page - 1)) / kBlock), dim * kBlock * 2);
 #pragma unroll
                 for (int d2 = 0; d2 < VT; d2 += 2) {
 #pragma unroll 1
@@ -840,18 +881,16 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
                 }
             }
         }
-        stage(kl[b], kr);
-        if constexpr (edge()) {
-            if (at + 1 < order.edges) clean_values(b ^ 1, key1);
-        }
-        stage(vl[b ^ 1], vr);
-        key0 = key1, key1 = key2, key2 = key3;
-        named0 = named1, named1 = named2, named2 = named3;
-        b ^= 1;
+        key0 = key1, key1 = key2, key2 = key3, key3 = key4;
+        named0 = named1, named1 = named2, named2 = named3, named3 = named4;
+        const uint32_t used_k = k0, used_v = v0;
+        k0 = k1, k1 = k2, k2 = used_k;
+        v0 = v1, v1 = v2, v2 = used_v;
         ++at;
     };
     while (at < order.edges) block(std::true_type{});
     while (at < order.count) block(std::false_type{});
+    wait_dma<0>();  // LDS is given back
 
 #pragma unroll
     for (int d = 0; d < VT; ++d) {
@@ -975,8 +1014,8 @@ hipError_t launch_dim(const AttendArgs &a, const AttendPlan &pl, const Partial &
     if (pl.rows == 16) {
         e = launch_rows<BF16, DM, 1>(a, pl, ws, stream);
     } else {
-        // Two blocks of keys and of values, and bf16's third query terms.
-        constexpr size_t lds = 4 * DM * 64 + (BF16 ? kWaves * DM * 64 : 0);
+        // Three blocks of keys and of values, and bf16's third query terms.
+        constexpr size_t lds = 6 * DM * 64 + (BF16 ? kWaves * (DM == 256 ? DM - 32 : DM) * 64 : 0);
         const auto kernel = attn_tile_kernel<BF16, DM>;
         if (lds > 65536 - 2048) {
             e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
