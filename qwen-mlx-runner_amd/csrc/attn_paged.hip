@@ -617,9 +617,11 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
 // P^T has to stand for step s of O^T = V^T P^T.
 //
 // The scores of block i + 1 are worked out while block i's are weighed: matrix
-// and vector instructions that do not wait for each other. Blocks go from
-// memory straight to a ring of three in LDS, two iterations ahead of their
-// use, with one barrier a block.
+// and vector instructions that do not wait for each other, and that stand in
+// the order in which they should issue, a step's operands read from LDS kAhead
+// steps before (scheduling barriers keep it). Blocks go from memory straight to
+// a ring of three in LDS, two iterations ahead of their use, with one barrier
+// a block.
 template <bool BF16, int DM>
 __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
     constexpr int R = 32 * kWaves, T = kTerms<BF16>, KS = DM / 16, VT = DM / 32;
@@ -627,6 +629,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     constexpr int kChunks = DM * 4;             // 16-byte chunks of a block
     constexpr int kEach = kChunks / kThreads;   // a thread's
     constexpr uint32_t kBytes = kChunks * 16;
+    constexpr int kAhead = 4;
     // Of a query's terms two stay in registers; the third of bf16 would not fit
     // beside O and waits in LDS, but for the last steps of the largest heads,
     // for which LDS is too small.
@@ -664,9 +667,19 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     if (threadIdx.x == 0) apart = -1;
 
     const Order order(from, to, lo_most, hi_least);
-    const auto *table = (const __attribute__((address_space(4))) uint32_t *)(c.table + size_t(t.seq) * c.columns);
+    // A page's name: 64 of them wait in a register, so that no scalar load's
+    // wait falls among those for LDS.
+    const uint32_t *table = c.table + size_t(t.seq) * c.columns;
     const uint32_t page_shift = __builtin_ctz(c.page);
-    auto page_of = [&](int key0) { return table[uint32_t(key0) >> page_shift]; };
+    uint32_t names = 0, names_at = 0x80000000u;
+    auto page_of = [&](int key0) {
+        const uint32_t column = uint32_t(key0) >> page_shift;
+        if (column - names_at >= 64) {
+            names_at = column;
+            names = table[min(column + l, c.columns - 1)];
+        }
+        return uint32_t(__builtin_amdgcn_readlane(names, column - names_at));
+    };
     const uint32_t lds0 = uint32_t(uintptr_t((__attribute__((address_space(3))) unsigned char *)lds));
     // Block `key0` of page `named` to the ring's slot at byte `to`. Nothing is
     // written for a page past the pool, whose scores count as hidden.
@@ -767,32 +780,30 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     uint32_t poison[(VT + 1) / 2] = {};  // of a lane's outputs, those that saw a value that is not finite
 
     const uint32_t key_at = g * 32 + (n & 7) + 2 * (n & 8) + (n & 16) / 2;  // where A's row n is in a key chunk pair
-    auto scores = [&](uint32_t at) {
-        const u4 *kb = reinterpret_cast<const u4 *>(lds + at);
-        f16v s0 = {};
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const u4 k = kb[s * 64 + key_at];
-            s0 = mfma32<BF16>(k, q[s][0], s0);
-            s0 = mfma32<BF16>(k, q[s][1], s0);
-            if constexpr (T == 3) s0 = mfma32<BF16>(k, s < kLow ? ql[s * 64 + l] : q_last[s < kLow ? 0 : s - kLow], s0);
-        }
-        return s0;
+    auto key_operand = [&](uint32_t at, int s) { return reinterpret_cast<const u4 *>(lds + at)[s * 64 + key_at]; };
+    auto value_operand = [&](uint32_t at, int i) {
+        return reinterpret_cast<const u4 *>(lds + at)[(i / VT * 2 + g) * dim + 32 * (i % VT) + n];
+    };
+    auto low_operand = [&](int s) { return s < kLow ? ql[s * 64 + l] : q_last[s < kLow ? 0 : s - kLow]; };
+    auto score_step = [&](f16v x, int s, u4 k, u4 low) {
+        x = mfma32<BF16>(k, q[s][0], x);
+        x = mfma32<BF16>(k, q[s][1], x);
+        if constexpr (T == 3) x = mfma32<BF16>(k, low, x);
+        return x;
     };
 
     f16v next = {};
     if (order.count > 0) {
         wait_dma<4 * kEach>();
         lds_barrier();
-        next = scores(k0);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) next = score_step(next, s, key_operand(k0, s), low_operand(s));
     }
     int at = 0;
     auto block = [&](auto edge) {
         f16v p = next;
         wait_dma<2 * kEach>();  // the next keys and these values are there
         lds_barrier();
-        fetch(c.k, named3, key3, k0);
-        fetch(c.v, named2, key2, v2);
         const int key4 = order.key(at + 4);
         const uint32_t named4 = page_of(key4);
         const bool held = named0 < c.pages;
@@ -820,42 +831,47 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         }
         const float off = kTop - (m == -INFINITY ? 0.f : m);
         if constexpr (edge()) lds_barrier();
-        next = scores(k1);
+
+        // Steps 0..KS-1: the next block's scores, and this one's weights.
+        // Steps KS..: the weights times the values.
+        constexpr int STEPS = KS + 2 * VT;
+        u4 ring[kAhead], low[2];
+        auto operand = [&](int i) { return i < KS ? key_operand(k1, i) : value_operand(v0, i - KS); };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ring[i] = operand(i);
+        if constexpr (T == 3) low[0] = low_operand(0), low[1] = low_operand(1);
+        __builtin_amdgcn_sched_barrier(0);
+        f16v ahead = {};
         u4 pt[2][T];
+        float x[8];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            float x[8];
+        for (int i = 0; i < STEPS; ++i) {
+            const u4 a_operand = ring[i % kAhead];
+            if (i < KS) {
+                ahead = score_step(ahead, i, a_operand, low[i % 2]);
+                if constexpr (T == 3)
+                    if (i + 2 < KS) low[i % 2] = low_operand(i + 2);
+            } else {
+                const int s = (i - KS) / VT, d = (i - KS) % VT;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = __builtin_amdgcn_exp2f(fmaf(p[8 * s + j], rs, off));
-                sum += x[j];
+                for (int j = 0; j < T; ++j) o[d] = mfma32<BF16>(a_operand, pt[s][j], o[d]);
             }
-            split8<BF16>(x, pt[s]);
-        }
-        const u4 *vb = reinterpret_cast<const u4 *>(lds + v0);
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-#pragma unroll
-            for (int d = 0; d < VT; ++d) {
-                const u4 v = vb[(2 * s + g) * dim + 32 * d + n];
-#pragma unroll
-                for (int i = 0; i < T; ++i) o[d] = mfma32<BF16>(v, pt[s][i], o[d]);
+            if (i + kAhead < STEPS) ring[i % kAhead] = operand(i + kAhead);
+            if (i == 0) {
+                fetch(c.k, named3, key3, k0);
+                fetch(c.v, named2, key2, v2);
             }
-        }
-        // Matrix instructions with the vector ones between them, two LDS reads
-        // ahead of their use.
-        next_are<kLdsRead, 2 * (T - 1)>();
+            if (i < KS) {
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            next_are<kMatrix, T>();
-            next_are<kVector, (BF16 ? 180 : 110) / KS>();
-            next_are<kLdsRead, T - 1>();
+                for (int j = i * 16 / KS; j < (i + 1) * 16 / KS; ++j) {
+                    x[j % 8] = __builtin_amdgcn_exp2f(fmaf(p[j], rs, off));
+                    sum += x[j % 8];
+                    if (j % 8 == 7) split8<BF16>(x, pt[j / 8]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int i = 0; i < 2 * VT; ++i) {
-            next_are<kMatrix, T>();
-            next_are<kLdsRead, 1>();
-        }
+        next = ahead;
         if constexpr (edge()) {
             if (apart == key0) {
                 // The rows that see one of the values left out become NaN.
