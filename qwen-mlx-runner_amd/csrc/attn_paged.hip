@@ -149,13 +149,6 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// The order of a stretch of code: groups of instructions of a kind.
-constexpr int kMatrix = 0x8, kVector = 0x2, kLdsRead = 0x100;
-template <int KIND, int COUNT>
-__device__ __forceinline__ void next_are() {
-    __builtin_amdgcn_sched_group_barrier(KIND, COUNT, 0);
-}
-
 // What a workgroup works on: a tile of query rows of one sequence and key
 // head. Row r of the sequence is token r / group, head r % group.
 struct Tile {
@@ -677,16 +670,23 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         if (column - names_at >= 64) {
             names_at = column;
             names = table[min(column + l, c.columns - 1)];
+            asm volatile("s_waitcnt vmcnt(0)" : "+v"(names));  // here, not at each use
         }
         return uint32_t(__builtin_amdgcn_readlane(names, column - names_at));
     };
     const uint32_t lds0 = uint32_t(uintptr_t((__attribute__((address_space(3))) unsigned char *)lds));
-    // Block `key0` of page `named` to the ring's slot at byte `to`. Nothing is
-    // written for a page past the pool, whose scores count as hidden.
-    auto fetch = [&](const uint16_t *pool, uint32_t named, int key0, uint32_t to) {
-        const bool held = named < c.pages;
-        const size_t at = attn::block_at(c, held ? named : 0, head, (uint32_t(key0) & (c.page - 1)) / kBlock);
-        const u4 rsrc = block_words(pool, at, held ? dim * kBlock * 2 : 0);
+    // Where the i-th block of the order is in either pool, all ones for a block
+    // of a page past the pool.
+    constexpr uint64_t kNowhere = ~uint64_t(0);
+    auto place_of = [&](int i) {
+        const int key = order.key(i);
+        const uint32_t named = page_of(key);
+        return named < c.pages ? uint64_t(attn::block_at(c, named, head, (uint32_t(key) & (c.page - 1)) / kBlock)) : kNowhere;
+    };
+    // That block to the ring's slot at byte `to`; zeros from nowhere.
+    auto fetch = [&](const uint16_t *pool, uint64_t at, uint32_t to) {
+        const bool held = at != kNowhere;
+        const u4 rsrc = block_words(pool, held ? at : 0, held ? dim * kBlock * 2 : 0);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) dma16(rsrc, l * 16, (i * kWaves + w) * 1024, lds0 + to + (i * kWaves + w) * 1024);
     };
@@ -713,20 +713,18 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 
     // Blocks, by their place in the order: this one and the three after; the
     // ring's slots of keys and of values in the order of their use.
-    int key0 = 0, key1 = 0, key2 = 0, key3 = 0;
-    uint32_t named0 = 0, named1 = 0, named2 = 0, named3 = 0;
+    uint64_t at0 = kNowhere, at1 = kNowhere, at2 = kNowhere, at3 = kNowhere;
     uint32_t k0 = 0, k1 = kBytes, k2 = 2 * kBytes, v0 = 3 * kBytes, v1 = 4 * kBytes, v2 = 5 * kBytes;
-    // What no load writes (dims past the head's, pages past the pool) is zero.
+    // What no load writes (dims past the head's) is zero.
     for (uint32_t i = threadIdx.x; i < 6 * kChunks; i += kThreads) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
     lds_barrier();
     if (order.count > 0) {
-        key0 = order.key(0), key1 = order.key(1), key2 = order.key(2), key3 = order.key(3);
-        named0 = page_of(key0), named1 = page_of(key1), named2 = page_of(key2), named3 = page_of(key3);
-        fetch(c.k, named0, key0, k0);
-        fetch(c.k, named1, key1, k1);
-        fetch(c.v, named0, key0, v0);
-        fetch(c.k, named2, key2, k2);
-        fetch(c.v, named1, key1, v1);
+        at0 = place_of(0), at1 = place_of(1), at2 = place_of(2), at3 = place_of(3);
+        fetch(c.k, at0, k0);
+        fetch(c.k, at1, k1);
+        fetch(c.v, at0, v0);
+        fetch(c.k, at2, k2);
+        fetch(c.v, at1, v1);
     }
 
     // Queries.
@@ -792,34 +790,47 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         return x;
     };
 
+    auto largest = [](f16v x) {
+        float most = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) most = fmaxf(most, x[i]);
+        return most;
+    };
     f16v next = {};
+    float next_most = 0.f;
     if (order.count > 0) {
         wait_dma<4 * kEach>();
         lds_barrier();
 #pragma unroll
         for (int s = 0; s < KS; ++s) next = score_step(next, s, key_operand(k0, s), low_operand(s));
+        next_most = largest(next);
     }
+    // Of the largest heads, O has its place in the accumulation registers: left
+    // to itself the compiler moves it to the others and back for every block.
+    auto stays = [](f16v &x) {
+        if constexpr (DM == 256) asm volatile("" : "+a"(x));
+    };
     int at = 0;
     auto block = [&](auto edge) {
         f16v p = next;
+#pragma unroll
+        for (int d = 0; d < VT; ++d) stays(o[d]);
         wait_dma<2 * kEach>();  // the next keys and these values are there
         lds_barrier();
-        const int key4 = order.key(at + 4);
-        const uint32_t named4 = page_of(key4);
-        const bool held = named0 < c.pages;
-        if (!held) p = f16v{} - INFINITY;
-        if constexpr (edge()) clean_values(v0, key0);
+        const bool held = at0 != kNowhere;
+        float most = next_most;
+        int key0 = 0;
         if constexpr (edge()) {
+            key0 = order.key(at);
+            clean_values(v0, key0);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int key = key0 + 16 * (i / 8) + 8 * int(g) + i % 8;
                 if (key < lo || key >= hi) p[i] = -INFINITY;
             }
+            most = largest(p);
         }
-        float most = p[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) most = fmaxf(most, p[i]);
-        most *= rs;
+        most = held ? most * rs : -INFINITY;
         if (__ballot(most > m + kLag) != 0) {
             most = fmaxf(most, __shfl_xor(most, 32));
             const float up = fmaxf(m, most);
@@ -827,9 +838,12 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
             m = up;
             sum *= f;
 #pragma unroll
-            for (int d = 0; d < VT; ++d) o[d] *= f;
+            for (int d = 0; d < VT; ++d) {
+                o[d] *= f;
+                stays(o[d]);
+            }
         }
-        const float off = kTop - (m == -INFINITY ? 0.f : m);
+        const float off = held ? kTop - (m == -INFINITY ? 0.f : m) : -INFINITY;
         if constexpr (edge()) lds_barrier();
 
         // Steps 0..KS-1: the next block's scores, and this one's weights.
@@ -842,6 +856,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         if constexpr (T == 3) low[0] = low_operand(0), low[1] = low_operand(1);
         __builtin_amdgcn_sched_barrier(0);
         f16v ahead = {};
+        uint64_t at4 = kNowhere;
         u4 pt[2][T];
         float x[8];
 #pragma unroll
@@ -857,10 +872,9 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
                 for (int j = 0; j < T; ++j) o[d] = mfma32<BF16>(a_operand, pt[s][j], o[d]);
             }
             if (i + kAhead < STEPS) ring[i % kAhead] = operand(i + kAhead);
-            if (i == 0) {
-                fetch(c.k, named3, key3, k0);
-                fetch(c.v, named2, key2, v2);
-            }
+            if (i == 0) fetch(c.k, at3, k0);
+            if (i == 1) fetch(c.v, at2, v2);
+            if (i == 2) at4 = place_of(at + 4);
             if (i < KS) {
 #pragma unroll
                 for (int j = i * 16 / KS; j < (i + 1) * 16 / KS; ++j) {
@@ -869,14 +883,14 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
                     if (j % 8 == 7) split8<BF16>(x, pt[j / 8]);
                 }
             }
+            if (i == KS + 1) next_most = largest(ahead);
             __builtin_amdgcn_sched_barrier(0);
         }
         next = ahead;
         if constexpr (edge()) {
             if (apart == key0) {
                 // The rows that see one of the values left out become NaN.
-                const auto again = block_rsrc(
-                    c.v, attn::block_at(c, named0, head, (uint32_t(key0) & (c.page - 1)) / kBlock), dim * kBlock * 2);
+                const auto again = block_rsrc(c.v, at0, dim * kBlock * 2);
 #pragma unroll
                 for (int d2 = 0; d2 < VT; d2 += 2) {
 #pragma unroll 1
@@ -897,8 +911,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
                 }
             }
         }
-        key0 = key1, key1 = key2, key2 = key3, key3 = key4;
-        named0 = named1, named1 = named2, named2 = named3, named3 = named4;
+        at0 = at1, at1 = at2, at2 = at3, at3 = at4;
         const uint32_t used_k = k0, used_v = v0;
         k0 = k1, k1 = k2, k2 = used_k;
         v0 = v1, v1 = v2, v2 = used_v;
