@@ -783,12 +783,18 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         return reinterpret_cast<const u4 *>(lds + at)[(i / VT * 2 + g) * dim + 32 * (i % VT) + n];
     };
     auto low_operand = [&](int s) { return s < kLow ? ql[s * 64 + l] : q_last[s < kLow ? 0 : s - kLow]; };
-    auto score_step = [&](f16v x, int s, u4 k, u4 low) {
-        x = mfma32<BF16>(k, q[s][0], x);
-        x = mfma32<BF16>(k, q[s][1], x);
-        if constexpr (T == 3) x = mfma32<BF16>(k, low, x);
-        return x;
+    // A matrix instruction that adds to the one before it waits half as long
+    // again: two sums in turn where there are registers for it (of 128 dims
+    // there are not, but two waves on a SIMD).
+    constexpr int SUMS = DM == 128 ? 1 : 2;
+    auto score_step = [&](f16v (&x)[SUMS], int s, u4 k, u4 low) {
+#pragma unroll
+        for (int i = 0; i < T; ++i) {
+            f16v &sum = x[(s * T + i) % SUMS];
+            sum = mfma32<BF16>(k, i == 2 ? low : q[s][i == 2 ? 0 : i], sum);
+        }
     };
+    auto total = [](const f16v (&x)[SUMS]) { return SUMS == 2 ? x[0] + x[SUMS - 1] : x[0]; };
 
     auto largest = [](f16v x) {
         float most = x[0];
@@ -801,8 +807,10 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     if (order.count > 0) {
         wait_dma<4 * kEach>();
         lds_barrier();
+        f16v first[SUMS] = {};
 #pragma unroll
-        for (int s = 0; s < KS; ++s) next = score_step(next, s, key_operand(k0, s), low_operand(s));
+        for (int s = 0; s < KS; ++s) score_step(first, s, key_operand(k0, s), low_operand(s));
+        next = total(first);
         next_most = largest(next);
     }
     // Of the largest heads, O has its place in the accumulation registers: left
@@ -846,47 +854,52 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         const float off = held ? kTop - (m == -INFINITY ? 0.f : m) : -INFINITY;
         if constexpr (edge()) lds_barrier();
 
-        // Steps 0..KS-1: the next block's scores, and this one's weights.
-        // Steps KS..: the weights times the values.
-        constexpr int STEPS = KS + 2 * VT;
+        // The next block's scores, and this one's weights between them; then
+        // the weights times the values, two tiles of dims in turn.
         u4 ring[kAhead], low[2];
         auto operand = [&](int i) { return i < KS ? key_operand(k1, i) : value_operand(v0, i - KS); };
+        auto take = [&](int i) {
+            const u4 x = ring[i % kAhead];
+            if (i + kAhead < KS + 2 * VT) ring[i % kAhead] = operand(i + kAhead);
+            return x;
+        };
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) ring[i] = operand(i);
         if constexpr (T == 3) low[0] = low_operand(0), low[1] = low_operand(1);
         __builtin_amdgcn_sched_barrier(0);
-        f16v ahead = {};
+        f16v ahead[SUMS] = {};
         uint64_t at4 = kNowhere;
         u4 pt[2][T];
         float x[8];
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const u4 a_operand = ring[i % kAhead];
-            if (i < KS) {
-                ahead = score_step(ahead, i, a_operand, low[i % 2]);
-                if constexpr (T == 3)
-                    if (i + 2 < KS) low[i % 2] = low_operand(i + 2);
-            } else {
-                const int s = (i - KS) / VT, d = (i - KS) % VT;
-#pragma unroll
-                for (int j = 0; j < T; ++j) o[d] = mfma32<BF16>(a_operand, pt[s][j], o[d]);
-            }
-            if (i + kAhead < STEPS) ring[i % kAhead] = operand(i + kAhead);
+        for (int i = 0; i < KS; ++i) {
+            score_step(ahead, i, take(i), low[i % 2]);
+            if constexpr (T == 3)
+                if (i + 2 < KS) low[i % 2] = low_operand(i + 2);
             if (i == 0) fetch(c.k, at3, k0);
             if (i == 1) fetch(c.v, at2, v2);
             if (i == 2) at4 = place_of(at + 4);
-            if (i < KS) {
 #pragma unroll
-                for (int j = i * 16 / KS; j < (i + 1) * 16 / KS; ++j) {
-                    x[j % 8] = __builtin_amdgcn_exp2f(fmaf(p[j], rs, off));
-                    sum += x[j % 8];
-                    if (j % 8 == 7) split8<BF16>(x, pt[j / 8]);
-                }
+            for (int j = i * 16 / KS; j < (i + 1) * 16 / KS; ++j) {
+                x[j % 8] = __builtin_amdgcn_exp2f(fmaf(p[j], rs, off));
+                sum += x[j % 8];
+                if (j % 8 == 7) split8<BF16>(x, pt[j / 8]);
             }
-            if (i == KS + 1) next_most = largest(ahead);
             __builtin_amdgcn_sched_barrier(0);
         }
-        next = ahead;
+#pragma unroll
+        for (int i = 0; i < 2 * VT; i += 2) {
+            const int s = i / VT, d = i % VT;
+            const u4 va = take(KS + i), vb = take(KS + i + 1);
+#pragma unroll
+            for (int j = 0; j < T; ++j) {
+                o[d] = mfma32<BF16>(va, pt[s][j], o[d]);
+                o[d + 1] = mfma32<BF16>(vb, pt[s][j], o[d + 1]);
+            }
+            if (i == 0) next = total(ahead);
+            if (i == 2) next_most = largest(next);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if constexpr (edge()) {
             if (apart == key0) {
                 // The rows that see one of the values left out become NaN.
