@@ -117,16 +117,8 @@ __device__ __forceinline__ u4 load16(__amdgpu_buffer_rsrc_t r, uint32_t offset, 
     return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, int(offset), int(more), 0));
 }
 
-// The same as four words in scalar registers, for dma16.
-__device__ __forceinline__ u4 block_words(const uint16_t *pool, size_t at, uint32_t bytes) {
-    const uint64_t p = reinterpret_cast<uint64_t>(pool + at);
-    return u4{uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(p))),
-              uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(p >> 32) & 0xFFFFu)),
-              uint32_t(__builtin_amdgcn_readfirstlane(bytes)), kRsrcWord3};
-}
-
 // A wave's 64 chunks of 16 bytes from memory straight to LDS, chunk after chunk
-// from byte `to`. The compiler does not see that they are on their way:
+// from byte `to`; `rsrc`: a buffer's four words. The compiler does not see that they are on their way:
 // wait_dma is the wait. The idle cycles are those a load has to keep from a
 // vector instruction that wrote its scalar operands, and from m0's own write.
 __device__ __forceinline__ void dma16(u4 rsrc, uint32_t offset, uint32_t more, uint32_t to) {
@@ -675,20 +667,26 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         return uint32_t(__builtin_amdgcn_readlane(names, column - names_at));
     };
     const uint32_t lds0 = uint32_t(uintptr_t((__attribute__((address_space(3))) unsigned char *)lds));
-    // Where the i-th block of the order is in either pool, all ones for a block
-    // of a page past the pool.
-    constexpr uint64_t kNowhere = ~uint64_t(0);
+    // The number of the order's i-th block in either pool, kNone for one of a
+    // page past the pool.
+    const uint32_t block_bytes = dim * kBlock * 2, page_blocks = c.page / kBlock;
     auto place_of = [&](int i) {
         const int key = order.key(i);
-        const uint32_t named = page_of(key);
-        return named < c.pages ? uint64_t(attn::block_at(c, named, head, (uint32_t(key) & (c.page - 1)) / kBlock)) : kNowhere;
+        const uint32_t named = page_of(key), in_page = (uint32_t(key) & (c.page - 1)) / kBlock;
+        return named < c.pages ? (named * c.kv_heads + head) * page_blocks + in_page : kNone;
+    };
+    auto words_of = [&](const uint16_t *pool, uint32_t at) {
+        const bool held = at != kNone;
+        const uint64_t p = reinterpret_cast<uint64_t>(pool) + uint64_t(held ? at : 0) * block_bytes;
+        return u4{uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(p))),
+                  uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(p >> 32) & 0xFFFFu)), held ? block_bytes : 0, kRsrcWord3};
     };
     // That block to the ring's slot at byte `to`; zeros from nowhere.
-    auto fetch = [&](const uint16_t *pool, uint64_t at, uint32_t to) {
-        const bool held = at != kNowhere;
-        const u4 rsrc = block_words(pool, held ? at : 0, held ? dim * kBlock * 2 : 0);
+    const uint32_t own_bytes = l * 16 + w * 1024, lds_own = lds0 + w * 1024;
+    auto fetch = [&](const uint16_t *pool, uint32_t at, uint32_t to) {
+        const u4 words = words_of(pool, at);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) dma16(rsrc, l * 16, (i * kWaves + w) * 1024, lds0 + to + (i * kWaves + w) * 1024);
+        for (int i = 0; i < kEach; ++i) dma16(words, own_bytes, i * kWaves * 1024, lds_own + to + i * kWaves * 1024);
     };
     // Values that no row of the tile sees may be anything: zeros. Those that are
     // not finite in a block that some rows see in part are zeros too, and
@@ -713,10 +711,11 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 
     // Blocks, by their place in the order: this one and the three after; the
     // ring's slots of keys and of values in the order of their use.
-    uint64_t at0 = kNowhere, at1 = kNowhere, at2 = kNowhere, at3 = kNowhere;
+    uint32_t at0 = kNone, at1 = kNone, at2 = kNone, at3 = kNone;
     uint32_t k0 = 0, k1 = kBytes, k2 = 2 * kBytes, v0 = 3 * kBytes, v1 = 4 * kBytes, v2 = 5 * kBytes;
     // What no load writes (dims past the head's) is zero.
-    for (uint32_t i = threadIdx.x; i < 6 * kChunks; i += kThreads) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
+    if (dim < DM)
+        for (uint32_t i = threadIdx.x; i < 6 * kChunks; i += kThreads) reinterpret_cast<u4 *>(lds)[i] = u4{0, 0, 0, 0};
     lds_barrier();
     if (order.count > 0) {
         at0 = place_of(0), at1 = place_of(1), at2 = place_of(2), at3 = place_of(3);
@@ -733,38 +732,36 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     {
         const uint32_t row = t.row0 + min(r, in_tile - 1);
         const float *src = a.q + size_t(t.first_token + row / group) * a.q_stride + size_t(head * group + row % group) * dim;
-        auto read = [&](int s, float (&x)[8]) {
-            const uint32_t d = 16 * s + 8 * g;
-            const f4 none = {0.f, 0.f, 0.f, 0.f};
-            const float *at = src + (d < dim ? d : 0);
-            const f4 x0 = *reinterpret_cast<const f4u *>(at), x1 = *reinterpret_cast<const f4u *>(at + 4);
-            *reinterpret_cast<f4 *>(x) = d < dim ? x0 * (a.scale * kLog2e) : none;
-            *reinterpret_cast<f4 *>(x + 4) = d < dim ? x1 * (a.scale * kLog2e) : none;
-        };
+        f4 x[KS][2];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[s][i] = *reinterpret_cast<const f4u *>(src + min(16 * s + 8 * g, dim - 8) + 4 * i);
+        }
+        float most = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const float f = 16 * s + 8 * g < dim ? a.scale * kLog2e : 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                x[s][i] = f == 0.f ? f4{0.f, 0.f, 0.f, 0.f} : x[s][i] * f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[s][i][j]));
+            }
+        }
         int e = 0;
         if constexpr (!BF16) {
-            float most = 0.f;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                float x[8];
-                read(s, x);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
-            }
             most = fmaxf(most, __shfl_xor(most, 32));
             if (most > 0.f && most < INFINITY) frexpf(most, &e), e -= 15;
             rs = ldexpf(1.f, e);
         }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            float x[8];
-            read(s, x);
-            if constexpr (!BF16) {
+            float y[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = ldexpf(x[j], -e);
-            }
+            for (int j = 0; j < 8; ++j) y[j] = BF16 ? x[s][j / 4][j % 4] : ldexpf(x[s][j / 4][j % 4], -e);
             u4 terms[T];
-            split8<BF16>(x, terms);
+            split8<BF16>(y, terms);
             q[s][0] = terms[0];
             q[s][1] = terms[1];
             if (s < kLow) ql[s * 64 + l] = terms[T - 1];
@@ -825,7 +822,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         for (int d = 0; d < VT; ++d) stays(o[d]);
         wait_dma<2 * kEach>();  // the next keys and these values are there
         lds_barrier();
-        const bool held = at0 != kNowhere;
+        const bool held = at0 != kNone;
         float most = next_most;
         int key0 = 0;
         if constexpr (edge()) {
@@ -868,23 +865,24 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         if constexpr (T == 3) low[0] = low_operand(0), low[1] = low_operand(1);
         __builtin_amdgcn_sched_barrier(0);
         f16v ahead[SUMS] = {};
-        uint64_t at4 = kNowhere;
+        uint32_t at4 = kNone;
         u4 pt[2][T];
         float x[8];
+        auto weigh = [&](int j) {
+            x[j % 8] = __builtin_amdgcn_exp2f(fmaf(p[j], rs, off));
+            sum += x[j % 8];
+            if (j % 8 == 7) split8<BF16>(x, pt[j / 8]);
+        };
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             score_step(ahead, i, take(i), low[i % 2]);
             if constexpr (T == 3)
                 if (i + 2 < KS) low[i % 2] = low_operand(i + 2);
-            if (i == 0) fetch(c.k, at3, k0);
-            if (i == 1) fetch(c.v, at2, v2);
-            if (i == 2) at4 = place_of(at + 4);
+            // The first half of the weights here, the other one while the first
+            // meets its values.
 #pragma unroll
-            for (int j = i * 16 / KS; j < (i + 1) * 16 / KS; ++j) {
-                x[j % 8] = __builtin_amdgcn_exp2f(fmaf(p[j], rs, off));
-                sum += x[j % 8];
-                if (j % 8 == 7) split8<BF16>(x, pt[j / 8]);
-            }
+            for (int j = i * 8 / KS; j < (i + 1) * 8 / KS; ++j) weigh(j);
+            if (KS < 8 && i == 0) fetch(c.k, at3, k0);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -896,14 +894,23 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
                 o[d] = mfma32<BF16>(va, pt[s][j], o[d]);
                 o[d + 1] = mfma32<BF16>(vb, pt[s][j], o[d + 1]);
             }
-            if (i == 0) next = total(ahead);
-            if (i == 2) next_most = largest(next);
+            if (s == 0) {
+#pragma unroll
+                for (int j = 8 + d * 8 / VT; j < 8 + (d + 2) * 8 / VT; ++j) weigh(j);
+            }
+            if (KS >= 8 && i == 0) fetch(c.k, at3, k0);
+            if (i == VT) next = total(ahead);
+            if (i == VT) fetch(c.v, at2, v2);
+            if (i == 2 * VT - 2) {
+                at4 = place_of(at + 4);
+                next_most = largest(next);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (edge()) {
             if (apart == key0) {
                 // The rows that see one of the values left out become NaN.
-                const auto again = block_rsrc(c.v, at0, dim * kBlock * 2);
+                const auto again = block_rsrc(c.v, size_t(at0) * (dim * kBlock), block_bytes);
 #pragma unroll
                 for (int d2 = 0; d2 < VT; d2 += 2) {
 #pragma unroll 1
