@@ -21,6 +21,8 @@
 // be as the B operand of O^T = V^T P^T. Scores never leave their lane.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "attn_common.hpp"
@@ -42,6 +44,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kMaxSplits = 512;  // key ranges of a tile, at most
+constexpr uint32_t kFewSplits = 16;   // that a wave joins alone
 constexpr uint32_t kRsrcWord3 = 0x00020000u;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
@@ -981,49 +984,65 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     if (pl.splits > 1 && split == 0 && g == 0) ws.place[size_t(unit) * R + r] = one_range || !real ? kNone : token * a.heads + qh;
 }
 
-// Adds the ranges of a row up: a workgroup a row, every wave a quarter of the
-// ranges, whose loads depend on nothing and are all in flight at once.
-template <int DM>
-__global__ __launch_bounds__(kThreads) void attn_join_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
-    constexpr int E = DM / 64;
+// Adds the ranges of a row up. WIDE: a workgroup a row, every wave a quarter of
+// the ranges, whose loads depend on nothing and are all in flight at once. For
+// few ranges a wave a row.
+template <int DM, bool WIDE>
+__global__ __launch_bounds__(kThreads) void attn_join_kernel(AttendArgs a, AttendPlan pl, Partial ws, uint32_t rows) {
+    constexpr int E = DM / 64, W = WIDE ? kWaves : 1;
     typedef float fe __attribute__((ext_vector_type(E)));
-    __shared__ float weight[kMaxSplits], part_o[kWaves][DM], part_l[kWaves];
+    __shared__ float weight[WIDE ? kMaxSplits : kWaves * kFewSplits], part_o[kWaves][WIDE ? DM : 1], part_l[kWaves];
     const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64;
-    const uint32_t place = ws.place[blockIdx.x];
+    const uint32_t at_row = WIDE ? blockIdx.x : blockIdx.x * kWaves + w;
+    if (at_row >= rows) return;
+    const uint32_t place = ws.place[at_row];
     if (place == kNone) return;
-    const uint32_t unit = blockIdx.x / pl.rows, r = blockIdx.x % pl.rows;
+    float *weights = WIDE ? weight : weight + w * kFewSplits;
+    const uint32_t unit = at_row / pl.rows, r = at_row % pl.rows;
     const size_t first = size_t(unit) * pl.splits * pl.rows + r;
     float top = -INFINITY, all = 0.f;
     for (uint32_t s = l; s < pl.splits; s += 64) top = fmaxf(top, ws.ml[first + size_t(s) * pl.rows].x);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
     // A range that saw nothing (its sum is 0) left no row.
-    for (uint32_t s = threadIdx.x; s < pl.splits; s += kThreads) {
+    for (uint32_t s = WIDE ? threadIdx.x : l; s < pl.splits; s += W * 64) {
         const float2 ml = ws.ml[first + size_t(s) * pl.rows];
         const float f = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? 1.f : exp2f(ml.x - top);
-        weight[s] = ml.y == 0.f ? -1.f : f;
+        weights[s] = ml.y == 0.f ? -1.f : f;
         all += f * ml.y;
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
-    if (l == 0) part_l[w] = all;
-    __syncthreads();
+    if constexpr (WIDE) {
+        if (l == 0) part_l[w] = all;
+        __syncthreads();
+    } else {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    }
     fe acc = {};
     const fe *o = reinterpret_cast<const fe *>(ws.o + first * DM) + l;
 #pragma unroll 8
-    for (uint32_t s = w; s < pl.splits; s += kWaves) {
+    for (uint32_t s = WIDE ? w : 0; s < pl.splits; s += W) {
         const fe x = o[size_t(s) * pl.rows * (DM / E)];
-        const float f = weight[s];
+        const float f = weights[s];
         if (f >= 0.f || f != f) acc += f * x;
     }
-    *reinterpret_cast<fe *>(&part_o[w][l * E]) = acc;
-    __syncthreads();
-    all = part_l[0] + part_l[1] + part_l[2] + part_l[3];
-    const float f = all == 0.f ? 0.f : 1.f / all;
-    const uint32_t d = threadIdx.x;
-    if (d < a.cache.dim)
-        a.out[size_t(place / a.heads) * a.out_stride + size_t(place % a.heads) * a.cache.dim + d] =
-            (part_o[0][d] + part_o[1][d] + part_o[2][d] + part_o[3][d]) * f;
+    float *y = a.out + size_t(place / a.heads) * a.out_stride + size_t(place % a.heads) * a.cache.dim;
+    if constexpr (WIDE) {
+        *reinterpret_cast<fe *>(&part_o[w][l * E]) = acc;
+        __syncthreads();
+        all = part_l[0] + part_l[1] + part_l[2] + part_l[3];
+        const float f = all == 0.f ? 0.f : 1.f / all;
+        const uint32_t d = threadIdx.x;
+        if (d < a.cache.dim) y[d] = (part_o[0][d] + part_o[1][d] + part_o[2][d] + part_o[3][d]) * f;
+    } else {
+        const float f = all == 0.f ? 0.f : 1.f / all;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (l * E + e < a.cache.dim) y[l * E + e] = acc[e] * f;
+    }
 }
 
 uint32_t wide_dim(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
@@ -1074,7 +1093,12 @@ hipError_t launch_dim(const AttendArgs &a, const AttendPlan &pl, const Partial &
         e = hipGetLastError();
     }
     if (e != hipSuccess || pl.splits == 1) return e;
-    attn_join_kernel<DM><<<pl.tiles * a.cache.kv_heads * pl.rows, kThreads, 0, stream>>>(a, pl, ws);
+    const uint32_t rows = pl.tiles * a.cache.kv_heads * pl.rows;
+    if (pl.splits <= kFewSplits) {
+        attn_join_kernel<DM, false><<<(rows + kWaves - 1) / kWaves, kThreads, 0, stream>>>(a, pl, ws, rows);
+    } else {
+        attn_join_kernel<DM, true><<<rows, kThreads, 0, stream>>>(a, pl, ws, rows);
+    }
     return hipGetLastError();
 }
 
@@ -1089,36 +1113,80 @@ hipError_t launch_type(const AttendArgs &a, const AttendPlan &pl, const Partial 
 
 }  // namespace
 
+// The plan is the cheapest of an estimate over both kernels and their numbers
+// of key ranges, from sizes alone. Fitted to MI355X timings (us), per dims 64,
+// 128 and 256, bf16 and f16:
+//   rows kernel  a workgroup starts and ends in 4 and takes `chain` for its four
+//                waves' blocks; a CU works a tile of 16 rows against a block off
+//                in `each` whatever is resident; keys and values come in at
+//                5.3 TB/s
+//   tile kernel  15 for start and end, `chain` a block alone, `each` a block of
+//                128 rows when the CU's two workgroups (one of 256 dims) overlap
+//   join         3, and each range's rows written and read once
+// Both sides where it decides, rows / tile kernel: 64 tokens of 24 heads of 256
+// over 4064 keys 36 / 47 us, 150 over 4150 61 / 76, 512 over 16512 (bf16) 640 /
+// 580; one prompt of 32 heads of 128 (f16), 500 tokens 19 / 25, 1000 43 / 43,
+// 2000 118 / 88, 4100 389 / 282.
+// Ranges, in the rows kernel: one token of 24/4 heads of 256 over 32768 keys in
+// 8, 16, 32, 64 and 128: 52, 35, 30, 31.6 and 32 us; 32 sequences of 8 heads of
+// 128 over up to 8001 in 1, 2 and 4: 105, 113 and 122; one over 600 keys in 1, 2
+// and 5: 9.5, 11.4 and 10.4.
 AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t workspace_limit) {
     const PagedCache &c = a.cache;
     const uint64_t group = a.heads / c.kv_heads;
-    AttendPlan pl;
     // Sequences with a row: at most n. Each takes whole tiles.
     const uint64_t n = c.seqs < c.tokens ? c.seqs : c.tokens;
-    const uint64_t each = c.tokens * group / n;  // rows of a sequence, on average
-    pl.rows = each <= 32 ? 16 : 128;
-    const uint64_t by_rows = n + (c.tokens * group - n) / pl.rows;
-    const uint64_t by_token = c.tokens * ((group + pl.rows - 1) / pl.rows);
-    pl.tiles = uint32_t(by_rows < by_token ? by_rows : by_token);
-    // The keys that a tile's rows see, at most: with a window those of its
-    // first row to those of its last.
-    const uint64_t across = (pl.rows + group - 1) / group + kBlock;
-    const uint64_t keys = a.window && a.window + across < a.max_keys ? a.window + across : a.max_keys;
-    // Ranges of keys until every CU has two workgroups; a range gives each
-    // wave a block at least.
-    const uint64_t units = uint64_t(pl.tiles) * c.kv_heads, want = 2 * uint64_t(lim.num_cus);
-    const uint64_t step = kWaves * kBlock;
-    uint64_t splits = units < want ? want / units : 1;
-    if (splits > kMaxSplits) splits = kMaxSplits;
-    pl.keys = uint32_t(((keys + splits - 1) / splits + step - 1) / step * step);
-    pl.splits = uint32_t((keys + pl.keys - 1) / pl.keys);
-    pl.workspace = workspace_of(a, pl);
-    while (pl.splits > 1 && pl.workspace > workspace_limit) {
-        pl.keys *= 2;
-        pl.splits = uint32_t((keys + pl.keys - 1) / pl.keys);
-        pl.workspace = workspace_of(a, pl);
+    const int wide = wide_dim(c.dim) == 64 ? 0 : wide_dim(c.dim) == 128 ? 1 : 2;
+    static constexpr double kRowsChain[3] = {0.35, 0.55, 1.2}, kTileChain[3] = {0.75, 1.2, 2.3};
+    static constexpr double kRowsEach[2][3] = {{0.07, 0.19, 0.34}, {0.09, 0.21, 0.42}};
+    static constexpr double kTileEach[2][3] = {{0.5, 1.08, 2.3}, {0.6, 1.45, 2.9}};
+    const double cus = lim.num_cus;
+    AttendPlan best;
+    double least = 0;
+    for (const uint32_t rows : {16u, 128u}) {
+        AttendPlan pl;
+        pl.rows = rows;
+        const uint64_t by_rows = n + (c.tokens * group - n) / rows;
+        const uint64_t by_token = c.tokens * ((group + rows - 1) / rows);
+        pl.tiles = uint32_t(by_rows < by_token ? by_rows : by_token);
+        // The keys that a tile's rows see, at most: with a window those of its
+        // first row to those of its last.
+        const uint64_t across = (rows + group - 1) / group + kBlock;
+        const uint64_t keys = a.window && a.window + across < a.max_keys ? a.window + across : a.max_keys;
+        // A range gives each wave of the rows kernel a block at least.
+        const uint64_t units = uint64_t(pl.tiles) * c.kv_heads, step = kWaves * kBlock;
+        const uint64_t most = (keys + step - 1) / step < kMaxSplits ? (keys + step - 1) / step : kMaxSplits;
+        uint64_t before = 0;
+        for (uint64_t s = 1; s <= most; s += s < 32 ? 1 : s / 8) {
+            pl.keys = uint32_t(((keys + s - 1) / s + step - 1) / step * step);
+            pl.splits = uint32_t((keys + pl.keys - 1) / pl.keys);
+            if (pl.splits == before) continue;
+            before = pl.splits;
+            pl.workspace = workspace_of(a, pl);
+            if (pl.workspace > workspace_limit) break;
+            const double blocks = pl.keys / kBlock, work = double(units) * pl.splits * blocks / cus;
+            double us;
+            if (rows == 16) {
+                const double rounds = std::ceil(double(units) * pl.splits / cus);
+                const double moved = double(n) * c.kv_heads * keys * c.dim * 4 / 5.3e6;
+                us = std::max({rounds * 4 + rounds * blocks / kWaves * kRowsChain[wide], work * kRowsEach[c.bf16][wide], moved});
+                if (pl.splits == 1) us = std::max({4 + blocks / kWaves * kRowsChain[wide], work * kRowsEach[c.bf16][wide], moved});
+            } else {
+                const double rounds = std::ceil(double(units) * pl.splits / (wide == 2 ? cus : 2 * cus));
+                us = std::max(rounds * (15 + blocks * kTileChain[wide]), 15 * rounds + work * kTileEach[c.bf16][wide]);
+                if (wide < 2) us = std::max(15 + blocks * kTileChain[wide], 15 * rounds + work * kTileEach[c.bf16][wide]);
+            }
+            if (pl.splits > 1) {
+                const double joined = double(c.tokens) * a.heads * pl.splits * wide_dim(c.dim) * 8;
+                us += 3 + joined / 4.0e6 + 0.02 * pl.splits;
+            }
+            if (best.rows == 0 || us < least) {
+                best = pl;
+                least = us;
+            }
+        }
     }
-    return pl;
+    return best;
 }
 
 const char *attend_kernel_name(const AttendPlan &pl) { return pl.rows == 16 ? "attn_rows_kernel" : "attn_tile_kernel"; }
