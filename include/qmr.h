@@ -316,6 +316,9 @@ int qmr_supported_bf16_quantization(uint32_t bits, size_t group);
  *            of 16 rows per workgroup; zero fields and ks = 0 leave them to
  *            its planner). Wide blocks of more than four RHS run on that
  *            kernel by default; any other rr runs them as blocks of four.
+ *   rr = -7: attn_paged on the kernel of tiles of 16 or 128 query rows with
+ *            ks = rows*1000 + key ranges (zero fields leave them to its
+ *            planner); any other rr leaves attention to its planner.
  * Shapes a forced kernel does not support fall back to the next one; pairs
  * that are not compiled fall back to the planner. */
 int qmr_set_gemv_plan(qmr_device *device, int rr, int ks);

@@ -289,9 +289,10 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
     const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = l % 16, g = l / 16;
     const uint32_t split = blockIdx.x % pl.splits, unit = blockIdx.x / pl.splits;  // unit: tile and key head
-    const uint32_t head = unit % c.kv_heads, group = a.heads / c.kv_heads, dim = c.dim;
+    const uint32_t head = unit % c.kv_heads, tile = unit / c.kv_heads;
+    const uint32_t group = a.heads / c.kv_heads, dim = c.dim;
     Tile t;
-    if (!find_tile(c, group, R, unit / c.kv_heads, t)) {
+    if (!find_tile(c, group, R, tile, t)) {
         if (pl.splits > 1 && split == 0 && threadIdx.x < R) ws.place[size_t(unit) * R + threadIdx.x] = kNone;
         return;
     }
@@ -628,11 +629,12 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     const PagedCache &c = a.cache;
     const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = l % 32, g = l / 32;
-    const uint32_t split = blockIdx.x % pl.splits, unit = blockIdx.x / pl.splits;
-    const uint32_t head = unit % c.kv_heads, group = a.heads / c.kv_heads, dim = c.dim;
+    const uint32_t split = blockIdx.x % pl.splits, unit = blockIdx.x / pl.splits;  // unit: tile and key head
+    const uint32_t head = unit % c.kv_heads, tile = unit / c.kv_heads;
+    const uint32_t group = a.heads / c.kv_heads, dim = c.dim;
     Tile t;
     // The last tiles first: they see the most keys.
-    if (!find_tile(c, group, R, pl.tiles - 1 - unit / c.kv_heads, t)) {
+    if (!find_tile(c, group, R, pl.tiles - 1 - tile, t)) {
         if (pl.splits > 1 && split == 0 && threadIdx.x < R) ws.place[size_t(unit) * R + threadIdx.x] = kNone;
         return;
     }
@@ -1118,9 +1120,9 @@ hipError_t launch_type(const AttendArgs &a, const AttendPlan &pl, const Partial 
 // 128 and 256, bf16 and f16:
 //   rows kernel  a workgroup starts and ends in 4 and takes `chain` for its four
 //                waves' blocks; a CU works a tile of 16 rows against a block off
-//                in `each` whatever is resident; keys and values come in at
-//                5.3 TB/s
-//   tile kernel  15 for start and end, `chain` a block alone, `each` a block of
+//                in `each` whatever is resident, and starts a tile in 2; keys and values come in at
+//                5.3 TB/s from 128 workgroups on, at half that from 37
+//   tile kernel  10 for start and end, `chain` a block alone, `each` a block of
 //                128 rows when the CU's two workgroups (one of 256 dims) overlap
 //   join         3, and each range's rows written and read once
 // Both sides where it decides, rows / tile kernel: 64 tokens of 24 heads of 256
@@ -1131,19 +1133,24 @@ hipError_t launch_type(const AttendArgs &a, const AttendPlan &pl, const Partial 
 // 8, 16, 32, 64 and 128: 52, 35, 30, 31.6 and 32 us; 32 sequences of 8 heads of
 // 128 over up to 8001 in 1, 2 and 4: 105, 113 and 122; one over 600 keys in 1, 2
 // and 5: 9.5, 11.4 and 10.4.
-AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t workspace_limit) {
+AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t workspace_limit, uint32_t force_rows,
+                       uint32_t force_splits) {
     const PagedCache &c = a.cache;
     const uint64_t group = a.heads / c.kv_heads;
     // Sequences with a row: at most n. Each takes whole tiles.
     const uint64_t n = c.seqs < c.tokens ? c.seqs : c.tokens;
     const int wide = wide_dim(c.dim) == 64 ? 0 : wide_dim(c.dim) == 128 ? 1 : 2;
-    static constexpr double kRowsChain[3] = {0.35, 0.55, 1.2}, kTileChain[3] = {0.75, 1.2, 2.3};
-    static constexpr double kRowsEach[2][3] = {{0.07, 0.19, 0.34}, {0.09, 0.21, 0.42}};
-    static constexpr double kTileEach[2][3] = {{0.5, 1.08, 2.3}, {0.6, 1.45, 2.9}};
+    static constexpr double kRowsChain[3] = {0.45, 0.75, 1.6};
+    static constexpr double kTileChain[2][3] = {{0.95, 1.2, 2.0}, {1.0, 1.4, 2.4}};
+    static constexpr double kRowsEach[2][3] = {{0.07, 0.19, 0.33}, {0.09, 0.21, 0.42}};
+    static constexpr double kTileEach[2][3] = {{1.1, 1.05, 2.1}, {1.2, 1.45, 2.6}};
     const double cus = lim.num_cus;
+    // Of the keys before a sequence's end, those that its average row sees.
+    const double share = a.causal ? 1 - std::min(1.0, double(c.tokens) / n / a.max_keys) / 2 : 1;
     AttendPlan best;
     double least = 0;
     for (const uint32_t rows : {16u, 128u}) {
+        if ((force_rows == 16 || force_rows == 128) && rows != force_rows) continue;
         AttendPlan pl;
         pl.rows = rows;
         const uint64_t by_rows = n + (c.tokens * group - n) / rows;
@@ -1156,25 +1163,34 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
         // A range gives each wave of the rows kernel a block at least.
         const uint64_t units = uint64_t(pl.tiles) * c.kv_heads, step = kWaves * kBlock;
         const uint64_t most = (keys + step - 1) / step < kMaxSplits ? (keys + step - 1) / step : kMaxSplits;
+        // Workgroups go to the eight XCDs in turn: tiles that read the same keys
+        // share one's L2 if their distance is a multiple of eight (six tokens
+        // of 24/4 heads over 16006 keys in 16, 18, 20 and 21 ranges: 25.0, 25.5,
+        // 25.4 and 31.8 us; four sequences of four tokens over 6004 in 6, 7 and
+        // 8: 28.5, 40.4 and 26.8).
+        const bool shared = rows == 16 && c.tokens * group > n * rows;
         uint64_t before = 0;
-        for (uint64_t s = 1; s <= most; s += s < 32 ? 1 : s / 8) {
+        const uint64_t first = force_splits == 0 ? 1 : std::min<uint64_t>(force_splits, most);
+        for (uint64_t s = first; s <= (force_splits == 0 ? most : first); s += s < 32 ? 1 : s / 8) {
             pl.keys = uint32_t(((keys + s - 1) / s + step - 1) / step * step);
             pl.splits = uint32_t((keys + pl.keys - 1) / pl.keys);
             if (pl.splits == before) continue;
+            const uint64_t streams = pl.splits * uint64_t(c.kv_heads);
+            if (shared && force_splits == 0 && pl.splits > 1 && streams > 8 && streams % 8 != 0) continue;
             before = pl.splits;
             pl.workspace = workspace_of(a, pl);
-            if (pl.workspace > workspace_limit) break;
-            const double blocks = pl.keys / kBlock, work = double(units) * pl.splits * blocks / cus;
+            if (pl.workspace > workspace_limit && pl.splits > 1) break;
+            const double blocks = pl.keys / kBlock, work = double(units) * pl.splits * blocks * share / cus;
+            const double rounds = std::ceil(double(units) * pl.splits / (rows == 128 && wide < 2 ? 2 * cus : cus));
             double us;
             if (rows == 16) {
-                const double rounds = std::ceil(double(units) * pl.splits / cus);
                 const double moved = double(n) * c.kv_heads * keys * c.dim * 4 / 5.3e6;
-                us = std::max({rounds * 4 + rounds * blocks / kWaves * kRowsChain[wide], work * kRowsEach[c.bf16][wide], moved});
-                if (pl.splits == 1) us = std::max({4 + blocks / kWaves * kRowsChain[wide], work * kRowsEach[c.bf16][wide], moved});
+                const double fed = std::max(1.0, 0.6 + 51 / (double(units) * pl.splits));
+                const double alone = 4 + blocks / kWaves * kRowsChain[wide];
+                us = std::max({alone, (rounds - 1) * alone * share, work * kRowsEach[c.bf16][wide] + 2 * double(units) * pl.splits / cus, moved * fed});
             } else {
-                const double rounds = std::ceil(double(units) * pl.splits / (wide == 2 ? cus : 2 * cus));
-                us = std::max(rounds * (15 + blocks * kTileChain[wide]), 15 * rounds + work * kTileEach[c.bf16][wide]);
-                if (wide < 2) us = std::max(15 + blocks * kTileChain[wide], 15 * rounds + work * kTileEach[c.bf16][wide]);
+                us = std::max({10 + blocks * kTileChain[c.bf16][wide], rounds * (10 + blocks * share * kTileChain[c.bf16][wide]),
+                               10 * rounds + work * kTileEach[c.bf16][wide]});
             }
             if (pl.splits > 1) {
                 const double joined = double(c.tokens) * a.heads * pl.splits * wide_dim(c.dim) * 8;
@@ -1186,6 +1202,8 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
             }
         }
     }
+    // A forced number of ranges whose workspace is too large.
+    if (best.rows == 0) return plan_attend(a, lim, workspace_limit, force_rows, 1);
     return best;
 }
 

@@ -313,7 +313,10 @@ struct AttendPlan {
     uint32_t keys = 0;      // keys of one range
     size_t workspace = 0;   // bytes of the ranges' partial results
 };
-AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t workspace_limit);
+// force_rows (16 or 128) and force_splits (tuning hook) are kept where they can
+// be; zeros leave the choice to the planner.
+AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t workspace_limit, uint32_t force_rows = 0,
+                       uint32_t force_splits = 0);
 hipError_t launch_attn_paged(const AttendArgs &a, const AttendPlan &pl, void *workspace, hipStream_t stream);
 const char *attend_kernel_name(const AttendPlan &pl);
 

@@ -956,7 +956,13 @@ hipError_t launch_attention(qmr_device *dev, const std::string &name, qmr_buffer
     a.window = p[12];
     std::memcpy(&a.scale, &p[13], 4);
     a.cache = cache_at(1, 7);
-    const qmr::AttendPlan pl = qmr::plan_attend(a, dev->limits, fixed ? QMR_STATIC_SCRATCH_BYTES : SIZE_MAX);
+    const qmr::GemvPlan f = dev->forced_plan;
+    const bool forced = f.rr == -7 && f.ks > 0;
+    // A plan without key ranges needs no workspace: the static scratch always
+    // has room for one.
+    const qmr::AttendPlan pl =
+        qmr::plan_attend(a, dev->limits, fixed ? QMR_STATIC_SCRATCH_BYTES : SIZE_MAX, forced ? uint32_t(f.ks / 1000) : 0,
+                         forced ? uint32_t(f.ks % 1000) : 0);
     if (fixed) {
         check_static_scratch(pl.workspace, "attention's key ranges");
         if (pl.workspace) mark_static_dirty(dev, pl.workspace);

@@ -8,6 +8,20 @@ from attention_cases import Batch, attend, attend64, check_attend, from_half, ma
 pytestmark = pytest.mark.gpu
 
 KINDS = ["bf16", "f16"]
+# The planner's choice, and each kernel with and without key ranges.
+PLANS = [0, 16001, 16003, 128001, 128002]
+
+
+def under_plans(gpu, call):
+    """(plan, call()) under each plan, the planner's last."""
+    try:
+        for plan in PLANS[1:]:
+            gpu.set_gemv_plan(-7, plan)
+            yield plan, call()
+    finally:
+        gpu.set_gemv_plan(0, 0)
+    yield 0, call()
+
 
 
 def run(gpu, kind, batch, heads, kv_heads, dim, seed=0, spread=1.0, **how):
@@ -15,10 +29,10 @@ def run(gpu, kind, batch, heads, kv_heads, dim, seed=0, spread=1.0, **how):
     q = (spread * rng.standard_normal((batch.tokens, heads, dim))).astype(np.float32)
     k, v = make_pool(batch, kv_heads, dim, kind, rng)
     scale = how.pop("scale", dim ** -0.5)
-    got = attend(gpu, kind, q, k, v, batch, scale, **how)
-    how = {n: how[n] for n in ("causal", "window", "max_keys") if n in how}
-    want, bound = attend64(q, from_half(k, kind), from_half(v, kind), batch, np.float32(scale).astype(np.float64), **how)
-    check_attend(got, want, bound, f"{kind} {heads}/{kv_heads}x{dim} {batch.new} {batch.lengths}")
+    mask = {n: how[n] for n in ("causal", "window", "max_keys") if n in how}
+    want, bound = attend64(q, from_half(k, kind), from_half(v, kind), batch, np.float32(scale).astype(np.float64), **mask)
+    for plan, got in under_plans(gpu, lambda: attend(gpu, kind, q, k, v, batch, scale, **how)):
+        check_attend(got, want, bound, f"plan {plan}: {kind} {heads}/{kv_heads}x{dim} {batch.new} {batch.lengths}")
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -77,6 +91,15 @@ def test_pages_past_the_pool_hold_nothing(gpu, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("column", [0, 1, 2, 3, 4])
+def test_dropped_pages_behind_garbage(gpu, kind, column):
+    # The last block's free slots hold NaN or infinities; a page that is not
+    # there comes after it, whichever block that is.
+    run(gpu, kind, Batch([3], [5 * 32 + 3], 32, dropped=((0, column),)), 2, 1, 64)
+    run(gpu, kind, Batch([3], [5 * 32 + 3], 32, dropped=((0, column), (0, (column + 1) % 5))), 2, 1, 256)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_many_sequences(gpu, kind):
     # More than a wave's 64, with empty ones among them.
     rng = np.random.default_rng(3)
@@ -115,8 +138,9 @@ def test_rising_scores(gpu, kind):
     for s, length in enumerate(batch.lengths):
         for j in range(length):
             k[batch.table[s, j // 32], 0, j % 32] = to_half(np.full(64, (j // 32) * (0.05 if j % 2 else 0.4)), kind)
-    got = attend(gpu, kind, q, k, v, batch, 0.3)
-    check_attend(got, *attend64(q, from_half(k, kind), from_half(v, kind), batch, float(np.float32(0.3))))
+    want, bound = attend64(q, from_half(k, kind), from_half(v, kind), batch, float(np.float32(0.3)))
+    for plan, got in under_plans(gpu, lambda: attend(gpu, kind, q, k, v, batch, 0.3)):
+        check_attend(got, want, bound, f"plan {plan}")
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -133,12 +157,24 @@ def test_hidden_values_do_not_reach_rows(gpu, kind, new):
     for pos, bits in ((at, nan), (12, inf)):  # the first two tokens still see position 12
         v[batch.table[0, pos // 32], 0, pos % 32, 5] = bits
         k[batch.table[0, pos // 32], 0, pos % 32, 7] = bits
-    got = attend(gpu, kind, q, k, v, batch, 0.125, window=90)
     want, bound = attend64(q, from_half(k, kind), from_half(v, kind), batch, 0.125, window=90)
     assert np.isfinite(want[2:-1]).all()
-    check_attend(got[2:-1], want[2:-1], bound[2:-1])
-    for i in (0, 1, -1):
-        assert not np.isfinite(want[i]).all() and not np.isfinite(got[i]).all()
+    for plan, got in under_plans(gpu, lambda: attend(gpu, kind, q, k, v, batch, 0.125, window=90)):
+        check_attend(got[2:-1], want[2:-1], bound[2:-1], f"plan {plan}")
+        for i in (0, 1, -1):
+            assert not np.isfinite(want[i]).all() and not np.isfinite(got[i]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_every_row_sees_a_value_that_is_not_finite(gpu, kind):
+    batch = Batch([5], [200], 32)
+    rng = np.random.default_rng(16)
+    k, v = make_pool(batch, 1, 64, kind, rng)
+    q = rng.standard_normal((5, 4, 64)).astype(np.float32)
+    v[batch.table[0, 2], 0, 9, 11] = to_half(np.array([np.nan], np.float32), kind)[0]
+    want, bound = attend64(q, from_half(k, kind), from_half(v, kind), batch, 0.125)
+    for plan, got in under_plans(gpu, lambda: attend(gpu, kind, q, k, v, batch, 0.125)):
+        check_attend(got, want, bound, f"plan {plan}")
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -148,8 +184,9 @@ def test_rows_repeat(gpu, kind):
     for batch, heads, kv in ((Batch([1], [3000], 64), 12, 2), (Batch([37, 1], [300, 900], 64), 6, 2)):
         q = rng.standard_normal((batch.tokens, heads, 128)).astype(np.float32)
         k, v = make_pool(batch, kv, 128, kind, rng)
-        first = attend(gpu, kind, q, k, v, batch, 0.09)
-        assert np.array_equal(first, attend(gpu, kind, q, k, v, batch, 0.09))
+        for plan, first in under_plans(gpu, lambda: attend(gpu, kind, q, k, v, batch, 0.09)):
+            gpu.set_gemv_plan(-7, plan)
+            assert np.array_equal(first, attend(gpu, kind, q, k, v, batch, 0.09)), plan
         want, bound = attend64(q, from_half(k, kind), from_half(v, kind), batch, float(np.float32(0.09)))
         check_attend(attend(gpu, kind, q, k, v, batch, 0.09, static=True), want, bound)
 
