@@ -1187,7 +1187,7 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
                 const double moved = double(n) * c.kv_heads * keys * c.dim * 4 / 5.3e6;
                 const double fed = std::max(1.0, 0.6 + 51 / (double(units) * pl.splits));
                 const double alone = 4 + blocks / kWaves * kRowsChain[wide];
-                us = std::max({alone, (rounds - 1) * alone * share, work * kRowsEach[c.bf16][wide] + 2 * double(units) * pl.splits / cus, moved * fed});
+                us = std::max({alone * (1 + 0.8 * (rounds - 1) * share), work * kRowsEach[c.bf16][wide] + 2 * double(units) * pl.splits / cus, moved * fed});
             } else {
                 us = std::max({10 + blocks * kTileChain[c.bf16][wide], rounds * (10 + blocks * share * kTileChain[c.bf16][wide]),
                                10 * rounds + work * kTileEach[c.bf16][wide]});
