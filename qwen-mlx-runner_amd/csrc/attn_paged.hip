@@ -166,10 +166,15 @@ __device__ __forceinline__ bool find_tile(const PagedCache &c, uint32_t group, u
         const uint32_t to = min(end, c.tokens), count = to > from ? to - from : 0;
         const uint32_t own = (count * group + R - 1) / R;
         uint32_t sum = own;
+        if (__ballot(own > 1) == 0) {  // decode: bits to count
+            const uint64_t some = __ballot(own != 0);
+            sum += __builtin_amdgcn_mbcnt_hi(uint32_t(some >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(some), 0));
+        } else {
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint32_t o = __shfl_up(sum, d);
-            if (l >= uint32_t(d)) sum += o;
+            for (int d = 1; d < 64; d *= 2) {
+                const uint32_t o = __shfl_up(sum, d);
+                if (l >= uint32_t(d)) sum += o;
+            }
         }
         const uint32_t total = __builtin_amdgcn_readlane(sum, 63);
         if (tile >= total) {
@@ -308,7 +313,31 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
     const int from = some ? int(from64) : 0;
     const int to = some ? int(min(from64 + int64_t(pl.keys), int64_t(hi_last))) : 0;
 
-    // The queries' loads go out first: thread (row % 16, p) has chunks p and
+    // Blocks w, w + 4, .. of the order. A block's keys are loaded while the
+    // block before is weighed, its values while its scores are worked out, the
+    // first ones while the queries are; the page after next is named by then.
+    // Pages are read as constants (scalar loads), whose wait does not wait for
+    // the blocks in flight. A page past the pool, or a block past the last,
+    // reads as zeros: no memory is touched.
+    const Order order(from, to, lo_last, hi_first);
+    const auto *table = (const __attribute__((address_space(4))) uint32_t *)(c.table + size_t(t.seq) * c.columns);
+    const uint32_t page_shift = __builtin_ctz(c.page);
+    auto page_of = [&](int key0) { return table[uint32_t(key0) >> page_shift]; };
+    auto rsrc_of = [&](const uint16_t *pool, uint32_t named, int key0, bool real) {
+        const bool held = real && named < c.pages;
+        const size_t at = attn::block_at(c, held ? named : 0, head, (uint32_t(key0) & (c.page - 1)) / kBlock);
+        return block_rsrc(pool, at, held ? dim * kBlock * 2 : 0);
+    };
+    int at = int(w), key0 = 0, next_key = 0;
+    uint32_t named = 0, next = 0;
+    if (at < order.count) {
+        key0 = order.key(at);
+        next_key = order.key(at + kWaves);
+        named = page_of(key0);
+        next = page_of(next_key);
+    }
+
+    // The queries' loads go out before the blocks': thread (row % 16, p) has chunks p and
     // p + 16 of 8 dims.
     constexpr int CH = (DM / 8 + 15) / 16;
     const uint32_t qn = threadIdx.x / 16, qp = threadIdx.x % 16;
@@ -329,21 +358,6 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
         }
     }
 
-    // Blocks w, w + 4, .. of the order. A block's keys are loaded while the
-    // block before is weighed, its values while its scores are worked out, the
-    // first ones while the queries are; the page after next is named by then.
-    // Pages are read as constants (scalar loads), whose wait does not wait for
-    // the blocks in flight. A page past the pool, or a block past the last,
-    // reads as zeros: no memory is touched.
-    const Order order(from, to, lo_last, hi_first);
-    const auto *table = (const __attribute__((address_space(4))) uint32_t *)(c.table + size_t(t.seq) * c.columns);
-    const uint32_t page_shift = __builtin_ctz(c.page);
-    auto page_of = [&](int key0) { return table[uint32_t(key0) >> page_shift]; };
-    auto rsrc_of = [&](const uint16_t *pool, uint32_t named, int key0, bool real) {
-        const bool held = real && named < c.pages;
-        const size_t at = attn::block_at(c, held ? named : 0, head, (uint32_t(key0) & (c.page - 1)) / kBlock);
-        return block_rsrc(pool, at, held ? dim * kBlock * 2 : 0);
-    };
     u4 k[KS][2];
     auto load_keys = [&](uint32_t named, int key0, bool real) {
         const auto r = rsrc_of(c.k, named, key0, real);
@@ -360,13 +374,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
 #pragma unroll
         for (int d = 0; d < VT; ++d) v[d] = load16(r, (g * dim + n) * 16, d * 256);
     };
-    int at = int(w), key0 = 0, next_key = 0;
-    uint32_t named = 0, next = 0;
     if (at < order.count) {
-        key0 = order.key(at);
-        next_key = order.key(at + kWaves);
-        named = page_of(key0);
-        next = page_of(next_key);
         load_keys(named, key0, true);
         load_values(named, key0, true);
     }
@@ -445,6 +453,8 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
 #pragma unroll
                     for (int j = 0; j < 2; ++j) scores[nb][j] = mfma16<BF16>(k[s][j], q, scores[nb][j]);
                 }
+                // Not all of them on their way at once, which would not fit.
+                if (DM == 256 && s % 2 == 1) __builtin_amdgcn_sched_barrier(0);
             }
         }
         const bool more = at + kWaves < order.count;
@@ -544,7 +554,11 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
     while (at < order.edges) block(std::true_type{});
     while (at < order.count) block(std::false_type{});
 
-    // Join the waves, 16 rows at a time.
+    // Join the waves, 16 rows at a time. (What a thread is in the workgroup is
+    // worked out again: the loop needs the registers.)
+    uint32_t thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));
+    const uint32_t jl = thread % 64, jn = jl % 16, jg = jl / 16, rn = thread / 16, rp = thread % 16;
     float *os = reinterpret_cast<float *>(lds);  // [kWaves][16][kPitch]
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -559,42 +573,43 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
                 if (poison[(nb * VT + d) / 8] >> ((nb * VT + d) % 8 * 4 + i) & 1) o[nb][d][i] = __builtin_nanf("");
         }
 #pragma unroll
-        for (int d = 0; d < VT; ++d) *reinterpret_cast<f4 *>(os + (w * 16 + n) * kPitch + 16 * d + 4 * g) = o[nb][d];
-        if (g == 0) {
-            wave_m[w][n] = m[nb];
-            wave_l[w][n] = all;
+        for (int d = 0; d < VT; ++d) *reinterpret_cast<f4 *>(os + (w * 16 + jn) * kPitch + 16 * d + 4 * jg) = o[nb][d];
+        if (jg == 0) {
+            wave_m[w][jn] = m[nb];
+            wave_l[w][jn] = all;
         }
         __syncthreads();
-        const size_t part = (size_t(unit) * pl.splits + split) * R + nb * 16;
-        for (uint32_t i = threadIdx.x; i < 16 * DM / 4; i += kThreads) {
-            const uint32_t rn = i / (DM / 4), d = i % (DM / 4) * 4, r = nb * 16 + rn;
-            float top = wave_m[0][rn];
+        // Sixteen threads a row, four dims at a time.
+        const uint32_t r = nb * 16 + rn;
+        const bool real = r < in_tile;
+        const uint32_t row = t.row0 + r, token = t.first_token + row / group, qh = head * group + row % group;
+        if (pl.splits > 1 && split == 0 && rp == 0)
+            ws.place[size_t(unit) * R + r] = one_range || !real ? kNone : token * a.heads + qh;
+        if (!real || (one_range && split > 0)) continue;
+        float top = wave_m[0][rn], f[kWaves], joined = 0.f;
 #pragma unroll
-            for (int k = 1; k < kWaves; ++k) top = fmaxf(top, wave_m[k][rn]);
-            float joined = 0.f;
+        for (int k = 1; k < kWaves; ++k) top = fmaxf(top, wave_m[k][rn]);
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            const float mk = wave_m[k][rn], lk = wave_l[k][rn];
+            f[k] = mk == -INFINITY ? (lk == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mk - top);
+            joined += f[k] * lk;
+        }
+        const size_t part = (size_t(unit) * pl.splits + split) * R + r;
+        const float over = joined == 0.f ? 0.f : 1.f / joined;
+        float *y = one_range ? a.out + size_t(token) * a.out_stride + size_t(qh) * dim : ws.o + part * DM;
+#pragma unroll
+        for (uint32_t d = rp * 4; d < DM; d += 64) {
             f4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < kWaves; ++k) {
-                const float f = wave_m[k][rn] == -INFINITY ? (wave_l[k][rn] == 0.f ? 0.f : 1.f) : exp2f(wave_m[k][rn] - top);
-                joined += f * wave_l[k][rn];
-                acc += f * *reinterpret_cast<const f4 *>(os + (k * 16 + rn) * kPitch + d);
+            for (int k = 0; k < kWaves; ++k) acc += f[k] * *reinterpret_cast<const f4 *>(os + (k * 16 + rn) * kPitch + d);
+            if (!one_range) {
+                if (joined != 0.f) *reinterpret_cast<f4 *>(y + d) = acc;
+            } else if (d < dim) {
+                *reinterpret_cast<f4u *>(y + d) = acc * over;
             }
-            const uint32_t row = t.row0 + r;
-            const bool real = r < in_tile;
-            const uint32_t place = (t.first_token + row / group) * a.heads + head * group + row % group;
-            if (one_range) {
-                if (split == 0 && real && d < dim) {
-                    const float f = joined == 0.f ? 0.f : 1.f / joined;
-                    float *y = a.out + size_t(t.first_token + row / group) * a.out_stride +
-                               size_t(head * group + row % group) * dim + d;
-                    *reinterpret_cast<f4u *>(y) = acc * f;
-                }
-            } else if (real) {
-                if (joined != 0.f) *reinterpret_cast<f4 *>(ws.o + (part + rn) * DM + d) = acc;
-                if (d == 0) ws.ml[part + rn] = make_float2(top, joined);
-            }
-            if (pl.splits > 1 && split == 0 && d == 0) ws.place[size_t(unit) * R + r] = one_range || !real ? kNone : place;
         }
+        if (!one_range && rp == 0) ws.ml[part] = make_float2(top, joined);
     }
 }
 
