@@ -275,21 +275,21 @@ __device__ __forceinline__ u4 ones_of(int first, int lo, int hi) {
     return halves_of(first, lo, hi) & kOne<BF16>;
 }
 
-// Few rows: R = 16 NB rows a workgroup, every wave all of them over its own
+// Few rows: 16 rows a workgroup, every wave all of them over its own
 // blocks of the range (block w, w + 4, ..), straight from memory into operand
 // registers, whole lines at a time; nothing is shared but the queries, which
 // wait in LDS as operands. The waves' m, l and O
 // are joined through LDS at the end.
-template <bool BF16, int DM, int NB>
-__global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
-    constexpr int R = 16 * NB, T = kTerms<BF16>, KS = DM / 32, VT = DM / 16;
+template <bool BF16, int DM>
+__global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
+    constexpr int R = 16, T = kTerms<BF16>, KS = DM / 32, VT = DM / 16;
     // f16 weights are up to 2^15, so that small ones stay normal; the maximum
     // lags by at most 2^kLag.
     constexpr float kTop = BF16 ? 0.f : 7.f, kLag = 8.f;
     constexpr int kPitch = DM + 4;  // LDS pitch of a joined row: 16 rows on different banks
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ float row_scale[R];
-    __shared__ float wave_m[kWaves][16], wave_l[kWaves][16];
+    __shared__ float wave_m[kWaves][R], wave_l[kWaves][R];
     const PagedCache &c = a.cache;
     const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t n = l % 16, g = l / 16;
@@ -341,21 +341,18 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
     // p + 16 of 8 dims.
     constexpr int CH = (DM / 8 + 15) / 16;
     const uint32_t qn = threadIdx.x / 16, qp = threadIdx.x % 16;
-    float x[NB][CH][8];
+    float x[CH][8];
+    const uint32_t q_row = t.row0 + min(qn, in_tile - 1);
+    const float *q_own = a.q + size_t(t.first_token + q_row / group) * a.q_stride + size_t(head * group + q_row % group) * dim;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const uint32_t r = nb * 16 + qn, row = t.row0 + min(r, in_tile - 1);
-        const float *q = a.q + size_t(t.first_token + row / group) * a.q_stride + size_t(head * group + row % group) * dim;
-#pragma unroll
-        for (int k = 0; k < CH; ++k) {
-            const uint32_t ch = qp + 16 * k;
-            const f4 none = {0.f, 0.f, 0.f, 0.f};
-            const bool in = r < in_tile && ch * 8 < dim;
-            const float *at = q + (ch * 8 < dim ? ch * 8 : 0);
-            const f4 x0 = *reinterpret_cast<const f4u *>(at), x1 = *reinterpret_cast<const f4u *>(at + 4);
-            *reinterpret_cast<f4 *>(x[nb][k]) = in ? x0 : none;
-            *reinterpret_cast<f4 *>(x[nb][k] + 4) = in ? x1 : none;
-        }
+    for (int k = 0; k < CH; ++k) {
+        const uint32_t ch = qp + 16 * k;
+        const f4 none = {0.f, 0.f, 0.f, 0.f};
+        const bool in = qn < in_tile && ch * 8 < dim;
+        const float *at = q_own + (ch * 8 < dim ? ch * 8 : 0);
+        const f4 x0 = *reinterpret_cast<const f4u *>(at), x1 = *reinterpret_cast<const f4u *>(at + 4);
+        *reinterpret_cast<f4 *>(x[k]) = in ? x0 : none;
+        *reinterpret_cast<f4 *>(x[k] + 4) = in ? x1 : none;
     }
 
     u4 k[KS][2];
@@ -380,60 +377,48 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
     }
 
     // The queries, as operands.
-    u4 *qs = reinterpret_cast<u4 *>(lds);  // [NB][KS][T][64 lanes]
+    u4 *qs = reinterpret_cast<u4 *>(lds);  // [KS][T][64 lanes]
+    float q_most = 0.f;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const uint32_t r = nb * 16 + qn;
-        float most = 0.f;
+    for (int k = 0; k < CH; ++k) {
 #pragma unroll
-        for (int k = 0; k < CH; ++k) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[nb][k][j] *= a.scale * kLog2e;
-                most = fmaxf(most, fabsf(x[nb][k][j]));
-            }
+        for (int j = 0; j < 8; ++j) {
+            x[k][j] *= a.scale * kLog2e;
+            q_most = fmaxf(q_most, fabsf(x[k][j]));
         }
-        int e = 0;
+    }
+    int e = 0;
+    if constexpr (!BF16) {
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) q_most = fmaxf(q_most, __shfl_xor(q_most, d));
+        if (q_most > 0.f && q_most < INFINITY) frexpf(q_most, &e), e -= 15;
+    }
+    if (qp == 0) row_scale[qn] = ldexpf(1.f, e);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+        const uint32_t ch = qp + 16 * k;
+        if (ch >= DM / 8) continue;
         if constexpr (!BF16) {
 #pragma unroll
-            for (int d = 1; d < 16; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-            if (most > 0.f && most < INFINITY) frexpf(most, &e), e -= 15;
+            for (int j = 0; j < 8; ++j) x[k][j] = ldexpf(x[k][j], -e);
         }
-        if (qp == 0) row_scale[r] = ldexpf(1.f, e);
+        u4 terms[T];
+        split8<BF16>(x[k], terms);
 #pragma unroll
-        for (int k = 0; k < CH; ++k) {
-            const uint32_t ch = qp + 16 * k;
-            if (ch >= DM / 8) continue;
-            if constexpr (!BF16) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[nb][k][j] = ldexpf(x[nb][k][j], -e);
-            }
-            u4 terms[T];
-            split8<BF16>(x[nb][k], terms);
-#pragma unroll
-            for (int i = 0; i < T; ++i) qs[((nb * KS + ch / 4) * T + i) * 64 + (ch % 4) * 16 + qn] = terms[i];
-        }
+        for (int i = 0; i < T; ++i) qs[(ch / 4 * T + i) * 64 + (ch % 4) * 16 + qn] = terms[i];
     }
     __syncthreads();
 
-    // What each row may see.
-    int lo[NB], hi[NB];
-    float rs[NB], m[NB], sum[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const uint32_t r = nb * 16 + n;
-        visible(a, t, (t.row0 + min(r, in_tile - 1)) / group, lo[nb], hi[nb]);
-        rs[nb] = row_scale[r];
-        m[nb] = -INFINITY;
-        sum[nb] = 0.f;
-    }
+    // What the lane's row may see.
+    int lo, hi;
+    visible(a, t, (t.row0 + min(n, in_tile - 1)) / group, lo, hi);
+    const float rs = row_scale[n];
+    float m = -INFINITY, sum = 0.f;
     // Of a lane's outputs, those that saw a value that is not finite.
-    uint32_t poison[(NB * VT + 7) / 8] = {};
-    f4 o[NB][VT];
+    uint32_t poison[(VT + 7) / 8] = {};
+    f4 o[VT];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int d = 0; d < VT; ++d) o[nb][d] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < VT; ++d) o[d] = f4{0.f, 0.f, 0.f, 0.f};
 
     auto block = [&](auto edge) {
         const bool held = named < c.pages;
@@ -441,21 +426,17 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
         // the block do not fit the registers together.
         uint32_t ql = l;
         if constexpr (DM == 256) asm volatile("" : "+v"(ql));
-        f4 scores[NB][2];
+        f4 scores[2] = {};
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            scores[nb][0] = scores[nb][1] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < KS; ++s) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
+            for (int i = 0; i < T; ++i) {
+                const u4 q = qs[(s * T + i) * 64 + ql];
 #pragma unroll
-                for (int i = 0; i < T; ++i) {
-                    const u4 q = qs[((nb * KS + s) * T + i) * 64 + ql];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) scores[nb][j] = mfma16<BF16>(k[s][j], q, scores[nb][j]);
-                }
-                // Not all of them on their way at once, which would not fit.
-                if (DM == 256 && s % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                for (int j = 0; j < 2; ++j) scores[j] = mfma16<BF16>(k[s][j], q, scores[j]);
             }
+            // Not all of them on their way at once, which would not fit.
+            if (DM == 256 && s % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
         const bool more = at + kWaves < order.count;
         load_keys(next, next_key, more);
@@ -483,66 +464,60 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
                         for (int i = 0; i < 4; ++i) v[d][i] &= ~not_finite<BF16>(v[d][i]);
                     }
                     const auto again = rsrc_of(c.v, named, key_now, true);
+                    const u4 seen = ones_of<BF16>(key_now + 8 * int(g), lo, hi);
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        const u4 seen = ones_of<BF16>(key_now + 8 * int(g), lo[nb], hi[nb]);
-#pragma unroll
-                        for (int d8 = 0; d8 < VT; d8 += 8) {
+                    for (int d8 = 0; d8 < VT; d8 += 8) {
 #pragma unroll 1
-                            for (int d = 0; d < 8 && d8 + d < VT; ++d) {
-                                u4 bad = load16(again, (g * dim + n) * 16, (d8 + d) * 256) & kept;
+                        for (int d = 0; d < 8 && d8 + d < VT; ++d) {
+                            u4 bad = load16(again, (g * dim + n) * 16, (d8 + d) * 256) & kept;
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) bad[i] = not_finite<BF16>(bad[i]) & kOne<BF16>;
-                                const f4 count = mfma16<BF16>(bad, seen, f4{0.f, 0.f, 0.f, 0.f});
-                                uint32_t bits = 0;
+                            for (int i = 0; i < 4; ++i) bad[i] = not_finite<BF16>(bad[i]) & kOne<BF16>;
+                            const f4 count = mfma16<BF16>(bad, seen, f4{0.f, 0.f, 0.f, 0.f});
+                            uint32_t bits = 0;
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) bits |= count[i] > 0.f ? 1u << i : 0u;
-                                poison[(nb * VT + d8) / 8] |= bits << (4 * ((nb * VT) % 8 + d));
-                            }
+                            for (int i = 0; i < 4; ++i) bits |= count[i] > 0.f ? 1u << i : 0u;
+                            poison[d8 / 8] |= bits << (4 * d);
                         }
                     }
                 }
             }
         }
+        float p[8];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            float p[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = scores[nb][0][i], p[4 + i] = scores[nb][1][i];
-            if constexpr (edge()) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int key = key_now + 8 * int(g) + e;
-                    if (key < lo[nb] || key >= hi[nb]) p[e] = -INFINITY;
-                }
-            }
-            float most = p[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) most = fmaxf(most, p[e]);
-            most = held ? most * rs[nb] : -INFINITY;
-            if (__ballot(most > m[nb] + kLag) != 0) {
-                most = fmaxf(most, __shfl_xor(most, 16));
-                most = fmaxf(most, __shfl_xor(most, 32));
-                const float up = fmaxf(m[nb], most);
-                const float f = up > m[nb] ? exp2f(m[nb] - up) : 1.f;
-                m[nb] = up;
-                sum[nb] *= f;
-#pragma unroll
-                for (int d = 0; d < VT; ++d) o[nb][d] *= f;
-            }
-            const float off = held ? kTop - (m[nb] == -INFINITY ? 0.f : m[nb]) : -INFINITY;
+        for (int i = 0; i < 4; ++i) p[i] = scores[0][i], p[4 + i] = scores[1][i];
+        if constexpr (edge()) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], rs[nb], off));
-                sum[nb] += p[e];
+                const int key = key_now + 8 * int(g) + e;
+                if (key < lo || key >= hi) p[e] = -INFINITY;
             }
-            u4 pt[T];
-            split8<BF16>(p, pt);
+        }
+        float most = p[0];
 #pragma unroll
-            for (int d = 0; d < VT; ++d) {
+        for (int e = 1; e < 8; ++e) most = fmaxf(most, p[e]);
+        most = held ? most * rs : -INFINITY;
+        if (__ballot(most > m + kLag) != 0) {
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const float up = fmaxf(m, most);
+            const float f = up > m ? exp2f(m - up) : 1.f;
+            m = up;
+            sum *= f;
 #pragma unroll
-                for (int i = 0; i < T; ++i) o[nb][d] = mfma16<BF16>(v[d], pt[i], o[nb][d]);
-            }
+            for (int d = 0; d < VT; ++d) o[d] *= f;
+        }
+        const float off = held ? kTop - (m == -INFINITY ? 0.f : m) : -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], rs, off));
+            sum += p[e];
+        }
+        u4 pt[T];
+        split8<BF16>(p, pt);
+#pragma unroll
+        for (int d = 0; d < VT; ++d) {
+#pragma unroll
+            for (int i = 0; i < T; ++i) o[d] = mfma16<BF16>(v[d], pt[i], o[d]);
         }
         load_values(next, next_key, more);
         at += kWaves;
@@ -554,63 +529,59 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 2 : 1) void attn_rows_kernel(At
     while (at < order.edges) block(std::true_type{});
     while (at < order.count) block(std::false_type{});
 
-    // Join the waves, 16 rows at a time. (What a thread is in the workgroup is
+    // Join the waves. (What a thread is in the workgroup is
     // worked out again: the loop needs the registers.)
     uint32_t thread = threadIdx.x;
     asm volatile("" : "+v"(thread));
     const uint32_t jl = thread % 64, jn = jl % 16, jg = jl / 16, rn = thread / 16, rp = thread % 16;
     float *os = reinterpret_cast<float *>(lds);  // [kWaves][16][kPitch]
+    float all = sum;
+    all += __shfl_xor(all, 16);
+    all += __shfl_xor(all, 32);
+    __syncthreads();
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        float all = sum[nb];
-        all += __shfl_xor(all, 16);
-        all += __shfl_xor(all, 32);
-        __syncthreads();
+    for (int d = 0; d < VT; ++d) {
 #pragma unroll
-        for (int d = 0; d < VT; ++d) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (poison[(nb * VT + d) / 8] >> ((nb * VT + d) % 8 * 4 + i) & 1) o[nb][d][i] = __builtin_nanf("");
-        }
-#pragma unroll
-        for (int d = 0; d < VT; ++d) *reinterpret_cast<f4 *>(os + (w * 16 + jn) * kPitch + 16 * d + 4 * jg) = o[nb][d];
-        if (jg == 0) {
-            wave_m[w][jn] = m[nb];
-            wave_l[w][jn] = all;
-        }
-        __syncthreads();
-        // Sixteen threads a row, four dims at a time.
-        const uint32_t r = nb * 16 + rn;
-        const bool real = r < in_tile;
-        const uint32_t row = t.row0 + r, token = t.first_token + row / group, qh = head * group + row % group;
-        if (pl.splits > 1 && split == 0 && rp == 0)
-            ws.place[size_t(unit) * R + r] = one_range || !real ? kNone : token * a.heads + qh;
-        if (!real || (one_range && split > 0)) continue;
-        float top = wave_m[0][rn], f[kWaves], joined = 0.f;
-#pragma unroll
-        for (int k = 1; k < kWaves; ++k) top = fmaxf(top, wave_m[k][rn]);
-#pragma unroll
-        for (int k = 0; k < kWaves; ++k) {
-            const float mk = wave_m[k][rn], lk = wave_l[k][rn];
-            f[k] = mk == -INFINITY ? (lk == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mk - top);
-            joined += f[k] * lk;
-        }
-        const size_t part = (size_t(unit) * pl.splits + split) * R + r;
-        const float over = joined == 0.f ? 0.f : 1.f / joined;
-        float *y = one_range ? a.out + size_t(token) * a.out_stride + size_t(qh) * dim : ws.o + part * DM;
-#pragma unroll
-        for (uint32_t d = rp * 4; d < DM; d += 64) {
-            f4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < kWaves; ++k) acc += f[k] * *reinterpret_cast<const f4 *>(os + (k * 16 + rn) * kPitch + d);
-            if (!one_range) {
-                if (joined != 0.f) *reinterpret_cast<f4 *>(y + d) = acc;
-            } else if (d < dim) {
-                *reinterpret_cast<f4u *>(y + d) = acc * over;
-            }
-        }
-        if (!one_range && rp == 0) ws.ml[part] = make_float2(top, joined);
+        for (int i = 0; i < 4; ++i)
+            if (poison[d / 8] >> (d % 8 * 4 + i) & 1) o[d][i] = __builtin_nanf("");
     }
+#pragma unroll
+    for (int d = 0; d < VT; ++d) *reinterpret_cast<f4 *>(os + (w * 16 + jn) * kPitch + 16 * d + 4 * jg) = o[d];
+    if (jg == 0) {
+        wave_m[w][jn] = m;
+        wave_l[w][jn] = all;
+    }
+    __syncthreads();
+    // Sixteen threads a row, four dims at a time.
+    const bool real = rn < in_tile;
+    const uint32_t row = t.row0 + rn, token = t.first_token + row / group, qh = head * group + row % group;
+    if (pl.splits > 1 && split == 0 && rp == 0)
+        ws.place[size_t(unit) * R + rn] = one_range || !real ? kNone : token * a.heads + qh;
+    if (!real || (one_range && split > 0)) return;
+    float top = wave_m[0][rn], f[kWaves], joined = 0.f;
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) top = fmaxf(top, wave_m[k][rn]);
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+        const float mk = wave_m[k][rn], lk = wave_l[k][rn];
+        f[k] = mk == -INFINITY ? (lk == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mk - top);
+        joined += f[k] * lk;
+    }
+    const size_t part = (size_t(unit) * pl.splits + split) * R + rn;
+    const float over = joined == 0.f ? 0.f : 1.f / joined;
+    float *y = one_range ? a.out + size_t(token) * a.out_stride + size_t(qh) * dim : ws.o + part * DM;
+#pragma unroll
+    for (uint32_t d = rp * 4; d < DM; d += 64) {
+        f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) acc += f[k] * *reinterpret_cast<const f4 *>(os + (k * 16 + rn) * kPitch + d);
+        if (!one_range) {
+            if (joined != 0.f) *reinterpret_cast<f4 *>(y + d) = acc;
+        } else if (d < dim) {
+            *reinterpret_cast<f4u *>(y + d) = acc * over;
+        }
+    }
+    if (!one_range && rp == 0) ws.ml[part] = make_float2(top, joined);
 }
 
 // Many rows: 128 rows a workgroup, 32 a wave, which keeps its queries' operands
@@ -1079,12 +1050,12 @@ size_t workspace_of(const AttendArgs &a, const AttendPlan &pl) {
     return units * pl.rows * (size_t(pl.splits) * (wide_dim(a.cache.dim) + 2) + 1) * 4;
 }
 
-template <bool BF16, int DM, int NB>
+template <bool BF16, int DM>
 hipError_t launch_rows(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, hipStream_t stream) {
-    const size_t queries = size_t(NB) * (DM / 32) * kTerms<BF16> * 1024;
+    const size_t queries = size_t(DM / 32) * kTerms<BF16> * 1024;
     const size_t joined = size_t(kWaves) * 16 * (DM + 4) * 4;
     const size_t lds = queries > joined ? queries : joined;
-    const auto kernel = attn_rows_kernel<BF16, DM, NB>;
+    const auto kernel = attn_rows_kernel<BF16, DM>;
     if (lds > 65536 - 2048) {
         const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
         if (e != hipSuccess) return e;
@@ -1097,7 +1068,7 @@ template <bool BF16, int DM>
 hipError_t launch_dim(const AttendArgs &a, const AttendPlan &pl, const Partial &ws, hipStream_t stream) {
     hipError_t e;
     if (pl.rows == 16) {
-        e = launch_rows<BF16, DM, 1>(a, pl, ws, stream);
+        e = launch_rows<BF16, DM>(a, pl, ws, stream);
     } else {
         // Three blocks of keys and of values, and bf16's third query terms.
         constexpr size_t lds = 6 * DM * 64 + (BF16 ? kWaves * (DM == 256 ? DM - 32 : DM) * 64 : 0);

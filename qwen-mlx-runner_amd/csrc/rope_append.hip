@@ -33,6 +33,11 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Four FP32 of a row, which need not lie on 16 bytes.
+struct Quad {
+    float x[4];
+};
+
 // What pair i turns by, for token t.
 __device__ __forceinline__ void turn_of(const RopeSpec &r, uint32_t tokens, uint32_t t, uint32_t i, float &c, float &s) {
     uint32_t axis = 0;
@@ -63,8 +68,8 @@ __device__ __forceinline__ void load_unit(const float *x, uint32_t u, const Rope
     const float *pb = halves ? pa + half : pa + V;
     float e[2 * V];
     if constexpr (V == 4) {
-        *reinterpret_cast<float4 *>(e) = *reinterpret_cast<const float4 *>(pa);
-        *reinterpret_cast<float4 *>(e + V) = *reinterpret_cast<const float4 *>(pb);
+        *reinterpret_cast<Quad *>(e) = *reinterpret_cast<const Quad *>(pa);
+        *reinterpret_cast<Quad *>(e + V) = *reinterpret_cast<const Quad *>(pb);
     } else {
 #pragma unroll
         for (int k = 0; k < V; ++k) e[k] = pa[k], e[V + k] = pb[k];
@@ -159,7 +164,7 @@ __device__ __forceinline__ void turns(const RopeSpec &r, uint32_t tokens, uint32
 template <int V>
 __device__ __forceinline__ void store_f32(float *y, uint32_t at, const float *e) {
     if constexpr (V == 4) {
-        *reinterpret_cast<float4 *>(y + at) = *reinterpret_cast<const float4 *>(e);
+        *reinterpret_cast<Quad *>(y + at) = *reinterpret_cast<const Quad *>(e);
     } else {
 #pragma unroll
         for (int k = 0; k < V; ++k) y[at + k] = e[k];
@@ -226,7 +231,7 @@ __device__ __forceinline__ bool slot_of(const PagedCache &c, uint32_t seq, int64
 // Waves [0, tokens * slices): query and key heads, turned. The others: values,
 // one wave a token and head.
 template <int V, int IT, bool BF16>
-__global__ __launch_bounds__(kThreads) void kv_append_rope_kernel(AppendArgs a, Spread sp, bool v_aligned) {
+__global__ __launch_bounds__(kThreads) void kv_append_rope_kernel(AppendArgs a, Spread sp) {
     const uint32_t wave = blockIdx.x * (kThreads / 64) + threadIdx.x / 64, l = threadIdx.x % 64;
     const PagedCache &c = a.cache;
     const uint32_t tokens = c.tokens, dim = c.dim;
@@ -288,13 +293,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_rope_kernel(AppendArgs a, 
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i) {
             if (i >= n) continue;
-            const float *xi = x + size_t(i) * a.v_stride + d0;
-            if (v_aligned) {
-                *reinterpret_cast<float4 *>(e[i]) = *reinterpret_cast<const float4 *>(xi);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) e[i][j] = xi[j];
-            }
+            *reinterpret_cast<Quad *>(e[i]) = *reinterpret_cast<const Quad *>(x + size_t(i) * a.v_stride + d0);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -315,8 +314,6 @@ __global__ __launch_bounds__(kThreads) void kv_append_rope_kernel(AppendArgs a, 
     }
 }
 
-bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-
 // Lanes, units and slices for rows of `heads` heads. A token's heads go to as
 // few waves as still give every CU eight, since each wave works out the
 // token's angles again.
@@ -336,8 +333,7 @@ Spread spread_of(uint32_t dim, uint32_t v, uint32_t tokens, uint32_t heads, cons
 }  // namespace
 
 hipError_t launch_rope_axes(const RopeArgs &a, const DeviceLimits &lim, hipStream_t stream) {
-    const bool wide = a.dim % 8 == 0 && a.rope.rotary % 8 == 0 && a.x_stride % 4 == 0 && a.y_stride % 4 == 0 &&
-                      aligned16(a.x) && aligned16(a.y);
+    const bool wide = a.dim % 8 == 0 && a.rope.rotary % 8 == 0;
     const Spread sp = spread_of(a.dim, wide ? 4 : 1, a.tokens, a.heads, lim);
     const uint64_t waves = uint64_t(a.tokens) * sp.slices;
     const uint32_t blocks = uint32_t((waves + kThreads / 64 - 1) / (kThreads / 64));
@@ -351,21 +347,18 @@ hipError_t launch_rope_axes(const RopeArgs &a, const DeviceLimits &lim, hipStrea
 
 hipError_t launch_kv_append_rope(const AppendArgs &a, const DeviceLimits &lim, hipStream_t stream) {
     const PagedCache &c = a.cache;
-    const bool norms = a.eps == 0.f || (aligned16(a.q_norm) && aligned16(a.k_norm));
-    const bool wide = a.rope.rotary % 8 == 0 && a.k_stride % 4 == 0 && aligned16(a.k) && norms &&
-                      (a.heads == 0 || (a.q_stride % 4 == 0 && a.out_stride % 4 == 0 && aligned16(a.q) && aligned16(a.q_out)));
-    const bool v_aligned = a.v_stride % 4 == 0 && aligned16(a.v);
+    const bool wide = a.rope.rotary % 8 == 0;
     const Spread sp = spread_of(c.dim, wide ? 4 : 1, c.tokens, a.heads + c.kv_heads, lim);
     const uint64_t waves = uint64_t(c.tokens) * (uint64_t(sp.slices) + c.kv_heads);
     const uint32_t blocks = uint32_t((waves + kThreads / 64 - 1) / (kThreads / 64));
     if (wide && c.bf16) {
-        kv_append_rope_kernel<4, 1, true><<<blocks, kThreads, 0, stream>>>(a, sp, v_aligned);
+        kv_append_rope_kernel<4, 1, true><<<blocks, kThreads, 0, stream>>>(a, sp);
     } else if (wide) {
-        kv_append_rope_kernel<4, 1, false><<<blocks, kThreads, 0, stream>>>(a, sp, v_aligned);
+        kv_append_rope_kernel<4, 1, false><<<blocks, kThreads, 0, stream>>>(a, sp);
     } else if (c.bf16) {
-        kv_append_rope_kernel<1, 2, true><<<blocks, kThreads, 0, stream>>>(a, sp, v_aligned);
+        kv_append_rope_kernel<1, 2, true><<<blocks, kThreads, 0, stream>>>(a, sp);
     } else {
-        kv_append_rope_kernel<1, 2, false><<<blocks, kThreads, 0, stream>>>(a, sp, v_aligned);
+        kv_append_rope_kernel<1, 2, false><<<blocks, kThreads, 0, stream>>>(a, sp);
     }
     return hipGetLastError();
 }
