@@ -14,6 +14,7 @@ from __future__ import annotations
 import atexit
 import ctypes as C
 import os
+import struct
 from dataclasses import dataclass
 from pathlib import Path
 from typing import Optional, Sequence
@@ -96,6 +97,7 @@ class FrameTiming:
 
 
 _lib: Optional[C.CDLL] = None
+_encodes: tuple = ()
 _alive = True  # cleared at interpreter exit: no handle is released after that
 
 
@@ -109,7 +111,7 @@ atexit.register(_at_exit)
 
 def lib() -> C.CDLL:
     """Load libqmr_hip.so once; raises if it has not been built."""
-    global _lib
+    global _lib, _encodes
     if _lib is not None:
         return _lib
     path = Path(os.environ.get("QMR_LIB", LIB_PATH))
@@ -177,6 +179,12 @@ def lib() -> C.CDLL:
         fn = getattr(L, name)
         fn.restype = res
         fn.argtypes = args
+    # Command.encode's own function objects, which take the arrays as bytes.
+    encodes = L["qmr_encode"], L["qmr_encode_static"]
+    for fn in encodes:
+        fn.restype = C.c_int
+        fn.argtypes = [vp, C.c_char_p, C.c_char_p, C.c_char_p, sz, C.c_char_p, sz, sz, sz]
+    _encodes = encodes
     _lib = L
     return L
 
@@ -186,9 +194,25 @@ def _check(code: int) -> None:
         raise QmrError(code, lib().qmr_last_error().decode())
 
 
+_structs: dict[tuple[str, int], struct.Struct] = {}
+
+
+def _packed(kind: str, values: Sequence[int]) -> bytes:
+    """Unsigned words ("I": 32 bits, "Q": 64), taken modulo their size. Packing
+    a list at once costs a tenth of a ctypes array filled from Python."""
+    key = (kind, len(values))
+    form = _structs.get(key)
+    if form is None:
+        form = _structs[key] = struct.Struct(f"={len(values)}{kind}")
+    try:
+        return form.pack(*values)
+    except struct.error:
+        mask = 0xFFFFFFFF if kind == "I" else 0xFFFFFFFFFFFFFFFF
+        return form.pack(*[int(v) & mask for v in values])
+
+
 def _u32(params: Sequence[int]):
-    arr = (C.c_uint32 * max(len(params), 1))(*[int(p) & 0xFFFFFFFF for p in params])
-    return arr
+    return (C.c_uint32 * max(len(params), 1)).from_buffer_copy(_packed("I", params) or bytes(4))
 
 
 def _s(v: Optional[str]) -> Optional[bytes]:
@@ -313,14 +337,14 @@ class Command:
         static_scratch=True calls qmr_encode_static instead: the same launch
         with its workspace in the GPU's static scratch, allocating nothing."""
         n = len(buffers)
-        bufs = (C.c_void_p * max(n, 1))(*[b.handle.value for b in buffers])
         offs = None
         if offsets is not None:
             if len(offsets) != n:
                 raise QmrError(QMR_ERR_INVALID, f"{name}: offset count must match buffers")
-            offs = (C.c_size_t * max(n, 1))(*[int(o) for o in offsets])
-        entry = lib().qmr_encode_static if static_scratch else lib().qmr_encode
-        _check(entry(self._h, name.encode(), bufs, offs, n, _u32(params), len(params), threads, group_size))
+            offs = _packed("Q", offsets)
+        bufs = _packed("Q", [b._h.value or 0 for b in buffers])
+        lib()
+        _check(_encodes[bool(static_scratch)](self._h, name.encode(), bufs, offs, n, _packed("I", params), len(params), threads, group_size))
 
     def mark(self) -> int:
         idx = C.c_int()
