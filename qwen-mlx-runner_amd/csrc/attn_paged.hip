@@ -275,11 +275,19 @@ __device__ __forceinline__ u4 ones_of(int first, int lo, int hi) {
     return halves_of(first, lo, hi) & kOne<BF16>;
 }
 
-// Few rows: 16 rows a workgroup, every wave all of them over its own
-// blocks of the range (block w, w + 4, ..), straight from memory into operand
-// registers, whole lines at a time; nothing is shared but the queries, which
-// wait in LDS as operands. The waves' m, l and O
-// are joined through LDS at the end.
+// Few rows: 16 rows a workgroup, every wave all of them over its own blocks of
+// the range (block w, w + 4, ..), straight from memory into operand registers,
+// whole lines at a time; nothing is shared but the queries, which wait in LDS
+// as operands. The waves' m, l and O are joined through LDS at the end. A wave
+// holds a block of keys and one of values (32 KB at 256 dims), a CU two
+// workgroups: 256 KB on their way, more than HBM needs. Sharing a block in LDS
+// between the waves, or 32 rows a workgroup, had fewer in flight or spilled.
+// Memory bounds it: 32 sequences of 8 heads of 128 over up to 8001 keys (521
+// MB) 104 us, 5.0 TB/s (repeated, so in part from the last-level cache; a large
+// copy reaches 4.8); one token of 24/4 heads of 256 over 32768 (134 MB) 28 us
+// with the join, 4.7 TB/s; over 1001 keys (4 MB) 10.9 us, of which the join
+// takes 3 and the first workgroup's chain of dependent steps (its sequence, its
+// page, keys and queries, products, waves joined) the rest.
 template <bool BF16, int DM>
 __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
     constexpr int R = 16, T = kTerms<BF16>, KS = DM / 32, VT = DM / 16;
@@ -539,11 +547,16 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
     all += __shfl_xor(all, 16);
     all += __shfl_xor(all, 32);
     __syncthreads();
+    uint32_t poisoned = poison[0];
 #pragma unroll
-    for (int d = 0; d < VT; ++d) {
+    for (int d = 8; d < VT; d += 8) poisoned |= poison[d / 8];
+    if (__ballot(poisoned != 0) != 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (poison[d / 8] >> (d % 8 * 4 + i) & 1) o[d][i] = __builtin_nanf("");
+        for (int d = 0; d < VT; ++d) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (poison[d / 8] >> (d % 8 * 4 + i) & 1) o[d][i] = __builtin_nanf("");
+        }
     }
 #pragma unroll
     for (int d = 0; d < VT; ++d) *reinterpret_cast<f4 *>(os + (w * 16 + jn) * kPitch + 16 * d + 4 * jg) = o[d];
@@ -1104,21 +1117,24 @@ hipError_t launch_type(const AttendArgs &a, const AttendPlan &pl, const Partial 
 // The plan is the cheapest of an estimate over both kernels and their numbers
 // of key ranges, from sizes alone. Fitted to MI355X timings (us), per dims 64,
 // 128 and 256, bf16 and f16:
-//   rows kernel  a workgroup starts and ends in 4 and takes `chain` for its four
-//                waves' blocks; a CU works a tile of 16 rows against a block off
-//                in `each` whatever is resident, and starts a tile in 2; keys and values come in at
-//                5.3 TB/s from 128 workgroups on, at half that from 37
+//   rows kernel  a workgroup takes `start`, `chain` for each round of its four
+//                waves' blocks, and less by `fewer` where waves have none, as a
+//                CU's cache then brings less; a CU works a tile of 16 rows
+//                against a block off in `each` whatever is resident, and starts
+//                a tile in 2; keys and values come in at 5.3 TB/s from 128
+//                workgroups on, at half that from 37
 //   tile kernel  10 for start and end, `chain` a block alone, `each` a block of
 //                128 rows when the CU's two workgroups (one of 256 dims) overlap
 //   join         3, and each range's rows written and read once
 // Both sides where it decides, rows / tile kernel: 64 tokens of 24 heads of 256
 // over 4064 keys 36 / 47 us, 150 over 4150 61 / 76, 512 over 16512 (bf16) 640 /
-// 580; one prompt of 32 heads of 128 (f16), 500 tokens 19 / 25, 1000 43 / 43,
-// 2000 118 / 88, 4100 389 / 282.
+// 540; one prompt of 32 heads of 128 (f16), 500 tokens 18 / 25, 1000 43 / 40,
+// 2000 118 / 84, 4100 389 / 267.
 // Ranges, in the rows kernel: one token of 24/4 heads of 256 over 32768 keys in
-// 8, 16, 32, 64 and 128: 52, 35, 30, 31.6 and 32 us; 32 sequences of 8 heads of
-// 128 over up to 8001 in 1, 2 and 4: 105, 113 and 122; one over 600 keys in 1, 2
-// and 5: 9.5, 11.4 and 10.4.
+// 8, 16, 32, 64 and 128: 52, 35, 30, 31.6 and 32 us; over 4001 in 16, 32 and 64:
+// 15.0, 13.7 and 15.4; over 1001 in 1, 8, 16 and 32 (of one block): 18.3, 11.7,
+// 11.3 and 10.9; over 101 in 1 and 4: 7.8 and 11; 32 sequences of 8 heads of 128
+// over up to 8001 in 1, 2 and 4: 105, 113 and 122.
 AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t workspace_limit, uint32_t force_rows,
                        uint32_t force_splits) {
     const PagedCache &c = a.cache;
@@ -1126,7 +1142,7 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
     // Sequences with a row: at most n. Each takes whole tiles.
     const uint64_t n = c.seqs < c.tokens ? c.seqs : c.tokens;
     const int wide = wide_dim(c.dim) == 64 ? 0 : wide_dim(c.dim) == 128 ? 1 : 2;
-    static constexpr double kRowsChain[3] = {0.45, 0.75, 1.6};
+    static constexpr double kRowsStart[3] = {4.5, 5.1, 6.3}, kRowsChain[3] = {0.39, 0.65, 1.45}, kRowsFewer[3] = {0.03, 0.07, 0.17};
     static constexpr double kTileChain[2][3] = {{0.95, 1.2, 2.0}, {1.0, 1.4, 2.4}};
     static constexpr double kRowsEach[2][3] = {{0.07, 0.19, 0.33}, {0.09, 0.21, 0.42}};
     static constexpr double kTileEach[2][3] = {{1.1, 1.05, 2.1}, {1.2, 1.45, 2.6}};
@@ -1146,9 +1162,11 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
         // first row to those of its last.
         const uint64_t across = (rows + group - 1) / group + kBlock;
         const uint64_t keys = a.window && a.window + across < a.max_keys ? a.window + across : a.max_keys;
-        // A range gives each wave of the rows kernel a block at least.
+        // A range is a block for each wave, or several; in the rows kernel also
+        // one or two blocks, which come through a CU's own cache the sooner.
         const uint64_t units = uint64_t(pl.tiles) * c.kv_heads, step = kWaves * kBlock;
-        const uint64_t most = (keys + step - 1) / step < kMaxSplits ? (keys + step - 1) / step : kMaxSplits;
+        const uint64_t least_keys = rows == 16 ? kBlock : step;
+        const uint64_t most = std::min<uint64_t>((keys + least_keys - 1) / least_keys, kMaxSplits);
         // Workgroups go to the eight XCDs in turn: tiles that read the same keys
         // share one's L2 if their distance is a multiple of eight (six tokens
         // of 24/4 heads over 16006 keys in 16, 18, 20 and 21 ranges: 25.0, 25.5,
@@ -1158,7 +1176,10 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
         uint64_t before = 0;
         const uint64_t first = force_splits == 0 ? 1 : std::min<uint64_t>(force_splits, most);
         for (uint64_t s = first; s <= (force_splits == 0 ? most : first); s += s < 32 ? 1 : s / 8) {
-            pl.keys = uint32_t(((keys + s - 1) / s + step - 1) / step * step);
+            const uint64_t even = (keys + s - 1) / s;
+            pl.keys = uint32_t(rows == 16 && even <= kBlock       ? kBlock
+                               : rows == 16 && even <= 2 * kBlock ? 2 * kBlock
+                                                                  : (even + step - 1) / step * step);
             pl.splits = uint32_t((keys + pl.keys - 1) / pl.keys);
             if (pl.splits == before) continue;
             const uint64_t streams = pl.splits * uint64_t(c.kv_heads);
@@ -1172,7 +1193,8 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
             if (rows == 16) {
                 const double moved = double(n) * c.kv_heads * keys * c.dim * 4 / 5.3e6;
                 const double fed = std::max(1.0, 0.6 + 51 / (double(units) * pl.splits));
-                const double alone = 4 + blocks / kWaves * kRowsChain[wide];
+                const double idle = std::max(0.0, kWaves - blocks);
+                const double alone = kRowsStart[wide] + std::ceil(blocks / kWaves) * kRowsChain[wide] - idle * idle * kRowsFewer[wide];
                 us = std::max({alone * (1 + 0.8 * (rounds - 1) * share), work * kRowsEach[c.bf16][wide] + 2 * double(units) * pl.splits / cus, moved * fed});
             } else {
                 us = std::max({10 + blocks * kTileChain[c.bf16][wide], rounds * (10 + blocks * share * kTileChain[c.bf16][wide]),
