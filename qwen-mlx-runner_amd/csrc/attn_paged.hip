@@ -280,8 +280,8 @@ __device__ __forceinline__ u4 ones_of(int first, int lo, int hi) {
 // whole lines at a time; nothing is shared but the queries, which wait in LDS
 // as operands. The waves' m, l and O are joined through LDS at the end. A wave
 // holds a block of keys and one of values (32 KB at 256 dims), a CU two
-// workgroups: 256 KB on their way, more than HBM needs. Sharing a block in LDS
-// between the waves, or 32 rows a workgroup, had fewer in flight or spilled.
+// workgroups: 256 KB on their way, more than HBM needs. 32 rows a workgroup
+// spilled registers.
 // Memory bounds it: 32 sequences of 8 heads of 128 over up to 8001 keys (521
 // MB) 104 us, 5.0 TB/s (repeated, so in part from the last-level cache; a large
 // copy reaches 4.8); one token of 24/4 heads of 256 over 32768 (134 MB) 28 us
@@ -610,6 +610,13 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
 // steps before (scheduling barriers keep it). Blocks go from memory straight to
 // a ring of three in LDS, two iterations ahead of their use, with one barrier
 // a block.
+//
+// The matrix cores bound it, at the card's power: their clock falls as they
+// fill. A prompt of 4100 tokens of 32/8 heads of 128 (f16) takes 266 us, 518
+// TFLOP/s of the formula and 1036 of the instructions, as each operand of FP32
+// is two terms; 512 tokens of 24/4 heads of 256 over 16513 keys (bf16, three
+// terms) 529 us, 387 and 1160. A large matrix product reaches 1166 in f16 and
+// 1227 in bf16.
 template <bool BF16, int DM>
 __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
     constexpr int R = 32 * kWaves, T = kTerms<BF16>, KS = DM / 16, VT = DM / 32;
@@ -987,7 +994,8 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 
 // Adds the ranges of a row up. WIDE: a workgroup a row, every wave a quarter of
 // the ranges, whose loads depend on nothing and are all in flight at once. For
-// few ranges a wave a row.
+// few ranges a wave a row (24 rows of 256 dims, 16 ranges: 11.4 us with the rows
+// kernel, 11.8 as WIDE). Of its 3 to 4 us most is one more launch.
 template <int DM, bool WIDE>
 __global__ __launch_bounds__(kThreads) void attn_join_kernel(AttendArgs a, AttendPlan pl, Partial ws, uint32_t rows) {
     constexpr int E = DM / 64, W = WIDE ? kWaves : 1;
@@ -1127,9 +1135,9 @@ hipError_t launch_type(const AttendArgs &a, const AttendPlan &pl, const Partial 
 //                128 rows when the CU's two workgroups (one of 256 dims) overlap
 //   join         3, and each range's rows written and read once
 // Both sides where it decides, rows / tile kernel: 64 tokens of 24 heads of 256
-// over 4064 keys 36 / 47 us, 150 over 4150 61 / 76, 512 over 16512 (bf16) 640 /
-// 540; one prompt of 32 heads of 128 (f16), 500 tokens 18 / 25, 1000 43 / 40,
-// 2000 118 / 84, 4100 389 / 267.
+// over 4064 keys (bf16) 38 / 45 us, 150 over 4150 60 / 71, 512 over 16512 552 /
+// 529; one prompt of 32 heads of 128 (f16), 500 tokens 18 / 25, 1000 40 / 42,
+// 2000 111 / 82, 4100 365 / 266.
 // Ranges, in the rows kernel: one token of 24/4 heads of 256 over 32768 keys in
 // 8, 16, 32, 64 and 128: 52, 35, 30, 31.6 and 32 us; over 4001 in 16, 32 and 64:
 // 15.0, 13.7 and 15.4; over 1001 in 1, 8, 16 and 32 (of one block): 18.3, 11.7,
