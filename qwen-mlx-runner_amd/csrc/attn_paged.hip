@@ -998,56 +998,63 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 // kernel, 11.8 as WIDE). Of its 3 to 4 us most is one more launch.
 template <int DM, bool WIDE>
 __global__ __launch_bounds__(kThreads) void attn_join_kernel(AttendArgs a, AttendPlan pl, Partial ws, uint32_t rows) {
-    constexpr int E = DM / 64, W = WIDE ? kWaves : 1;
+    constexpr int E = DM / 64, kFirst = 8;
     typedef float fe __attribute__((ext_vector_type(E)));
-    __shared__ float weight[WIDE ? kMaxSplits : kWaves * kFewSplits], part_o[kWaves][WIDE ? DM : 1], part_l[kWaves];
+    __shared__ float weight[kWaves][WIDE ? kMaxSplits : kFewSplits], part_o[kWaves][WIDE ? DM : 1];
     const uint32_t l = threadIdx.x % 64, w = threadIdx.x / 64;
     const uint32_t at_row = WIDE ? blockIdx.x : blockIdx.x * kWaves + w;
     if (at_row >= rows) return;
-    const uint32_t place = ws.place[at_row];
-    if (place == kNone) return;
-    float *weights = WIDE ? weight : weight + w * kFewSplits;
     const uint32_t unit = at_row / pl.rows, r = at_row % pl.rows;
     const size_t first = size_t(unit) * pl.splits * pl.rows + r;
-    float top = -INFINITY, all = 0.f;
-    for (uint32_t s = l; s < pl.splits; s += 64) top = fmaxf(top, ws.ml[first + size_t(s) * pl.rows].x);
+    // What the wave adds first is loaded before its weights are known.
+    const uint32_t from = WIDE ? w : 0, by = WIDE ? kWaves : 1;
+    const fe *o = reinterpret_cast<const fe *>(ws.o + first * DM) + l;
+    auto part_of = [&](uint32_t s) { return o[size_t(s) * pl.rows * (DM / E)]; };
+    auto ml_of = [&](uint32_t s) { return ws.ml[first + size_t(s) * pl.rows]; };
+    const uint32_t place = ws.place[at_row];
+    const float2 own = l < pl.splits ? ml_of(l) : make_float2(-INFINITY, 0.f);
+    fe ahead[kFirst];
+#pragma unroll
+    for (uint32_t i = 0; i < kFirst; ++i) ahead[i] = part_of(min(from + i * by, pl.splits - 1));
+
+    float top = own.x, all = 0.f;
+    for (uint32_t s = l + 64; s < pl.splits; s += 64) top = fmaxf(top, ml_of(s).x);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
     // A range that saw nothing (its sum is 0) left no row.
-    for (uint32_t s = WIDE ? threadIdx.x : l; s < pl.splits; s += W * 64) {
-        const float2 ml = ws.ml[first + size_t(s) * pl.rows];
+    auto weigh = [&](uint32_t s, float2 ml) {
         const float f = ml.y == 0.f ? 0.f : ml.x == -INFINITY ? 1.f : exp2f(ml.x - top);
-        weights[s] = ml.y == 0.f ? -1.f : f;
+        weight[w][s] = ml.y == 0.f ? -1.f : f;
         all += f * ml.y;
-    }
+    };
+    if (l < pl.splits) weigh(l, own);
+    for (uint32_t s = l + 64; s < pl.splits; s += 64) weigh(s, ml_of(s));
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
-    if constexpr (WIDE) {
-        if (l == 0) part_l[w] = all;
-        __syncthreads();
-    } else {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
     fe acc = {};
-    const fe *o = reinterpret_cast<const fe *>(ws.o + first * DM) + l;
-#pragma unroll 8
-    for (uint32_t s = WIDE ? w : 0; s < pl.splits; s += W) {
-        const fe x = o[size_t(s) * pl.rows * (DM / E)];
-        const float f = weights[s];
+    auto add = [&](uint32_t s, fe x) {
+        const float f = weight[w][s];
         if (f >= 0.f || f != f) acc += f * x;
-    }
-    float *y = a.out + size_t(place / a.heads) * a.out_stride + size_t(place % a.heads) * a.cache.dim;
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kFirst; ++i)
+        if (from + i * by < pl.splits) add(from + i * by, ahead[i]);
+#pragma unroll 8
+    for (uint32_t s = from + kFirst * by; s < pl.splits; s += by) add(s, part_of(s));
+    const float f = all == 0.f ? 0.f : 1.f / all;
     if constexpr (WIDE) {
         *reinterpret_cast<fe *>(&part_o[w][l * E]) = acc;
         __syncthreads();
-        all = part_l[0] + part_l[1] + part_l[2] + part_l[3];
-        const float f = all == 0.f ? 0.f : 1.f / all;
+    }
+    if (place == kNone) return;
+    float *y = a.out + size_t(place / a.heads) * a.out_stride + size_t(place % a.heads) * a.cache.dim;
+    if constexpr (WIDE) {
         const uint32_t d = threadIdx.x;
         if (d < a.cache.dim) y[d] = (part_o[0][d] + part_o[1][d] + part_o[2][d] + part_o[3][d]) * f;
     } else {
-        const float f = all == 0.f ? 0.f : 1.f / all;
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (l * E + e < a.cache.dim) y[l * E + e] = acc[e] * f;
