@@ -57,7 +57,13 @@ __device__ __forceinline__ void turn_of(const RopeSpec &r, uint32_t tokens, uint
 // V at `first` and V at `second` of the row (halves), or 2V in sequence.
 template <int V, int IT>
 struct Part {
-    float a[IT][V], b[IT][V], c[IT][V], s[IT][V];
+    float a[IT][V], b[IT][V];
+};
+
+// What those pairs turn by.
+template <int V, int IT>
+struct Turns {
+    float c[IT][V], s[IT][V];
 };
 
 template <int V>
@@ -102,62 +108,66 @@ __device__ __forceinline__ void store_unit(uint32_t u, const RopeSpec &r, const 
     f(halves ? at + half : at + V, e + V);
 }
 
-// One head row through a group of `lanes` lanes: load, norm, turn.
+// One head row for a group of `lanes` lanes.
 template <int V, int IT>
-__device__ __forceinline__ void turn_row(const float *x, const float *norm, float eps, uint32_t dim, const RopeSpec &r,
-                                         uint32_t lane, uint32_t lanes, uint32_t units, Part<V, IT> &p) {
-    float sum = 0.f;
+__device__ __forceinline__ void load_row(const float *x, const RopeSpec &r, uint32_t lane, uint32_t lanes, uint32_t units,
+                                         Part<V, IT> &p) {
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
         const uint32_t u = lane + k * lanes;
 #pragma unroll
         for (int j = 0; j < V; ++j) p.a[k][j] = p.b[k][j] = 0.f;
-        if (u < units) {
-            load_unit<V>(x, u, r, p.a[k], p.b[k]);
+        if (u < units) load_unit<V>(x, u, r, p.a[k], p.b[k]);
+    }
+}
+
+// Its RMS norm, with the weights of the lane's own elements.
+template <int V, int IT>
+__device__ __forceinline__ void norm_row(const Part<V, IT> &weights, float eps, uint32_t dim, uint32_t lanes, Part<V, IT> &p) {
+    float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum += p.a[k][j] * p.a[k][j] + p.b[k][j] * p.b[k][j];
+    for (int k = 0; k < IT; ++k) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += p.a[k][j] * p.a[k][j] + p.b[k][j] * p.b[k][j];
+    }
+    for (uint32_t d = 1; d < lanes; d *= 2) sum += __shfl_xor(sum, d);
+    const float f = 1.f / sqrtf(sum / float(dim) + eps);
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            p.a[k][j] = p.a[k][j] * f * weights.a[k][j];
+            p.b[k][j] = p.b[k][j] * f * weights.b[k][j];
         }
     }
-    if (eps > 0.f) {
-        for (uint32_t d = 1; d < lanes; d *= 2) sum += __shfl_xor(sum, d);
-        const float f = 1.f / sqrtf(sum / float(dim) + eps);
-#pragma unroll
-        for (int k = 0; k < IT; ++k) {
-            const uint32_t u = lane + k * lanes;
-            if (u < units) {
-                float wa[V], wb[V];
-                load_unit<V>(norm, u, r, wa, wb);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    p.a[k][j] = p.a[k][j] * f * wa[j];
-                    p.b[k][j] = p.b[k][j] * f * wb[j];
-                }
-            }
-        }
-    }
+}
+
+template <int V, int IT>
+__device__ __forceinline__ void turn_row(const RopeSpec &r, uint32_t lane, uint32_t lanes, const Turns<V, IT> &turns,
+                                         Part<V, IT> &p) {
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
         if ((lane + k * lanes) * V >= r.rotary / 2) continue;  // passes as it is, infinities too
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float a = p.a[k][j], b = p.b[k][j];
-            p.a[k][j] = a * p.c[k][j] - b * p.s[k][j];
-            p.b[k][j] = b * p.c[k][j] + a * p.s[k][j];
+            p.a[k][j] = a * turns.c[k][j] - b * turns.s[k][j];
+            p.b[k][j] = b * turns.c[k][j] + a * turns.s[k][j];
         }
     }
 }
 
 template <int V, int IT>
-__device__ __forceinline__ void turns(const RopeSpec &r, uint32_t tokens, uint32_t t, uint32_t lane, uint32_t lanes,
-                                      uint32_t units, Part<V, IT> &p) {
+__device__ __forceinline__ void turns_of(const RopeSpec &r, uint32_t tokens, uint32_t t, uint32_t lane, uint32_t lanes,
+                                         Turns<V, IT> &turns) {
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
         const uint32_t u = lane + k * lanes;
 #pragma unroll
-        for (int j = 0; j < V; ++j) p.c[k][j] = 1.f, p.s[k][j] = 0.f;
+        for (int j = 0; j < V; ++j) turns.c[k][j] = 1.f, turns.s[k][j] = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (u * V < r.rotary / 2) turn_of(r, tokens, t, u * V + j, p.c[k][j], p.s[k][j]);
+            if (u * V < r.rotary / 2) turn_of(r, tokens, t, u * V + j, turns.c[k][j], turns.s[k][j]);
     }
 }
 
@@ -176,6 +186,7 @@ __device__ __forceinline__ void store_f32(float *y, uint32_t at, const float *e)
 // token are worked out once a group.
 struct Spread {
     uint32_t lanes, units, heads_each, slices;  // slices: waves of one token
+    uint32_t span = 1;                          // tokens of a wave of values
 };
 
 // Memory bounds it: 4352 tokens of 16 heads of 72 (40 MB) 8.7 us, 4.6 TB/s, as
@@ -186,14 +197,15 @@ __global__ __launch_bounds__(kThreads) void rope_axes_kernel(RopeArgs a, Spread 
     const uint32_t t = wave / sp.slices;
     if (t >= a.tokens) return;
     const uint32_t group = l / sp.lanes, lane = l % sp.lanes, groups = 64 / sp.lanes;
-    Part<V, IT> p;
-    turns<V, IT>(a.rope, a.tokens, t, lane, sp.lanes, sp.units, p);
+    Turns<V, IT> turns;
+    turns_of<V, IT>(a.rope, a.tokens, t, lane, sp.lanes, turns);
     const uint32_t h0 = (wave % sp.slices) * sp.heads_each * groups + group;
     for (uint32_t k = 0; k < sp.heads_each; ++k) {
         const uint32_t h = h0 + k * groups;
         if (h >= a.heads) break;
-        turn_row<V, IT>(a.x + size_t(t) * a.x_stride + size_t(h) * a.dim, nullptr, 0.f, a.dim, a.rope, lane, sp.lanes,
-                        sp.units, p);
+        Part<V, IT> p;
+        load_row<V, IT>(a.x + size_t(t) * a.x_stride + size_t(h) * a.dim, a.rope, lane, sp.lanes, sp.units, p);
+        turn_row<V, IT>(a.rope, lane, sp.lanes, turns, p);
         float *y = a.y + size_t(t) * a.y_stride + size_t(h) * a.dim;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
@@ -218,7 +230,7 @@ __device__ __forceinline__ void place_of(const PagedCache &c, uint32_t t, uint32
     pos = -1;
     end = t + 1;
     if (seq >= c.seqs || c.starts[seq] > t) return;
-    end = c.starts[seq + 1] < c.tokens ? c.starts[seq + 1] : c.tokens;
+    end = max(min(c.starts[seq + 1], c.tokens), t + 1);  // past t whatever the starts hold
     pos = int64_t(c.lengths[seq]) - int64_t(c.starts[seq + 1] - t);
 }
 
@@ -230,14 +242,47 @@ __device__ __forceinline__ bool slot_of(const PagedCache &c, uint32_t seq, int64
     return page < c.pages;
 }
 
+// Slots first..first+n-1 of the value chunks at `to` from tokens t..t+n-1.
+template <bool BF16>
+__device__ __forceinline__ void append_values(const AppendArgs &a, uint16_t *to, uint32_t first, uint32_t t, uint32_t h, uint32_t n) {
+    const uint32_t dim = a.cache.dim;
+    const float *x = a.v + size_t(t) * a.v_stride + size_t(h) * dim;
+    for (uint32_t d0 = threadIdx.x % 64 * 4; d0 < dim; d0 += 256) {
+        float e[8][4];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            if (i >= n) continue;
+            *reinterpret_cast<Quad *>(e[i]) = *reinterpret_cast<const Quad *>(x + size_t(i) * a.v_stride + d0);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint16_t *chunk = to + size_t(d0 + j) * 8;
+            if (n == 8) {
+                uint4 w;
+                w.x = attn::half_bits<BF16>(e[0][j]) | uint32_t(attn::half_bits<BF16>(e[1][j])) << 16;
+                w.y = attn::half_bits<BF16>(e[2][j]) | uint32_t(attn::half_bits<BF16>(e[3][j])) << 16;
+                w.z = attn::half_bits<BF16>(e[4][j]) | uint32_t(attn::half_bits<BF16>(e[5][j])) << 16;
+                w.w = attn::half_bits<BF16>(e[6][j]) | uint32_t(attn::half_bits<BF16>(e[7][j])) << 16;
+                *reinterpret_cast<uint4 *>(chunk) = w;
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    if (i < n) chunk[first + i] = attn::half_bits<BF16>(e[i][j]);
+            }
+        }
+    }
+}
+
 // Waves [0, tokens * slices): query and key heads, turned. The others: values,
-// one wave a token and head.
+// one wave `span` tokens and a head.
 //
-// 2011 tokens of 24/4 heads of 256 with norms (124 MB) 30 us, 4.1 TB/s of a
-// copy's 4.8: the angles, norms and layouts take vector instructions beside the
-// stream. Loading a row before the last one is turned made it 34: registers. One
-// token 5.2 us, 48 of 32/8 heads of 128 4.3: a launch and its chain of loads
-// (the token's sequence, its length, its page).
+// 2011 tokens of 24/4 heads of 256 with norms (124 MB) 36 us, 3.4 TB/s, and 26
+// from the last-level cache; a large copy reaches 4.8 and the rotation alone 4.3
+// at this size: angles, norms and layouts take vector instructions beside the
+// stream. With the norms' weights loaded for each row 41 us, a wave of values a
+// token 38, a row loaded before the last one is turned 41. One token 5.5 us, 48
+// of 32/8 heads of 128 4.2: a launch and its chain of loads (the token's
+// sequence, its length, its page).
 template <int V, int IT, bool BF16>
 __global__ __launch_bounds__(kThreads) void kv_append_rope_kernel(AppendArgs a, Spread sp) {
     const uint32_t wave = blockIdx.x * (kThreads / 64) + threadIdx.x / 64, l = threadIdx.x % 64;
@@ -248,19 +293,26 @@ __global__ __launch_bounds__(kThreads) void kv_append_rope_kernel(AppendArgs a, 
     if (wave < tokens * sp.slices) {
         const uint32_t t = wave / sp.slices;
         const uint32_t group = l / sp.lanes, lane = l % sp.lanes, groups = 64 / sp.lanes;
+        const uint32_t h0 = (wave % sp.slices) * sp.heads_each * groups + group, heads = a.heads + c.kv_heads;
+        Part<V, IT> q_norm, k_norm;
+        if (a.eps > 0.f) {
+            load_row<V, IT>(a.q_norm, a.rope, lane, sp.lanes, sp.units, q_norm);
+            load_row<V, IT>(a.k_norm, a.rope, lane, sp.lanes, sp.units, k_norm);
+        }
         place_of(c, t, seq, pos, end);
         const bool kept = slot_of(c, seq, pos, page, slot);
-        Part<V, IT> p;
-        turns<V, IT>(a.rope, tokens, t, lane, sp.lanes, sp.units, p);
-        const uint32_t h0 = (wave % sp.slices) * sp.heads_each * groups + group;
+        Turns<V, IT> turns;
+        turns_of<V, IT>(a.rope, tokens, t, lane, sp.lanes, turns);
         for (uint32_t k = 0; k < sp.heads_each; ++k) {
             const uint32_t h = h0 + k * groups;
-            if (h >= a.heads + c.kv_heads) break;
+            if (h >= heads) break;
             const bool key = h >= a.heads;
             const uint32_t kh = h - a.heads;
-            const float *x = key ? a.k + size_t(t) * a.k_stride + size_t(kh) * dim
-                                 : a.q + size_t(t) * a.q_stride + size_t(h) * dim;
-            turn_row<V, IT>(x, key ? a.k_norm : a.q_norm, a.eps, dim, a.rope, lane, sp.lanes, sp.units, p);
+            Part<V, IT> p;
+            load_row<V, IT>(key ? a.k + size_t(t) * a.k_stride + size_t(kh) * dim : a.q + size_t(t) * a.q_stride + size_t(h) * dim,
+                            a.rope, lane, sp.lanes, sp.units, p);
+            if (a.eps > 0.f) norm_row<V, IT>(key ? k_norm : q_norm, a.eps, dim, sp.lanes, p);
+            turn_row<V, IT>(a.rope, lane, sp.lanes, turns, p);
             float *y = a.q_out + size_t(t) * a.out_stride + size_t(h) * dim;
             uint16_t *row = c.k + attn::key_row(c, page, kh, slot);
 #pragma unroll
@@ -287,45 +339,24 @@ __global__ __launch_bounds__(kThreads) void kv_append_rope_kernel(AppendArgs a, 
         }
         return;
     }
-    const uint32_t at = wave - tokens * sp.slices;
-    const uint32_t t = at / c.kv_heads, h = at % c.kv_heads;
-    if (t >= tokens) return;
-    place_of(c, t, seq, pos, end);
-    // One wave leads a chunk: its first slot's, or the first new token's.
-    if (pos < 0 || (pos % 8 != 0 && t != c.starts[seq]) || !slot_of(c, seq, pos, page, slot)) return;
-    const uint32_t n = min(8 - slot % 8, end - t);
-    uint16_t *to = c.v + attn::value_chunk(c, page, h, slot);
-    const float *x = a.v + size_t(t) * a.v_stride + size_t(h) * dim;
-    for (uint32_t d0 = l * 4; d0 < dim; d0 += 256) {
-        float e[8][4];
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-            if (i >= n) continue;
-            *reinterpret_cast<Quad *>(e[i]) = *reinterpret_cast<const Quad *>(x + size_t(i) * a.v_stride + d0);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint16_t *chunk = to + size_t(d0 + j) * 8;
-            if (n == 8) {
-                uint4 w;
-                w.x = attn::half_bits<BF16>(e[0][j]) | uint32_t(attn::half_bits<BF16>(e[1][j])) << 16;
-                w.y = attn::half_bits<BF16>(e[2][j]) | uint32_t(attn::half_bits<BF16>(e[3][j])) << 16;
-                w.z = attn::half_bits<BF16>(e[4][j]) | uint32_t(attn::half_bits<BF16>(e[5][j])) << 16;
-                w.w = attn::half_bits<BF16>(e[6][j]) | uint32_t(attn::half_bits<BF16>(e[7][j])) << 16;
-                *reinterpret_cast<uint4 *>(chunk) = w;
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    if (i < n) chunk[slot % 8 + i] = attn::half_bits<BF16>(e[i][j]);
-            }
-        }
+    const uint32_t at = wave - tokens * sp.slices, h = at % c.kv_heads;
+    uint32_t t = at / c.kv_heads * sp.span;
+    const uint32_t last = min(t + sp.span, tokens);
+    while (t < last) {
+        place_of(c, t, seq, pos, end);
+        const uint32_t in_chunk = uint32_t(pos) % 8;
+        // A chunk's first slot leads it, or the first new token.
+        if (pos >= 0 && (in_chunk == 0 || t == c.starts[seq]) && slot_of(c, seq, pos, page, slot))
+            append_values<BF16>(a, c.v + attn::value_chunk(c, page, h, slot), slot % 8, t, h, min(8 - in_chunk, end - t));
+        t = pos < 0 ? t + 1 : min(t + 8 - in_chunk, end);
     }
 }
 
 // Lanes, units and slices for rows of `heads` heads. A token's heads go to as
 // few waves as still give every CU eight, since each wave works out the
-// token's angles again (2011 tokens as above with four, eight, 16 and 32: 33.5,
-// 31.8, 31.5 and 32.3 us; 4352 of 16 heads of 72 10.7, 10.7, 10.7 and 12.4).
+// token's angles again (2011 tokens as above with four, eight and 16: 34.6, 35.9
+// and 36.3 us; the rotation of 4352 of 16 heads of 72 8.7 with each, 10.2 with
+// 32).
 Spread spread_of(uint32_t dim, uint32_t v, uint32_t tokens, uint32_t heads, const DeviceLimits &lim) {
     Spread s;
     s.units = dim / (2 * v);
@@ -357,8 +388,10 @@ hipError_t launch_rope_axes(const RopeArgs &a, const DeviceLimits &lim, hipStrea
 hipError_t launch_kv_append_rope(const AppendArgs &a, const DeviceLimits &lim, hipStream_t stream) {
     const PagedCache &c = a.cache;
     const bool wide = a.rope.rotary % 8 == 0;
-    const Spread sp = spread_of(c.dim, wide ? 4 : 1, c.tokens, a.heads + c.kv_heads, lim);
-    const uint64_t waves = uint64_t(c.tokens) * (uint64_t(sp.slices) + c.kv_heads);
+    Spread sp = spread_of(c.dim, wide ? 4 : 1, c.tokens, a.heads + c.kv_heads, lim);
+    // One token of eight leads a chunk where sequences have many.
+    sp.span = c.tokens / 8 >= c.seqs ? 8 : 1;
+    const uint64_t waves = uint64_t(c.tokens) * sp.slices + uint64_t((c.tokens + sp.span - 1) / sp.span) * c.kv_heads;
     const uint32_t blocks = uint32_t((waves + kThreads / 64 - 1) / (kThreads / 64));
     if (wide && c.bf16) {
         kv_append_rope_kernel<4, 1, true><<<blocks, kThreads, 0, stream>>>(a, sp);
