@@ -122,7 +122,7 @@ int qmr_command_begin(qmr_device *device, qmr_command **out);
  * `name` is a reference kernel name (matvec_affine, matvec_affine_bf16,
  * matmul_affine, matmul_affine_bf16, embed_affine, embed_affine_bf16,
  * matvec_f16, matmul_f16, embed_f16, copy_f32) or one of this library's additions
- * (matmul_affine_wide[_bf16], see below). `offsets` may be NULL (all zero) or
+ * (matmul_affine_wide[_bf16], rope_axes, attn_paged_bf16, .., see below). `offsets` may be NULL (all zero) or
  * hold one 4-byte-aligned byte offset per buffer. `params`, `threads` and
  * `group_size` follow dispatch_layout (src/gpu.rs:1041-1294). */
 int qmr_encode(qmr_command *command, const char *name, qmr_buffer *const *buffers,
@@ -133,21 +133,22 @@ int qmr_encode(qmr_command *command, const char *name, qmr_buffer *const *buffer
  * harnesses that forbid hipMalloc). Same arguments, validation and kernels;
  * it calls no hipMalloc, hipFree or allocating library routine. The
  * workspace its kernels need (the row-band kernel's split sums, the split-K
- * kernel's partial sums and counters, the wide block's activation images)
- * comes from a static scratch array of QMR_STATIC_SCRATCH_BYTES that each GPU
+ * kernel's partial sums and counters, the wide block's activation images,
+ * attention's results of key ranges) comes from a static scratch array of QMR_STATIC_SCRATCH_BYTES that each GPU
  * holds from library load until the process ends; a launch needing more is
  * rejected with QMR_ERR_INVALID before anything is enqueued. (Of the wide
  * blocks these are Q4 ones of group 64 and more than eight RHS over whole 256
  * columns, codes, scales and biases 16-byte aligned; the others run in
  * passes over fewer RHS, or as blocks of four, that fit the scratch, and do
- * so in qmr_encode too.) Workspace that
+ * so in qmr_encode too. attn_paged is planned with as many key ranges as fit:
+ * its bits are qmr_encode's wherever both plans agree, as for single tokens.) Workspace that
  * must start at zero (split sums tagged with a fixed epoch, arrival counters)
  * is cleared by a fill kernel inside the call when earlier launches may have
  * left it non-zero: the split-K kernel and the row-band kernel's GEMV and
  * block forms (plain or residual) clear every slot and counter they take, so
  * after the first fill the region stays zero from call to call and needs no
  * fill until a wide block, a group 32 block of three or four RHS on the wide
- * kernel, the row-band MLP form or a failed command has used it. All calls on one GPU share its scratch: calls whose launches
+ * kernel, the row-band MLP form, attn_paged or a failed command has used it. All calls on one GPU share its scratch: calls whose launches
  * overlap in time (other streams, other device handles on the same GPU)
  * race. */
 #define QMR_STATIC_SCRATCH_BYTES (8u << 20)
@@ -345,7 +346,8 @@ int qmr_set_read_plan(qmr_device *device, uint32_t workgroups, uint32_t unroll, 
 int qmr_set_band_wait_fault(qmr_device *device, int enabled);
 /* Bytes of device workspace this handle has allocated for its kernels (the
  * row-band split sums, the split-K partial sums and counters, the wide
- * block's activation images); qmr_encode_static allocates none. */
+ * block's activation images, attention's results of key ranges);
+ * qmr_encode_static allocates none. */
 size_t qmr_device_workspace_bytes(const qmr_device *device);
 /* Reference pipeline label selected by the last successful qmr_encode. */
 const char *qmr_last_kernel(const qmr_device *device);

@@ -44,7 +44,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kMaxSplits = 512;  // key ranges of a tile, at most
-constexpr uint32_t kFewSplits = 4;    // that a wave joins alone
+constexpr uint32_t kFewSplits = 16;   // that a wave joins alone, at most
 constexpr uint32_t kRsrcWord3 = 0x00020000u;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
@@ -996,7 +996,8 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 // the ranges, whose loads depend on nothing and are all in flight at once. For
 // few ranges a wave a row (one token of 24/4 heads of 256 over 2001 keys, 4, 8 and
 // 16 ranges, rows kernel and join: 16.2, 13.5 and 12.2 us, as WIDE 16.2, 13.0 and
-// 11.4). Of its 3 us most is one more launch.
+// 11.4; 12288 rows of 256 dims in 5 ranges, the join alone: 15.8, as WIDE 18.6).
+// Of its 3 us with few rows most is one more launch.
 template <int DM, bool WIDE>
 __global__ __launch_bounds__(kThreads) void attn_join_kernel(AttendArgs a, AttendPlan pl, Partial ws, uint32_t rows) {
     constexpr int E = DM / 64, kFirst = 8;
@@ -1111,7 +1112,7 @@ hipError_t launch_dim(const AttendArgs &a, const AttendPlan &pl, const Partial &
     }
     if (e != hipSuccess || pl.splits == 1) return e;
     const uint32_t rows = pl.tiles * a.cache.kv_heads * pl.rows;
-    if (pl.splits <= kFewSplits) {
+    if (pl.splits <= 4 || (pl.splits <= kFewSplits && rows >= 4096)) {
         attn_join_kernel<DM, false><<<(rows + kWaves - 1) / kWaves, kThreads, 0, stream>>>(a, pl, ws, rows);
     } else {
         attn_join_kernel<DM, true><<<rows, kThreads, 0, stream>>>(a, pl, ws, rows);
