@@ -265,12 +265,12 @@ int qmr_supported_bf16_quantization(uint32_t bits, size_t group);
  *     keys, causal, window, scale as FP32 bits. Query head h reads key-value
  *     head h / (q heads / kv heads). A token at position p sees the positions
  *     below min(lengths[s], most keys), with causal = 1 those up to p, and with
- *     a window w > 0 those past p - w; positions of pages not below `pages`
- *     hold nothing. A row that sees no key is zero. What it does not see does
- *     not reach it, be it NaN; a key or value that it sees and that is not
- *     finite makes it not finite. `most keys` bounds the lengths that the
- *     launch is planned for. Results are near FP32 arithmetic's: no operand is
- *     rounded below 22 bits.
+ *     a window w > 0 (of causal attention) those past p - w; positions of pages
+ *     not below `pages` hold nothing. A row that sees no key is zero. What it
+ *     does not see does not reach it, be it NaN; a key or value that it sees and
+ *     that is not finite makes it not finite. `most keys` bounds the lengths that
+ *     the launch is planned for. Results are near FP32 arithmetic's: no operand
+ *     is rounded below 22 bits.
  *   "matvec_affine_f16meta", "matmul_affine_f16meta", "embed_affine_f16meta"
  *     As the FP32-metadata names, with scales/biases stored as IEEE binary16
  *     (the dtype MLX checkpoints ship). The reference expands F16 metadata

@@ -121,8 +121,8 @@ __device__ __forceinline__ u4 load16(__amdgpu_buffer_rsrc_t r, uint32_t offset, 
 }
 
 // A wave's 64 chunks of 16 bytes from memory straight to LDS, chunk after chunk
-// from byte `to`; `rsrc`: a buffer's four words. The compiler does not see that they are on their way:
-// wait_dma is the wait. The idle cycles are those a load has to keep from a
+// from byte `to`; `rsrc`: a buffer's four words. The compiler does not see that
+// they are on their way: wait_dma is the wait. The idle cycles are those a load has to keep from a
 // vector instruction that wrote its scalar operands, and from m0's own write.
 __device__ __forceinline__ void dma16(u4 rsrc, uint32_t offset, uint32_t more, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
@@ -345,8 +345,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
         next = page_of(next_key);
     }
 
-    // The queries' loads go out before the blocks': thread (row % 16, p) has chunks p and
-    // p + 16 of 8 dims.
+    // The queries' loads go out before the blocks': thread (row % 16, p) has
+    // chunks p and p + 16 of 8 dims.
     constexpr int CH = (DM / 8 + 15) / 16;
     const uint32_t qn = threadIdx.x / 16, qp = threadIdx.x % 16;
     float x[CH][8];
@@ -537,8 +537,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
     while (at < order.edges) block(std::true_type{});
     while (at < order.count) block(std::false_type{});
 
-    // Join the waves. (What a thread is in the workgroup is
-    // worked out again: the loop needs the registers.)
+    // Join the waves. (What a thread is in the workgroup is worked out again:
+    // the loop needs the registers.)
     uint32_t thread = threadIdx.x;
     asm volatile("" : "+v"(thread));
     const uint32_t jl = thread % 64, jn = jl % 16, jg = jl / 16, rn = thread / 16, rp = thread % 16;
