@@ -285,7 +285,7 @@ __device__ __forceinline__ u4 ones_of(int first, int lo, int hi) {
 // Memory bounds it: 32 sequences of 8 heads of 128 over up to 8001 keys (521
 // MB) 104 us, 5.0 TB/s (repeated, so in part from the last-level cache; a large
 // copy reaches 4.8); one token of 24/4 heads of 256 over 32768 (134 MB) 28 us
-// with the join, 4.7 TB/s; over 1001 keys (4 MB) 10.9 us, of which the join
+// with the join, 4.8 TB/s; over 1001 keys (4 MB) 10.2 us, of which the join
 // takes 3 and the first workgroup's chain of dependent steps (its sequence, its
 // page, keys and queries, products, waves joined) the rest.
 template <bool BF16, int DM>
@@ -1150,7 +1150,7 @@ hipError_t launch_type(const AttendArgs &a, const AttendPlan &pl, const Partial 
 // Ranges, in the rows kernel: one token of 24/4 heads of 256 over 32768 keys in
 // 8, 16, 32, 64 and 128: 52, 35, 30, 31.6 and 32 us; over 4001 in 16, 32 and 64:
 // 15.0, 13.7 and 15.4; over 1001 in 1, 8, 16 and 32 (of one block): 18.3, 11.7,
-// 11.3 and 10.9; over 101 in 1 and 4: 7.8 and 11; 32 sequences of 8 heads of 128
+// 11.3 and 10.8; over 101 in 1 and 4: 7.8 and 11; 32 sequences of 8 heads of 128
 // over up to 8001 in 1, 2 and 4: 105, 113 and 122.
 AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t workspace_limit, uint32_t force_rows,
                        uint32_t force_splits) {
