@@ -296,7 +296,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_rope_kernel(AppendArgs a, 
         const uint32_t h0 = (wave % sp.slices) * sp.heads_each * groups + group, heads = a.heads + c.kv_heads;
         Part<V, IT> q_norm, k_norm;
         if (a.eps > 0.f) {
-            load_row<V, IT>(a.q_norm, a.rope, lane, sp.lanes, sp.units, q_norm);
+            if (a.heads > 0) load_row<V, IT>(a.q_norm, a.rope, lane, sp.lanes, sp.units, q_norm);  // else no view
             load_row<V, IT>(a.k_norm, a.rope, lane, sp.lanes, sp.units, k_norm);
         }
         place_of(c, t, seq, pos, end);
