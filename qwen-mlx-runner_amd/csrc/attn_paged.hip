@@ -198,7 +198,9 @@ __device__ __forceinline__ void visible(const AttendArgs &a, const Tile &t, uint
     const int pos = t.context + int(token);
     hi = a.causal ? min(pos + 1, t.length) : t.length;
     hi = max(min(hi, int(a.max_keys)), 0);
-    lo = a.window ? max(pos - int(a.window) + 1, 0) : 0;
+    // pos - window is taken where it is not negative: a window may be as long as
+    // INT32_MAX, and a sequence's first new tokens may stand before position 0.
+    lo = a.window && pos >= int(a.window) ? pos - int(a.window) + 1 : 0;
 }
 
 // The order of a range's blocks: those that some row sees in part first (the
