@@ -110,6 +110,15 @@ __device__ __forceinline__ void split8(const float (&x)[8], u4 (&t)[kTerms<BF16>
     }
 }
 
+// The power of two that brings a row's queries, `most` at most, to 2^14..2^15. Not
+// below FP32's normal numbers: as a factor of 0 it would make NaN of the minus
+// infinity of a key that is not seen.
+__device__ __forceinline__ int query_exponent(float most) {
+    int e;
+    frexpf(most, &e);
+    return max(e - 15, -126);
+}
+
 // A block of keys or values as a buffer of its own bytes: loads past it give
 // zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const uint16_t *pool, size_t at, uint32_t bytes) {
@@ -401,7 +410,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
     if constexpr (!BF16) {
 #pragma unroll
         for (int d = 1; d < 16; d *= 2) q_most = fmaxf(q_most, __shfl_xor(q_most, d));
-        if (q_most > 0.f && q_most < INFINITY) frexpf(q_most, &e), e -= 15;
+        if (q_most > 0.f && q_most < INFINITY) e = query_exponent(q_most);
     }
     if (qp == 0) row_scale[qn] = ldexpf(1.f, e);
 #pragma unroll
@@ -765,7 +774,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         int e = 0;
         if constexpr (!BF16) {
             most = fmaxf(most, __shfl_xor(most, 32));
-            if (most > 0.f && most < INFINITY) frexpf(most, &e), e -= 15;
+            if (most > 0.f && most < INFINITY) e = query_exponent(most);
             rs = ldexpf(1.f, e);
         }
 #pragma unroll

@@ -40,3 +40,16 @@ def test_windows_longer_than_every_position(gpu, kind, window):
     assert np.abs(want[3:5]).max() > 0.1 and (want[:3] == 0).all()
     for plan, got in under_plans(gpu, lambda: attend(gpu, kind, q, k, v, batch, 0.125, window=window)):
         check_attend(got, want, bound, f"plan {plan}")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [2e-40, 1e-41, 1e-44])
+def test_queries_near_zero(gpu, kind, size):
+    # Scores that vanish, beside keys that a row does not see: plain means.
+    batch = Batch([1, 3, 40], [20, 37, 200], 32)
+    q, k, v = inputs(kind, batch, 4, 2, 64, 3)
+    q = (q * size).astype(np.float32)
+    assert (np.abs(q).reshape(batch.tokens, -1).max(axis=1) > 0).all()
+    want, bound = attend64(q, from_half(k, kind), from_half(v, kind), batch, 0.5)
+    for plan, got in under_plans(gpu, lambda: attend(gpu, kind, q, k, v, batch, 0.5)):
+        check_attend(got, want, bound, f"plan {plan}")
