@@ -504,6 +504,9 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
         float p[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] = scores[0][i], p[4 + i] = scores[1][i];
+        // A page past the pool: no weight, be the query NaN.
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = held ? p[e] : -INFINITY;
         if constexpr (edge()) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -514,7 +517,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
         float most = p[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) most = fmaxf(most, p[e]);
-        most = held ? most * rs : -INFINITY;
+        most *= rs;
         if (__ballot(most > m + kLag) != 0) {
             most = fmaxf(most, __shfl_xor(most, 16));
             most = fmaxf(most, __shfl_xor(most, 32));
@@ -525,7 +528,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
 #pragma unroll
             for (int d = 0; d < VT; ++d) o[d] *= f;
         }
-        const float off = held ? kTop - (m == -INFINITY ? 0.f : m) : -INFINITY;
+        const float off = kTop - (m == -INFINITY ? 0.f : m);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], rs, off));
@@ -846,6 +849,11 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         lds_barrier();
         const bool held = at0 != kNone;
         float most = next_most;
+        if (!held) {  // a page past the pool: no weight, be the query NaN
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = -INFINITY;
+            most = -INFINITY;
+        }
         int key0 = 0;
         if constexpr (edge()) {
             key0 = order.key(at);
@@ -857,7 +865,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
             }
             most = largest(p);
         }
-        most = held ? most * rs : -INFINITY;
+        most *= rs;
         if (__ballot(most > m + kLag) != 0) {
             most = fmaxf(most, __shfl_xor(most, 32));
             const float up = fmaxf(m, most);
@@ -870,7 +878,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
                 stays(o[d]);
             }
         }
-        const float off = held ? kTop - (m == -INFINITY ? 0.f : m) : -INFINITY;
+        const float off = kTop - (m == -INFINITY ? 0.f : m);
         if constexpr (edge()) lds_barrier();
 
         // The next block's scores, and this one's weights between them; then

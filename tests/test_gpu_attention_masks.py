@@ -53,3 +53,18 @@ def test_queries_near_zero(gpu, kind, size):
     want, bound = attend64(q, from_half(k, kind), from_half(v, kind), batch, 0.5)
     for plan, got in under_plans(gpu, lambda: attend(gpu, kind, q, k, v, batch, 0.5)):
         check_attend(got, want, bound, f"plan {plan}")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [3, 140])
+def test_queries_that_see_nothing_are_zero_whatever_they_hold(gpu, kind, new):
+    # All pages of the first sequence are past the pool; the second has no cache.
+    batch = Batch([new, 2, 1], [300, 0, 40], 32, dropped=tuple((0, c) for c in range(10)))
+    q, k, v = inputs(kind, batch, 4, 2, 64, 2)
+    clean = q.copy()
+    q[:new:2, :, 5], q[1:new:2, :, 6] = np.nan, np.inf
+    q[new:new + 2, 1, 0] = np.nan
+    want, bound = attend64(clean, from_half(k, kind), from_half(v, kind), batch, 0.125)
+    assert (want[:new + 2] == 0).all()
+    for plan, got in under_plans(gpu, lambda: attend(gpu, kind, q, k, v, batch, 0.125)):
+        check_attend(got, want, bound, f"plan {plan}")
