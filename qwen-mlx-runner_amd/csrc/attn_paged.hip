@@ -286,6 +286,25 @@ __device__ __forceinline__ u4 ones_of(int first, int lo, int hi) {
     return halves_of(first, lo, hi) & kOne<BF16>;
 }
 
+// Whether one of a block's keys lo..hi-1 (counted from its first) is not finite.
+// An infinite key can give a score of minus infinity, which has no weight and
+// leaves no mark on its row; a wave that has met such a score looks at the keys
+// of all its blocks once more.
+template <bool BF16>
+__device__ __forceinline__ bool sees_bad_key(__amdgpu_buffer_rsrc_t block, uint32_t dim, int lo, int hi) {
+    const uint32_t l = threadIdx.x % 64, place = 16 * (l / 4 % 2) + 4 * (l / 8 % 4) + l % 4;  // of slot l % 32
+    uint32_t bad = 0;
+#pragma unroll 1
+    for (uint32_t ch = l / 32; ch < dim / 8; ch += 2) {
+        const u4 x = load16(block, (ch * kBlock + place) * 16, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= not_finite<BF16>(x[i]);
+    }
+    const uint64_t some = __ballot(bad != 0);
+    auto below = [](int n) { return n >= 32 ? 0xFFFFFFFFu : (1u << max(n, 0)) - 1; };
+    return ((uint32_t(some) | uint32_t(some >> 32)) & below(hi) & ~below(lo)) != 0;
+}
+
 // Few rows: 16 rows a workgroup, every wave all of them over its own blocks of
 // the range (block w, w + 4, ..), straight from memory into operand registers,
 // whole lines at a time; nothing is shared but the queries, which wait in LDS
@@ -432,7 +451,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
     int lo, hi;
     visible(a, t, (t.row0 + min(n, in_tile - 1)) / group, lo, hi);
     const float rs = row_scale[n];
-    float m = -INFINITY, sum = 0.f;
+    float m = -INFINITY, off = kTop, sum = 0.f;  // off: kTop - m
+    bool deep = false, gap = false;              // the wave has met a score of minus infinity, a page past the pool
     // Of a lane's outputs, those that saw a value that is not finite.
     uint32_t poison[(VT + 7) / 8] = {};
     f4 o[VT];
@@ -458,7 +478,6 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
             if (DM == 256 && s % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
         const bool more = at + kWaves < order.count;
-        load_keys(next, next_key, more);
         const int key_now = key0;
         if constexpr (edge()) {
             // Values that no row sees may be anything: zero them.
@@ -504,34 +523,42 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
         float p[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] = scores[0][i], p[4 + i] = scores[1][i];
-        // A page past the pool: no weight, be the query NaN.
+        // Of the keys that are seen the least score: minus infinity for some infinite
+        // keys.
+        float least = INFINITY;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = held ? p[e] : -INFINITY;
-        if constexpr (edge()) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int key = key_now + 8 * int(g) + e;
-                if (key < lo || key >= hi) p[e] = -INFINITY;
-            }
+        for (int e = 0; e < 8; ++e) {
+            const int key = key_now + 8 * int(g) + e;
+            const bool seen = !edge() || (key >= lo && key < hi);
+            least = fminf(least, seen ? p[e] : INFINITY);
+            if (!seen) p[e] = -INFINITY;
         }
         float most = p[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) most = fmaxf(most, p[e]);
         most *= rs;
-        if (__ballot(most > m + kLag) != 0) {
-            most = fmaxf(most, __shfl_xor(most, 16));
-            most = fmaxf(most, __shfl_xor(most, 32));
-            const float up = fmaxf(m, most);
-            const float f = up > m ? exp2f(m - up) : 1.f;
-            m = up;
-            sum *= f;
+        auto small = [&] { return least == -INFINITY; };
+        if (held & (__ballot((most > m + kLag) | small()) != 0)) {
+            if (__ballot(most > m + kLag) != 0) {
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                const float up = fmaxf(m, most);
+                const float f = up > m ? exp2f(m - up) : 1.f;
+                m = up;
+                off = kTop - (m == -INFINITY ? 0.f : m);
+                sum *= f;
 #pragma unroll
-            for (int d = 0; d < VT; ++d) o[d] *= f;
+                for (int d = 0; d < VT; ++d) o[d] *= f;
+            }
+            deep |= __ballot(small()) != 0;
         }
-        const float off = kTop - (m == -INFINITY ? 0.f : m);
+        // A page past the pool has no weight.
+        const float less = held ? off : -INFINITY;
+        gap |= !held;
+        load_keys(next, next_key, more);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], rs, off));
+            p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], rs, less));
             sum += p[e];
         }
         u4 pt[T];
@@ -550,6 +577,26 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
     };
     while (at < order.edges) block(std::true_type{});
     while (at < order.count) block(std::false_type{});
+    // A query that is not finite gives the blocks of pages past the pool weights of
+    // NaN: a row that sees no key is zero all the same.
+    if (gap && __ballot(sum != sum) != 0) {
+        bool sees = false;
+        for (int i = int(w); i < order.count; i += kWaves) {
+            const int key = order.key(i);
+            sees |= page_of(key) < c.pages && max(lo, key) < min(hi, key + int(kBlock));
+        }
+        if (!sees) {
+            m = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int d = 0; d < VT; ++d) o[d] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    if (deep) {
+        for (int i = int(w); i < order.count; i += kWaves) {
+            const int key = order.key(i);
+            if (sees_bad_key<BF16>(rsrc_of(c.k, page_of(key), key, true), dim, lo - key, hi - key)) sum = __builtin_nanf("");
+        }
+    }
 
     // Join the waves. (What a thread is in the workgroup is worked out again:
     // the loop needs the registers.)
@@ -824,8 +871,17 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         for (int i = 1; i < 16; ++i) most = fmaxf(most, x[i]);
         return most;
     };
+    auto smallest = [](f16v x) {
+        float least = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) least = fminf(least, x[i]);
+        return least;
+    };
     f16v next = {};
-    float next_most = 0.f;
+    float off = kTop;                  // kTop - m
+    bool raise = false, few = false;   // the next block raises m; has infinite keys
+    bool deep = false, gap = false;    // the wave has met a score of minus infinity, a page past the pool
+    auto small = [](float least) { return least == -INFINITY; };
     if (order.count > 0) {
         wait_dma<4 * kEach>();
         lds_barrier();
@@ -833,7 +889,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 #pragma unroll
         for (int s = 0; s < KS; ++s) score_step(first, s, key_operand(k0, s), low_operand(s));
         next = total(first);
-        next_most = largest(next);
+        raise = at0 != kNone;
     }
     // Of the largest heads, O has its place in the accumulation registers: left
     // to itself the compiler moves it to the others and back for every block.
@@ -847,39 +903,44 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         for (int d = 0; d < VT; ++d) stays(o[d]);
         wait_dma<2 * kEach>();  // the next keys and these values are there
         lds_barrier();
-        const bool held = at0 != kNone;
-        float most = next_most;
-        if (!held) {  // a page past the pool: no weight, be the query NaN
-#pragma unroll
-            for (int i = 0; i < 16; ++i) p[i] = -INFINITY;
-            most = -INFINITY;
-        }
         int key0 = 0;
+        float least = 0.f;
         if constexpr (edge()) {
             key0 = order.key(at);
             clean_values(v0, key0);
+            least = INFINITY;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int key = key0 + 16 * (i / 8) + 8 * int(g) + i % 8;
-                if (key < lo || key >= hi) p[i] = -INFINITY;
+                const bool seen = key >= lo && key < hi;
+                least = fminf(least, seen ? p[i] : INFINITY);
+                if (!seen) p[i] = -INFINITY;
             }
-            most = largest(p);
+            raise = (at0 != kNone) & (__ballot(largest(p) * rs > m + kLag) != 0);
+            few = (at0 != kNone) & (__ballot(small(least)) != 0);
         }
-        most *= rs;
-        if (__ballot(most > m + kLag) != 0) {
+        if (raise) {
+            float most = largest(p) * rs;
             most = fmaxf(most, __shfl_xor(most, 32));
             const float up = fmaxf(m, most);
             const float f = up > m ? exp2f(m - up) : 1.f;
             m = up;
+            off = kTop - (m == -INFINITY ? 0.f : m);
             sum *= f;
+            if constexpr (!edge()) least = smallest(p);
+            few = __ballot(small(least)) != 0;
 #pragma unroll
             for (int d = 0; d < VT; ++d) {
+                stays(o[d]);
                 o[d] *= f;
                 stays(o[d]);
             }
         }
-        const float off = kTop - (m == -INFINITY ? 0.f : m);
+        // A page past the pool has no weight.
+        const float less = at0 != kNone ? off : -INFINITY;
+        gap |= at0 == kNone;
         if constexpr (edge()) lds_barrier();
+        deep |= few;
 
         // The next block's scores, and this one's weights between them; then
         // the weights times the values, two tiles of dims in turn.
@@ -899,7 +960,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         u4 pt[2][T];
         float x[8];
         auto weigh = [&](int j) {
-            x[j % 8] = __builtin_amdgcn_exp2f(fmaf(p[j], rs, off));
+            x[j % 8] = __builtin_amdgcn_exp2f(fmaf(p[j], rs, less));
             sum += x[j % 8];
             if (j % 8 == 7) split8<BF16>(x, pt[j / 8]);
         };
@@ -933,7 +994,8 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
             if (i == VT) fetch(c.v, at2, v2);
             if (i == 2 * VT - 2) {
                 at4 = place_of(at + 4);
-                next_most = largest(next);
+                raise = (at1 != kNone) & (__ballot(largest(next) * rs > m + kLag) != 0);
+                few = (at1 != kNone) & (__ballot(small(smallest(next))) != 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -970,6 +1032,28 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
     while (at < order.edges) block(std::true_type{});
     while (at < order.count) block(std::false_type{});
     wait_dma<0>();  // LDS is given back
+    // As in the rows kernel: rows that see no key, and infinite keys.
+    if (gap && __ballot(sum != sum) != 0) {
+        bool sees = false;
+        for (int i = 0; i < order.count; ++i) {
+            const int key = order.key(i);
+            sees |= place_of(i) != kNone && max(lo, key) < min(hi, key + int(kBlock));
+        }
+        if (!sees) {
+            m = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int d = 0; d < VT; ++d) o[d] = f16v{};
+        }
+    }
+    if (deep) {
+        for (int i = 0; i < order.count; ++i) {
+            const int key = order.key(i);
+            const uint32_t named = place_of(i);
+            if (named == kNone) continue;
+            if (sees_bad_key<BF16>(block_rsrc(c.k, size_t(named) * (dim * kBlock), block_bytes), dim, lo - key, hi - key))
+                sum = __builtin_nanf("");
+        }
+    }
 
 #pragma unroll
     for (int d = 0; d < VT; ++d) {

@@ -68,3 +68,40 @@ def test_queries_that_see_nothing_are_zero_whatever_they_hold(gpu, kind, new):
     assert (want[:new + 2] == 0).all()
     for plan, got in under_plans(gpu, lambda: attend(gpu, kind, q, k, v, batch, 0.125)):
         check_attend(got, want, bound, f"plan {plan}")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("element", [1.0, -1.0, 0.3, -0.3])
+@pytest.mark.parametrize("infinity", [np.inf, -np.inf])
+def test_keys_that_are_not_finite(gpu, kind, element, infinity):
+    # Rows that see the key are NaN or infinite, be the score it gives plus or
+    # minus infinity, and whether the query's element has 16 bits or more; rows
+    # that do not are as without it.
+    batch = Batch([40, 1, 1], [130, 300, 1], 32)
+    q, k, v = inputs(kind, batch, 4, 2, 64, 4)
+    q[..., 7] = element
+    want, bound = attend64(q, from_half(k, kind), from_half(v, kind), batch, 0.125)
+    bits = to_half(np.float32([infinity]), kind)[0]
+    for s, pos in ((0, 110), (1, 45), (2, 0)):
+        k[batch.table[s, pos // 32], 0, pos % 32, 7] = bits
+    sees = np.zeros((42, 4), bool)  # key-value head 0 is that of query heads 0 and 1
+    sees[20:, :2] = True
+    for plan, got in under_plans(gpu, lambda: attend(gpu, kind, q, k, v, batch, 0.125)):
+        assert not np.isfinite(got[sees]).any(), plan
+        check_attend(got[~sees], want[~sees], bound[~sees], f"plan {plan}")
+
+
+@pytest.mark.parametrize("new", [3, 60])
+def test_scores_below_fp32_have_no_weight(gpu, new):
+    # A finite key of bf16 whose product with the query is past FP32's range.
+    batch = Batch([new], [200], 32)
+    q, k, v = inputs("bf16", batch, 2, 1, 64, 5)
+    q[..., 7] = 10.0
+    row = (batch.table[0, 1], 0, 8, 7)
+    k[row] = 0
+    _, bound = attend64(q, from_half(k, "bf16"), from_half(v, "bf16"), batch, 0.125)
+    k[row] = to_half(np.float32([-1000.0]), "bf16")[0]
+    want, _ = attend64(q, from_half(k, "bf16"), from_half(v, "bf16"), batch, 0.125)
+    k[row] = to_half(np.float32([-3e38]), "bf16")[0]
+    for plan, got in under_plans(gpu, lambda: attend(gpu, "bf16", q, k, v, batch, 0.125)):
+        check_attend(got, want, bound, f"plan {plan}")
