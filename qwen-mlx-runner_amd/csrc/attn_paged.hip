@@ -871,17 +871,10 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         for (int i = 1; i < 16; ++i) most = fmaxf(most, x[i]);
         return most;
     };
-    auto smallest = [](f16v x) {
-        float least = x[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) least = fminf(least, x[i]);
-        return least;
-    };
     f16v next = {};
-    float off = kTop;                  // kTop - m
-    bool raise = false, few = false;   // the next block raises m; has infinite keys
-    bool deep = false, gap = false;    // the wave has met a score of minus infinity, a page past the pool
-    auto small = [](float least) { return least == -INFINITY; };
+    float next_most = 0.f;
+    float least_to = 0.f;            // the least exponent of a weight, but for those of the masked blocks
+    bool deep = false, gap = false;  // the wave has met a score of minus infinity in these, a page past the pool
     if (order.count > 0) {
         wait_dma<4 * kEach>();
         lds_barrier();
@@ -889,7 +882,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
 #pragma unroll
         for (int s = 0; s < KS; ++s) score_step(first, s, key_operand(k0, s), low_operand(s));
         next = total(first);
-        raise = at0 != kNone;
+        next_most = largest(next);
     }
     // Of the largest heads, O has its place in the accumulation registers: left
     // to itself the compiler moves it to the others and back for every block.
@@ -903,12 +896,14 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         for (int d = 0; d < VT; ++d) stays(o[d]);
         wait_dma<2 * kEach>();  // the next keys and these values are there
         lds_barrier();
+        const bool held = at0 != kNone;
+        gap |= !held;
+        float most = next_most;
         int key0 = 0;
-        float least = 0.f;
         if constexpr (edge()) {
             key0 = order.key(at);
             clean_values(v0, key0);
-            least = INFINITY;
+            float least = INFINITY;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int key = key0 + 16 * (i / 8) + 8 * int(g) + i % 8;
@@ -916,31 +911,24 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
                 least = fminf(least, seen ? p[i] : INFINITY);
                 if (!seen) p[i] = -INFINITY;
             }
-            raise = (at0 != kNone) & (__ballot(largest(p) * rs > m + kLag) != 0);
-            few = (at0 != kNone) & (__ballot(small(least)) != 0);
+            deep |= __ballot(least == -INFINITY) != 0;
+            most = largest(p);
         }
-        if (raise) {
-            float most = largest(p) * rs;
+        most = held ? most * rs : -INFINITY;
+        if (__ballot(most > m + kLag) != 0) {
             most = fmaxf(most, __shfl_xor(most, 32));
             const float up = fmaxf(m, most);
             const float f = up > m ? exp2f(m - up) : 1.f;
             m = up;
-            off = kTop - (m == -INFINITY ? 0.f : m);
             sum *= f;
-            if constexpr (!edge()) least = smallest(p);
-            few = __ballot(small(least)) != 0;
 #pragma unroll
             for (int d = 0; d < VT; ++d) {
-                stays(o[d]);
                 o[d] *= f;
                 stays(o[d]);
             }
         }
-        // A page past the pool has no weight.
-        const float less = at0 != kNone ? off : -INFINITY;
-        gap |= at0 == kNone;
+        const float off = held ? kTop - (m == -INFINITY ? 0.f : m) : -INFINITY;
         if constexpr (edge()) lds_barrier();
-        deep |= few;
 
         // The next block's scores, and this one's weights between them; then
         // the weights times the values, two tiles of dims in turn.
@@ -960,7 +948,9 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
         u4 pt[2][T];
         float x[8];
         auto weigh = [&](int j) {
-            x[j % 8] = __builtin_amdgcn_exp2f(fmaf(p[j], rs, less));
+            const float to = fmaf(p[j], rs, off);
+            x[j % 8] = __builtin_amdgcn_exp2f(to);
+            if constexpr (!edge()) least_to = fminf(least_to, to);
             sum += x[j % 8];
             if (j % 8 == 7) split8<BF16>(x, pt[j / 8]);
         };
@@ -994,8 +984,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
             if (i == VT) fetch(c.v, at2, v2);
             if (i == 2 * VT - 2) {
                 at4 = place_of(at + 4);
-                raise = (at1 != kNone) & (__ballot(largest(next) * rs > m + kLag) != 0);
-                few = (at1 != kNone) & (__ballot(small(smallest(next))) != 0);
+                next_most = largest(next);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -1045,7 +1034,7 @@ __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(
             for (int d = 0; d < VT; ++d) o[d] = f16v{};
         }
     }
-    if (deep) {
+    if (deep || __ballot(least_to == -INFINITY) != 0) {
         for (int i = 0; i < order.count; ++i) {
             const int key = order.key(i);
             const uint32_t named = place_of(i);
