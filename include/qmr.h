@@ -269,8 +269,10 @@ int qmr_supported_bf16_quantization(uint32_t bits, size_t group);
  *     not below `pages` hold nothing. A row that sees no key is zero. What it
  *     does not see does not reach it, be it NaN; a key or value that it sees and
  *     that is not finite makes it not finite. `most keys` bounds the lengths that
- *     the launch is planned for. Results are near FP32 arithmetic's: no operand
- *     is rounded below 22 bits.
+ *     the launch is planned for. Results are near FP32 arithmetic's: with
+ *     a BF16 cache queries and weights keep 24 bits. With an F16 cache they keep
+ *     22, but a query's element is off by 2^-39 of its row's largest and a weight
+ *     by 2^-36 of its row's where that is more.
  *   "matvec_affine_f16meta", "matmul_affine_f16meta", "embed_affine_f16meta"
  *     As the FP32-metadata names, with scales/biases stored as IEEE binary16
  *     (the dtype MLX checkpoints ship). The reference expands F16 metadata

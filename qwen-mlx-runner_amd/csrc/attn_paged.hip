@@ -7,12 +7,13 @@
 // keys with the running maximum m and sum l of each row, in 32 bits, in powers
 // of two (q carries scale * log2 e).
 //
-// Products run on the matrix cores in the cache's own 16-bit type, with no
-// bit of the 32-bit side lost: an FP32 operand is the sum of two f16 terms
-// (22 bits; queries scaled by a power of two a row so that the second term
-// stays normal) or three bf16 terms (24 bits). That is two or three times the
-// matrix work, which a call of few rows has to spare, and an error near 32-bit
-// arithmetic's own, as every product of this library has.
+// Products run on the matrix cores in the cache's own 16-bit type: an FP32
+// operand is the sum of two f16 terms (22 bits) or three bf16 terms (24 bits).
+// That is two or three times the matrix work, which a call of few rows has to
+// spare, and an error near 32-bit arithmetic's own, as every product of this
+// library has. f16 spans 40 powers of two: queries are scaled by a power of two
+// a row, so that an element is off by 2^-39 of the row's largest where that is
+// more than its own 22 bits; weights are off by 2^-36 of the largest (kTop).
 //
 // Operand placement (v_mfma_f32_16x16x32: A row and B column lane % 16, K
 // chunk lane / 16; D[i][j] in lane j + 16 (i / 4), element i % 4): S^T = K Q^T
@@ -35,6 +36,8 @@ using attn::kBlock;
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -86,9 +89,14 @@ __device__ __forceinline__ float less_half(float x, uint32_t h) {
     return r;
 }
 
-// Eight FP32 values as kTerms vectors of eight halves that add up to them:
-// truncated terms, each exact in what the ones before leave (the last f16 one
-// rounds at 2^-22).
+// Two f16 in a word, to nearest.
+__device__ __forceinline__ uint32_t two_halves(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{lo, hi}), h2));
+}
+
+// Eight FP32 values as kTerms vectors of eight halves that add up to them, each
+// term exact in what the ones before leave: bf16 ones truncated, f16 ones to
+// nearest (the second rounds at 2^-23).
 template <bool BF16>
 __device__ __forceinline__ void split8(const float (&x)[8], u4 (&t)[kTerms<BF16>]) {
 #pragma unroll
@@ -103,9 +111,8 @@ __device__ __forceinline__ void split8(const float (&x)[8], u4 (&t)[kTerms<BF16>
                 b -= __uint_as_float(ub & 0xFFFF0000u);
             }
         } else {
-            const auto hi = __builtin_amdgcn_cvt_pkrtz(a, b);
-            t[0][i] = __builtin_bit_cast(uint32_t, hi);
-            t[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(less_half<0>(a, t[0][i]), less_half<1>(b, t[0][i])));
+            t[0][i] = two_halves(a, b);
+            t[1][i] = two_halves(less_half<0>(a, t[0][i]), less_half<1>(b, t[0][i]));
         }
     }
 }
@@ -321,9 +328,15 @@ __device__ __forceinline__ bool sees_bad_key(__amdgpu_buffer_rsrc_t block, uint3
 template <bool BF16, int DM>
 __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
     constexpr int R = 16, T = kTerms<BF16>, KS = DM / 32, VT = DM / 16;
-    // f16 weights are up to 2^15, so that small ones stay normal; the maximum
-    // lags by at most 2^kLag.
-    constexpr float kTop = BF16 ? 0.f : 7.f, kLag = 8.f;
+    // The maximum lags by at most 2^kLag. f16 weights reach from 2^kTop to 2^15, as
+    // far from the type's smallest step as it allows: their second term rounds at
+    // 2^-25, 2^-36 of the row's largest. That counts where the row's weight is on a
+    // key whose value is near zero (the first position of many a sequence) and its
+    // output is what small weights make of the others. Of 4096 keys 14 nats below
+    // such a key 2.8e-4 were lost with a top of 2^7, a lag of 2^8 and truncated
+    // terms, and 4e-6, the scores' own rounding, are now; the shorter lag takes
+    // 0.3% of a prompt, one of 2^2 2%.
+    constexpr float kTop = BF16 ? 0.f : 11.f, kLag = BF16 ? 8.f : 4.f;
     constexpr int kPitch = DM + 4;  // LDS pitch of a joined row: 16 rows on different banks
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ float row_scale[R];
@@ -681,7 +694,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
 template <bool BF16, int DM>
 __global__ __launch_bounds__(kThreads, DM == 256 ? 1 : 2) void attn_tile_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
     constexpr int R = 32 * kWaves, T = kTerms<BF16>, KS = DM / 16, VT = DM / 32;
-    constexpr float kTop = BF16 ? 0.f : 7.f, kLag = 8.f;
+    constexpr float kTop = BF16 ? 0.f : 11.f, kLag = BF16 ? 8.f : 4.f;
     constexpr int kChunks = DM * 4;             // 16-byte chunks of a block
     constexpr int kEach = kChunks / kThreads;   // a thread's
     constexpr uint32_t kBytes = kChunks * 16;
