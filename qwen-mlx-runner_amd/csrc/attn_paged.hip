@@ -144,7 +144,7 @@ __device__ __forceinline__ void dma16(u4 rsrc, uint32_t offset, uint32_t more, u
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(more))
-                 : "memory");
+                 : "memory", "m0");
 }
 
 // Until at most LATER of this wave's loads are on their way.
