@@ -37,3 +37,12 @@ def gpus():
     yield handles
     for g in handles.values():
         g.close()
+
+
+@pytest.fixture(autouse=True)
+def planner(request):
+    """The handles above outlive a test; a plan that it forces does not."""
+    shared = {n: request.getfixturevalue(n) for n in ("gpu", "gpus") if n in request.fixturenames}
+    yield
+    for handle in [*([shared["gpu"]] if "gpu" in shared else []), *shared.get("gpus", {}).values()]:
+        handle.set_gemv_plan(0, 0)
