@@ -140,12 +140,17 @@ __device__ __forceinline__ u4 load16(__amdgpu_buffer_rsrc_t r, uint32_t offset, 
 // from byte `to`; `rsrc`: a buffer's four words. The compiler does not see that
 // they are on their way: wait_dma is the wait. The idle cycles are those a load has to keep from a
 // vector instruction that wrote its scalar operands, and from m0's own write.
+// (m0 is a register that the compiler allots to nothing, and it warns of the
+// name; its own writes of m0 are merged across what does not say that it is written.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma16(u4 rsrc, uint32_t offset, uint32_t more, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(more))
                  : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // Until at most LATER of this wave's loads are on their way.
 template <int LATER>
