@@ -325,10 +325,11 @@ __device__ __forceinline__ bool sees_bad_key(__amdgpu_buffer_rsrc_t block, uint3
 // workgroups: 256 KB on their way, more than HBM needs. 32 rows a workgroup
 // spilled registers.
 // Memory bounds it: 32 sequences of 8 heads of 128 over up to 8001 keys (521
-// MB) 104 us, 5.0 TB/s (repeated, so in part from the last-level cache; a large
+// MB) 105 us, 5.0 TB/s (repeated, so in part from the last-level cache; a large
 // copy reaches 4.8); one token of 24/4 heads of 256 over 32768 (134 MB) 28 us
-// with the join, 4.8 TB/s; over 1001 keys (4 MB) 10.2 us, of which the join
-// takes 3 and the first workgroup's chain of dependent steps (its sequence, its
+// with the join, 4.8 TB/s, and 34.9 over one of four caches in turn, which the
+// last-level cache does not hold; over 1001 keys (4 MB) 10.5 us, of which the
+// join takes 3 and the first workgroup's chain of dependent steps (its sequence, its
 // page, keys and queries, products, waves joined) the rest.
 template <bool BF16, int DM>
 __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, AttendPlan pl, Partial ws) {
@@ -691,8 +692,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_rows_kernel(AttendArgs a, At
 // a block.
 //
 // The matrix cores bound it, at the card's power: their clock falls as they
-// fill. A prompt of 4100 tokens of 32/8 heads of 128 (f16) takes 266 us, 518
-// TFLOP/s of the formula and 1036 of the instructions, as each operand of FP32
+// fill. A prompt of 4100 tokens of 32/8 heads of 128 (f16) takes 278 us, 495
+// TFLOP/s of the formula and 990 of the instructions, as each operand of FP32
 // is two terms; 512 tokens of 24/4 heads of 256 over 16513 keys (bf16, three
 // terms) 529 us, 387 and 1160. A large matrix product reaches 1166 in f16 and
 // 1227 in bf16.
@@ -1253,15 +1254,15 @@ hipError_t launch_type(const AttendArgs &a, const AttendPlan &pl, const Partial 
 //   tile kernel  10 for start and end, `chain` a block alone, `each` a block of
 //                128 rows when the CU's two workgroups (one of 256 dims) overlap
 //   join         3, and each range's rows written and read once
-// Both sides where it decides, rows / tile kernel: 64 tokens of 24 heads of 256
-// over 4064 keys (bf16) 38 / 45 us, 150 over 4150 60 / 71, 512 over 16512 552 /
-// 529; one prompt of 32 heads of 128 (f16), 500 tokens 18 / 25, 1000 40 / 42,
-// 2000 111 / 82, 4100 365 / 266.
-// Ranges, in the rows kernel: one token of 24/4 heads of 256 over 32768 keys in
-// 8, 16, 32, 64 and 128: 52, 35, 30, 31.6 and 32 us; over 4001 in 16, 32 and 64:
-// 15.0, 13.7 and 15.4; over 1001 in 1, 8, 16 and 32 (of one block): 18.3, 11.7,
-// 11.3 and 10.8; over 101 in 1 and 4: 7.8 and 11; 32 sequences of 8 heads of 128
-// over up to 8001 in 1, 2 and 4: 105, 113 and 122.
+// Both sides where it decides, rows / tile kernel in its best number of ranges:
+// 64 tokens of 24 heads of 256 over 4064 keys (bf16) 34 / 42 us, 150 over 4150 58
+// / 69, 512 over 16512 569 / 540; one prompt of 32 heads of 128 (f16), 500 tokens
+// 19 / 25, 1000 40 / 41, 2000 114 / 85, 4100 375 / 280.
+// Ranges, in the rows kernel (four caches in turn): one token of 24/4 heads of 256
+// over 32768 keys in 8, 16, 32, 64 and 128: 83, 50, 35, 33.5 and 35.5 us; over 4001
+// in 16, 32 and 64: 13.9, 13.3 and 15.2; over 1001 in 1, 8, 16 and 32 (of one
+// block): 17.6, 11.1, 10.6 and 10.5; over 101 in 1 and 4: 7.7 and 9.8; 32 sequences
+// of 8 heads of 128 over up to 8001 in 1, 2 and 4: 106, 109 and 117.
 AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t workspace_limit, uint32_t force_rows,
                        uint32_t force_splits) {
     const PagedCache &c = a.cache;
@@ -1296,9 +1297,9 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
         const uint64_t most = std::min<uint64_t>((keys + least_keys - 1) / least_keys, kMaxSplits);
         // Workgroups go to the eight XCDs in turn: tiles that read the same keys
         // share one's L2 if their distance is a multiple of eight (six tokens
-        // of 24/4 heads over 16006 keys in 16, 18, 20 and 21 ranges: 25.0, 25.5,
-        // 25.4 and 31.8 us; four sequences of four tokens over 6004 in 6, 7 and
-        // 8: 28.5, 40.4 and 26.8).
+        // of 24/4 heads over 16006 keys in 16, 18, 20 and 21 ranges: 23.8, 22.9,
+        // 22.9 and 28.7 us; four sequences of four tokens over 6004 in 6, 7 and
+        // 8: 33.3, 38.3 and 29.9).
         const bool shared = rows == 16 && c.tokens * group > n * rows;
         uint64_t before = 0;
         const uint64_t first = force_splits == 0 ? 1 : std::min<uint64_t>(force_splits, most);

@@ -279,10 +279,10 @@ __device__ __forceinline__ void append_values(const AppendArgs &a, uint16_t *to,
 // 2011 tokens of 24/4 heads of 256 with norms (124 MB) 36 us, 3.4 TB/s, and 26
 // from the last-level cache; a large copy reaches 4.8 and the rotation alone 4.3
 // at this size: angles, norms and layouts take vector instructions beside the
-// stream. With the norms' weights loaded for each row 41 us, a wave of values a
-// token 38, a row loaded before the last one is turned 41. One token 5.5 us, 48
-// of 32/8 heads of 128 4.2: a launch and its chain of loads (the token's
-// sequence, its length, its page).
+// stream (7.1 million of a wave, 12 us of four SIMDs a CU). With the norms'
+// weights loaded for each row 41 us, a wave of values a token 38, a row loaded
+// before the last one is turned 41. One token 5.4 us, 48 of 32/8 heads of 128 4.2:
+// a launch and its chain of loads (the token's sequence, its length, its page).
 template <int V, int IT, bool BF16>
 __global__ __launch_bounds__(kThreads) void kv_append_rope_kernel(AppendArgs a, Spread sp) {
     const uint32_t wave = blockIdx.x * (kThreads / 64) + threadIdx.x / 64, l = threadIdx.x % 64;
@@ -355,8 +355,9 @@ __global__ __launch_bounds__(kThreads) void kv_append_rope_kernel(AppendArgs a, 
 // Lanes, units and slices for rows of `heads` heads. A token's heads go to as
 // few waves as still give every CU eight, since each wave works out the
 // token's angles again (2011 tokens as above with four, eight and 16: 34.6, 35.9
-// and 36.3 us; the rotation of 4352 of 16 heads of 72 8.7 with each, 10.2 with
-// 32).
+// and 36.3 us: four make one wave a token, eight two of 13 and one step, which
+// is what they lose by; the rotation of 4352 of 16 heads of 72 8.7 with each, 10.2
+// with 32).
 Spread spread_of(uint32_t dim, uint32_t v, uint32_t tokens, uint32_t heads, const DeviceLimits &lim) {
     Spread s;
     s.units = dim / (2 * v);

@@ -142,8 +142,8 @@ class Attention:
         return (self.heads + 2 * self.kv_heads) * self.dim
 
     def cache(self, gpu: Gpu, pages: Pages) -> tuple[Buffer, Buffer]:
-        """Keys and values of this layer; positions that no token was written
-        to are never read."""
+        """Keys and values of this layer; what stands where no token was
+        written reaches no row."""
         size = 2 * pages.pages * self.kv_heads * pages.page * self.dim
         return gpu.alloc(size), gpu.alloc(size)
 
