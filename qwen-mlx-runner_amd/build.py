@@ -40,10 +40,13 @@ SOURCES = [
     ("affine_mfma.hip", ["-x", "hip"]),
     ("affine_rows.hip", ["-x", "hip"]),
     ("affine_tile.hip", ["-x", "hip"]),
+    ("attn_linear.hip", ["-x", "hip"]),
     ("attn_paged.hip", ["-x", "hip"]),
+    ("conv_causal.hip", ["-x", "hip"]),
     ("dense_mfma.hip", ["-x", "hip"]),
     ("misc_kernels.hip", ["-x", "hip"]),
     ("rope_append.hip", ["-x", "hip"]),
+    ("sample_logits.hip", ["-x", "hip"]),
     ("wide_mfma.hip", ["-x", "hip"]),
 ]
 

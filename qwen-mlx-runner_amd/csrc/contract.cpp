@@ -61,6 +61,10 @@ bool is_attention_name(const std::string &name) {
     return name == "rope_axes" || is_append_name(name) || is_attend_name(name);
 }
 
+bool is_linear_name(const std::string &name) { return name == "conv_causal" || name == "attn_linear"; }
+
+bool is_sample_name(const std::string &name) { return name == "sample_logits"; }
+
 RopeWords rope_words(const std::string &name, const uint32_t *p) {
     const bool append = is_append_name(name);
     const uint32_t *w = p + (append ? 10 : 6);
@@ -204,12 +208,102 @@ Layout attention_layout(const std::string &name, const uint32_t *p, size_t np) {
     return out;
 }
 
+// Layouts of conv_causal, attn_linear and sample_logits (no reference
+// counterpart).
+Layout linear_layout(const std::string &name, const uint32_t *p, size_t np) {
+    const bool conv = name == "conv_causal", sample = is_sample_name(name);
+    const size_t count = conv ? 10 : sample ? 3 : 21;
+    ensure(np == count, name + ": expected " + std::to_string(count) + " parameters");
+    auto bytes = [&](std::initializer_list<size_t> v) -> size_t {
+        size_t size = 1;
+        for (size_t b : v) ensure(!mul_overflow(size, b, &size), "GPU shape overflow");
+        return size;
+    };
+    auto rows = [&](size_t tokens, size_t width, size_t stride) -> size_t {
+        ensure(stride >= width, name + ": a row stride is shorter than its row");
+        return bytes({tokens - 1, stride, 4}) + bytes({width, 4});
+    };
+    auto threads = [&](std::initializer_list<size_t> v) -> size_t {
+        const size_t n = bytes(v);
+        ensure(n <= UINT32_MAX, "GPU element index overflow");
+        return n;
+    };
+    auto positive = [&](std::initializer_list<size_t> idx) {
+        for (size_t i : idx) ensure(p[i] > 0, name + ": dimensions must be nonzero");
+    };
+    auto flags = [&](std::initializer_list<size_t> idx) {
+        for (size_t i : idx) ensure(p[i] <= 1, name + ": switches must be 0 or 1");
+    };
+    auto float_word = [&](size_t i) {
+        float v;
+        std::memcpy(&v, &p[i], 4);
+        return v;
+    };
+    Layout out;
+    if (sample) {
+        positive({0, 1});
+        ensure(p[1] <= 1u << 24, name + ": a vocabulary has at most 2^24 tokens");
+        const size_t row = bytes({p[0], 4});
+        out.sizes = {rows(p[0], p[1], p[2]), row, row, row, row, row, row, row};
+        out.threads = threads({p[0], 1024});
+        return out;
+    }
+    const size_t seqs = p[0], tokens = p[1];
+    const size_t starts = bytes({seqs + 1, 4}), slots = bytes({seqs, 4});
+    if (conv) {
+        const size_t channels = p[2], width = p[3];
+        positive({0, 1, 2, 8});
+        ensure(width >= 2 && width <= 4, name + ": filters have two through four taps");
+        flags({6, 7, 9});
+        ensure(p[8] < 1u << 31, name + ": too many slots");
+        const size_t span = (channels + 3) / 4;
+        threads({tokens + seqs, span});
+        ensure(span <= size_t(65535) * 16, name + ": too many channels");
+        out.sizes = {rows(tokens, channels, p[4]), bytes({channels, width, 4}), p[7] ? bytes({channels, 4}) : 0, starts,
+                     slots, bytes({p[8], width - 1, channels, 4}), rows(tokens, channels, p[5])};
+        out.threads = threads({tokens, span});
+        return out;
+    }
+    positive({0, 1, 2, 3, 4, 5, 13, 19});
+    const size_t k_heads = p[2], v_heads = p[3], dk = p[4], dv = p[5];
+    ensure(v_heads % k_heads == 0, name + ": value heads must be a multiple of the key heads");
+    ensure(dk % 8 == 0 && dk <= 256 && dv % 8 == 0 && dv <= 256,
+           name + ": head dimensions must be multiples of 8, at most 256");
+    flags({14, 15, 20});
+    ensure(p[19] < 1u << 31, name + ": too many slots");
+    const float scale = float_word(16), qk_eps = float_word(17), out_eps = float_word(18);
+    ensure(std::isfinite(scale) && scale > 0.f, name + ": the scale must be finite and positive");
+    ensure((p[17] == 0 || (std::isfinite(qk_eps) && qk_eps > 0.f)) && (p[18] == 0 || (std::isfinite(out_eps) && out_eps > 0.f)),
+           name + ": epsilons must be finite and positive, or 0 for no norm");
+    const size_t kw = bytes({k_heads, dk}), vw = bytes({v_heads, dv});
+    const bool gates = p[14] == 1, delta = p[15] == 1, normed = p[18] != 0;
+    const size_t head = v_heads * 4;
+    threads({seqs, v_heads, 1024});
+    threads({tokens + seqs, v_heads, 32});
+    out.sizes = {rows(tokens, kw, p[6]),
+                 rows(tokens, kw, p[7]),
+                 rows(tokens, vw, p[8]),
+                 p[9] == 0 ? head : rows(tokens, v_heads, p[9]),  // stride 0: one row for all tokens
+                 delta ? rows(tokens, v_heads, p[10]) : 0,
+                 gates ? head : 0,
+                 gates ? head : 0,
+                 normed ? rows(tokens, vw, p[11]) : 0,
+                 normed ? dv * 4 : 0,
+                 starts,
+                 slots,
+                 bytes({p[19], v_heads, dk, dv, 4}),
+                 rows(tokens, vw, p[12])};
+    out.threads = threads({tokens, v_heads, 32});
+    return out;
+}
+
 }  // namespace
 
 // dispatch_layout, matrix part (src/gpu.rs:1041-1172), plus this library's
-// F16-metadata, wide-block and attention names.
+// F16-metadata, wide-block, attention, linear-attention and sampling names.
 Layout dispatch_layout(const std::string &name, const uint32_t *p, size_t np) {
     if (is_attention_name(name)) return attention_layout(name, p, np);
+    if (is_linear_name(name) || is_sample_name(name)) return linear_layout(name, p, np);
     size_t count;
     if (name == "copy_f32") {
         count = 1;

@@ -100,6 +100,10 @@ struct RopeWords {
     uint32_t rotary, adjacent, dealt, axes, sections[4];
 };
 RopeWords rope_words(const std::string &name, const uint32_t *p);
+// Names of a linear-attention layer (conv_causal, attn_linear) and of the
+// choice of a token (sample_logits), with no reference counterpart.
+bool is_linear_name(const std::string &name);
+bool is_sample_name(const std::string &name);
 // Rows of a_len and b_len bytes, one every `stride` bytes from a and from b,
 // of which none of a's shares a byte with one of b's.
 bool strided_rows_disjoint(size_t a, size_t a_len, size_t b, size_t b_len, size_t stride);

@@ -1,7 +1,7 @@
 // Launch interface between the host runtime (runtime.cpp) and the HIP
 // kernels (affine_rows.hip, affine_mfma.hip, affine_gemv.hip, affine_tile.hip,
 // dense_mfma.hip, misc_kernels.hip, wide_mfma.hip, rope_append.hip,
-// attn_paged.hip).
+// attn_paged.hip, conv_causal.hip, attn_linear.hip, sample_logits.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -319,6 +319,59 @@ AttendPlan plan_attend(const AttendArgs &a, const DeviceLimits &lim, size_t work
                        uint32_t force_splits = 0);
 hipError_t launch_attn_paged(const AttendArgs &a, const AttendPlan &pl, void *workspace, hipStream_t stream);
 const char *attend_kernel_name(const AttendPlan &pl);
+
+// New tokens of some sequences, each of which has a state in a slot of a pool:
+// sequence s has the tokens starts[s]..starts[s+1]-1, at most the first `most`
+// of them, and the slot slots[s], whose bit 31 says that its state is taken as
+// zeros. Slots past the pool and slots that an earlier sequence names keep
+// nothing. See sequences.hpp.
+struct Sequences {
+    const uint32_t *starts;  // [seqs + 1]
+    const uint32_t *slots;   // [seqs]
+    uint32_t seqs, tokens, most, pool;
+};
+
+// Causal convolution, a filter a channel. See conv_causal.hip.
+struct ConvArgs {
+    const float *x;     // [tokens] rows of channels
+    const float *w;     // [channels][width]
+    const float *bias;  // [channels] or null
+    float *state;       // [pool][width - 1][channels]
+    float *y;
+    uint32_t channels, width, x_stride, y_stride;
+    bool silu, keep;    // keep: states are replaced
+    Sequences seq;
+};
+hipError_t launch_conv_causal(const ConvArgs &a, const DeviceLimits &lim, hipStream_t stream);
+
+// Linear attention with a state and a decay for each value head. See
+// attn_linear.hip.
+struct LinearArgs {
+    const float *q, *k, *v;       // rows of k_heads * dk, k_heads * dk and v_heads * dv
+    const float *a, *b;           // rows of v_heads: decays, and the delta rule's factors
+    const float *a_log, *dt_bias; // [v_heads], used when gates
+    const float *z, *norm;        // rows of v_heads * dv and [dv], used when out_eps > 0
+    float *state;                 // [pool][v_heads][dk][dv]
+    float *out;                   // rows of v_heads * dv
+    uint32_t k_heads, v_heads, dk, dv;
+    uint32_t q_stride, k_stride, v_stride, a_stride, b_stride, z_stride, out_stride;
+    bool gates, delta, keep;
+    float scale, qk_eps, out_eps;  // eps 0: no norm
+    Sequences seq;
+};
+hipError_t launch_attn_linear(const LinearArgs &a, const DeviceLimits &lim, hipStream_t stream);
+
+// A token from each row of logits. See sample_logits.hip.
+struct SampleArgs {
+    const float *logits;  // [rows] of vocab, one every `stride` floats
+    const float *temperature;
+    const uint32_t *top_k;
+    const float *top_p, *min_p, *uniform;
+    uint32_t *tokens;
+    float *probs;
+    uint32_t rows, vocab, stride;
+};
+hipError_t launch_sample_logits(const SampleArgs &a, const DeviceLimits &lim, hipStream_t stream);
 
 // The plan the GEMV launcher would use (for tests and tuning reports).
 GemvPlan plan_affine_gemv(const AffineArgs &a, GemvPlan forced, const DeviceLimits &lim);

@@ -887,6 +887,102 @@ void check_attention_views(const std::string &name, qmr_buffer *const *buffers, 
     for (size_t i = 0; i < last; ++i) apart(last, i);
 }
 
+// Views of the linear-attention and sampling names: what is written shares no
+// byte with another view, except that rows may stand beside other rows of one
+// buffer.
+void check_linear_views(const std::string &name, qmr_buffer *const *buffers, const size_t *offsets,
+                        const std::vector<size_t> &sizes, const uint32_t *p) {
+    auto off = [&](size_t i) -> size_t { return offsets ? offsets[i] : 0; };
+    const bool conv = name == "conv_causal", sample = qmr::is_sample_name(name);
+    // The FP32 rows of a view: its width and stride in bytes, 0 for other views.
+    auto row = [&](size_t i, size_t &width, size_t &stride) {
+        size_t floats = 0, step = 0;
+        if (conv) {
+            if (i == 0 || i == 6) floats = p[2], step = p[i == 0 ? 4 : 5];
+        } else if (!sample) {
+            if (i == 0 || i == 1) floats = size_t(p[2]) * p[4], step = p[6 + i];
+            if (i == 2 || i == 7 || i == 12) floats = size_t(p[3]) * p[5], step = p[i == 2 ? 8 : i == 7 ? 11 : 12];
+            if (i == 3 || i == 4) floats = p[3], step = p[6 + i];
+        }
+        width = step ? floats * 4 : 0;
+        stride = step * 4;
+    };
+    for (size_t out = conv ? 5 : sample ? 6 : 11; out < sizes.size(); ++out) {
+        for (size_t i = 0; i < sizes.size(); ++i) {
+            if (i == out || buffers[i] != buffers[out] || sizes[i] == 0 || sizes[out] == 0 ||
+                !qmr::ranges_overlap(off(i), sizes[i], off(out), sizes[out]))
+                continue;
+            size_t wo, so, wi, si;
+            row(out, wo, so);
+            row(i, wi, si);
+            ensure(wo != 0 && wi != 0 && so == si && qmr::strided_rows_disjoint(off(out), wo, off(i), wi, so),
+                   name + ": output overlaps input buffer " + std::to_string(i));
+        }
+    }
+}
+
+// conv_causal, attn_linear and sample_logits.
+hipError_t launch_linear(qmr_device *dev, const std::string &name, qmr_buffer *const *buffers, const size_t *offsets,
+                         const uint32_t *p, unsigned char *) {
+    auto ptr = [&](size_t i) -> char * { return static_cast<char *>(buffers[i]->ptr) + (offsets ? offsets[i] : 0); };
+    auto f32 = [&](size_t i) { return reinterpret_cast<float *>(ptr(i)); };
+    auto u32 = [&](size_t i) { return reinterpret_cast<uint32_t *>(ptr(i)); };
+    if (qmr::is_sample_name(name)) {
+        start_gpu(dev);
+        return qmr::launch_sample_logits({f32(0), f32(1), u32(2), f32(3), f32(4), f32(5), u32(6), f32(7), p[0], p[1], p[2]},
+                                         dev->limits, dev->stream);
+    }
+    if (name == "conv_causal") {
+        qmr::ConvArgs a{};
+        a.x = f32(0);
+        a.w = f32(1);
+        a.bias = p[7] ? f32(2) : nullptr;
+        a.state = f32(5);
+        a.y = f32(6);
+        a.channels = p[2];
+        a.width = p[3];
+        a.x_stride = p[4];
+        a.y_stride = p[5];
+        a.silu = p[6] == 1;
+        a.keep = p[9] == 1;
+        a.seq = {u32(3), u32(4), p[0], p[1], UINT32_MAX, p[8]};
+        start_gpu(dev);
+        return qmr::launch_conv_causal(a, dev->limits, dev->stream);
+    }
+    qmr::LinearArgs a{};
+    a.q = f32(0);
+    a.k = f32(1);
+    a.v = f32(2);
+    a.a = f32(3);
+    a.b = f32(4);
+    a.a_log = f32(5);
+    a.dt_bias = f32(6);
+    a.z = f32(7);
+    a.norm = f32(8);
+    a.state = f32(11);
+    a.out = f32(12);
+    a.k_heads = p[2];
+    a.v_heads = p[3];
+    a.dk = p[4];
+    a.dv = p[5];
+    a.q_stride = p[6];
+    a.k_stride = p[7];
+    a.v_stride = p[8];
+    a.a_stride = p[9];
+    a.b_stride = p[10];
+    a.z_stride = p[11];
+    a.out_stride = p[12];
+    a.gates = p[14] == 1;
+    a.delta = p[15] == 1;
+    a.keep = p[20] == 1;
+    std::memcpy(&a.scale, &p[16], 4);
+    std::memcpy(&a.qk_eps, &p[17], 4);
+    std::memcpy(&a.out_eps, &p[18], 4);
+    a.seq = {u32(9), u32(10), p[0], p[1], p[13], p[19]};
+    start_gpu(dev);
+    return qmr::launch_attn_linear(a, dev->limits, dev->stream);
+}
+
 // rope_axes, kv_append_rope_* and attn_paged_*.
 hipError_t launch_attention(qmr_device *dev, const std::string &name, qmr_buffer *const *buffers, const size_t *offsets,
                             const uint32_t *p, unsigned char *fixed) {
@@ -1403,6 +1499,9 @@ static int encode_command(qmr_command *command, const char *cname, qmr_buffer *c
         const bool attention = qmr::is_attention_name(name);
         ensure(!dev->reference || !attention, "Attention dispatch is unavailable in reference mode");
         if (attention) check_attention_views(name, buffers, offsets, layout.sizes, params);
+        const bool linear = qmr::is_linear_name(name) || qmr::is_sample_name(name);
+        ensure(!dev->reference || !linear, "Linear attention and sampling are unavailable in reference mode");
+        if (linear) check_linear_views(name, buffers, offsets, layout.sizes, params);
         if (qmr::starts_with(name, "matmul_") || name == "copy_f32" || name == "read_checksum" || fused) {
             const size_t out = nbuffers - 1;
             for (size_t i = 0; i < out; ++i) {
@@ -1466,9 +1565,11 @@ static int encode_command(qmr_command *command, const char *cname, qmr_buffer *c
         hipError_t e = hipSuccess;
         // Families that launch without workspace start the frame's GPU time
         // here; the others start it after their workspace is in place.
-        if (!qmr::starts_with(name, "mat") && !fused && !attention) start_gpu(dev);
+        if (!qmr::starts_with(name, "mat") && !fused && !attention && !linear) start_gpu(dev);
         if (attention) {
             e = launch_attention(dev, name, buffers, offsets, params, fixed);
+        } else if (linear) {
+            e = launch_linear(dev, name, buffers, offsets, params, fixed);
         } else if (qmr::starts_with(name, "embed_affine")) {
             e = qmr::launch_embed_affine(reinterpret_cast<const uint32_t *>(ptr(0)), ptr(1), ptr(2),
                                          meta, params[0], params[1], params[2], params[3],
