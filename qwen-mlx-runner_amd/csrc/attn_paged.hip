@@ -28,19 +28,27 @@
 
 #include "attn_common.hpp"
 #include "kernels.hpp"
+#include "wave_ops.hpp"
 
 namespace qmr {
 namespace {
 
 using attn::kBlock;
 
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+using wave::dma16;
+using wave::f2;
+using wave::f4;
+using wave::h2;
+using wave::h8;
+using wave::kRsrcWord3;
+using wave::lds_barrier;
+using wave::less_half;
+using wave::two_halves;
+using wave::u4;
+using wave::wait_dma;
+
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f2 __attribute__((ext_vector_type(2)));
-typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef f4 f4u __attribute__((aligned(4)));  // rows of FP32 need no more
 
 constexpr int kWaves = 4;
@@ -48,7 +56,6 @@ constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kMaxSplits = 512;  // key ranges of a tile, at most
 constexpr uint32_t kFewSplits = 16;   // that a wave joins alone, at most
-constexpr uint32_t kRsrcWord3 = 0x00020000u;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
 // Terms of an FP32 operand in the cache's type.
@@ -75,23 +82,6 @@ __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
 
 __device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) {  // lo >> 16 | hi & 0xFFFF0000
     return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-}
-
-// x - the low (0) or high (1) f16 of h, in one instruction.
-template <int HIGH>
-__device__ __forceinline__ float less_half(float x, uint32_t h) {
-    float r;
-    if constexpr (HIGH) {
-        asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
-    } else {
-        asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
-    }
-    return r;
-}
-
-// Two f16 in a word, to nearest.
-__device__ __forceinline__ uint32_t two_halves(float lo, float hi) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{lo, hi}), h2));
 }
 
 // Eight FP32 values as kTerms vectors of eight halves that add up to them, each
@@ -134,35 +124,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const uint16_t *poo
 
 __device__ __forceinline__ u4 load16(__amdgpu_buffer_rsrc_t r, uint32_t offset, uint32_t more) {
     return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(r, int(offset), int(more), 0));
-}
-
-// A wave's 64 chunks of 16 bytes from memory straight to LDS, chunk after chunk
-// from byte `to`; `rsrc`: a buffer's four words. The compiler does not see that
-// they are on their way: wait_dma is the wait. The idle cycles are those a load has to keep from a
-// vector instruction that wrote its scalar operands, and from m0's own write.
-// (m0 is a register that the compiler allots to nothing, and it warns of the
-// name; its own writes of m0 are merged across what does not say that it is written.)
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void dma16(u4 rsrc, uint32_t offset, uint32_t more, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 :
-                 : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(more))
-                 : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
-// Until at most LATER of this wave's loads are on their way.
-template <int LATER>
-__device__ __forceinline__ void wait_dma() {
-    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LATER) : "memory");
-}
-
-// A barrier that orders LDS alone: loads stay in flight across it.
-__device__ __forceinline__ void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // What a workgroup works on: a tile of query rows of one sequence and key
