@@ -41,6 +41,7 @@ SOURCES = [
     ("affine_rows.hip", ["-x", "hip"]),
     ("affine_tile.hip", ["-x", "hip"]),
     ("attn_linear.hip", ["-x", "hip"]),
+    ("attn_linear_chunks.hip", ["-x", "hip"]),
     ("attn_paged.hip", ["-x", "hip"]),
     ("conv_causal.hip", ["-x", "hip"]),
     ("dense_mfma.hip", ["-x", "hip"]),

@@ -12,36 +12,20 @@
 #include <hip/hip_runtime.h>
 
 #include "kernels.hpp"
+#include "linear_common.hpp"
 #include "sequences.hpp"
 
 namespace qmr {
 namespace {
 
+using linear::gate_of;
+using linear::log_decay;
+using linear::Quad;
+using linear::quad_at;
+using linear::sigmoid;
+
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-
-// Four FP32 of a row, which need not lie on 16 bytes.
-struct Quad {
-    float x[4];
-};
-
-__device__ __forceinline__ Quad quad_at(const float *p, bool there) {
-    return there ? *reinterpret_cast<const Quad *>(p) : Quad{};
-}
-
-// The log of the decay of value head h at token t.
-__device__ __forceinline__ float log_decay(const LinearArgs &a, size_t t, uint32_t h) {
-    const float x = a.a[t * a.a_stride + h];
-    if (!a.gates) return x;
-    const float y = x + a.dt_bias[h];
-    // Past 20, log(1 + e^y) is y to 2^-33 of it.
-    return -expf(a.a_log[h]) * (y > 20.f ? y : log1pf(expf(y)));
-}
-
-__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
-
-// What the output norm multiplies an element of its head by, apart from 1 / rms.
-__device__ __forceinline__ float gate_of(float z, float norm) { return norm * z * sigmoid(z); }
 
 // Token after token, a workgroup a sequence and value head. A thread has R rows
 // of four columns of the state in registers, CG threads a row. One sum over
@@ -193,7 +177,8 @@ void go_tokens(const LinearArgs &a, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_attn_linear(const LinearArgs &a, const DeviceLimits &, hipStream_t stream) {
+hipError_t launch_attn_linear(const LinearArgs &a, const LinearPlan &pl, void *workspace, hipStream_t stream) {
+    if (pl.chunks) return launch_linear_chunks(a, pl, workspace, stream);
     if (a.dv <= 32) {
         go_tokens<8>(a, stream);
     } else if (a.dv <= 64) {
@@ -204,6 +189,10 @@ hipError_t launch_attn_linear(const LinearArgs &a, const DeviceLimits &, hipStre
         go_tokens<64>(a, stream);
     }
     return hipGetLastError();
+}
+
+const char *linear_kernel_name(const LinearPlan &pl) {
+    return pl.chunks ? "linear_scan_kernel" : "attn_linear_tokens_kernel";
 }
 
 }  // namespace qmr

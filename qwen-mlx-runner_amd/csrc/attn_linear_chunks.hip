@@ -1,0 +1,797 @@
+// Linear attention over chunks of 32 tokens, on the matrix cores (attn_linear.hip
+// says what is computed). In a chunk, with G the running sum of the log decays
+// in it, S the state before it and c the factor that normalises a row:
+//
+//   A_ij = beta_i e^(G_i - G_j) k_i . k_j  (j < i)          T = (I + A)^-1
+//   R_i  = beta_i (v_i - e^(G_i) S^T k_i)                    U = T R
+//   M_ij = scale e^(G_i - G_j) q_i . k_j  (j <= i)
+//   o_i  = scale e^(G_i) S^T q_i + (M U)_i
+//   S'   = e^(G_32) S + sum_j e^(G_32 - G_j) k_j U_j^T
+//
+// (without the delta rule U = V). Exponents are differences that are never
+// positive where decays do not grow, so nothing overflows on the way.
+//
+// Three launches. linear_prepare_kernel has a workgroup a chunk and key head:
+// everything that does not depend on the state, all chunks at once, left in the
+// workspace as the operands that the matrix instructions take. linear_scan_kernel
+// goes through a sequence's chunks: a workgroup has some 16-column tiles of a
+// value head's state, a wave one, in its accumulators; the next chunk's operands
+// come to LDS meanwhile. linear_norm_kernel norms the outputs, whose rows the
+// workgroups of a head share.
+//
+// Columns of the state do not meet until the output norm, so a wave needs
+// nothing of another one, and S, R and U need not leave its registers: a product
+// leaves column n of its 16x16 tiles in lanes n, n + 16, n + 32 and n + 48, four
+// rows each, and that is where the next product takes its operand from if its
+// left side counts the rows in the same order (slot 8g + 4h + i of 32 is row
+// 16h + 4g + i). The operands in the workspace do.
+//
+// Precision: FP32 values are two f16 terms, the second what the first leaves
+// (22 bits), a product three matrix instructions (the product of the two second
+// terms, 2^-22 of it, is left out); sums are FP32. One FP32 matrix instruction
+// would take 5.3 times as long as those three. Rows of q and k are scaled by
+// powers of two to 2^3..2^4, a column of S, R and U to at most 2^15, so that the
+// terms stay among the normal f16 numbers as far as they matter.
+//
+// The chunk's algebra has products of tokens with later ones, by zero: a value
+// that is not finite would reach tokens before it. A chunk that has some, or
+// whose T is not small (keys longer than 1, where the recurrence itself is not
+// stable), is done token after token by the same waves.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "kernels.hpp"
+#include "linear_common.hpp"
+#include "sequences.hpp"
+#include "wave_ops.hpp"
+
+namespace qmr {
+namespace {
+
+using linear::gate_of;
+using linear::log_decay;
+using linear::Quad;
+using linear::quad_at;
+using linear::sigmoid;
+using wave::dma16;
+using wave::f4;
+using wave::h8;
+using wave::kRsrcWord3;
+using wave::lds_barrier;
+using wave::less_half;
+using wave::two_halves;
+using wave::u4;
+using wave::wait_dma;
+using wave::wave_lds_sync;
+
+constexpr uint32_t kChunk = 32;
+constexpr uint32_t kTile = 1024;         // bytes of one f16 operand of 16 x 32
+constexpr uint32_t kOut = 0x80000000u;   // buffer offset past every range
+constexpr float kForget = -1000.f;       // e^-1000 is 0 in FP32 whatever it meets
+constexpr int kScore = 2;                // M's entries are products of scaled rows by 2^-kScore
+constexpr int kSolve = 4;                // T's entries are by 2^kSolve
+
+// A chunk's operands. Of a key head: Q [2 tiles of 16 tokens][blocks][2 terms],
+// K^T [2 * blocks tiles of 16 dims][2 terms], K as Q (delta rule). Of a value
+// head: M [2][2 terms], scalars, T as M (delta rule).
+constexpr uint32_t kScalars = 4 * kTile;  // where they stand
+enum Scalar : uint32_t { kBeta = 0, kX = 32, kQ = 64, kM = 96, kU = 128, kWhole = 160, kMost = 161, kWild = 162 };
+
+__device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+// Two terms of each side.
+__device__ __forceinline__ f4 mfma3(u4 ah, u4 al, u4 bh, u4 bl, f4 c) {
+    c = mfma(al, bh, c);
+    c = mfma(ah, bl, c);
+    return mfma(ah, bh, c);
+}
+
+// Eight values as terms, to nearest both.
+__device__ __forceinline__ void terms(const float (&x)[8], u4 &hi, u4 &lo) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        hi[i] = two_halves(x[2 * i], x[2 * i + 1]);
+        lo[i] = two_halves(less_half<0>(x[2 * i], hi[i]), less_half<1>(x[2 * i + 1], hi[i]));
+    }
+}
+
+// The largest of a column's four lanes.
+__device__ __forceinline__ float column_max(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ float column_sum(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+__device__ __forceinline__ int exponent(float x) {  // |x| < 2^it; 0 for what is not finite
+    return __builtin_amdgcn_frexp_expf(x);
+}
+
+__device__ __forceinline__ u4 rsrc_of(const void *p, uint32_t bytes) {
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    return u4{uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(at))),
+              uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(at >> 32) & 0xFFFFu)),
+              uint32_t(__builtin_amdgcn_readfirstlane(bytes)), kRsrcWord3};
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float *p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), 0, int(bytes), kRsrcWord3);
+}
+
+// Which chunks a pass has, and where their operands are.
+struct Pass {
+    unsigned char *operands;  // [chunk][k_heads * k_bytes + v_heads * v_bytes]
+    float *from, *to;         // a state [v_heads][dk][dv] that the last pass left, or this one leaves; the last one leaves none
+    uint32_t first, last;
+    uint32_t k_bytes, v_bytes;
+    uint32_t columns;         // workgroups of a head
+
+    __device__ unsigned char *of_key(const LinearArgs &a, uint32_t chunk, uint32_t h) const {
+        return operands + size_t(chunk - first) * (size_t(a.k_heads) * k_bytes + size_t(a.v_heads) * v_bytes) + size_t(h) * k_bytes;
+    }
+    __device__ unsigned char *of_value(const LinearArgs &a, uint32_t chunk, uint32_t h) const {
+        return of_key(a, chunk, a.k_heads) + size_t(h) * v_bytes;
+    }
+};
+
+constexpr int kPrepare = 256;
+
+template <int KB>
+struct PrepareLds {
+    static constexpr uint32_t kGram = 0;                        // [2][32][33] FP32: q k, k k
+    static constexpr uint32_t kRows = 2 * 32 * 33 * 4;          // [4][32] FP32 of rows
+    static constexpr uint32_t kRest = kRows + 4 * 32 * 4;       // terms of q and k, then each wave's own
+    static constexpr uint32_t kTerms = 4 * kTile * KB;          // of q, or of k
+    static constexpr uint32_t kA = 0, kMT = 32 * 36 * 4, kG = kMT + 8 * kTile, kWave = kG + 32 * 8 + 32 * 4;
+    static constexpr uint32_t kBytes = kRest + (2 * kTerms > 4 * kWave ? 2 * kTerms : 4 * kWave);
+};
+
+template <int KB, bool DELTA>
+__global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, Pass pass) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    using L = PrepareLds<KB>;
+    float *gram = reinterpret_cast<float *>(lds + L::kGram);
+    float *rows = reinterpret_cast<float *>(lds + L::kRows);  // c of k, c of q, bad
+    unsigned char *rest = lds + L::kRest;
+
+    const uint32_t chunk = pass.first + blockIdx.x, kh = blockIdx.y, tid = threadIdx.x;
+    const uint32_t l = tid % 64, w = __builtin_amdgcn_readfirstlane(tid / 64), g = l / 16, m = l % 16;
+    uint32_t s, part, first, count;
+    if (!seq::part_of(a.seq, chunk, kChunk, s, part)) return;
+    seq::tokens_of(a.seq, s, first, count);
+    const uint32_t t0 = part * kChunk, n = min(kChunk, count - t0);
+    const size_t token0 = size_t(first) + t0;
+    unsigned char *out = pass.of_key(a, chunk, kh);
+    constexpr uint32_t kOutKt = L::kTerms, kOutK = 2 * L::kTerms;
+
+    // Eight lanes a token: 4-dim pieces seg, seg + 8, ..
+    {
+        const uint32_t i = tid / 8, seg = tid % 8;
+        const bool real = i < n;
+        const float *qr = a.q + (token0 + i) * a.q_stride + size_t(kh) * a.dk;
+        const float *kr = a.k + (token0 + i) * a.k_stride + size_t(kh) * a.dk;
+        Quad x[2][KB];
+#pragma unroll
+        for (int u = 0; u < KB; ++u) {
+            const uint32_t d = (seg + 8 * u) * 4;
+            x[0][u] = quad_at(qr + d, real && d < a.dk);
+            x[1][u] = quad_at(kr + d, real && d < a.dk);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float top = 0.f, sum = 0.f;
+#pragma unroll
+            for (int u = 0; u < KB; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    top = fmaxf(top, fabsf(x[r][u].x[j]));
+                    sum = fmaf(x[r][u].x[j], x[r][u].x[j], sum);
+                }
+#pragma unroll
+            for (int d = 1; d < 8; d *= 2) {
+                top = fmaxf(top, __shfl_xor(top, d));
+                sum += __shfl_xor(sum, d);
+            }
+            const int p = top > 0.f ? min(4 - exponent(top), 120) : 0;  // the largest to 2^3..2^4
+            const float f = a.qk_eps > 0.f ? 1.f / sqrtf(sum + a.qk_eps) : 1.f;
+            if (seg == 0) {
+                rows[32 * (1 - r) + i] = top > 0.f ? ldexpf(f, -p) : 0.f;
+                rows[64 + 32 * r + i] = sum < INFINITY ? 0.f : 1.f;
+            }
+            const float by = ldexpf(1.f, p);
+#pragma unroll
+            for (int u = 0; u < KB; ++u) {
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float b0 = x[r][u].x[2 * j] * by, b1 = x[r][u].x[2 * j + 1] * by;
+                    hi[j] = two_halves(b0, b1);
+                    lo[j] = two_halves(less_half<0>(b0, hi[j]), less_half<1>(b1, hi[j]));
+                }
+                const uint32_t at = ((i / 16 * KB + u) * 2) * kTile + (seg % 4 * 16 + i % 16) * 16 + seg / 4 * 8;
+                unsigned char *to = rest + r * L::kTerms + at;
+                *reinterpret_cast<uint2 *>(to) = uint2{hi[0], hi[1]};
+                *reinterpret_cast<uint2 *>(to + kTile) = uint2{lo[0], lo[1]};
+                if (r == 0 || DELTA) {
+                    to = out + (r ? kOutK : 0) + at;
+                    *reinterpret_cast<uint2 *>(to) = uint2{hi[0], hi[1]};
+                    *reinterpret_cast<uint2 *>(to + kTile) = uint2{lo[0], lo[1]};
+                }
+            }
+        }
+    }
+    __syncthreads();
+
+    // K^T: four dims and eight tokens at a time.
+    for (uint32_t it = tid; it < 64 * KB; it += kPrepare) {
+        const uint32_t quad = it / 32 * 4 + it % 4, gt = it / 4 % 4, hl = it / 16 % 2;
+        uint2 x[2][4];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[tt][e] = *reinterpret_cast<const uint2 *>(rest + L::kTerms + ((tt * KB + quad / 8) * 2 + hl) * kTile +
+                                                            (quad % 4 * 16 + 4 * gt + e) * 16 + quad / 4 % 2 * 8);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            u4 y;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint2 x0 = x[k / 2][k % 2 * 2], x1 = x[k / 2][k % 2 * 2 + 1];
+                const uint32_t lo = d < 2 ? x0.x : x0.y, hi = d < 2 ? x1.x : x1.y;
+                y[k] = __builtin_amdgcn_perm(hi, lo, d % 2 ? 0x07060302u : 0x05040100u);
+            }
+            *reinterpret_cast<u4 *>(out + kOutKt + (quad / 4 * 2 + hl) * kTile + (gt * 16 + quad % 4 * 4 + d) * 16) = y;
+        }
+    }
+    // Products of rows: tiles (0, 0), (1, 0), (1, 1).
+    if (w < 3) {
+        const uint32_t rt = w > 0, ct = w == 2;
+        f4 qk{}, kk{};
+        auto term = [&](uint32_t r, uint32_t tile, uint32_t kb, uint32_t hl) {
+            return *reinterpret_cast<const u4 *>(rest + r * L::kTerms + ((tile * KB + kb) * 2 + hl) * kTile + l * 16);
+        };
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            const u4 bh = term(1, ct, kb, 0), bl = term(1, ct, kb, 1);
+            qk = mfma3(term(0, rt, kb, 0), term(0, rt, kb, 1), bh, bl, qk);
+            if constexpr (DELTA) kk = mfma3(term(1, rt, kb, 0), term(1, rt, kb, 1), bh, bl, kk);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            gram[(rt * 16 + 4 * g + i) * 33 + ct * 16 + m] = qk[i];
+            if constexpr (DELTA) gram[(32 + rt * 16 + 4 * g + i) * 33 + ct * 16 + m] = kk[i];
+        }
+    }
+    __syncthreads();
+
+    // A wave a value head of this key head.
+    unsigned char *own = rest + w * L::kWave;
+    float *A = reinterpret_cast<float *>(own + L::kA);  // [32][36]
+    unsigned char *mt = own + L::kMT;                   // M, T
+    double *Gs = reinterpret_cast<double *>(own + L::kG);
+    float *by_row = reinterpret_cast<float *>(own + L::kG + 32 * 8);
+    const uint32_t group = a.v_heads / a.k_heads, j = l % 32;
+    const float ck = rows[j], cq = rows[32 + j];
+    const bool bad_rows = rows[64 + j] + rows[96 + j] > 0.f;
+    float top = ck;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    const float part_of_top = top > 0.f ? ck / top : 0.f;
+    for (uint32_t vh = w; vh < group; vh += kPrepare / 64) {
+        const uint32_t h = kh * group + vh;
+        const bool real = j < n;
+        float step = real ? log_decay(a, token0 + j, h) : 0.f;
+        step = step < kForget ? kForget : step;
+        const float beta = DELTA ? (real ? sigmoid(a.b[(token0 + j) * a.b_stride + h]) : 0.f) : 1.f;
+        double G = step;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const double before = __shfl_up(G, d, 32);
+            if (j >= uint32_t(d)) G += before;
+        }
+        const double all = __shfl(G, 31, 32);
+        Gs[j] = G;
+        by_row[j] = beta * ck;
+        wave_lds_sync();
+        bool bad = bad_rows;
+#pragma unroll 4
+        for (uint32_t r = 0; r < 16; ++r) {
+            const uint32_t i = 2 * r + l / 32;
+            const float e = i >= j ? expf(float(Gs[i] - G)) : 0.f;
+            const float x = i >= j ? ldexpf(gram[i * 33 + j], -kScore) * part_of_top * e : 0.f;
+            bad |= !(fabsf(x) < 60000.f);
+            const uint32_t hi = two_halves(x, x), lo = two_halves(less_half<0>(x, hi), 0.f);
+            unsigned char *to = mt + i / 16 * 2 * kTile + (j % 16 / 4 * 16 + i % 16) * 16 + j / 16 * 8 + j % 4 * 2;
+            *reinterpret_cast<uint16_t *>(to) = uint16_t(hi);
+            *reinterpret_cast<uint16_t *>(to + kTile) = uint16_t(lo);
+            if constexpr (DELTA) A[i * 36 + j] = i > j ? by_row[i] * ck * gram[(32 + i) * 33 + j] * e : 0.f;
+        }
+        float rows_of_t = 1.f;
+        if constexpr (DELTA) {
+            wave_lds_sync();
+            // Column j of T, row after row.
+            float x[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                float even = uint32_t(i) == j ? 1.f : 0.f, odd = 0.f;
+#pragma unroll
+                for (int c = 0; c < i; ++c) {
+                    if (c % 2) odd = fmaf(-A[i * 36 + c], x[c], odd);
+                    else even = fmaf(-A[i * 36 + c], x[c], even);
+                }
+                x[i] = even + odd;
+                asm volatile("" : "+v"(x[i]) : : "memory");  // or all of A is loaded at once
+            }
+            rows_of_t = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                bad |= !(fabsf(x[i]) < 2.f);
+                rows_of_t = fmaxf(rows_of_t, fabsf(x[i]));
+                const float t = ldexpf(x[i], kSolve);
+                const uint32_t hi = two_halves(t, t), lo = two_halves(less_half<0>(t, hi), 0.f);
+                unsigned char *to = mt + (4 + l / 32) * kTile + i / 16 * 2 * kTile + (j % 16 / 4 * 16 + i % 16) * 16 + j / 16 * 8 + j % 4 * 2;
+                *reinterpret_cast<uint16_t *>(to) = uint16_t(l < 32 ? hi : lo);
+            }
+            // A row of T adds up to no more than its columns' largest do.
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) rows_of_t += __shfl_xor(rows_of_t, d);
+        }
+        wave_lds_sync();
+        const float grown = expf(float(G)), left = expf(float(all - G)), whole = expf(float(all));
+        const float of_q = a.scale * grown * cq, of_x = beta * grown * ck, of_u = left * ck;
+        const float of_m = ldexpf(a.scale * cq * top, kScore);
+        bad |= !(fabsf(of_q) < INFINITY) || !(fabsf(of_x) < INFINITY) || !(of_u < INFINITY) || !(fabsf(of_m) < INFINITY) ||
+               !(whole < INFINITY);
+        float most = of_u;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+        const bool wild = __ballot(bad) != 0;
+        unsigned char *to = pass.of_value(a, chunk, h);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            *reinterpret_cast<u4 *>(to + p * kTile + l * 16) = *reinterpret_cast<const u4 *>(mt + p * kTile + l * 16);
+            if constexpr (DELTA)
+                *reinterpret_cast<u4 *>(to + kScalars + kTile + p * kTile + l * 16) =
+                    *reinterpret_cast<const u4 *>(mt + (4 + p) * kTile + l * 16);
+        }
+        float *scalars = reinterpret_cast<float *>(to + kScalars);
+        if (l < 32) {
+            scalars[kBeta + j] = beta;
+            scalars[kX + j] = of_x;
+            scalars[kQ + j] = of_q;
+            scalars[kM + j] = of_m;
+            scalars[kU + j] = of_u;
+        }
+        if (l == 0) {
+            scalars[kWhole] = whole;
+            // What a chunk adds to a column of the state, at most, by the largest
+            // of R (32 tokens, dims up to 2^4).
+            scalars[kMost] = ldexpf(most * rows_of_t, 9);
+            reinterpret_cast<uint32_t *>(scalars)[kWild] = wild;
+        }
+        wave_lds_sync();
+    }
+}
+
+// One wave's columns of a chunk, token after token, for chunks whose algebra
+// would not hold. S: the state itself, tile t's lane has rows 16t + 4g + i.
+template <int TD>
+__device__ void tokens_of_chunk(const LinearArgs &a, size_t token0, uint32_t n, uint32_t h, uint32_t col, f4 (&S)[TD]) {
+    const uint32_t g = threadIdx.x % 64 / 16, kh = h / (a.v_heads / a.k_heads);
+    const bool has = col < a.dv;
+    for (uint32_t t = 0; t < n; ++t) {
+        const size_t token = token0 + t;
+        const float *qr = a.q + token * a.q_stride + size_t(kh) * a.dk, *kr = a.k + token * a.k_stride + size_t(kh) * a.dk;
+        float kk = 0.f, qq = 0.f, qk = 0.f, sk = 0.f, sq = 0.f;
+#pragma unroll
+        for (int td = 0; td < TD; ++td) {
+            const uint32_t d = 16 * td + 4 * g;
+            const Quad q = quad_at(qr + d, d < a.dk), k = quad_at(kr + d, d < a.dk);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                kk = fmaf(k.x[i], k.x[i], kk);
+                qq = fmaf(q.x[i], q.x[i], qq);
+                qk = fmaf(q.x[i], k.x[i], qk);
+                sk = fmaf(S[td][i], k.x[i], sk);
+                sq = fmaf(S[td][i], q.x[i], sq);
+            }
+        }
+        kk = column_sum(kk);
+        qq = column_sum(qq);
+        qk = column_sum(qk);
+        sk = column_sum(sk);
+        sq = column_sum(sq);
+        const float decay = expf(log_decay(a, token, h));
+        const float v = has ? a.v[token * a.v_stride + size_t(h) * a.dv + col] : 0.f;
+        const float fk = a.qk_eps > 0.f ? 1.f / sqrtf(kk + a.qk_eps) : 1.f;
+        const float fq = (a.qk_eps > 0.f ? 1.f / sqrtf(qq + a.qk_eps) : 1.f) * a.scale;
+        const float u = a.delta ? sigmoid(a.b[token * a.b_stride + h]) * (v - decay * (sk * fk)) : v;
+        if (g == 0 && has)
+            a.out[token * a.out_stride + size_t(h) * a.dv + col] = fq * (decay * sq + qk * fk * u);
+#pragma unroll
+        for (int td = 0; td < TD; ++td) {
+            const uint32_t d = 16 * td + 4 * g;
+            const Quad k = quad_at(kr + d, d < a.dk);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S[td][i] = fmaf(k.x[i] * fk, u, decay * S[td][i]);
+        }
+    }
+}
+
+template <int KB, int NC, bool DELTA>
+struct ScanLds {
+    static constexpr uint32_t kKey = (DELTA ? 12 : 8) * kTile * KB, kValue = (DELTA ? 9 : 5) * kTile;
+    static constexpr uint32_t kStage = kKey + kValue;
+    static constexpr uint32_t kStages = 2 * kStage <= 150 * 1024 ? 2 : 1;
+    static constexpr uint32_t kBytes = kStages * kStage;
+};
+
+template <int KB, int NC, bool DELTA>
+__global__ __launch_bounds__(NC * 64) void linear_scan_kernel(LinearArgs a, Pass pass) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    using L = ScanLds<KB, NC, DELTA>;
+    constexpr int TD = 2 * KB;
+    const uint32_t lds0 = uint32_t(uintptr_t((__attribute__((address_space(3))) unsigned char *)lds));
+    const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), g = l / 16;
+
+    // Workgroups go to the eight dies in turn: all those of a key head to one,
+    // whose cache then has its operands once.
+    const uint32_t group = a.v_heads / a.k_heads, of_unit = group * pass.columns;
+    const uint32_t unit = blockIdx.x % 8 + blockIdx.x / 8 / of_unit * 8, in_unit = blockIdx.x / 8 % of_unit;
+    if (unit >= a.seq.seqs * a.k_heads) return;
+    const uint32_t s = unit / a.k_heads, kh = unit % a.k_heads, h = kh * group + in_unit / pass.columns;
+    const uint32_t tile = in_unit % pass.columns * NC + w, col = tile * 16 + l % 16;
+
+    uint32_t first, count;
+    seq::tokens_of(a.seq, s, first, count);
+    if (count == 0) return;
+    const uint32_t begin = seq::parts_before(a.seq, s, kChunk), end = begin + (count + kChunk - 1) / kChunk;
+    const uint32_t c0 = max(begin, pass.first), c1 = min(end, pass.last);
+    if (c0 >= c1) return;
+    const bool starts = c0 == begin, ends = c1 == end;
+    bool read;
+    const uint32_t slot = seq::slot_of(a.seq, s, read);
+
+    const uint32_t state_bytes = a.dk * a.dv * 4;
+    const bool has = col < a.dv;
+    float *pool = a.state + (size_t(slot == seq::kNoSlot ? 0 : slot) * a.v_heads + h) * a.dk * a.dv;
+    const float *from = starts ? pool : pass.from + size_t(h) * a.dk * a.dv;
+    // Of a buffer's rows these lanes have 4g + i of every 16; what is past the
+    // head's dimensions or the sequence's tokens is past the buffer.
+    const uint32_t state_at = has ? (4 * g * a.dv + col) * 4 : kOut;
+    const uint32_t values_at = has ? (4 * g * a.v_stride + col) * 4 : kOut, out_at = has ? (4 * g * a.out_stride + col) * 4 : kOut;
+    f4 S[TD];
+    {
+        const auto r = buffer_of(from, !starts || read ? state_bytes : 0);
+#pragma unroll
+        for (int t = 0; t < TD; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                S[t][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, int(state_at + (16 * t + i) * a.dv * 4), 0, 0));
+    }
+
+    auto fetch = [&](uint32_t chunk, uint32_t to) {
+        const u4 keys = rsrc_of(pass.of_key(a, chunk, kh), L::kKey), values = rsrc_of(pass.of_value(a, chunk, h), L::kValue);
+        constexpr int kPieces = L::kStage / kTile, kOfKey = L::kKey / kTile;
+        uint32_t piece = w * kTile;
+        asm volatile("" : "+s"(piece));  // counted here, not kept in registers for every piece
+#pragma unroll
+        for (int p = 0; p < kPieces; p += NC, piece += NC * kTile) {
+            if (p + NC <= kOfKey || piece < L::kKey) {
+                dma16(keys, l * 16, piece, to + piece);
+            } else if (p + NC <= kPieces || piece < L::kStage) {
+                dma16(values, l * 16, piece - L::kKey, to + piece);
+            }
+        }
+    };
+    float next[8];  // the values of the chunk to come: tokens 16h + 4g + i at 4h + i
+    auto load_values = [&](uint32_t chunk) {
+        const uint32_t t0 = (chunk - begin) * kChunk, n = min(kChunk, count - t0);
+        const auto r = buffer_of(a.v + (size_t(first) + t0) * a.v_stride + size_t(h) * a.dv, ((n - 1) * a.v_stride + a.dv) * 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            next[e] = __uint_as_float(
+                __builtin_amdgcn_raw_buffer_load_b32(r, int(values_at + (16 * (e / 4) + e % 4) * a.v_stride * 4), 0, 0));
+    };
+
+    // S is kept by 2^scale, a column's own.
+    int scale = 0;
+    auto biggest = [&] {
+        float top = 0.f;
+#pragma unroll
+        for (int t = 0; t < TD; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(S[t][i]));
+        return column_max(top);
+    };
+    auto rescale = [&](int to) {
+#pragma unroll
+        for (int t = 0; t < TD; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S[t][i] = ldexpf(S[t][i], to - scale);
+        scale = to;
+    };
+    auto fitting = [](float top) { return max(-113, min(15 - exponent(top), 110)); };
+    rescale(fitting(biggest()));
+
+    if constexpr (L::kStages == 2) fetch(c0, lds0);
+    load_values(c0);
+    for (uint32_t c = c0; c < c1; ++c) {
+        const uint32_t at = L::kStages == 2 ? (c - c0) % 2 * L::kStage : 0;
+        if constexpr (L::kStages == 1) {
+            lds_barrier();  // nobody reads the last chunk's
+            fetch(c, lds0);
+        }
+        wait_dma<0>();
+        lds_barrier();
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = next[e];
+        if (c + 1 < c1) {
+            if constexpr (L::kStages == 2) fetch(c + 1, lds0 + (L::kStage - at));
+            load_values(c + 1);
+        }
+        if (tile * 16 >= a.dv) continue;
+
+        const unsigned char *keys = lds + at, *values = keys + L::kKey;
+        const float *scalars = reinterpret_cast<const float *>(values + kScalars);
+        const uint32_t t0 = (c - begin) * kChunk, n = min(kChunk, count - t0);
+        float odd = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) odd = fmaf(v[e], 0.f, odd);
+        if (reinterpret_cast<const uint32_t *>(scalars)[kWild] != 0 || __ballot(odd != 0.f) != 0) {
+            rescale(0);
+            tokens_of_chunk<TD>(a, size_t(first) + t0, n, h, col, S);
+            rescale(fitting(biggest()));
+            continue;
+        }
+        auto tile_at = [&](const unsigned char *p) { return *reinterpret_cast<const u4 *>(p + l * 16); };
+        auto of_rows = [&](uint32_t which, int half) { return *reinterpret_cast<const f4 *>(scalars + which + 16 * half + 4 * g); };
+        const float whole = scalars[kWhole], most = scalars[kMost];
+        const float top = biggest();
+
+        // S^T k and S^T q.
+        f4 x[2] = {}, o[2] = {};
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            float both[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) both[e] = S[2 * kb + e / 4][e % 4];
+            u4 sh, sl;
+            terms(both, sh, sl);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t p = (half * KB + kb) * 2 * kTile;
+                if constexpr (DELTA) {
+                    const unsigned char *k = keys + 8 * kTile * KB + p;
+                    x[half] = mfma3(tile_at(k), tile_at(k + kTile), sh, sl, x[half]);
+                }
+                o[half] = mfma3(tile_at(keys + p), tile_at(keys + p + kTile), sh, sl, o[half]);
+            }
+        }
+        // R, by 2^up.
+        float r[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const f4 beta = of_rows(kBeta, half), of_x = of_rows(kX, half);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                r[4 * half + i] = DELTA ? beta[i] * v[4 * half + i] - of_x[i] * ldexpf(x[half][i], -scale) : v[4 * half + i];
+        }
+        float r_top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r_top = fmaxf(r_top, fabsf(r[e]));
+        r_top = column_max(r_top);
+        const int up = max(-113, min(13 - exponent(r_top), 110));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = ldexpf(r[e], up);
+        u4 uh, ul;
+        terms(r, uh, ul);
+        // U, by 2^up (and 2^kSolve until its terms are made).
+        float u[8];
+        int u_up = up;
+        if constexpr (DELTA) {
+            f4 y[2] = {};
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const unsigned char *t = values + kScalars + kTile + half * 2 * kTile;
+                y[half] = mfma3(tile_at(t), tile_at(t + kTile), uh, ul, y[half]);
+            }
+            float small[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                u[e] = y[e / 4][e % 4];
+                small[e] = u[e] * 0.00390625f;  // 2^-8: below 2^15 while rows of T add up to 2^6
+            }
+            terms(small, uh, ul);
+            u_up = up + kSolve;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = r[e];
+        }
+        // The next state's scale: below 2^15 whatever the chunk adds.
+        const int to = min(fitting(ldexpf(whole * top, -scale) + most * r_top), scale + 100);
+        // M U and the outputs.
+        {
+            const auto rows = buffer_of(a.out + (size_t(first) + t0) * a.out_stride + size_t(h) * a.dv,
+                                        ((n - 1) * a.out_stride + a.dv) * 4);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const unsigned char *p = values + half * 2 * kTile;
+                const f4 y = mfma3(tile_at(p), tile_at(p + kTile), uh, ul, f4{});
+                const f4 of_q = of_rows(kQ, half), of_m = of_rows(kM, half);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float out = of_q[i] * ldexpf(o[half][i], -scale) + of_m[i] * ldexpf(y[i], (DELTA ? 8 : 0) - u_up);
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(out), rows, int(out_at + (16 * half + i) * a.out_stride * 4),
+                                                          0, 0);
+                }
+            }
+        }
+        // The next state.
+        const float keep = ldexpf(whole, to - scale);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const f4 of_u = of_rows(kU, half);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[4 * half + i] = u[4 * half + i] * ldexpf(of_u[i], to - u_up);
+        }
+        terms(u, uh, ul);
+#pragma unroll
+        for (int t = 0; t < TD; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S[t][i] *= keep;
+            const unsigned char *p = keys + 4 * kTile * KB + t * 2 * kTile;
+            S[t] = mfma3(tile_at(p), tile_at(p + kTile), uh, ul, S[t]);
+        }
+        scale = to;
+    }
+    wait_dma<0>();  // LDS is given back
+    if (tile * 16 >= a.dv || (ends ? !a.keep || slot == seq::kNoSlot : pass.to == nullptr)) return;
+    rescale(0);
+    const auto r = buffer_of(ends ? pool : pass.to + size_t(h) * a.dk * a.dv, state_bytes);
+#pragma unroll
+    for (int t = 0; t < TD; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(S[t][i]), r, int(state_at + (16 * t + i) * a.dv * 4), 0, 0);
+}
+
+constexpr int kNorm = 256;
+
+// The RMS norm and gate of the outputs, where they are: `lanes` lanes a head's
+// row of a token. A workgroup has a chunk's tokens and `heads` heads.
+__global__ __launch_bounds__(kNorm) void linear_norm_kernel(LinearArgs a, uint32_t first_chunk, uint32_t lanes, uint32_t heads) {
+    uint32_t s, part, first, count;
+    if (!seq::part_of(a.seq, first_chunk + blockIdx.x, kChunk, s, part)) return;
+    seq::tokens_of(a.seq, s, first, count);
+    const uint32_t t0 = part * kChunk, n = min(kChunk, count - t0);
+    const uint32_t h0 = blockIdx.y * heads, own = min(heads, a.v_heads - h0);
+    const uint32_t lane = threadIdx.x % lanes, col = lane * 4;
+    const bool has = col < a.dv;
+    const Quad norm = quad_at(a.norm + col, has);
+    for (uint32_t row = threadIdx.x / lanes; row < n * own; row += kNorm / lanes) {
+        const size_t token = size_t(first) + t0 + row / own;
+        const uint32_t h = h0 + row % own;
+        float *out = a.out + token * a.out_stride + size_t(h) * a.dv + col;
+        Quad o = quad_at(out, has);
+        const Quad z = quad_at(a.z + token * a.z_stride + size_t(h) * a.dv + col, has);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum = fmaf(o.x[i], o.x[i], sum);
+        for (uint32_t d = 1; d < lanes; d *= 2) sum += __shfl_xor(sum, d);
+        const float f = 1.f / sqrtf(sum / float(a.dv) + a.out_eps);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o.x[i] = o.x[i] * f * gate_of(z.x[i], norm.x[i]);
+        if (has) *reinterpret_cast<Quad *>(out) = o;
+    }
+}
+
+template <int KB, bool DELTA>
+hipError_t go_prepare(const LinearArgs &a, const Pass &pass, hipStream_t stream) {
+    const auto kernel = linear_prepare_kernel<KB, DELTA>;
+    constexpr uint32_t lds = PrepareLds<KB>::kBytes;
+    const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
+    if (e != hipSuccess) return e;
+    kernel<<<dim3(pass.last - pass.first, a.k_heads), kPrepare, lds, stream>>>(a, pass);
+    return hipGetLastError();
+}
+
+template <int KB, int NC, bool DELTA>
+hipError_t go_scan(const LinearArgs &a, const Pass &pass, hipStream_t stream) {
+    const auto kernel = linear_scan_kernel<KB, NC, DELTA>;
+    constexpr uint32_t lds = ScanLds<KB, NC, DELTA>::kBytes;
+    const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
+    if (e != hipSuccess) return e;
+    const uint32_t units = (a.seq.seqs * a.k_heads + 7) / 8 * 8;
+    kernel<<<units * (a.v_heads / a.k_heads) * pass.columns, NC * 64, lds, stream>>>(a, pass);
+    return hipGetLastError();
+}
+
+template <int KB, bool DELTA>
+hipError_t go_pass(const LinearArgs &a, const LinearPlan &pl, const Pass &pass, hipStream_t stream) {
+    const hipError_t e = go_prepare<KB, DELTA>(a, pass, stream);
+    if (e != hipSuccess) return e;
+    switch (pl.columns) {
+        case 2: return go_scan<KB, 2, DELTA>(a, pass, stream);
+        case 4: return go_scan<KB, 4, DELTA>(a, pass, stream);
+        default: return go_scan<KB, 8, DELTA>(a, pass, stream);
+    }
+}
+
+}  // namespace
+
+LinearPlan plan_linear(const LinearArgs &a, const DeviceLimits &lim, size_t limit, uint32_t form, uint32_t columns) {
+    LinearPlan pl;
+    const Sequences &q = a.seq;
+    const uint32_t longest = std::min(q.most, q.tokens);
+    if (form == 1 || (form == 0 && longest < 16)) return pl;
+    // Rows that a buffer's 32-bit offsets reach over a chunk.
+    if (a.v_stride > 1u << 22 || a.out_stride > 1u << 22) return pl;
+    const uint32_t tiles = (a.dv + 15) / 16;
+    pl.blocks = a.dk <= 64 ? 2 : a.dk <= 128 ? 4 : 8;
+    pl.columns = columns ? columns : 2;
+    pl.parts = uint32_t(std::min<uint64_t>(q.tokens, uint64_t(q.tokens) / kChunk + q.seqs));
+    pl.k_bytes = size_t(a.delta ? 12 : 8) * kTile * pl.blocks;
+    pl.v_bytes = size_t(a.delta ? 9 : 5) * kTile;
+    if (columns == 0)
+        while (pl.columns < 8 && uint64_t(std::min(q.seqs, pl.parts)) * a.v_heads * ((tiles + pl.columns - 1) / pl.columns) >
+                                     2 * uint64_t(lim.num_cus))
+            pl.columns *= 2;
+    const size_t each = a.k_heads * pl.k_bytes + a.v_heads * pl.v_bytes;
+    limit = std::min(limit, size_t(256) << 20);
+    pl.per_pass = pl.parts;
+    if (each * pl.parts > limit) {
+        pl.carry_bytes = (size_t(a.v_heads) * a.dk * a.dv * 4 + 255) / 256 * 256;
+        if (limit < 2 * pl.carry_bytes + each) return LinearPlan{};
+        pl.per_pass = uint32_t((limit - 2 * pl.carry_bytes) / each);
+    }
+    pl.workspace = 2 * pl.carry_bytes + each * pl.per_pass;
+    pl.chunks = true;
+    return pl;
+}
+
+// The workspace holds the operands of so many chunks; more go in passes, and
+// the state of a sequence that a pass leaves unfinished goes from one to the
+// next.
+hipError_t launch_linear_chunks(const LinearArgs &a, const LinearPlan &pl, void *workspace, hipStream_t stream) {
+    Pass pass{};
+    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    pass.operands = ws + 2 * pl.carry_bytes;
+    pass.k_bytes = uint32_t(pl.k_bytes);
+    pass.v_bytes = uint32_t(pl.v_bytes);
+    pass.columns = ((a.dv + 15) / 16 + pl.columns - 1) / pl.columns;
+    hipError_t e = hipSuccess;
+    uint32_t turn = 0;
+    for (uint32_t c = 0; c < pl.parts && e == hipSuccess; c += pl.per_pass, ++turn) {
+        pass.first = c;
+        pass.last = std::min(pl.parts, c + pl.per_pass);
+        pass.from = reinterpret_cast<float *>(ws + (turn % 2) * pl.carry_bytes);
+        pass.to = pass.last < pl.parts ? reinterpret_cast<float *>(ws + (1 - turn % 2) * pl.carry_bytes) : nullptr;
+        switch (pl.blocks * 2 + a.delta) {
+            case 4: e = go_pass<2, false>(a, pl, pass, stream); break;
+            case 5: e = go_pass<2, true>(a, pl, pass, stream); break;
+            case 8: e = go_pass<4, false>(a, pl, pass, stream); break;
+            case 9: e = go_pass<4, true>(a, pl, pass, stream); break;
+            case 16: e = go_pass<8, false>(a, pl, pass, stream); break;
+            default: e = go_pass<8, true>(a, pl, pass, stream); break;
+        }
+    }
+    if (e != hipSuccess || !(a.out_eps > 0.f)) return e;
+    uint32_t lanes = 2;
+    while (lanes * 4 < a.dv) lanes *= 2;
+    const uint32_t heads = 4;
+    linear_norm_kernel<<<dim3(pl.parts, (a.v_heads + heads - 1) / heads), kNorm, 0, stream>>>(a, 0, lanes, heads);
+    return hipGetLastError();
+}
+
+}  // namespace qmr

@@ -359,7 +359,25 @@ struct LinearArgs {
     float scale, qk_eps, out_eps;  // eps 0: no norm
     Sequences seq;
 };
-hipError_t launch_attn_linear(const LinearArgs &a, const DeviceLimits &lim, hipStream_t stream);
+// What a launch does, from sizes alone: where the sequences are is known on the
+// device.
+struct LinearPlan {
+    bool chunks = false;      // chunks of 32 tokens on the matrix cores; else token after token
+    uint32_t blocks = 0;      // 32-wide blocks of the key dimension, 2, 4 or 8
+    uint32_t columns = 0;     // 16-column tiles of a workgroup
+    uint32_t parts = 0;       // chunks of all sequences, at most
+    uint32_t per_pass = 0;    // chunks whose operands the workspace holds
+    size_t k_bytes = 0, v_bytes = 0;  // operands of a chunk, of one key and one value head
+    size_t carry_bytes = 0;   // a state between passes
+    size_t workspace = 0;
+};
+// `form` (tuning hook): 1 token after token, 2 chunks where they are possible, 0
+// the planner's choice; `columns` 2, 4 or 8, or 0.
+LinearPlan plan_linear(const LinearArgs &a, const DeviceLimits &lim, size_t workspace_limit, uint32_t form = 0,
+                       uint32_t columns = 0);
+hipError_t launch_attn_linear(const LinearArgs &a, const LinearPlan &pl, void *workspace, hipStream_t stream);
+hipError_t launch_linear_chunks(const LinearArgs &a, const LinearPlan &pl, void *workspace, hipStream_t stream);
+const char *linear_kernel_name(const LinearPlan &pl);
 
 // A token from each row of logits. See sample_logits.hip.
 struct SampleArgs {

@@ -79,6 +79,10 @@ struct qmr_device {
     // Workspace of the paged attention's key ranges.
     unsigned char *ws_attend = nullptr;
     size_t ws_attend_bytes = 0;
+    // Workspace of linear attention's chunks: their operands, and states
+    // between passes over them.
+    unsigned char *ws_linear = nullptr;
+    size_t ws_linear_bytes = 0;
     // This GPU's copy of the static scratch (the workspace of
     // qmr_encode_static, which allocates nothing), and how many of its
     // leading bytes may be non-zero (shared by every handle on the GPU).
@@ -923,7 +927,7 @@ void check_linear_views(const std::string &name, qmr_buffer *const *buffers, con
 
 // conv_causal, attn_linear and sample_logits.
 hipError_t launch_linear(qmr_device *dev, const std::string &name, qmr_buffer *const *buffers, const size_t *offsets,
-                         const uint32_t *p, unsigned char *) {
+                         const uint32_t *p, unsigned char *fixed) {
     auto ptr = [&](size_t i) -> char * { return static_cast<char *>(buffers[i]->ptr) + (offsets ? offsets[i] : 0); };
     auto f32 = [&](size_t i) { return reinterpret_cast<float *>(ptr(i)); };
     auto u32 = [&](size_t i) { return reinterpret_cast<uint32_t *>(ptr(i)); };
@@ -979,8 +983,26 @@ hipError_t launch_linear(qmr_device *dev, const std::string &name, qmr_buffer *c
     std::memcpy(&a.qk_eps, &p[17], 4);
     std::memcpy(&a.out_eps, &p[18], 4);
     a.seq = {u32(9), u32(10), p[0], p[1], p[13], p[19]};
+    const qmr::GemvPlan f = dev->forced_plan;
+    const bool forced = f.rr == -8 && f.ks > 0;
+    // Token after token needs no workspace: the static scratch always has room
+    // for a plan.
+    const qmr::LinearPlan pl = qmr::plan_linear(a, dev->limits, fixed ? QMR_STATIC_SCRATCH_BYTES : SIZE_MAX,
+                                                forced ? uint32_t(f.ks / 100) : 0, forced ? uint32_t(f.ks % 100) : 0);
+    if (fixed) {
+        check_static_scratch(pl.workspace, "linear attention's operands");
+        if (pl.workspace) mark_static_dirty(dev, pl.workspace);
+    } else if (pl.workspace > dev->ws_linear_bytes) {
+        check_hip(hipStreamSynchronize(dev->stream), "hipStreamSynchronize");
+        if (dev->ws_linear) hipFree(dev->ws_linear);
+        dev->ws_linear = nullptr;
+        dev->ws_linear_bytes = 0;
+        check_hip(hipMalloc(&dev->ws_linear, pl.workspace), "hipMalloc (linear attention workspace)");
+        dev->ws_linear_bytes = pl.workspace;
+    }
+    dev->last_hip = qmr::linear_kernel_name(pl);
     start_gpu(dev);
-    return qmr::launch_attn_linear(a, dev->limits, dev->stream);
+    return qmr::launch_attn_linear(a, pl, fixed ? fixed : dev->ws_linear, dev->stream);
 }
 
 // rope_axes, kv_append_rope_* and attn_paged_*.
@@ -1156,6 +1178,7 @@ void qmr_device_close(qmr_device *device) {
     }
     if (device->ws_wide) hipFree(device->ws_wide);
     if (device->ws_attend) hipFree(device->ws_attend);
+    if (device->ws_linear) hipFree(device->ws_linear);
     if (device->ws_slots) hipFree(device->ws_slots);
     if (device->ws_counters) hipFree(device->ws_counters);
     if (device->status_host) hipHostFree(device->status_host);
@@ -1892,7 +1915,7 @@ int qmr_gemv_plan(const qmr_device *device, uint32_t rows, uint32_t cols, uint32
 size_t qmr_device_workspace_bytes(const qmr_device *device) {
     if (!device) return 0;
     return device->ws_slots_bytes + device->ws_counter_count * sizeof(uint32_t) +
-           device->ws_wide_bytes + device->ws_attend_bytes;
+           device->ws_wide_bytes + device->ws_attend_bytes + device->ws_linear_bytes;
 }
 
 size_t qmr_device_max_lds(const qmr_device *device) {

@@ -53,12 +53,25 @@ __device__ __forceinline__ bool part_of(const Sequences &q, uint32_t id, uint32_
         if (past) {
             const uint32_t at = __ffsll(static_cast<unsigned long long>(past)) - 1;
             s = base + at;
-            part = id - (__shfl(up_to, at) - __shfl(own, at));
+            part = id - (__builtin_amdgcn_readlane(up_to, at) - __builtin_amdgcn_readlane(own, at));
             return true;
         }
-        id -= __shfl(up_to, 63);
+        id -= __builtin_amdgcn_readlane(up_to, 63);
     }
     return false;
+}
+
+// The number that sequence s's first part has. For whole waves.
+__device__ __forceinline__ uint32_t parts_before(const Sequences &q, uint32_t s, uint32_t size) {
+    const uint32_t l = threadIdx.x % 64;
+    uint32_t sum = 0;
+    for (uint32_t base = 0; base < s; base += 64) {
+        uint32_t first = 0, count = 0;
+        if (base + l < s) tokens_of(q, base + l, first, count);
+        sum += (count + size - 1) / size;
+    }
+    for (uint32_t d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    return __builtin_amdgcn_readfirstlane(sum);
 }
 
 }  // namespace seq
