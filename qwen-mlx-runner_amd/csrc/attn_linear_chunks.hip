@@ -55,7 +55,10 @@ using linear::Quad;
 using linear::quad_at;
 using linear::sigmoid;
 using wave::dma16;
+using wave::dma4;
+using wave::f2;
 using wave::f4;
+using wave::h2;
 using wave::h8;
 using wave::kRsrcWord3;
 using wave::lds_barrier;
@@ -89,12 +92,25 @@ __device__ __forceinline__ f4 mfma3(u4 ah, u4 al, u4 bh, u4 bl, f4 c) {
     return mfma(ah, bh, c);
 }
 
-// Eight values as terms, to nearest both.
-__device__ __forceinline__ void terms(const float (&x)[8], u4 &hi, u4 &lo) {
+// Eight values as terms, to nearest both. `minus`: -1 that the compiler does
+// not see through, for the instruction that multiplies an f16 into FP32.
+__device__ __forceinline__ void terms(const float (&x)[8], float minus, u4 &hi, u4 &lo) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        hi[i] = two_halves(x[2 * i], x[2 * i + 1]);
-        lo[i] = two_halves(less_half<0>(x[2 * i], hi[i]), less_half<1>(x[2 * i + 1], hi[i]));
+        const h2 h = __builtin_convertvector((f2{x[2 * i], x[2 * i + 1]}), h2);
+        hi[i] = __builtin_bit_cast(uint32_t, h);
+        lo[i] = two_halves(__builtin_fmaf(float(h[0]), minus, x[2 * i]), __builtin_fmaf(float(h[1]), minus, x[2 * i + 1]));
+    }
+}
+
+// So many times: a matrix instruction, then others that may run beside it.
+template <int TIMES, int VALU, int LDS>
+__device__ __forceinline__ void in_turn() {
+#pragma unroll
+    for (int i = 0; i < TIMES; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if constexpr (LDS > 0) __builtin_amdgcn_sched_group_barrier(0x100, LDS, 0);
+        if constexpr (VALU > 0) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
     }
 }
 
@@ -430,17 +446,18 @@ __device__ void tokens_of_chunk(const LinearArgs &a, size_t token0, uint32_t n, 
 template <int KB, int NC, bool DELTA>
 struct ScanLds {
     static constexpr uint32_t kKey = (DELTA ? 12 : 8) * kTile * KB, kValue = (DELTA ? 9 : 5) * kTile;
-    static constexpr uint32_t kStage = kKey + kValue;
-    static constexpr uint32_t kStages = 2 * kStage <= 150 * 1024 ? 2 : 1;
+    static constexpr uint32_t kV = kChunk * NC * 16 * 4;  // the workgroup's columns of the values
+    static constexpr uint32_t kStage = kKey + kValue + kV;
+    static constexpr uint32_t kStages = 2 * kStage <= 160 * 1024 ? 2 : 1;
     static constexpr uint32_t kBytes = kStages * kStage;
 };
 
-template <int KB, int NC, bool DELTA>
-__global__ __launch_bounds__(NC * 64) void linear_scan_kernel(LinearArgs a, Pass pass) {
+// A workgroup's waves: NC with a 16-column tile each, and NL that load.
+template <int KB, int NC, int NL, bool DELTA>
+__global__ __launch_bounds__((NC + NL) * 64, KB == 8 ? 1 : 2) void linear_scan_kernel(LinearArgs a, Pass pass) {
     extern __shared__ __align__(16) unsigned char lds[];
     using L = ScanLds<KB, NC, DELTA>;
     constexpr int TD = 2 * KB;
-    const uint32_t lds0 = uint32_t(uintptr_t((__attribute__((address_space(3))) unsigned char *)lds));
     const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), g = l / 16;
 
     // Workgroups go to the eight dies in turn: all those of a key head to one,
@@ -449,7 +466,6 @@ __global__ __launch_bounds__(NC * 64) void linear_scan_kernel(LinearArgs a, Pass
     const uint32_t unit = blockIdx.x % 8 + blockIdx.x / 8 / of_unit * 8, in_unit = blockIdx.x / 8 % of_unit;
     if (unit >= a.seq.seqs * a.k_heads) return;
     const uint32_t s = unit / a.k_heads, kh = unit % a.k_heads, h = kh * group + in_unit / pass.columns;
-    const uint32_t tile = in_unit % pass.columns * NC + w, col = tile * 16 + l % 16;
 
     uint32_t first, count;
     seq::tokens_of(a.seq, s, first, count);
@@ -457,18 +473,52 @@ __global__ __launch_bounds__(NC * 64) void linear_scan_kernel(LinearArgs a, Pass
     const uint32_t begin = seq::parts_before(a.seq, s, kChunk), end = begin + (count + kChunk - 1) / kChunk;
     const uint32_t c0 = max(begin, pass.first), c1 = min(end, pass.last);
     if (c0 >= c1) return;
+
+    const uint32_t lds0 = uint32_t(uintptr_t((__attribute__((address_space(3))) unsigned char *)lds));
+    auto stage_of = [&](uint32_t c) { return L::kStages == 2 ? (c - c0) % 2 * L::kStage : 0; };
+    if (w >= NC) {
+        // A chunk ahead of the others: every barrier says that a chunk is there
+        // and that the one before is no longer read.
+        constexpr uint32_t kAt = NC * 16;  // columns of the workgroup
+        const uint32_t col0 = in_unit % pass.columns * kAt + l % kAt;
+        const uint32_t values_at = col0 < a.dv ? (l / kAt * a.v_stride + col0) * 4 : kOut;
+        for (uint32_t c = c0; c < c1; ++c) {
+            const uint32_t to = lds0 + stage_of(c), t0 = (c - begin) * kChunk, n = min(kChunk, count - t0);
+            const u4 keys = rsrc_of(pass.of_key(a, c, kh), L::kKey), values = rsrc_of(pass.of_value(a, c, h), L::kValue);
+            const u4 v = rsrc_of(a.v + (size_t(first) + t0) * a.v_stride + size_t(h) * a.dv, ((n - 1) * a.v_stride + a.dv) * 4);
+            if (L::kStages == 1 && c > c0) lds_barrier();
+            uint32_t piece = (w - NC) * 256, row = (w - NC) * (64 / kAt) * a.v_stride * 4;
+            asm volatile("" : "+s"(piece), "+s"(row));  // counted here, not kept in registers for every piece
+#pragma unroll
+            for (uint32_t p = 0; p < L::kV; p += NL * 256, piece += NL * 256, row += NL * (64 / kAt) * a.v_stride * 4)
+                dma4(v, values_at + row, 0, to + L::kKey + L::kValue + piece);  // past the rows, zeros
+            piece = (w - NC) * kTile;
+            asm volatile("" : "+s"(piece));
+#pragma unroll
+            for (uint32_t p = 0; p < L::kKey + L::kValue; p += NL * kTile, piece += NL * kTile) {
+                if (p + NL * kTile <= L::kKey || piece < L::kKey) {
+                    dma16(keys, l * 16, piece, to + piece);
+                } else if (p + NL * kTile <= L::kKey + L::kValue || piece < L::kKey + L::kValue) {
+                    dma16(values, l * 16, piece - L::kKey, to + piece);
+                }
+            }
+            wait_dma<0>();
+            lds_barrier();
+        }
+        return;
+    }
+
     const bool starts = c0 == begin, ends = c1 == end;
     bool read;
     const uint32_t slot = seq::slot_of(a.seq, s, read);
-
-    const uint32_t state_bytes = a.dk * a.dv * 4;
+    const uint32_t tile = in_unit % pass.columns * NC + w, col = tile * 16 + l % 16, state_bytes = a.dk * a.dv * 4;
     const bool has = col < a.dv;
     float *pool = a.state + (size_t(slot == seq::kNoSlot ? 0 : slot) * a.v_heads + h) * a.dk * a.dv;
     const float *from = starts ? pool : pass.from + size_t(h) * a.dk * a.dv;
     // Of a buffer's rows these lanes have 4g + i of every 16; what is past the
     // head's dimensions or the sequence's tokens is past the buffer.
-    const uint32_t state_at = has ? (4 * g * a.dv + col) * 4 : kOut;
-    const uint32_t values_at = has ? (4 * g * a.v_stride + col) * 4 : kOut, out_at = has ? (4 * g * a.out_stride + col) * 4 : kOut;
+    uint32_t state_at = has ? (4 * g * a.dv + col) * 4 : kOut;
+    const uint32_t out_at = has ? (4 * g * a.out_stride + col) * 4 : kOut;
     f4 S[TD];
     {
         const auto r = buffer_of(from, !starts || read ? state_bytes : 0);
@@ -478,30 +528,8 @@ __global__ __launch_bounds__(NC * 64) void linear_scan_kernel(LinearArgs a, Pass
             for (int i = 0; i < 4; ++i)
                 S[t][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, int(state_at + (16 * t + i) * a.dv * 4), 0, 0));
     }
-
-    auto fetch = [&](uint32_t chunk, uint32_t to) {
-        const u4 keys = rsrc_of(pass.of_key(a, chunk, kh), L::kKey), values = rsrc_of(pass.of_value(a, chunk, h), L::kValue);
-        constexpr int kPieces = L::kStage / kTile, kOfKey = L::kKey / kTile;
-        uint32_t piece = w * kTile;
-        asm volatile("" : "+s"(piece));  // counted here, not kept in registers for every piece
-#pragma unroll
-        for (int p = 0; p < kPieces; p += NC, piece += NC * kTile) {
-            if (p + NC <= kOfKey || piece < L::kKey) {
-                dma16(keys, l * 16, piece, to + piece);
-            } else if (p + NC <= kPieces || piece < L::kStage) {
-                dma16(values, l * 16, piece - L::kKey, to + piece);
-            }
-        }
-    };
-    float next[8];  // the values of the chunk to come: tokens 16h + 4g + i at 4h + i
-    auto load_values = [&](uint32_t chunk) {
-        const uint32_t t0 = (chunk - begin) * kChunk, n = min(kChunk, count - t0);
-        const auto r = buffer_of(a.v + (size_t(first) + t0) * a.v_stride + size_t(h) * a.dv, ((n - 1) * a.v_stride + a.dv) * 4);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            next[e] = __uint_as_float(
-                __builtin_amdgcn_raw_buffer_load_b32(r, int(values_at + (16 * (e / 4) + e % 4) * a.v_stride * 4), 0, 0));
-    };
+    float minus = -1.f;
+    asm volatile("" : "+s"(minus));
 
     // S is kept by 2^scale, a column's own.
     int scale = 0;
@@ -523,142 +551,195 @@ __global__ __launch_bounds__(NC * 64) void linear_scan_kernel(LinearArgs a, Pass
     auto fitting = [](float top) { return max(-113, min(15 - exponent(top), 110)); };
     rescale(fitting(biggest()));
 
-    if constexpr (L::kStages == 2) fetch(c0, lds0);
-    load_values(c0);
-    for (uint32_t c = c0; c < c1; ++c) {
-        const uint32_t at = L::kStages == 2 ? (c - c0) % 2 * L::kStage : 0;
-        if constexpr (L::kStages == 1) {
-            lds_barrier();  // nobody reads the last chunk's
-            fetch(c, lds0);
-        }
-        wait_dma<0>();
+    // Two loops, so that a chunk that is done token after token costs the others
+    // no register moves where the paths would meet.
+    uint32_t c = c0;
+    const bool idle = tile * 16 >= a.dv;
+    auto enter = [&] {  // the chunk's operands are there
+        if (L::kStages == 1 && c > c0) lds_barrier();
         lds_barrier();
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = next[e];
-        if (c + 1 < c1) {
-            if constexpr (L::kStages == 2) fetch(c + 1, lds0 + (L::kStage - at));
-            load_values(c + 1);
-        }
-        if (tile * 16 >= a.dv) continue;
-
-        const unsigned char *keys = lds + at, *values = keys + L::kKey;
+    };
+    if (idle) {
+        for (; c < c1; ++c) enter();
+    }
+    while (c < c1) {
+        bool slow = false;
+        do {
+        enter();
+        const unsigned char *keys = lds + stage_of(c), *values = keys + L::kKey;
         const float *scalars = reinterpret_cast<const float *>(values + kScalars);
         const uint32_t t0 = (c - begin) * kChunk, n = min(kChunk, count - t0);
-        float odd = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) odd = fmaf(v[e], 0.f, odd);
-        if (reinterpret_cast<const uint32_t *>(scalars)[kWild] != 0 || __ballot(odd != 0.f) != 0) {
-            rescale(0);
-            tokens_of_chunk<TD>(a, size_t(first) + t0, n, h, col, S);
-            rescale(fitting(biggest()));
-            continue;
-        }
-        auto tile_at = [&](const unsigned char *p) { return *reinterpret_cast<const u4 *>(p + l * 16); };
+        // LDS answers late: operands are asked for well before the matrix
+        // instructions that take them, into registers that the last ones left.
+        struct Terms {
+            u4 hi, lo;
+        };
+        auto at = [&](const unsigned char *p) {
+            return Terms{*reinterpret_cast<const u4 *>(p + l * 16), *reinterpret_cast<const u4 *>(p + kTile + l * 16)};
+        };
+        // A sum waits for the matrix instruction before it some time longer than
+        // that one keeps the others: as many sums as there are go on in turn.
+        auto step = [&](int which, const Terms &m, u4 hi, u4 lo, f4 &c) {
+            c = mfma(which == 0 ? m.lo : m.hi, which == 1 ? lo : hi, c);
+        };
         auto of_rows = [&](uint32_t which, int half) { return *reinterpret_cast<const f4 *>(scalars + which + 16 * half + 4 * g); };
         const float whole = scalars[kWhole], most = scalars[kMost];
-        const float top = biggest();
-
-        // S^T k and S^T q.
-        f4 x[2] = {}, o[2] = {};
+        const uint32_t wild = reinterpret_cast<const uint32_t *>(scalars)[kWild];
+        float v[8];  // tokens 16h + 4g + i at 4h + i
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = reinterpret_cast<const float *>(values + L::kValue)[(16 * (e / 4) + 4 * g + e % 4) * (NC * 16) + w * 16 + l % 16];
+        f4 beta[2], of_x[2], of_q[2], of_m[2], of_u[2];
+        Terms tk[2][KB], tq[2][KB], tt[2], tm[2], tu[TD];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            beta[half] = of_rows(kBeta, half);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+                if constexpr (DELTA) tk[half][kb] = at(keys + 8 * kTile * KB + (half * KB + kb) * 2 * kTile);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        u4 sh[KB], sl[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             float both[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) both[e] = S[2 * kb + e / 4][e % 4];
-            u4 sh, sl;
-            terms(both, sh, sl);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t p = (half * KB + kb) * 2 * kTile;
-                if constexpr (DELTA) {
-                    const unsigned char *k = keys + 8 * kTile * KB + p;
-                    x[half] = mfma3(tile_at(k), tile_at(k + kTile), sh, sl, x[half]);
-                }
-                o[half] = mfma3(tile_at(keys + p), tile_at(keys + p + kTile), sh, sl, o[half]);
-            }
+            terms(both, minus, sh[kb], sl[kb]);
         }
-        // R, by 2^up.
-        float r[8];
+        __builtin_amdgcn_sched_barrier(0);
+        // S^T k; meanwhile R's part that does not wait for it, all by 2^scale.
+        f4 x2[2][2] = {}, o2[2][2] = {}, x[2], o[2];  // blocks 0, 2, .. and 1, 3, ..
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const f4 beta = of_rows(kBeta, half), of_x = of_rows(kX, half);
+            of_x[half] = of_rows(kX, half);
+            if constexpr (DELTA) tt[half] = at(values + kScalars + kTile + half * 2 * kTile);
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                r[4 * half + i] = DELTA ? beta[i] * v[4 * half + i] - of_x[i] * ldexpf(x[half][i], -scale) : v[4 * half + i];
+        for (int kb = 0; kb < KB; kb += 2) {
+            if constexpr (DELTA) {
+#pragma unroll
+                for (int m = 0; m < 12; ++m)
+                    step(m / 4, tk[m % 2][kb + m / 2 % 2], sh[kb + m / 2 % 2], sl[kb + m / 2 % 2], x2[m % 2][m / 2 % 2]);
+            }
+#pragma unroll
+            for (int m = 0; m < 4; ++m) tq[m % 2][kb + m / 2] = at(keys + (m % 2 * KB + kb + m / 2) * 2 * kTile);
+        }
+        float r[8];
+        {
+            const float by = ldexpf(1.f, scale);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[e] = v[e] * (DELTA ? beta[e / 4][e % 4] * by : by);
+        }
+        float odd = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) odd = fmaf(v[e], 0.f, odd);
+        const float top = biggest();
+        if constexpr (DELTA) in_turn<6 * KB, 2, 1>();
+        __builtin_amdgcn_sched_barrier(0);
+        slow = __builtin_amdgcn_readfirstlane(wild) != 0 || __ballot(odd != 0.f) != 0;
+        if (slow) break;
+        // S^T q; meanwhile R and its terms, by 2^up more; the next state's scale:
+        // below 2^15 whatever the chunk adds.
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            tm[half] = at(values + half * 2 * kTile);
+            of_u[half] = of_rows(kU, half);
+            of_q[half] = of_rows(kQ, half);
+            of_m[half] = of_rows(kM, half);
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; kb += 2) {
+#pragma unroll
+            for (int m = 0; m < 12; ++m)
+                step(m / 4, tq[m % 2][kb + m / 2 % 2], sh[kb + m / 2 % 2], sl[kb + m / 2 % 2], o2[m % 2][m / 2 % 2]);
+#pragma unroll
+            for (int t = 2 * kb; t < 2 * kb + 4; ++t) tu[t] = at(keys + 4 * kTile * KB + t * 2 * kTile);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            x[half] = x2[half][0] + x2[half][1];
+            o[half] = o2[half][0] + o2[half][1];
+        }
+        if constexpr (DELTA) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[e] = fmaf(-of_x[e / 4][e % 4], x[e / 4][e % 4], r[e]);
         }
         float r_top = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) r_top = fmaxf(r_top, fabsf(r[e]));
         r_top = column_max(r_top);
-        const int up = max(-113, min(13 - exponent(r_top), 110));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r[e] = ldexpf(r[e], up);
+        const int up = max(-113, min((DELTA ? 5 : 13) - exponent(r_top), 110));
+        int to = min(scale + 15 - exponent(fmaf(most, r_top, whole * top)), scale + 100);
+        to = max(-113, min(to, 110));
         u4 uh, ul;
-        terms(r, uh, ul);
-        // U, by 2^up (and 2^kSolve until its terms are made).
+        {
+            const float by = ldexpf(1.f, up);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[e] *= by;
+        }
+        terms(r, minus, uh, ul);
+        in_turn<6 * KB, 3, 1>();
+        __builtin_amdgcn_sched_barrier(0);
+        // U, by 2^(scale + up + kSolve): below 2^15 while rows of T add up to 2^6.
         float u[8];
-        int u_up = up;
         if constexpr (DELTA) {
             f4 y[2] = {};
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const unsigned char *t = values + kScalars + kTile + half * 2 * kTile;
-                y[half] = mfma3(tile_at(t), tile_at(t + kTile), uh, ul, y[half]);
-            }
-            float small[8];
+            for (int m = 0; m < 6; ++m) step(m / 2, tt[m % 2], uh, ul, y[m % 2]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                u[e] = y[e / 4][e % 4];
-                small[e] = u[e] * 0.00390625f;  // 2^-8: below 2^15 while rows of T add up to 2^6
-            }
-            terms(small, uh, ul);
-            u_up = up + kSolve;
+            for (int e = 0; e < 8; ++e) u[e] = y[e / 4][e % 4];
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) u[e] = r[e];
         }
-        // The next state's scale: below 2^15 whatever the chunk adds.
-        const int to = min(fitting(ldexpf(whole * top, -scale) + most * r_top), scale + 100);
-        // M U and the outputs.
         {
-            const auto rows = buffer_of(a.out + (size_t(first) + t0) * a.out_stride + size_t(h) * a.dv,
-                                        ((n - 1) * a.out_stride + a.dv) * 4);
+            const float keep = ldexpf(whole, to - scale);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const unsigned char *p = values + half * 2 * kTile;
-                const f4 y = mfma3(tile_at(p), tile_at(p + kTile), uh, ul, f4{});
-                const f4 of_q = of_rows(kQ, half), of_m = of_rows(kM, half);
+            for (int t = 0; t < TD; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float out = of_q[i] * ldexpf(o[half][i], -scale) + of_m[i] * ldexpf(y[i], (DELTA ? 8 : 0) - u_up);
-                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(out), rows, int(out_at + (16 * half + i) * a.out_stride * 4),
-                                                          0, 0);
-                }
-            }
+                for (int i = 0; i < 4; ++i) S[t][i] *= keep;
+            const float by = ldexpf(1.f, to - scale - up - (DELTA ? kSolve : 0));
+            of_u[0] *= by;
+            of_u[1] *= by;
         }
-        // The next state.
-        const float keep = ldexpf(whole, to - scale);
+        if constexpr (DELTA) in_turn<6, 6, 0>();
+        __builtin_amdgcn_sched_barrier(0);
+        u4 wh, wl;
+        {
+            float left[8];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const f4 of_u = of_rows(kU, half);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) u[4 * half + i] = u[4 * half + i] * ldexpf(of_u[i], to - u_up);
+            for (int e = 0; e < 8; ++e) left[e] = u[e] * of_u[e / 4][e % 4];
+            terms(left, minus, wh, wl);
+            if constexpr (DELTA) terms(u, minus, uh, ul);
         }
-        terms(u, uh, ul);
+        __builtin_amdgcn_sched_barrier(0);
+        // The next state, M U and the outputs.
 #pragma unroll
-        for (int t = 0; t < TD; ++t) {
+        for (int m = 0; m < 3 * TD; ++m) step(m / TD, tu[m % TD], wh, wl, S[m % TD]);
+        f4 y[2] = {};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) S[t][i] *= keep;
-            const unsigned char *p = keys + 4 * kTile * KB + t * 2 * kTile;
-            S[t] = mfma3(tile_at(p), tile_at(p + kTile), uh, ul, S[t]);
+        for (int m = 0; m < 6; ++m) step(m / 2, tm[m % 2], uh, ul, y[m % 2]);
+        const auto rows = buffer_of(a.out + (size_t(first) + t0) * a.out_stride + size_t(h) * a.dv, ((n - 1) * a.out_stride + a.dv) * 4);
+        const float one = ldexpf(1.f, -scale), of_y = ldexpf(1.f, (DELTA ? -kSolve : 0) - up - scale);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float out = of_q[e / 4][e % 4] * (o[e / 4][e % 4] * one) + of_m[e / 4][e % 4] * (y[e / 4][e % 4] * of_y);
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(out), rows, int(out_at + (16 * (e / 4) + e % 4) * a.out_stride * 4), 0, 0);
         }
         scale = to;
+        } while (++c < c1);
+        if (!slow) break;
+        rescale(0);
+        const uint32_t t0 = (c - begin) * kChunk;
+        tokens_of_chunk<TD>(a, size_t(first) + t0, min(kChunk, count - t0), h, col, S);
+        rescale(fitting(biggest()));
+        ++c;
     }
-    wait_dma<0>();  // LDS is given back
     if (tile * 16 >= a.dv || (ends ? !a.keep || slot == seq::kNoSlot : pass.to == nullptr)) return;
     rescale(0);
     const auto r = buffer_of(ends ? pool : pass.to + size_t(h) * a.dk * a.dv, state_bytes);
+    asm volatile("" : "+v"(state_at));  // or all of the addresses wait in registers for this
 #pragma unroll
     for (int t = 0; t < TD; ++t)
 #pragma unroll
@@ -706,14 +787,14 @@ hipError_t go_prepare(const LinearArgs &a, const Pass &pass, hipStream_t stream)
     return hipGetLastError();
 }
 
-template <int KB, int NC, bool DELTA>
+template <int KB, int NC, int NL, bool DELTA>
 hipError_t go_scan(const LinearArgs &a, const Pass &pass, hipStream_t stream) {
-    const auto kernel = linear_scan_kernel<KB, NC, DELTA>;
+    const auto kernel = linear_scan_kernel<KB, NC, NL, DELTA>;
     constexpr uint32_t lds = ScanLds<KB, NC, DELTA>::kBytes;
     const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
     if (e != hipSuccess) return e;
     const uint32_t units = (a.seq.seqs * a.k_heads + 7) / 8 * 8;
-    kernel<<<units * (a.v_heads / a.k_heads) * pass.columns, NC * 64, lds, stream>>>(a, pass);
+    kernel<<<units * (a.v_heads / a.k_heads) * pass.columns, (NC + NL) * 64, lds, stream>>>(a, pass);
     return hipGetLastError();
 }
 
@@ -722,9 +803,8 @@ hipError_t go_pass(const LinearArgs &a, const LinearPlan &pl, const Pass &pass, 
     const hipError_t e = go_prepare<KB, DELTA>(a, pass, stream);
     if (e != hipSuccess) return e;
     switch (pl.columns) {
-        case 2: return go_scan<KB, 2, DELTA>(a, pass, stream);
-        case 4: return go_scan<KB, 4, DELTA>(a, pass, stream);
-        default: return go_scan<KB, 8, DELTA>(a, pass, stream);
+        case 2: return go_scan<KB, 2, 4, DELTA>(a, pass, stream);
+        default: return go_scan<KB, 4, 4, DELTA>(a, pass, stream);
     }
 }
 
@@ -744,7 +824,7 @@ LinearPlan plan_linear(const LinearArgs &a, const DeviceLimits &lim, size_t limi
     pl.k_bytes = size_t(a.delta ? 12 : 8) * kTile * pl.blocks;
     pl.v_bytes = size_t(a.delta ? 9 : 5) * kTile;
     if (columns == 0)
-        while (pl.columns < 8 && uint64_t(std::min(q.seqs, pl.parts)) * a.v_heads * ((tiles + pl.columns - 1) / pl.columns) >
+        while (pl.columns < 4 && uint64_t(std::min(q.seqs, pl.parts)) * a.v_heads * ((tiles + pl.columns - 1) / pl.columns) >
                                      2 * uint64_t(lim.num_cus))
             pl.columns *= 2;
     const size_t each = a.k_heads * pl.k_bytes + a.v_heads * pl.v_bytes;

@@ -49,6 +49,14 @@ __device__ __forceinline__ void dma16(u4 rsrc, uint32_t offset, uint32_t more, u
                  : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(more))
                  : "memory", "m0");
 }
+
+// The same of 64 words.
+__device__ __forceinline__ void dma4(u4 rsrc, uint32_t offset, uint32_t more, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(more))
+                 : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 // Until at most LATER of this wave's loads are on their way.
