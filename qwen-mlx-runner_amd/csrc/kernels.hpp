@@ -389,7 +389,14 @@ struct SampleArgs {
     float *probs;
     uint32_t rows, vocab, stride;
 };
-hipError_t launch_sample_logits(const SampleArgs &a, const DeviceLimits &lim, hipStream_t stream);
+struct SamplePlan {
+    bool whole = false;       // a row fits a workgroup's LDS
+    uint32_t slice = 0, slices = 0;  // logits of a slice, slices of a row
+    uint32_t rows = 0;        // rows at a time
+    size_t workspace = 0;
+};
+SamplePlan plan_sample(const SampleArgs &a, const DeviceLimits &lim, size_t workspace_limit);
+hipError_t launch_sample_logits(const SampleArgs &a, const SamplePlan &pl, void *workspace, hipStream_t stream);
 
 // The plan the GEMV launcher would use (for tests and tuning reports).
 GemvPlan plan_affine_gemv(const AffineArgs &a, GemvPlan forced, const DeviceLimits &lim);

@@ -79,8 +79,8 @@ struct qmr_device {
     // Workspace of the paged attention's key ranges.
     unsigned char *ws_attend = nullptr;
     size_t ws_attend_bytes = 0;
-    // Workspace of linear attention's chunks: their operands, and states
-    // between passes over them.
+    // Workspace of linear attention's chunks (their operands, and states
+    // between passes over them) and of sampled rows.
     unsigned char *ws_linear = nullptr;
     size_t ws_linear_bytes = 0;
     // This GPU's copy of the static scratch (the workspace of
@@ -925,6 +925,25 @@ void check_linear_views(const std::string &name, qmr_buffer *const *buffers, con
     }
 }
 
+// The workspace of linear attention and sampling: the device's, grown to `need`
+// bytes, or with `fixed` (qmr_encode_static) the static scratch.
+unsigned char *linear_workspace(qmr_device *dev, size_t need, unsigned char *fixed, const char *what) {
+    if (fixed) {
+        check_static_scratch(need, what);
+        if (need) mark_static_dirty(dev, need);
+        return fixed;
+    }
+    if (need > dev->ws_linear_bytes) {
+        check_hip(hipStreamSynchronize(dev->stream), "hipStreamSynchronize");
+        if (dev->ws_linear) hipFree(dev->ws_linear);
+        dev->ws_linear = nullptr;
+        dev->ws_linear_bytes = 0;
+        check_hip(hipMalloc(&dev->ws_linear, need), "hipMalloc (linear attention and sampling workspace)");
+        dev->ws_linear_bytes = need;
+    }
+    return dev->ws_linear;
+}
+
 // conv_causal, attn_linear and sample_logits.
 hipError_t launch_linear(qmr_device *dev, const std::string &name, qmr_buffer *const *buffers, const size_t *offsets,
                          const uint32_t *p, unsigned char *fixed) {
@@ -932,9 +951,12 @@ hipError_t launch_linear(qmr_device *dev, const std::string &name, qmr_buffer *c
     auto f32 = [&](size_t i) { return reinterpret_cast<float *>(ptr(i)); };
     auto u32 = [&](size_t i) { return reinterpret_cast<uint32_t *>(ptr(i)); };
     if (qmr::is_sample_name(name)) {
+        const qmr::SampleArgs a{f32(0), f32(1), u32(2), f32(3), f32(4), f32(5), u32(6), f32(7), p[0], p[1], p[2]};
+        const qmr::SamplePlan pl = qmr::plan_sample(a, dev->limits, fixed ? QMR_STATIC_SCRATCH_BYTES : SIZE_MAX);
+        unsigned char *workspace = linear_workspace(dev, pl.workspace, fixed, "bins of sampled rows");
+        dev->last_hip = "sample_pick_kernel";
         start_gpu(dev);
-        return qmr::launch_sample_logits({f32(0), f32(1), u32(2), f32(3), f32(4), f32(5), u32(6), f32(7), p[0], p[1], p[2]},
-                                         dev->limits, dev->stream);
+        return qmr::launch_sample_logits(a, pl, workspace, dev->stream);
     }
     if (name == "conv_causal") {
         qmr::ConvArgs a{};
@@ -989,20 +1011,10 @@ hipError_t launch_linear(qmr_device *dev, const std::string &name, qmr_buffer *c
     // for a plan.
     const qmr::LinearPlan pl = qmr::plan_linear(a, dev->limits, fixed ? QMR_STATIC_SCRATCH_BYTES : SIZE_MAX,
                                                 forced ? uint32_t(f.ks / 100) : 0, forced ? uint32_t(f.ks % 100) : 0);
-    if (fixed) {
-        check_static_scratch(pl.workspace, "linear attention's operands");
-        if (pl.workspace) mark_static_dirty(dev, pl.workspace);
-    } else if (pl.workspace > dev->ws_linear_bytes) {
-        check_hip(hipStreamSynchronize(dev->stream), "hipStreamSynchronize");
-        if (dev->ws_linear) hipFree(dev->ws_linear);
-        dev->ws_linear = nullptr;
-        dev->ws_linear_bytes = 0;
-        check_hip(hipMalloc(&dev->ws_linear, pl.workspace), "hipMalloc (linear attention workspace)");
-        dev->ws_linear_bytes = pl.workspace;
-    }
+    unsigned char *workspace = linear_workspace(dev, pl.workspace, fixed, "linear attention's operands");
     dev->last_hip = qmr::linear_kernel_name(pl);
     start_gpu(dev);
-    return qmr::launch_attn_linear(a, pl, fixed ? fixed : dev->ws_linear, dev->stream);
+    return qmr::launch_attn_linear(a, pl, workspace, dev->stream);
 }
 
 // rope_axes, kv_append_rope_* and attn_paged_*.

@@ -17,20 +17,38 @@
 // tokens. They are worked out in 64 bits: with weights of 32, one draw in a
 // hundred of a broad row would fall on the other side of a border.
 //
-// Nothing is sorted. The borders of top k and top p are a logit and a number of
-// ties at it, found digit by digit: a histogram of the next eight bits of those
-// that agree in the bits before, counts for top k, weights for top p.
+// Nothing is sorted. A token's place is one number, its logit's bits above its
+// index's, so that every border is a place and there are no ties. Rows go over
+// the chip in slices, and what decides is narrowed down in four launches:
+//
+//   sample_max     the largest and smallest logit of each slice
+//   sample_bins    tokens and weight by bins of logits, at most a 16th of the
+//                  temperature wide, of each slice and of the row
+//   sample_gather  from the row's bins, those that a border may fall into; the
+//                  tokens in them, and each slice's weight above them
+//   sample_pick    a workgroup a row: the borders among those tokens, the slice
+//                  that the number falls into, and the token there
+//
+// A row that fits sample_pick's LDS needs that launch alone. One that has too
+// many tokens in its bins (many equal logits) is worked on by sample_pick
+// alone, which reads it once a digit of the borders.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "kernels.hpp"
 
 namespace qmr {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
 using u64 = unsigned long long;
 
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr uint32_t kBins = kThreads;     // a thread a bin; the last: weights that round to nothing
+constexpr uint32_t kPerNat = 16;         // bins of a temperature: 511 of them reach below 2^-45
+constexpr uint32_t kCandidates = 8192;   // of a row, at most
+constexpr uint32_t kSliceStep = 4096;
 constexpr uint32_t kNone = 0xffffffffu;
 
 // Ordered as the logits are; NaN and -infinity are 0. Both zeros are one logit.
@@ -44,6 +62,11 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+// A token's place, larger for those kept first.
+__device__ __forceinline__ u64 place_of(uint32_t key, uint32_t i) { return u64(key) << 32 | uint32_t(~i); }
+__device__ __forceinline__ uint32_t key_at(u64 place) { return uint32_t(place >> 32); }
+__device__ __forceinline__ uint32_t index_at(u64 place) { return ~uint32_t(place); }
+
 // n weights of at most 2^shift add up to 2^62 at most.
 __host__ __device__ constexpr uint32_t shift_of(uint32_t n) {
     uint32_t bits = 10;
@@ -51,19 +74,35 @@ __host__ __device__ constexpr uint32_t shift_of(uint32_t n) {
     return 62 - bits;
 }
 
-// What a row's weights are made with.
+// A row's weights and bins, from its largest and smallest logit.
 struct Weights {
-    float max;
+    uint32_t top;
+    float max, half_max, per_bin;  // bins: half the distance from the largest, times per_bin
     double temperature;
     double one;  // 2^shift
+    float min_p;
 
+    __device__ Weights(const SampleArgs &a, uint32_t row, uint32_t top_, uint32_t least)
+        : top(top_), max(logit_of(top_)), temperature(a.temperature[row]), one(double(u64(1) << shift_of(a.vocab))), min_p(a.min_p[row]) {
+        half_max = 0.5f * max;
+        const float width = half_max - 0.5f * logit_of(least);
+        // Narrow rows take all bins but the last, which then is empty.
+        per_bin = fminf(fmaxf(2.f * kPerNat / a.temperature[row], width > 0.f ? float(kBins - 2) / width : 0.f), 1e38f);
+    }
+    __device__ bool greedy() const { return !(temperature > 0); }
     __device__ double plain(uint32_t key) const {
-        const float x = logit_of(key);
-        if (x == max) return 1.0;
+        if (key == top) return 1.0;
         if (max == INFINITY) return 0.0;
-        return exp((double(x) - double(max)) / temperature);
+        return exp((double(logit_of(key)) - double(max)) / temperature);
     }
     __device__ u64 whole(uint32_t key) const { return u64(__double2ll_rn(plain(key) * one)); }
+    __device__ bool likely(uint32_t key) const { return key == top || !(min_p > 0.f) || plain(key) >= double(min_p); }
+    // Never smaller for a smaller logit, whatever rounds.
+    __device__ uint32_t bin(uint32_t key) const {
+        if (key == top) return 0;
+        const float z = (half_max - 0.5f * logit_of(key)) * per_bin;
+        return z < float(kBins - 1) ? uint32_t(z) : kBins - 1;
+    }
 };
 
 template <typename T>
@@ -74,6 +113,16 @@ __device__ __forceinline__ T block_sum(T v, T *room) {
     __syncthreads();
     v = 0;
     for (int w = 0; w < kWaves; ++w) v += room[w];
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T block_max(T v, T *room) {
+    for (int d = 1; d < 64; d *= 2) v = max(v, T(__shfl_xor(v, d)));
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = v;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) v = max(v, room[w]);
     return v;
 }
 
@@ -91,183 +140,460 @@ __device__ __forceinline__ T block_scan(T v, T *room) {
     return v;
 }
 
-// A border: keys above `key` are kept, and of those at it the first `ties` by
-// index.
-struct Border {
-    uint32_t key = 0;
-    uint32_t ties = 0;
+// What the launches leave for each other, a row.
+struct Work {
+    u64 *best;         // [rows][slices] a slice's first place
+    uint32_t *least;   // [rows][slices] its smallest key, of those kept at all
+    uint32_t *count;   // [rows][kBins]
+    u64 *weight;       // [rows][kBins]
+    uint32_t *found;   // [rows] candidates
+    u64 *of_slice;     // [rows][slices][kBins] weight
+    u64 *sure;         // [rows][slices] weight above the bins of the candidates
+    u64 *candidates;   // [rows][kCandidates]
+    uint32_t slices, slice;
 };
 
-// A workgroup a row.
-__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
-    __shared__ u64 bins[256];
+// A row's largest and smallest key from its slices'.
+__device__ __forceinline__ void extremes(const Work &w, uint32_t row, u64 &best, uint32_t &least, u64 *room) {
+    best = 0;
+    uint32_t low = 0;  // upside down
+    for (uint32_t i = threadIdx.x; i < w.slices; i += kThreads) {
+        best = max(best, w.best[size_t(row) * w.slices + i]);
+        low = max(low, ~w.least[size_t(row) * w.slices + i]);
+    }
+    best = block_max(best, room);
+    least = ~uint32_t(block_max(u64(low), room));
+}
+
+__global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, Work w) {
     __shared__ u64 room[kWaves];
-    __shared__ u64 found[2];
-    const uint32_t row = blockIdx.x, n = a.vocab, tid = threadIdx.x;
+    const uint32_t row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
     const float *x = a.logits + size_t(row) * a.stride;
-
-    uint32_t top = 0;
-    u64 valid = 0;
-    for (uint32_t i = tid; i < n; i += kThreads) {
+    for (uint32_t i = slice * kThreads + tid; i < kBins; i += w.slices * kThreads) {
+        w.count[size_t(row) * kBins + i] = 0;
+        w.weight[size_t(row) * kBins + i] = 0;
+    }
+    if (slice == 0 && tid == 0) w.found[row] = 0;
+    u64 best = 0;
+    uint32_t low = 0;
+    const uint32_t end = min((slice + 1) * w.slice, a.vocab);
+#pragma unroll 8
+    for (uint32_t i = slice * w.slice + tid; i < end; i += kThreads) {
         const uint32_t key = key_of(x[i]);
-        top = max(top, key);
-        valid += key != 0;
+        if (key == 0) continue;
+        best = max(best, place_of(key, i));
+        low = max(low, ~key);
     }
-    for (int d = 1; d < 64; d *= 2) top = max(top, uint32_t(__shfl_xor(top, d)));
-    if (tid % 64 == 0) room[tid / 64] = top;
+    best = block_max(best, room);
+    low = uint32_t(block_max(u64(low), room));
+    if (tid == 0) {
+        w.best[size_t(row) * w.slices + slice] = best;
+        w.least[size_t(row) * w.slices + slice] = ~low;
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Work w) {
+    __shared__ u64 room[kWaves], weight[kBins];
+    __shared__ uint32_t count[kBins];
+    const uint32_t row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
+    const float *x = a.logits + size_t(row) * a.stride;
+    u64 best;
+    uint32_t least;
+    extremes(w, row, best, least, room);
+    const Weights of(a, row, key_at(best), least);
+    if (best == 0 || of.greedy()) return;
+    weight[tid] = 0;
+    count[tid] = 0;
     __syncthreads();
-    for (int w = 0; w < kWaves; ++w) top = max(top, uint32_t(room[w]));
-    valid = block_sum(valid, room);
-    if (top == 0) {
-        if (tid == 0) a.tokens[row] = kNone, a.probs[row] = 0.f;
-        return;
+    const uint32_t end = min((slice + 1) * w.slice, a.vocab);
+#pragma unroll 4
+    for (uint32_t i = slice * w.slice + tid; i < end; i += kThreads) {
+        const uint32_t key = key_of(x[i]);
+        if (key == 0) continue;
+        const uint32_t bin = of.bin(key);
+        if (bin == kBins - 1) continue;
+        atomicAdd(&count[bin], 1u);
+        atomicAdd(&weight[bin], of.whole(key));
     }
-
-    const float temperature = a.temperature[row];
-    const Weights weights{logit_of(top), double(temperature), double(u64(1) << shift_of(n))};
-    const bool greedy = !(temperature > 0.f);
-
-    // Walks the keys from the largest down to where `before(sum)` no longer
-    // holds, sums of amount(key) over the keys of `in`; `sum` is then that of
-    // the keys above the border.
-    auto descend = [&](auto in, auto amount, auto inside, u64 &above) {
-        uint32_t prefix = 0;
-        above = 0;
-        for (int digit = 3; digit >= 0; --digit) {
-            const int low = 8 * digit;
-            __syncthreads();
-            if (tid < 256) bins[tid] = 0;
-            __syncthreads();
-            for (uint32_t i = tid; i < n; i += kThreads) {
-                const uint32_t key = key_of(x[i]);
-                if (key == 0 || !in(key, i)) continue;
-                if (digit < 3 && (key >> (low + 8)) != (prefix >> (low + 8))) continue;
-                atomicAdd(&bins[(key >> low) & 255], amount(key));
-            }
-            __syncthreads();
-            if (tid == 0) {
-                // The last bin, from above, whose first key may still be inside.
-                u64 sum = above;
-                uint32_t at = 0, some = 0;
-                u64 up_to = above;
-                for (int b = 255; b >= 0; --b) {
-                    if (bins[b] == 0) continue;
-                    if (some && !inside(sum)) break;
-                    at = b;
-                    up_to = sum;
-                    some = 1;
-                    sum += bins[b];
-                }
-                found[0] = at;
-                found[1] = up_to;
-            }
-            __syncthreads();
-            prefix |= uint32_t(found[0]) << low;
-            above = found[1];
-        }
-        return prefix;
-    };
-
-    // Top k.
-    Border k{0, kNone};
-    const uint32_t most = a.top_k[row];
-    if (greedy) {
-        k = {top, 1};
-    } else if (most > 0 && most < valid) {
-        u64 above;
-        k.key = descend([](uint32_t, uint32_t) { return true; }, [](uint32_t) { return u64(1); },
-                        [&](u64 sum) { return sum < most; }, above);
-        k.ties = uint32_t(most - above);
+    __syncthreads();
+    const uint32_t n = count[tid];
+    const u64 sum = weight[tid];
+    w.of_slice[(size_t(row) * w.slices + slice) * kBins + tid] = sum;
+    if (n) {
+        atomicAdd(&w.count[size_t(row) * kBins + tid], n);
+        atomicAdd(&w.weight[size_t(row) * kBins + tid], sum);
     }
-    // The index of the last tie that a border keeps.
-    auto last_tie = [&](const Border &b, u64 ties) -> uint32_t {
-        if (b.key == 0 || ties >= n) return n;
-        u64 before = 0;
-        for (uint32_t base = 0; base < n; base += kThreads) {
-            const uint32_t i = base + tid;
-            const u64 tie = i < n && key_of(x[i]) == b.key;
-            const u64 up_to = before + block_scan(tie, room);
-            __syncthreads();
-            if (tie && up_to == ties) found[0] = i;
-            if (tid == kThreads - 1) room[0] = up_to;
-            __syncthreads();
-            before = room[0];
-            const bool done = before >= ties;
-            const uint32_t at = uint32_t(found[0]);
-            __syncthreads();
-            if (done) return at;
-        }
-        return n;
-    };
-    uint32_t k_last = last_tie(k, k.ties);
-    auto in_k = [&](uint32_t key, uint32_t i) { return key > k.key || (key == k.key && i <= k_last); };
+}
 
-    // Top p.
-    Border p{0, kNone};
-    const float part = a.top_p[row];
-    uint32_t p_last = n;
-    if (!greedy && part < 1.f) {
-        u64 all = 0;
-        for (uint32_t i = tid; i < n; i += kThreads) {
-            const uint32_t key = key_of(x[i]);
-            if (key && in_k(key, i)) all += weights.whole(key);
-        }
-        const double target = fmax(double(part), 0.0) * double(block_sum(all, room));
-        u64 above;
-        p.key = descend(in_k, [&](uint32_t key) { return weights.whole(key); },
-                        [&](u64 sum) { return double(sum) < target; }, above);
-        // Ties: the one before which `above` and j of their weight stand.
-        const u64 w = weights.whole(p.key);
-        p.ties = 1;
-        if (w == 0) {
-            p.ties = double(above) < target || above == 0 ? kNone : 1;
-        } else {
-            u64 j = target > double(above) ? u64((target - double(above)) / double(w)) : 0;
-            while (j > 0 && double(above + (j - 1) * w) >= target) --j;
-            while (double(above + j * w) < target) ++j;
-            p.ties = uint32_t(max(j, u64(1)));
-        }
-        p_last = last_tie(p, p.ties);
-    }
-    const float min_p = a.min_p[row];
-    auto kept = [&](uint32_t i) -> uint32_t {
-        const uint32_t key = i < n ? key_of(x[i]) : 0;
-        if (key == 0 || !in_k(key, i)) return 0;
-        if (key < p.key || (key == p.key && i > p_last)) return 0;
-        if (key != top && min_p > 0.f && weights.plain(key) < double(min_p)) return 0;
-        return key;
-    };
+// Which bins the borders may fall into.
+struct Bounds {
+    uint32_t first, last;  // between them tokens may be kept or not; all above are
+    uint32_t k_bin;        // where top k ends; kNone: it keeps all
+    u64 above;             // weight above `first`
+    u64 above_k;           // weight above k_bin, or of all
+    uint32_t k_rank;       // so many of k_bin are kept by top k
+    bool p;                // top p has a border
+};
 
-    u64 total = 0;
-    for (uint32_t i = tid; i < n; i += kThreads) {
-        const uint32_t key = kept(i);
-        if (key) total += weights.whole(key);
-    }
-    total = block_sum(total, room);
-    const double u = fmin(fmax(double(a.uniform[row]), 0.0), 1.0);
-    const u64 target = min(u64(u * double(total)), total - 1);
-    u64 before = 0;
-    for (uint32_t base = 0; base < n; base += kThreads) {
-        const uint32_t key = kept(base + tid);
-        const u64 w = key ? weights.whole(key) : 0;
-        const u64 up_to = before + block_scan(w, room);
-        if (w && up_to > target && up_to - w <= target) {
-            a.tokens[row] = base + tid;
-            a.probs[row] = float(double(w) / double(total));
+__device__ Bounds bounds_of(const SampleArgs &a, const Work &w, uint32_t row, const Weights &of, u64 *room, u64 *found) {
+    const uint32_t tid = threadIdx.x, k = a.top_k[row];
+    const float p = a.top_p[row];
+    const uint32_t n = w.count[size_t(row) * kBins + tid];
+    const u64 sum = w.weight[size_t(row) * kBins + tid];
+    const u64 tokens = block_scan(u64(n), room), weight = block_scan(sum, room);
+    Bounds b;
+    if (tid < 4) found[tid] = kNone;
+    __syncthreads();
+    // A border past the last bin but one is none: what is there weighs nothing.
+    if (k > 0 && tokens >= k && tokens - n < k) found[0] = tid;
+    if (tid == kBins - 1) found[1] = weight;
+    __syncthreads();
+    b.k_bin = uint32_t(found[0]);
+    u64 most = found[1], least = most;
+    __syncthreads();
+    if (b.k_bin != kNone) {
+        if (tid == b.k_bin) {
+            found[1] = weight;
+            found[2] = weight - sum;
+            found[3] = k - (tokens - n);
         }
         __syncthreads();
-        if (tid == kThreads - 1) room[0] = up_to;
+        most = found[1];
+        least = found[2];
+        b.k_rank = uint32_t(found[3]);
         __syncthreads();
-        before = room[0];
+    } else {
+        b.k_rank = 0;
+    }
+    b.above_k = least;
+    b.first = b.k_bin;
+    b.last = b.k_bin;
+    b.p = p < 1.f;
+    if (b.p) {
+        // The first bin up to which the weight that top p asks for stands, with
+        // the least and with the most that top k may keep.
+        const double lo = fmax(double(p), 0.0) * double(least) * (1 - 1e-12), hi = fmax(double(p), 0.0) * double(most) * (1 + 1e-12);
+        const bool in_lo = double(weight) >= lo, in_hi = double(weight) >= hi;
+        const bool was_lo = tid > 0 && double(weight - sum) >= lo, was_hi = tid > 0 && double(weight - sum) >= hi;
+        if (tid < 2) found[tid] = kBins - 1;
         __syncthreads();
+        if (in_lo && !was_lo) found[0] = tid;
+        if (in_hi && !was_hi) found[1] = tid;
+        __syncthreads();
+        b.first = min(b.first, uint32_t(found[0]));
+        b.last = min(b.last, uint32_t(found[1]));
+        __syncthreads();
+    }
+    if (of.min_p > 0.f) {
+        // Where the weight min_p stands, give or take a bin for what rounds.
+        const double z = of.temperature * -log(double(fminf(of.min_p, 1.f))) * 0.5 * double(of.per_bin);
+        const uint32_t at = z < double(kBins) ? uint32_t(z) : kBins;
+        b.first = min(b.first, at > 0 ? at - 1 : 0);
+        b.last = min(b.last, at + 1);
+    }
+    if (b.first == kNone) b.first = kBins;  // no border: all is kept
+    if (tid == 0) found[0] = 0;
+    __syncthreads();
+    if (b.first > 0 && tid == min(b.first, kBins) - 1) found[0] = weight;
+    __syncthreads();
+    b.above = found[0];
+    __syncthreads();
+    return b;
+}
+
+__global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a, Work w) {
+    __shared__ u64 room[kWaves], found[4];
+    const uint32_t row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
+    const float *x = a.logits + size_t(row) * a.stride;
+    u64 best;
+    uint32_t least;
+    extremes(w, row, best, least, room);
+    const Weights of(a, row, key_at(best), least);
+    if (best == 0 || of.greedy()) return;
+    const Bounds b = bounds_of(a, w, row, of, room, found);
+    const u64 own = w.of_slice[(size_t(row) * w.slices + slice) * kBins + tid];
+    const u64 sure = block_sum(tid < b.first ? own : u64(0), room);
+    if (tid == 0) w.sure[size_t(row) * w.slices + slice] = sure;
+    if (b.first == kBins) return;
+    const uint32_t end = min((slice + 1) * w.slice, a.vocab);
+#pragma unroll 8
+    for (uint32_t i = slice * w.slice + tid; i < end; i += kThreads) {
+        const uint32_t key = key_of(x[i]);
+        if (key == 0) continue;
+        const uint32_t bin = of.bin(key);
+        if (bin == kBins - 1 || ((bin < b.first || bin > b.last) && bin != b.k_bin)) continue;
+        const uint32_t at = atomicAdd(&w.found[row], 1u);
+        if (at < kCandidates) w.candidates[size_t(row) * kCandidates + at] = place_of(key, i);
+    }
+}
+
+// A workgroup a row from here on. Both the row and its candidates are given as
+// each(f): f(place, key) for all of them, spread over the threads.
+struct PickLds {
+    u64 bins[256];
+    u64 room[kWaves];
+    u64 found[4];
+};
+
+// The last place, from the first one down, before which `inside(sum)` holds,
+// sums of amount(key) over the places that each() gives and `in` takes, from
+// `above` on (the first if it holds nowhere, 0 if there are none): digit by digit, a histogram of the next eight bits of those that
+// agree in the bits before.
+template <typename Each, typename In, typename Amount, typename Inside>
+__device__ u64 border_of(PickLds &lds, Each each, In in, Amount amount, Inside inside, u64 above) {
+    const uint32_t tid = threadIdx.x;
+    u64 prefix = 0;
+    for (int low = 56; low >= 0; low -= 8) {
+        __syncthreads();
+        if (tid < 256) lds.bins[tid] = 0;
+        if (tid < 2) lds.found[tid] = 0;
+        __syncthreads();
+        // The number of places beside their amounts, which may be nothing.
+        each([&](u64 place) {
+            if (!in(place) || (low < 56 && place >> (low + 8) != prefix >> (low + 8))) return;
+            atomicAdd(&lds.bins[place >> low & 255], amount(key_at(place)) << 1);
+            atomicOr(&lds.bins[place >> low & 255], 1ull);
+        });
+        __syncthreads();
+        const bool own = tid < 256;
+        const u64 bin = own ? lds.bins[255 - tid] : 0;  // from the largest down
+        const u64 sum = bin >> 1, before = above + block_scan(sum, lds.room) - sum;
+        // Bins in order: inside() holds up to some of them, of which the last is taken.
+        if (own && bin != 0 && inside(before)) atomicMax(&lds.found[0], u64(tid) + 1);
+        __syncthreads();
+        uint32_t at = uint32_t(lds.found[0]);
+        if (at == 0) {  // not even the first: it is taken all the same
+            if (own && bin != 0) atomicMax(&lds.found[1], 256 - u64(tid));
+            __syncthreads();
+            if (lds.found[1] == 0) return 0;  // no places
+            at = 257 - uint32_t(lds.found[1]);
+        }
+        if (tid == at - 1) lds.found[2] = before;
+        __syncthreads();
+        above = lds.found[2];
+        prefix |= u64(256 - at) << low;
+    }
+    return prefix;
+}
+
+// Draws from what is kept, from `base + tid` on in steps of a workgroup:
+// weight(i) of token i, 0 if it is not kept; `before` of their weight stands
+// before the first. `target` falls into them.
+template <typename Weight>
+__device__ void draw(const SampleArgs &a, uint32_t row, PickLds &lds, uint32_t begin, uint32_t end, Weight weight, u64 before, u64 target,
+                     u64 total) {
+    for (uint32_t base = begin; base < end; base += kThreads) {
+        const uint32_t i = base + threadIdx.x;
+        const u64 own = i < end ? weight(i) : 0;
+        const u64 up_to = before + block_scan(own, lds.room);
+        if (own && up_to > target && up_to - own <= target) {
+            a.tokens[row] = i;
+            a.probs[row] = float(double(own) / double(total));
+        }
+        __syncthreads();
+        if (threadIdx.x == kThreads - 1) lds.found[3] = up_to;
+        __syncthreads();
+        before = lds.found[3];
         if (before > target) return;
     }
 }
 
+__device__ __forceinline__ u64 target_of(const SampleArgs &a, uint32_t row, u64 total) {
+    const double u = fmin(fmax(double(a.uniform[row]), 0.0), 1.0);
+    return min(u64(u * double(total)), total - 1);
+}
+
+// `whole`: rows that fit the candidates' LDS, with no launch before this one.
+__global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a, Work w, bool whole) {
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    u64 *places = reinterpret_cast<u64 *>(dynamic);            // [kCandidates]
+    u64 *of_slices = places + (whole ? a.vocab : kCandidates);  // [slices]
+    __shared__ PickLds lds;
+    const uint32_t row = blockIdx.x, tid = threadIdx.x;
+    const float *x = a.logits + size_t(row) * a.stride;
+    u64 best = 0;
+    uint32_t least = 0, n = 0;
+    if (whole) {
+        n = a.vocab;
+        uint32_t low = 0;
+        for (uint32_t i = tid; i < n; i += kThreads) {
+            const uint32_t key = key_of(x[i]);
+            const u64 place = key ? place_of(key, i) : 0;
+            places[i] = place;
+            best = max(best, place);
+            if (key) low = max(low, ~key);
+        }
+        best = block_max(best, lds.room);
+        least = ~uint32_t(block_max(u64(low), lds.room));
+    } else {
+        extremes(w, row, best, least, lds.room);
+    }
+    const Weights of(a, row, key_at(best), least);
+    if (best == 0 || of.greedy()) {
+        if (tid == 0) {
+            a.tokens[row] = best ? index_at(best) : kNone;
+            a.probs[row] = best ? 1.f : 0.f;
+        }
+        return;
+    }
+    Bounds b{};
+    if (!whole) {
+        b = bounds_of(a, w, row, of, lds.room, lds.found);
+        n = b.first < kBins ? w.found[row] : 0;
+    }
+    const bool listed = whole || n <= kCandidates;
+    if (!whole && listed) {
+        for (uint32_t i = tid; i < n; i += kThreads) places[i] = w.candidates[size_t(row) * kCandidates + i];
+    }
+    __syncthreads();
+    auto each = [&](auto f) {
+        if (listed) {
+            for (uint32_t i = tid; i < n; i += kThreads)
+                if (places[i]) f(places[i]);
+        } else {
+            for (uint32_t i = tid; i < a.vocab; i += kThreads) {
+                const uint32_t key = key_of(x[i]);
+                if (key) f(place_of(key, i));
+            }
+        }
+    };
+    const bool bins = listed && !whole;  // the places are those of some bins
+
+    // Top k.
+    const uint32_t k = a.top_k[row];
+    const float p = a.top_p[row];
+    u64 k_border = 0, kept_by_k = 0;
+    if (bins ? b.k_bin != kNone : k > 0 && k < a.vocab) {
+        const u64 rank = bins ? b.k_rank : k;
+        k_border = border_of(
+            lds, each, [&](u64 place) { return !bins || of.bin(key_at(place)) == b.k_bin; }, [](uint32_t) { return u64(1); },
+            [&](u64 before) { return before < rank; }, 0);
+    }
+    // Top p, of what top k keeps.
+    u64 p_border = 0;
+    if (p < 1.f) {
+        u64 sum = 0;
+        if (!bins || b.k_bin != kNone)
+            each([&](u64 place) {
+                if (place >= k_border && (!bins || of.bin(key_at(place)) == b.k_bin)) sum += of.whole(key_at(place));
+            });
+        kept_by_k = block_sum(sum, lds.room) + (bins ? b.above_k : 0);
+        const double target = fmax(double(p), 0.0) * double(kept_by_k);
+        p_border = border_of(
+            lds, each, [&](u64 place) { return place >= k_border && (!bins || of.bin(key_at(place)) <= b.last); },
+            [&](uint32_t key) { return of.whole(key); }, [&](u64 before) { return double(before) < target; }, bins ? b.above : 0);
+    }
+    const u64 border = max(k_border, p_border);
+    auto weight = [&](uint32_t i) -> u64 {
+        const uint32_t key = key_of(x[i]);
+        return key && place_of(key, i) >= border && of.likely(key) ? of.whole(key) : 0;
+    };
+    if (!bins) {
+        u64 sum = 0;
+        each([&](u64 place) {
+            if (place >= border && of.likely(key_at(place))) sum += of.whole(key_at(place));
+        });
+        const u64 total = block_sum(sum, lds.room);
+        draw(a, row, lds, 0, a.vocab, weight, 0, target_of(a, row, total), total);
+        return;
+    }
+    // The slice that the number falls into.
+    for (uint32_t s = tid; s < w.slices; s += kThreads) of_slices[s] = w.sure[size_t(row) * w.slices + s];
+    __syncthreads();
+    each([&](u64 place) {
+        const uint32_t key = key_at(place), bin = of.bin(key);
+        if (place >= border && bin >= b.first && bin <= b.last && of.likely(key)) atomicAdd(&of_slices[index_at(place) / w.slice], of.whole(key));
+    });
+    __syncthreads();
+    u64 sum = 0;
+    for (uint32_t s = tid; s < w.slices; s += kThreads) sum += of_slices[s];
+    const u64 total = block_sum(sum, lds.room), target = target_of(a, row, total);
+    u64 before = 0;
+    for (uint32_t base = 0; base < w.slices; base += kThreads) {
+        const u64 own = base + tid < w.slices ? of_slices[base + tid] : 0, up_to = before + block_scan(own, lds.room);
+        if (own && up_to > target && up_to - own <= target) {
+            lds.found[0] = base + tid;
+            lds.found[1] = up_to - own;
+        }
+        if (tid == kThreads - 1) lds.found[2] = up_to;
+        __syncthreads();
+        before = lds.found[2];
+        if (before > target) break;
+        __syncthreads();
+    }
+    const uint32_t slice = uint32_t(lds.found[0]);
+    before = lds.found[1];
+    __syncthreads();
+    draw(a, row, lds, slice * w.slice, min((slice + 1) * w.slice, a.vocab), weight, before, target, total);
+}
+
+size_t row_bytes(uint32_t slices) {
+    return size_t(slices) * (8 + 4 + 8 + kBins * 8) + kBins * 12 + 4 + size_t(kCandidates) * 8 + 64;
+}
+
 }  // namespace
 
-hipError_t launch_sample_logits(const SampleArgs &a, const DeviceLimits &, hipStream_t stream) {
-    sample_row_kernel<<<a.rows, kThreads, 0, stream>>>(a);
+// Slices of at least 4096 logits, eight a thread, and more where there are rows
+// enough to fill the chip four times over.
+SamplePlan plan_sample(const SampleArgs &a, const DeviceLimits &lim, size_t limit) {
+    SamplePlan pl;
+    pl.whole = a.vocab <= kCandidates;
+    pl.rows = a.rows;
+    if (pl.whole) return pl;
+    pl.slice = kSliceStep;
+    const uint64_t most = uint64_t(lim.num_cus) * 4;
+    while (uint64_t(a.rows) * ((a.vocab + pl.slice - 1) / pl.slice) > most && pl.slice < a.vocab) pl.slice += kSliceStep;
+    limit = std::min(limit, size_t(64) << 20);
+    while (row_bytes((a.vocab + pl.slice - 1) / pl.slice) > limit) pl.slice *= 2;
+    pl.slices = (a.vocab + pl.slice - 1) / pl.slice;
+    pl.rows = uint32_t(std::min<uint64_t>(a.rows, limit / row_bytes(pl.slices)));
+    pl.workspace = pl.rows * row_bytes(pl.slices);
+    return pl;
+}
+
+hipError_t launch_sample_logits(const SampleArgs &all, const SamplePlan &pl, void *workspace, hipStream_t stream) {
+    SampleArgs a = all;
+    for (uint32_t row = 0; row < all.rows; row += pl.rows) {
+        const uint32_t n = std::min(pl.rows, all.rows - row);
+        a.logits = all.logits + size_t(row) * all.stride;
+        a.temperature = all.temperature + row;
+        a.top_k = all.top_k + row;
+        a.top_p = all.top_p + row;
+        a.min_p = all.min_p + row;
+        a.uniform = all.uniform + row;
+        a.tokens = all.tokens + row;
+        a.probs = all.probs + row;
+        a.rows = n;
+        Work w{};
+        w.slices = pl.slices;
+        w.slice = pl.slice;
+        uint32_t lds = all.vocab * 8;
+        if (!pl.whole) {
+            unsigned char *at = static_cast<unsigned char *>(workspace);
+            auto take = [&](size_t bytes) {
+                unsigned char *p = at;
+                at += (bytes + 7) / 8 * 8;
+                return p;
+            };
+            const size_t slices = size_t(n) * pl.slices;
+            w.best = reinterpret_cast<u64 *>(take(slices * 8));
+            w.weight = reinterpret_cast<u64 *>(take(size_t(n) * kBins * 8));
+            w.of_slice = reinterpret_cast<u64 *>(take(slices * kBins * 8));
+            w.sure = reinterpret_cast<u64 *>(take(slices * 8));
+            w.candidates = reinterpret_cast<u64 *>(take(size_t(n) * kCandidates * 8));
+            w.least = reinterpret_cast<uint32_t *>(take(slices * 4));
+            w.count = reinterpret_cast<uint32_t *>(take(size_t(n) * kBins * 4));
+            w.found = reinterpret_cast<uint32_t *>(take(size_t(n) * 4));
+            lds = kCandidates * 8 + pl.slices * 8;
+            const dim3 grid(pl.slices, n);
+            sample_max_kernel<<<grid, kThreads, 0, stream>>>(a, w);
+            sample_bins_kernel<<<grid, kThreads, 0, stream>>>(a, w);
+            sample_gather_kernel<<<grid, kThreads, 0, stream>>>(a, w);
+        }
+        const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(sample_pick_kernel), lds);
+        if (e != hipSuccess) return e;
+        sample_pick_kernel<<<n, kThreads, lds, stream>>>(a, w, pl.whole);
+    }
     return hipGetLastError();
 }
 
