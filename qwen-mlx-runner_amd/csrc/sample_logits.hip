@@ -67,9 +67,10 @@ __device__ __forceinline__ u64 place_of(uint32_t key, uint32_t i) { return u64(k
 __device__ __forceinline__ uint32_t key_at(u64 place) { return uint32_t(place >> 32); }
 __device__ __forceinline__ uint32_t index_at(u64 place) { return ~uint32_t(place); }
 
-// n weights of at most 2^shift add up to 2^62 at most.
+// n weights of at most 2^shift add up to 2^62 at most; a weight and 2^52 are a
+// double's whole number.
 __host__ __device__ constexpr uint32_t shift_of(uint32_t n) {
-    uint32_t bits = 10;
+    uint32_t bits = 12;
     while ((uint64_t(1) << bits) < n) ++bits;
     return 62 - bits;
 }
@@ -78,12 +79,13 @@ __host__ __device__ constexpr uint32_t shift_of(uint32_t n) {
 struct Weights {
     uint32_t top;
     float max, half_max, per_bin;  // bins: half the distance from the largest, times per_bin
-    double temperature;
-    double one;  // 2^shift
+    double temperature, per_octave;  // per_octave: log2(e) / temperature
+    int shift;
     float min_p;
 
     __device__ Weights(const SampleArgs &a, uint32_t row, uint32_t top_, uint32_t least)
-        : top(top_), max(logit_of(top_)), temperature(a.temperature[row]), one(double(u64(1) << shift_of(a.vocab))), min_p(a.min_p[row]) {
+        : top(top_), max(logit_of(top_)), temperature(a.temperature[row]), shift(shift_of(a.vocab)), min_p(a.min_p[row]) {
+        per_octave = 1.4426950408889634 / temperature;
         half_max = 0.5f * max;
         const float width = half_max - 0.5f * logit_of(least);
         // Narrow rows take all bins but the last, which then is empty.
@@ -95,7 +97,28 @@ struct Weights {
         if (max == INFINITY) return 0.0;
         return exp((double(logit_of(key)) - double(max)) / temperature);
     }
-    __device__ u64 whole(uint32_t key) const { return u64(__double2ll_rn(plain(key) * one)); }
+    // 2^t = 2^n 2^f, |f| <= 1/2, from the exponential's series: the term after the
+    // last is below 2^-52. Added to 2^52 the weight is rounded to a whole number
+    // and stands in the mantissa's low bits.
+    __device__ u64 whole(uint32_t key) const {
+        const double t = (double(logit_of(key)) - double(max)) * per_octave;
+        if (!(t > -64.0)) return key == top ? u64(1) << shift : 0;  // also where both are infinite
+        const double n = rint(t), y = (t - n) * 0.6931471805599453;
+        double e = 1.0 / 479001600;
+        e = fma(e, y, 1.0 / 39916800);
+        e = fma(e, y, 1.0 / 3628800);
+        e = fma(e, y, 1.0 / 362880);
+        e = fma(e, y, 1.0 / 40320);
+        e = fma(e, y, 1.0 / 5040);
+        e = fma(e, y, 1.0 / 720);
+        e = fma(e, y, 1.0 / 120);
+        e = fma(e, y, 1.0 / 24);
+        e = fma(e, y, 1.0 / 6);
+        e = fma(e, y, 0.5);
+        e = fma(e, y, 1.0);
+        e = fma(e, y, 1.0);
+        return u64(__double_as_longlong(ldexp(e, int(n) + shift) + 0x1p52)) & ((u64(1) << 52) - 1);
+    }
     __device__ bool likely(uint32_t key) const { return key == top || !(min_p > 0.f) || plain(key) >= double(min_p); }
     // Never smaller for a smaller logit, whatever rounds.
     __device__ uint32_t bin(uint32_t key) const {
@@ -140,8 +163,18 @@ __device__ __forceinline__ T block_scan(T v, T *room) {
     return v;
 }
 
+// Which bins the borders may fall into.
+struct Bounds {
+    uint32_t first, last;  // between them tokens may be kept or not; all above are
+    uint32_t k_bin;        // where top k ends; kNone: it keeps all
+    uint32_t k_rank;       // so many of k_bin are kept by top k
+    u64 above;             // weight above `first`
+    u64 above_k;           // weight above k_bin, or of all
+};
+
 // What the launches leave for each other, a row.
 struct Work {
+    Bounds *bounds;    // [rows]
     u64 *best;         // [rows][slices] a slice's first place
     uint32_t *least;   // [rows][slices] its smallest key, of those kept at all
     uint32_t *count;   // [rows][kBins]
@@ -192,11 +225,24 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, Work
     }
 }
 
+// Eight logits of a thread, a workgroup's width apart; -infinity past the end.
+constexpr int kAhead = 8;
+struct Ahead {
+    float x[kAhead];
+    __device__ __forceinline__ void load(const float *p, uint32_t i, uint32_t end) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) x[j] = i + j * kThreads < end ? p[i + j * kThreads] : -INFINITY;
+    }
+};
+
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Work w) {
     __shared__ u64 room[kWaves], weight[kBins];
     __shared__ uint32_t count[kBins];
     const uint32_t row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
     const float *x = a.logits + size_t(row) * a.stride;
+    const uint32_t begin = slice * w.slice + tid, end = min((slice + 1) * w.slice, a.vocab);
+    Ahead ahead;
+    ahead.load(x, begin, end);  // on their way while the slices' largest is found
     u64 best;
     uint32_t least;
     extremes(w, row, best, least, room);
@@ -205,15 +251,17 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Wor
     weight[tid] = 0;
     count[tid] = 0;
     __syncthreads();
-    const uint32_t end = min((slice + 1) * w.slice, a.vocab);
-#pragma unroll 4
-    for (uint32_t i = slice * w.slice + tid; i < end; i += kThreads) {
-        const uint32_t key = key_of(x[i]);
-        if (key == 0) continue;
-        const uint32_t bin = of.bin(key);
-        if (bin == kBins - 1) continue;
-        atomicAdd(&count[bin], 1u);
-        atomicAdd(&weight[bin], of.whole(key));
+    for (uint32_t i = begin; i < end; i += kAhead * kThreads) {
+        const Ahead now = ahead;
+        ahead.load(x, i + kAhead * kThreads, end);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const uint32_t key = key_of(now.x[j]);
+            const uint32_t bin = key ? of.bin(key) : kBins - 1;
+            if (bin == kBins - 1) continue;
+            atomicAdd(&count[bin], 1u);
+            atomicAdd(&weight[bin], of.whole(key));
+        }
     }
     __syncthreads();
     const uint32_t n = count[tid];
@@ -224,16 +272,6 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Wor
         atomicAdd(&w.weight[size_t(row) * kBins + tid], sum);
     }
 }
-
-// Which bins the borders may fall into.
-struct Bounds {
-    uint32_t first, last;  // between them tokens may be kept or not; all above are
-    uint32_t k_bin;        // where top k ends; kNone: it keeps all
-    u64 above;             // weight above `first`
-    u64 above_k;           // weight above k_bin, or of all
-    uint32_t k_rank;       // so many of k_bin are kept by top k
-    bool p;                // top p has a border
-};
 
 __device__ Bounds bounds_of(const SampleArgs &a, const Work &w, uint32_t row, const Weights &of, u64 *room, u64 *found) {
     const uint32_t tid = threadIdx.x, k = a.top_k[row];
@@ -268,8 +306,7 @@ __device__ Bounds bounds_of(const SampleArgs &a, const Work &w, uint32_t row, co
     b.above_k = least;
     b.first = b.k_bin;
     b.last = b.k_bin;
-    b.p = p < 1.f;
-    if (b.p) {
+    if (p < 1.f) {
         // The first bin up to which the weight that top p asks for stands, with
         // the least and with the most that top k may keep.
         const double lo = fmax(double(p), 0.0) * double(least) * (1 - 1e-12), hi = fmax(double(p), 0.0) * double(most) * (1 + 1e-12);
@@ -302,99 +339,144 @@ __device__ Bounds bounds_of(const SampleArgs &a, const Work &w, uint32_t row, co
 }
 
 __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a, Work w) {
-    __shared__ u64 room[kWaves], found[4];
+    constexpr uint32_t kRoom = 2048;
+    __shared__ u64 room[kWaves], found[4], places[kRoom];
+    __shared__ uint32_t here, first;
     const uint32_t row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
     const float *x = a.logits + size_t(row) * a.stride;
+    const uint32_t begin = slice * w.slice + tid, end = min((slice + 1) * w.slice, a.vocab);
+    Ahead ahead;
+    ahead.load(x, begin, end);
+    const u64 own = w.of_slice[(size_t(row) * w.slices + slice) * kBins + tid];
     u64 best;
     uint32_t least;
     extremes(w, row, best, least, room);
     const Weights of(a, row, key_at(best), least);
     if (best == 0 || of.greedy()) return;
+    if (tid == 0) here = 0;
     const Bounds b = bounds_of(a, w, row, of, room, found);
-    const u64 own = w.of_slice[(size_t(row) * w.slices + slice) * kBins + tid];
     const u64 sure = block_sum(tid < b.first ? own : u64(0), room);
     if (tid == 0) w.sure[size_t(row) * w.slices + slice] = sure;
+    if (slice == 0 && tid == 0) w.bounds[row] = b;
     if (b.first == kBins) return;
-    const uint32_t end = min((slice + 1) * w.slice, a.vocab);
-#pragma unroll 8
-    for (uint32_t i = slice * w.slice + tid; i < end; i += kThreads) {
-        const uint32_t key = key_of(x[i]);
-        if (key == 0) continue;
-        const uint32_t bin = of.bin(key);
-        if (bin == kBins - 1 || ((bin < b.first || bin > b.last) && bin != b.k_bin)) continue;
-        const uint32_t at = atomicAdd(&w.found[row], 1u);
-        if (at < kCandidates) w.candidates[size_t(row) * kCandidates + at] = place_of(key, i);
+    for (uint32_t i = begin; i < end; i += kAhead * kThreads) {
+        const Ahead now = ahead;
+        ahead.load(x, i + kAhead * kThreads, end);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const uint32_t key = key_of(now.x[j]);
+            const uint32_t bin = key ? of.bin(key) : kBins - 1;
+            if (bin == kBins - 1 || ((bin < b.first || bin > b.last) && bin != b.k_bin)) continue;
+            const uint32_t at = atomicAdd(&here, 1u);
+            const u64 place = place_of(key, i + j * kThreads);
+            if (at < kRoom) {
+                places[at] = place;
+            } else {
+                const uint32_t to = atomicAdd(&w.found[row], 1u);
+                if (to < kCandidates) w.candidates[size_t(row) * kCandidates + to] = place;
+            }
+        }
     }
+    __syncthreads();
+    const uint32_t n = min(here, kRoom);
+    if (tid == 0 && n) first = atomicAdd(&w.found[row], n);
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += kThreads)
+        if (first + i < kCandidates) w.candidates[size_t(row) * kCandidates + first + i] = places[i];
 }
 
 // A workgroup a row from here on. Both the row and its candidates are given as
 // each(f): f(place, key) for all of them, spread over the threads.
 struct PickLds {
-    u64 bins[256];
+    u64 amounts[256];
+    u64 some[256];       // a place of each bin
+    uint32_t counts[256];
     u64 room[kWaves];
     u64 found[4];
 };
 
 // The last place, from the first one down, before which `inside(sum)` holds,
 // sums of amount(key) over the places that each() gives and `in` takes, from
-// `above` on (the first if it holds nowhere, 0 if there are none): digit by digit, a histogram of the next eight bits of those that
-// agree in the bits before.
+// `above` on (the first if it holds nowhere, 0 if there are none): a histogram
+// of the first eight bits in which they differ, then of the next eight of those
+// in the border's bin, until that has one.
 template <typename Each, typename In, typename Amount, typename Inside>
 __device__ u64 border_of(PickLds &lds, Each each, In in, Amount amount, Inside inside, u64 above) {
     const uint32_t tid = threadIdx.x;
-    u64 prefix = 0;
-    for (int low = 56; low >= 0; low -= 8) {
+    u64 top = 0, rest = 0;  // rest: the smallest, upside down
+    each([&](u64 place) {
+        if (in(place)) top = max(top, place), rest = max(rest, ~place);
+    });
+    top = block_max(top, lds.room);
+    rest = ~block_max(rest, lds.room);
+    if (top == 0) return 0;
+    if (top == rest) return top;
+    // The window's bits, and those above it.
+    const int high = 64 - __clzll(static_cast<long long>(top ^ rest));
+    int width = min(8, high), low = high - width;
+    u64 prefix = high < 64 ? top >> high : 0;
+    for (;;) {
         __syncthreads();
-        if (tid < 256) lds.bins[tid] = 0;
+        if (tid < 256) lds.amounts[tid] = 0, lds.some[tid] = 0, lds.counts[tid] = 0;
         if (tid < 2) lds.found[tid] = 0;
         __syncthreads();
-        // The number of places beside their amounts, which may be nothing.
         each([&](u64 place) {
-            if (!in(place) || (low < 56 && place >> (low + 8) != prefix >> (low + 8))) return;
-            atomicAdd(&lds.bins[place >> low & 255], amount(key_at(place)) << 1);
-            atomicOr(&lds.bins[place >> low & 255], 1ull);
+            if (!in(place) || place >> low >> width != prefix) return;
+            const uint32_t bin = 255 - uint32_t(place >> low & ((1u << width) - 1));  // the largest first
+            atomicAdd(&lds.amounts[bin], amount(key_at(place)));
+            atomicAdd(&lds.counts[bin], 1u);
+            lds.some[bin] = place;
         });
         __syncthreads();
-        const bool own = tid < 256;
-        const u64 bin = own ? lds.bins[255 - tid] : 0;  // from the largest down
-        const u64 sum = bin >> 1, before = above + block_scan(sum, lds.room) - sum;
-        // Bins in order: inside() holds up to some of them, of which the last is taken.
-        if (own && bin != 0 && inside(before)) atomicMax(&lds.found[0], u64(tid) + 1);
-        __syncthreads();
-        uint32_t at = uint32_t(lds.found[0]);
-        if (at == 0) {  // not even the first: it is taken all the same
-            if (own && bin != 0) atomicMax(&lds.found[1], 256 - u64(tid));
-            __syncthreads();
-            if (lds.found[1] == 0) return 0;  // no places
-            at = 257 - uint32_t(lds.found[1]);
+        const u64 sum = tid < 256 ? lds.amounts[tid] : 0, before = above + block_scan(sum, lds.room) - sum;
+        // inside() holds up to some of the bins, of which the last is taken.
+        if (tid < 256 && lds.counts[tid] != 0) {
+            if (inside(before)) atomicMax(&lds.found[0], u64(tid) + 1);
+            atomicMax(&lds.found[1], 256 - u64(tid));
         }
-        if (tid == at - 1) lds.found[2] = before;
         __syncthreads();
+        const uint32_t at = lds.found[0] ? uint32_t(lds.found[0]) - 1 : 256 - uint32_t(lds.found[1]);
+        if (tid == at) lds.found[2] = before;
+        __syncthreads();
+        if (lds.counts[at] == 1) return lds.some[at];
         above = lds.found[2];
-        prefix |= u64(256 - at) << low;
+        prefix = prefix << width | (255 - at);
+        width = min(8, low);
+        low -= width;
     }
-    return prefix;
 }
 
-// Draws from what is kept, from `base + tid` on in steps of a workgroup:
-// weight(i) of token i, 0 if it is not kept; `before` of their weight stands
-// before the first. `target` falls into them.
+// Draws from what tokens begin..end-1 keep: weight(i) of token i, 0 if it is not
+// kept; `before` of the weight stands before them, and `target` falls into them.
 template <typename Weight>
 __device__ void draw(const SampleArgs &a, uint32_t row, PickLds &lds, uint32_t begin, uint32_t end, Weight weight, u64 before, u64 target,
                      u64 total) {
-    for (uint32_t base = begin; base < end; base += kThreads) {
-        const uint32_t i = base + threadIdx.x;
-        const u64 own = i < end ? weight(i) : 0;
-        const u64 up_to = before + block_scan(own, lds.room);
-        if (own && up_to > target && up_to - own <= target) {
-            a.tokens[row] = i;
-            a.probs[row] = float(double(own) / double(total));
+    constexpr uint32_t kEach = 8;  // of a thread, in sequence
+    for (uint32_t base = begin; base < end; base += kEach * kThreads) {
+        const uint32_t first = base + threadIdx.x * kEach;
+        u64 own[kEach], sum = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; ++j) {
+            own[j] = first + j < end ? weight(first + j) : 0;
+            sum += own[j];
         }
-        __syncthreads();
+        u64 up_to = before + block_scan(sum, lds.room);
         if (threadIdx.x == kThreads - 1) lds.found[3] = up_to;
+        if (up_to > target && up_to - sum <= target) {
+            up_to -= sum;
+#pragma unroll
+            for (uint32_t j = 0; j < kEach; ++j) {
+                up_to += own[j];
+                if (up_to > target && up_to - own[j] <= target) {
+                    a.tokens[row] = first + j;
+                    a.probs[row] = float(double(own[j]) / double(total));
+                }
+            }
+        }
         __syncthreads();
         before = lds.found[3];
         if (before > target) return;
+        __syncthreads();
     }
 }
 
@@ -438,7 +520,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a, Wor
     }
     Bounds b{};
     if (!whole) {
-        b = bounds_of(a, w, row, of, lds.room, lds.found);
+        b = w.bounds[row];
         n = b.first < kBins ? w.found[row] : 0;
     }
     const bool listed = whole || n <= kCandidates;
@@ -528,7 +610,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a, Wor
 }
 
 size_t row_bytes(uint32_t slices) {
-    return size_t(slices) * (8 + 4 + 8 + kBins * 8) + kBins * 12 + 4 + size_t(kCandidates) * 8 + 64;
+    return size_t(slices) * (8 + 4 + 8 + kBins * 8) + kBins * 12 + 4 + size_t(kCandidates) * 8 + sizeof(Bounds) + 64;
 }
 
 }  // namespace
@@ -576,6 +658,7 @@ hipError_t launch_sample_logits(const SampleArgs &all, const SamplePlan &pl, voi
                 return p;
             };
             const size_t slices = size_t(n) * pl.slices;
+            w.bounds = reinterpret_cast<Bounds *>(take(n * sizeof(Bounds)));
             w.best = reinterpret_cast<u64 *>(take(slices * 8));
             w.weight = reinterpret_cast<u64 *>(take(size_t(n) * kBins * 8));
             w.of_slice = reinterpret_cast<u64 *>(take(slices * kBins * 8));
