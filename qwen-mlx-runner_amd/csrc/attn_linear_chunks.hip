@@ -62,7 +62,6 @@ using wave::h2;
 using wave::h8;
 using wave::kRsrcWord3;
 using wave::lds_barrier;
-using wave::less_half;
 using wave::two_halves;
 using wave::u4;
 using wave::wait_dma;
@@ -162,13 +161,54 @@ constexpr int kPrepare = 256;
 
 template <int KB>
 struct PrepareLds {
-    static constexpr uint32_t kGram = 0;                        // [2][32][33] FP32: q k, k k
-    static constexpr uint32_t kRows = 2 * 32 * 33 * 4;          // [4][32] FP32 of rows
+    static constexpr uint32_t kPitch = 36;                      // floats of a row of 32
+    static constexpr uint32_t kSquare = 32 * kPitch * 4;
+    static constexpr uint32_t kGram = 0;                        // q k, k k
+    static constexpr uint32_t kRows = 2 * kSquare;              // [4][32] FP32 of rows
     static constexpr uint32_t kRest = kRows + 4 * 32 * 4;       // terms of q and k, then each wave's own
     static constexpr uint32_t kTerms = 4 * kTile * KB;          // of q, or of k
-    static constexpr uint32_t kA = 0, kMT = 32 * 36 * 4, kG = kMT + 8 * kTile, kWave = kG + 32 * 8 + 32 * 4;
+    static constexpr uint32_t kA = 0, kT = kSquare, kG = 2 * kSquare, kWave = kG + 32 * 8 + 32 * 4;
     static constexpr uint32_t kBytes = kRest + (2 * kTerms > 4 * kWave ? 2 * kTerms : 4 * kWave);
 };
+
+__device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// T = (I + A)^-1 for A [32][pitch] below its diagonal, a wave's: two blocks of
+// 16 on the diagonal, a lane a column, then T21 = -T22 (A21 T11) in FP32
+// matrix instructions. (A lane a column of all 32 takes 496 products in place
+// of 120, and each row waits for the one before it.)
+template <uint32_t PITCH>
+__device__ __forceinline__ void invert(const float *A, float *T) {
+    const uint32_t l = threadIdx.x % 64, g = l / 16, m = l % 16, at = l / 16 % 2 * 16;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float even = uint32_t(i) == m ? 1.f : 0.f, odd = 0.f;
+#pragma unroll
+        for (int c = 0; c < i; ++c) {
+            const float v = A[(at + i) * PITCH + at + c];
+            if (c % 2) odd = fmaf(-v, x[c], odd);
+            else even = fmaf(-v, x[c], even);
+        }
+        x[i] = even + odd;
+    }
+    if (l < 32) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) T[(at + i) * PITCH + at + m] = x[i];
+    }
+    wave_lds_sync();
+    // Step s has columns 4g + s of the left side and those rows of the right.
+    const f4 a21 = *reinterpret_cast<const f4 *>(A + (16 + m) * PITCH + 4 * g);
+    const f4 t22 = *reinterpret_cast<const f4 *>(T + (16 + m) * PITCH + 16 + 4 * g);
+    f4 y{}, z{};
+#pragma unroll
+    for (int s = 0; s < 4; ++s) y = mfma4(a21[s], T[(4 * g + s) * PITCH + m], y);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) z = mfma4(t22[s], y[s], z);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) T[(16 + 4 * g + i) * PITCH + m] = -z[i];
+    wave_lds_sync();
+}
 
 template <int KB, bool DELTA>
 __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, Pass pass) {
@@ -229,8 +269,9 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const float b0 = x[r][u].x[2 * j] * by, b1 = x[r][u].x[2 * j + 1] * by;
-                    hi[j] = two_halves(b0, b1);
-                    lo[j] = two_halves(less_half<0>(b0, hi[j]), less_half<1>(b1, hi[j]));
+                    const h2 h = __builtin_convertvector((f2{b0, b1}), h2);
+                    hi[j] = __builtin_bit_cast(uint32_t, h);
+                    lo[j] = two_halves(b0 - float(h[0]), b1 - float(h[1]));
                 }
                 const uint32_t at = ((i / 16 * KB + u) * 2) * kTile + (seg % 4 * 16 + i % 16) * 16 + seg / 4 * 8;
                 unsigned char *to = rest + r * L::kTerms + at;
@@ -283,16 +324,16 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            gram[(rt * 16 + 4 * g + i) * 33 + ct * 16 + m] = qk[i];
-            if constexpr (DELTA) gram[(32 + rt * 16 + 4 * g + i) * 33 + ct * 16 + m] = kk[i];
+            gram[(rt * 16 + 4 * g + i) * L::kPitch + ct * 16 + m] = qk[i];
+            if constexpr (DELTA) gram[(32 + rt * 16 + 4 * g + i) * L::kPitch + ct * 16 + m] = kk[i];
         }
     }
     __syncthreads();
 
-    // A wave a value head of this key head.
+    // A wave a value head of this key head. Lanes have a token each (twice), and
+    // then of rows m and 16 + m the columns 4g.. and 16 + 4g.., as operands do.
     unsigned char *own = rest + w * L::kWave;
-    float *A = reinterpret_cast<float *>(own + L::kA);  // [32][36]
-    unsigned char *mt = own + L::kMT;                   // M, T
+    float *A = reinterpret_cast<float *>(own + L::kA), *T = reinterpret_cast<float *>(own + L::kT);
     double *Gs = reinterpret_cast<double *>(own + L::kG);
     float *by_row = reinterpret_cast<float *>(own + L::kG + 32 * 8);
     const uint32_t group = a.v_heads / a.k_heads, j = l % 32;
@@ -301,7 +342,10 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
     float top = ck;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    const float part_of_top = top > 0.f ? ck / top : 0.f;
+    const float of_top = top > 0.f ? 1.f / top : 0.f;
+    f4 cks[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) cks[half] = *reinterpret_cast<const f4 *>(rows + 16 * half + 4 * g);
     for (uint32_t vh = w; vh < group; vh += kPrepare / 64) {
         const uint32_t h = kh * group + vh;
         const bool real = j < n;
@@ -318,50 +362,68 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
         Gs[j] = G;
         by_row[j] = beta * ck;
         wave_lds_sync();
+        unsigned char *to = pass.of_value(a, chunk, h);
         bool bad = bad_rows;
-#pragma unroll 4
-        for (uint32_t r = 0; r < 16; ++r) {
-            const uint32_t i = 2 * r + l / 32;
-            const float e = i >= j ? expf(float(Gs[i] - G)) : 0.f;
-            const float x = i >= j ? ldexpf(gram[i * 33 + j], -kScore) * part_of_top * e : 0.f;
-            bad |= !(fabsf(x) < 60000.f);
-            const uint32_t hi = two_halves(x, x), lo = two_halves(less_half<0>(x, hi), 0.f);
-            unsigned char *to = mt + i / 16 * 2 * kTile + (j % 16 / 4 * 16 + i % 16) * 16 + j / 16 * 8 + j % 4 * 2;
-            *reinterpret_cast<uint16_t *>(to) = uint16_t(hi);
-            *reinterpret_cast<uint16_t *>(to + kTile) = uint16_t(lo);
-            if constexpr (DELTA) A[i * 36 + j] = i > j ? by_row[i] * ck * gram[(32 + i) * 33 + j] * e : 0.f;
+#pragma unroll
+        for (uint32_t half = 0; half < 2; ++half) {  // rows
+            const uint32_t i = 16 * half + m;
+            const double Gi = Gs[i];
+            const float of_row = by_row[i];
+            float M[8];
+#pragma unroll
+            for (uint32_t c = 0; c < 2; ++c) {  // columns
+                const uint32_t j0 = 16 * c + 4 * g;
+                f4 below{};
+#pragma unroll
+                for (uint32_t q = 0; q < 4; ++q) M[4 * c + q] = 0.f;
+                if (c <= half) {
+                    const f4 qk = *reinterpret_cast<const f4 *>(gram + i * L::kPitch + j0);
+                    f4 kk{};
+                    if constexpr (DELTA) kk = *reinterpret_cast<const f4 *>(gram + (32 + i) * L::kPitch + j0);
+#pragma unroll
+                    for (uint32_t q = 0; q < 4; ++q) {
+                        const float e = i >= j0 + q ? expf(float(Gi - Gs[j0 + q])) : 0.f;
+                        M[4 * c + q] = i >= j0 + q ? ldexpf(qk[q], -kScore) * (cks[c][q] * of_top) * e : 0.f;
+                        below[q] = i > j0 + q ? of_row * cks[c][q] * kk[q] * e : 0.f;
+                        bad |= !(fabsf(M[4 * c + q]) < 60000.f);
+                    }
+                }
+                if constexpr (DELTA) *reinterpret_cast<f4 *>(A + i * L::kPitch + j0) = below;
+            }
+            u4 hi, lo;
+            terms(M, -1.f, hi, lo);
+            *reinterpret_cast<u4 *>(to + 2 * half * kTile + l * 16) = hi;
+            *reinterpret_cast<u4 *>(to + (2 * half + 1) * kTile + l * 16) = lo;
         }
         float rows_of_t = 1.f;
         if constexpr (DELTA) {
             wave_lds_sync();
-            // Column j of T, row after row.
-            float x[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                float even = uint32_t(i) == j ? 1.f : 0.f, odd = 0.f;
-#pragma unroll
-                for (int c = 0; c < i; ++c) {
-                    if (c % 2) odd = fmaf(-A[i * 36 + c], x[c], odd);
-                    else even = fmaf(-A[i * 36 + c], x[c], even);
-                }
-                x[i] = even + odd;
-                asm volatile("" : "+v"(x[i]) : : "memory");  // or all of A is loaded at once
-            }
+            invert<L::kPitch>(A, T);
             rows_of_t = 0.f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                bad |= !(fabsf(x[i]) < 2.f);
-                rows_of_t = fmaxf(rows_of_t, fabsf(x[i]));
-                const float t = ldexpf(x[i], kSolve);
-                const uint32_t hi = two_halves(t, t), lo = two_halves(less_half<0>(t, hi), 0.f);
-                unsigned char *to = mt + (4 + l / 32) * kTile + i / 16 * 2 * kTile + (j % 16 / 4 * 16 + i % 16) * 16 + j / 16 * 8 + j % 4 * 2;
-                *reinterpret_cast<uint16_t *>(to) = uint16_t(l < 32 ? hi : lo);
-            }
-            // A row of T adds up to no more than its columns' largest do.
+            for (uint32_t half = 0; half < 2; ++half) {
+                const uint32_t i = 16 * half + m;
+                float x[8], sum = 0.f;
 #pragma unroll
-            for (int d = 1; d < 32; d *= 2) rows_of_t += __shfl_xor(rows_of_t, d);
+                for (uint32_t c = 0; c < 2; ++c) {
+                    const f4 t = c <= half ? *reinterpret_cast<const f4 *>(T + i * L::kPitch + 16 * c + 4 * g) : f4{};
+#pragma unroll
+                    for (uint32_t q = 0; q < 4; ++q) {
+                        bad |= !(fabsf(t[q]) < 2.f);
+                        sum += fabsf(t[q]);
+                        x[4 * c + q] = ldexpf(t[q], kSolve);
+                    }
+                }
+                rows_of_t = fmaxf(rows_of_t, column_sum(sum));
+                u4 hi, lo;
+                terms(x, -1.f, hi, lo);
+                unsigned char *t = to + kScalars + kTile + 2 * half * kTile + l * 16;
+                *reinterpret_cast<u4 *>(t) = hi;
+                *reinterpret_cast<u4 *>(t + kTile) = lo;
+            }
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) rows_of_t = fmaxf(rows_of_t, __shfl_xor(rows_of_t, d));
         }
-        wave_lds_sync();
         const float grown = expf(float(G)), left = expf(float(all - G)), whole = expf(float(all));
         const float of_q = a.scale * grown * cq, of_x = beta * grown * ck, of_u = left * ck;
         const float of_m = ldexpf(a.scale * cq * top, kScore);
@@ -371,14 +433,6 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
         const bool wild = __ballot(bad) != 0;
-        unsigned char *to = pass.of_value(a, chunk, h);
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            *reinterpret_cast<u4 *>(to + p * kTile + l * 16) = *reinterpret_cast<const u4 *>(mt + p * kTile + l * 16);
-            if constexpr (DELTA)
-                *reinterpret_cast<u4 *>(to + kScalars + kTile + p * kTile + l * 16) =
-                    *reinterpret_cast<const u4 *>(mt + (4 + p) * kTile + l * 16);
-        }
         float *scalars = reinterpret_cast<float *>(to + kScalars);
         if (l < 32) {
             scalars[kBeta + j] = beta;
