@@ -75,8 +75,7 @@ constexpr int kScore = 2;                // M's entries are products of scaled r
 constexpr int kSolve = 4;                // T's entries are by 2^kSolve
 
 // A chunk's operands. Of a key head: Q [2 tiles of 16 tokens][blocks][2 terms],
-// K^T [2 * blocks tiles of 16 dims][2 terms], K as Q (delta rule). Of a value
-// head: M [2][2 terms], scalars, T as M (delta rule).
+// and K. Of a value head: M [2][2 terms], scalars, T as M (delta rule).
 constexpr uint32_t kScalars = 4 * kTile;  // where they stand
 enum Scalar : uint32_t { kBeta = 0, kX = 32, kQ = 64, kM = 96, kU = 128, kWhole = 160, kMost = 161, kWild = 162 };
 
@@ -138,7 +137,9 @@ __device__ __forceinline__ u4 rsrc_of(const void *p, uint32_t bytes) {
 }
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float *p, uint32_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p), 0, int(bytes), kRsrcWord3);
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    const uint64_t same = uint64_t(__builtin_amdgcn_readfirstlane(uint32_t(at >> 32))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(at)));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<float *>(same), 0, __builtin_amdgcn_readfirstlane(int(bytes)), kRsrcWord3);
 }
 
 // Which chunks a pass has, and where their operands are.
@@ -226,7 +227,6 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
     const uint32_t t0 = part * kChunk, n = min(kChunk, count - t0);
     const size_t token0 = size_t(first) + t0;
     unsigned char *out = pass.of_key(a, chunk, kh);
-    constexpr uint32_t kOutKt = L::kTerms, kOutK = 2 * L::kTerms;
 
     // Eight lanes a token: 4-dim pieces seg, seg + 8, ..
     {
@@ -277,38 +277,14 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
                 unsigned char *to = rest + r * L::kTerms + at;
                 *reinterpret_cast<uint2 *>(to) = uint2{hi[0], hi[1]};
                 *reinterpret_cast<uint2 *>(to + kTile) = uint2{lo[0], lo[1]};
-                if (r == 0 || DELTA) {
-                    to = out + (r ? kOutK : 0) + at;
-                    *reinterpret_cast<uint2 *>(to) = uint2{hi[0], hi[1]};
-                    *reinterpret_cast<uint2 *>(to + kTile) = uint2{lo[0], lo[1]};
-                }
+                to = out + r * L::kTerms + at;
+                *reinterpret_cast<uint2 *>(to) = uint2{hi[0], hi[1]};
+                *reinterpret_cast<uint2 *>(to + kTile) = uint2{lo[0], lo[1]};
             }
         }
     }
     __syncthreads();
 
-    // K^T: four dims and eight tokens at a time.
-    for (uint32_t it = tid; it < 64 * KB; it += kPrepare) {
-        const uint32_t quad = it / 32 * 4 + it % 4, gt = it / 4 % 4, hl = it / 16 % 2;
-        uint2 x[2][4];
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                x[tt][e] = *reinterpret_cast<const uint2 *>(rest + L::kTerms + ((tt * KB + quad / 8) * 2 + hl) * kTile +
-                                                            (quad % 4 * 16 + 4 * gt + e) * 16 + quad / 4 % 2 * 8);
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            u4 y;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint2 x0 = x[k / 2][k % 2 * 2], x1 = x[k / 2][k % 2 * 2 + 1];
-                const uint32_t lo = d < 2 ? x0.x : x0.y, hi = d < 2 ? x1.x : x1.y;
-                y[k] = __builtin_amdgcn_perm(hi, lo, d % 2 ? 0x07060302u : 0x05040100u);
-            }
-            *reinterpret_cast<u4 *>(out + kOutKt + (quad / 4 * 2 + hl) * kTile + (gt * 16 + quad % 4 * 4 + d) * 16) = y;
-        }
-    }
     // Products of rows: tiles (0, 0), (1, 0), (1, 1).
     if (w < 3) {
         const uint32_t rt = w > 0, ct = w == 2;
@@ -455,7 +431,7 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
 // One wave's columns of a chunk, token after token, for chunks whose algebra
 // would not hold. S: the state itself, tile t's lane has rows 16t + 4g + i.
 template <int TD>
-__device__ void tokens_of_chunk(const LinearArgs &a, size_t token0, uint32_t n, uint32_t h, uint32_t col, f4 (&S)[TD]) {
+__device__ __forceinline__ void tokens_of_chunk(const LinearArgs &a, size_t token0, uint32_t n, uint32_t h, uint32_t col, f4 (&S)[TD]) {
     const uint32_t g = threadIdx.x % 64 / 16, kh = h / (a.v_heads / a.k_heads);
     const bool has = col < a.dv;
     for (uint32_t t = 0; t < n; ++t) {
@@ -497,22 +473,29 @@ __device__ void tokens_of_chunk(const LinearArgs &a, size_t token0, uint32_t n, 
     }
 }
 
-template <int KB, int NC, bool DELTA>
-struct ScanLds {
-    static constexpr uint32_t kKey = (DELTA ? 12 : 8) * kTile * KB, kValue = (DELTA ? 9 : 5) * kTile;
+// How a workgroup's waves share the work: NC 16-column tiles, of each SPLIT parts
+// of the key dimension, a wave each, and NL waves that load.
+template <int KB, int NC, int SPLIT, int NL, bool DELTA>
+struct Scan {
+    static constexpr int kWorkers = NC * SPLIT, kThreads = (kWorkers + NL) * 64;
+    static constexpr uint32_t kTerms = 4 * kTile * KB;  // of Q, or of K
+    static constexpr uint32_t kKey = 2 * kTerms, kValue = (DELTA ? 9 : 5) * kTile;
     static constexpr uint32_t kV = kChunk * NC * 16 * 4;  // the workgroup's columns of the values
     static constexpr uint32_t kStage = kKey + kValue + kV;
-    static constexpr uint32_t kStages = 2 * kStage <= 160 * 1024 ? 2 : 1;
-    static constexpr uint32_t kBytes = kStages * kStage;
+    // What the waves of a tile tell each other: sums over their parts.
+    static constexpr uint32_t kX = 2 * kTile, kO = kTile, kTop = 256, kTold = kX + kO + kTop;
+    static constexpr uint32_t kShared = SPLIT > 1 ? kWorkers * kTold + kWorkers * 4 : 0;
+    static constexpr uint32_t kStages = 2 * kStage + kShared <= 160 * 1024 ? 2 : 1;
+    static constexpr uint32_t kBytes = kStages * kStage + kShared;
 };
 
-// A workgroup's waves: NC with a 16-column tile each, and NL that load.
-template <int KB, int NC, int NL, bool DELTA>
-__global__ __launch_bounds__((NC + NL) * 64, KB == 8 ? 1 : 2) void linear_scan_kernel(LinearArgs a, Pass pass) {
+template <int KB, int NC, int SPLIT, int NL, bool DELTA>
+__global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1) void linear_scan_kernel(LinearArgs a, Pass pass) {
     extern __shared__ __align__(16) unsigned char lds[];
-    using L = ScanLds<KB, NC, DELTA>;
-    constexpr int TD = 2 * KB;
-    const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), g = l / 16;
+    using L = Scan<KB, NC, SPLIT, NL, DELTA>;
+    constexpr int KW = KB / SPLIT, TD = 2 * KW;  // a wave's blocks and tiles of the key dimension
+    constexpr int kWorkers = L::kWorkers;
+    const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), g = l / 16, m = l % 16;
 
     // Workgroups go to the eight dies in turn: all those of a key head to one,
     // whose cache then has its operands once.
@@ -530,23 +513,38 @@ __global__ __launch_bounds__((NC + NL) * 64, KB == 8 ? 1 : 2) void linear_scan_k
 
     const uint32_t lds0 = uint32_t(uintptr_t((__attribute__((address_space(3))) unsigned char *)lds));
     auto stage_of = [&](uint32_t c) { return L::kStages == 2 ? (c - c0) % 2 * L::kStage : 0; };
-    if (w >= NC) {
-        // A chunk ahead of the others: every barrier says that a chunk is there
-        // and that the one before is no longer read.
+    // Whether a chunk is done token after token: the operands say so, or, where
+    // waves share a tile, one of them does (all then, as they meet at barriers).
+    unsigned char *shared = lds + L::kStages * L::kStage;
+    uint32_t *odd_waves = reinterpret_cast<uint32_t *>(shared + kWorkers * L::kTold);
+    auto is_wild = [&](uint32_t c) {
+        return reinterpret_cast<const uint32_t *>(lds + stage_of(c) + L::kKey + kScalars)[kWild];
+    };
+    auto some_odd = [&] {
+        uint32_t some = 0;
+#pragma unroll
+        for (int k = 0; k < kWorkers; ++k) some |= odd_waves[k];
+        return some;
+    };
+    if (w >= kWorkers) {
+        // A chunk ahead of the others: every first barrier says that a chunk is
+        // there and that the one before is no longer read.
         constexpr uint32_t kAt = NC * 16;  // columns of the workgroup
         const uint32_t col0 = in_unit % pass.columns * kAt + l % kAt;
         const uint32_t values_at = col0 < a.dv ? (l / kAt * a.v_stride + col0) * 4 : kOut;
+        const uint32_t own = w - kWorkers;
+        if (SPLIT > 1) lds_barrier();
         for (uint32_t c = c0; c < c1; ++c) {
             const uint32_t to = lds0 + stage_of(c), t0 = (c - begin) * kChunk, n = min(kChunk, count - t0);
             const u4 keys = rsrc_of(pass.of_key(a, c, kh), L::kKey), values = rsrc_of(pass.of_value(a, c, h), L::kValue);
             const u4 v = rsrc_of(a.v + (size_t(first) + t0) * a.v_stride + size_t(h) * a.dv, ((n - 1) * a.v_stride + a.dv) * 4);
             if (L::kStages == 1 && c > c0) lds_barrier();
-            uint32_t piece = (w - NC) * 256, row = (w - NC) * (64 / kAt) * a.v_stride * 4;
+            uint32_t piece = own * 256, row = own * (64 / kAt) * a.v_stride * 4;
             asm volatile("" : "+s"(piece), "+s"(row));  // counted here, not kept in registers for every piece
 #pragma unroll
             for (uint32_t p = 0; p < L::kV; p += NL * 256, piece += NL * 256, row += NL * (64 / kAt) * a.v_stride * 4)
                 dma4(v, values_at + row, 0, to + L::kKey + L::kValue + piece);  // past the rows, zeros
-            piece = (w - NC) * kTile;
+            piece = own * kTile;
             asm volatile("" : "+s"(piece));
 #pragma unroll
             for (uint32_t p = 0; p < L::kKey + L::kValue; p += NL * kTile, piece += NL * kTile) {
@@ -556,22 +554,39 @@ __global__ __launch_bounds__((NC + NL) * 64, KB == 8 ? 1 : 2) void linear_scan_k
                     dma16(values, l * 16, piece - L::kKey, to + piece);
                 }
             }
+            // With two stages the others are a chunk behind.
+            if (SPLIT > 1 && L::kStages == 2 && c > c0) {
+                lds_barrier();
+                if (is_wild(c - 1) | some_odd()) {
+                    lds_barrier();
+                    lds_barrier();
+                }
+            }
             wait_dma<0>();
             lds_barrier();
+            if (SPLIT > 1 && (L::kStages == 1 || c + 1 == c1)) {
+                lds_barrier();
+                if (is_wild(c) | some_odd()) {
+                    lds_barrier();
+                    lds_barrier();
+                }
+            }
         }
+        if (SPLIT > 1) lds_barrier();
         return;
     }
 
     const bool starts = c0 == begin, ends = c1 == end;
     bool read;
     const uint32_t slot = seq::slot_of(a.seq, s, read);
-    const uint32_t tile = in_unit % pass.columns * NC + w, col = tile * 16 + l % 16, state_bytes = a.dk * a.dv * 4;
-    const bool has = col < a.dv;
+    const uint32_t in_group = w / SPLIT, split = w % SPLIT, partner = w ^ (SPLIT - 1);
+    const uint32_t tile = in_unit % pass.columns * NC + in_group, col = tile * 16 + m, state_bytes = a.dk * a.dv * 4;
+    const bool has = col < a.dv, idle = tile * 16 >= a.dv;
     float *pool = a.state + (size_t(slot == seq::kNoSlot ? 0 : slot) * a.v_heads + h) * a.dk * a.dv;
     const float *from = starts ? pool : pass.from + size_t(h) * a.dk * a.dv;
     // Of a buffer's rows these lanes have 4g + i of every 16; what is past the
     // head's dimensions or the sequence's tokens is past the buffer.
-    uint32_t state_at = has ? (4 * g * a.dv + col) * 4 : kOut;
+    uint32_t state_at = has ? ((split * 16 * TD + 4 * g) * a.dv + col) * 4 : kOut;
     const uint32_t out_at = has ? (4 * g * a.out_stride + col) * 4 : kOut;
     f4 S[TD];
     {
@@ -583,7 +598,9 @@ __global__ __launch_bounds__((NC + NL) * 64, KB == 8 ? 1 : 2) void linear_scan_k
                 S[t][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, int(state_at + (16 * t + i) * a.dv * 4), 0, 0));
     }
     float minus = -1.f;
-    asm volatile("" : "+s"(minus));
+    asm volatile("" : "+v"(minus));
+    unsigned char *told = shared + w * L::kTold;
+    const unsigned char *heard = shared + partner * L::kTold;
 
     // S is kept by 2^scale, a column's own.
     int scale = 0;
@@ -603,194 +620,313 @@ __global__ __launch_bounds__((NC + NL) * 64, KB == 8 ? 1 : 2) void linear_scan_k
         scale = to;
     };
     auto fitting = [](float top) { return max(-113, min(15 - exponent(top), 110)); };
-    rescale(fitting(biggest()));
+    {
+        float top = biggest();
+        if constexpr (SPLIT > 1) {
+            *reinterpret_cast<float *>(told + L::kX + L::kO + l * 4) = top;
+            lds_barrier();
+            top = fmaxf(top, *reinterpret_cast<const float *>(heard + L::kX + L::kO + l * 4));
+        }
+        rescale(fitting(top));
+    }
 
-    // Two loops, so that a chunk that is done token after token costs the others
-    // no register moves where the paths would meet.
-    uint32_t c = c0;
-    const bool idle = tile * 16 >= a.dv;
-    auto enter = [&] {  // the chunk's operands are there
+    // Outputs of the chunk before that wait for the other part's sum over S.
+    float waits[4], of_heard[4];
+    auto rows_of = [&](uint32_t c) {
+        const uint32_t t0 = (c - begin) * kChunk, n = min(kChunk, count - t0);
+        return buffer_of(a.out + (size_t(first) + t0) * a.out_stride + size_t(h) * a.dv, ((n - 1) * a.out_stride + a.dv) * 4);
+    };
+    auto finish = [&](uint32_t c) {
+        const f4 o = *reinterpret_cast<const f4 *>(heard + L::kX + l * 16);
+        const auto rows = rows_of(c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(fmaf(of_heard[i], o[i], waits[i])), rows,
+                                                  int(out_at + (16 * split + i) * a.out_stride * 4), 0, 0);
+    };
+    auto enter = [&](uint32_t c) {  // the chunk's operands are there
         if (L::kStages == 1 && c > c0) lds_barrier();
         lds_barrier();
     };
-    if (idle) {
-        for (; c < c1; ++c) enter();
+    // Token after token: one wave of a tile has the whole state, which comes to
+    // it by way of the chunk's own place in LDS.
+    auto tokens = [&](uint32_t c) {
+        const uint32_t t0 = (c - begin) * kChunk, n = min(kChunk, count - t0);
+        rescale(0);
+        if constexpr (SPLIT == 1) {
+            tokens_of_chunk<TD>(a, size_t(first) + t0, n, h, col, S);
+            rescale(fitting(biggest()));
+        } else {
+            f4 *room = reinterpret_cast<f4 *>(lds + stage_of(c)) + in_group * (TD * 64) + l;
+            if (split == 1) {
+#pragma unroll
+                for (int t = 0; t < TD; ++t) room[t * 64] = S[t];
+            }
+            lds_barrier();
+            if (split == 0 && !idle) {
+                f4 all[SPLIT * TD];
+#pragma unroll
+                for (int t = 0; t < TD; ++t) {
+                    all[t] = S[t];
+                    all[TD + t] = room[t * 64];
+                }
+                tokens_of_chunk<SPLIT * TD>(a, size_t(first) + t0, n, h, col, all);
+                float top = 0.f;
+#pragma unroll
+                for (int t = 0; t < SPLIT * TD; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(all[t][i]));
+                *reinterpret_cast<float *>(told + L::kX + L::kO + l * 4) = column_max(top);
+#pragma unroll
+                for (int t = 0; t < TD; ++t) {
+                    S[t] = all[t];
+                    room[t * 64] = all[TD + t];
+                }
+            }
+            lds_barrier();
+            if (split == 1) {
+#pragma unroll
+                for (int t = 0; t < TD; ++t) S[t] = room[t * 64];
+            }
+            rescale(fitting(*reinterpret_cast<const float *>(split == 0 ? told + L::kX + L::kO + l * 4 : heard + L::kX + L::kO + l * 4)));
+        }
+    };
+
+    uint32_t c = c0;
+    if (SPLIT == 1 && idle) {
+        for (; c < c1; ++c) enter(c);
     }
+    bool pending = false;
+    // Two loops, so that a chunk that is done token after token costs the others
+    // no register moves where the paths would meet.
     while (c < c1) {
         bool slow = false;
         do {
-        enter();
-        const unsigned char *keys = lds + stage_of(c), *values = keys + L::kKey;
-        const float *scalars = reinterpret_cast<const float *>(values + kScalars);
-        const uint32_t t0 = (c - begin) * kChunk, n = min(kChunk, count - t0);
-        // LDS answers late: operands are asked for well before the matrix
-        // instructions that take them, into registers that the last ones left.
-        struct Terms {
-            u4 hi, lo;
-        };
-        auto at = [&](const unsigned char *p) {
-            return Terms{*reinterpret_cast<const u4 *>(p + l * 16), *reinterpret_cast<const u4 *>(p + kTile + l * 16)};
-        };
-        // A sum waits for the matrix instruction before it some time longer than
-        // that one keeps the others: as many sums as there are go on in turn.
-        auto step = [&](int which, const Terms &m, u4 hi, u4 lo, f4 &c) {
-            c = mfma(which == 0 ? m.lo : m.hi, which == 1 ? lo : hi, c);
-        };
-        auto of_rows = [&](uint32_t which, int half) { return *reinterpret_cast<const f4 *>(scalars + which + 16 * half + 4 * g); };
-        const float whole = scalars[kWhole], most = scalars[kMost];
-        const uint32_t wild = reinterpret_cast<const uint32_t *>(scalars)[kWild];
-        float v[8];  // tokens 16h + 4g + i at 4h + i
+            enter(c);
+            if constexpr (SPLIT > 1)
+                if (pending) finish(c - 1);
+            pending = false;
+            const unsigned char *keys = lds + stage_of(c), *values = keys + L::kKey;
+            const float *scalars = reinterpret_cast<const float *>(values + kScalars);
+            // LDS answers late: operands are asked for well before the matrix
+            // instructions that take them, into registers that the last ones left.
+            struct Terms {
+                u4 hi, lo;
+            };
+            auto at = [&](const unsigned char *p) {
+                return Terms{*reinterpret_cast<const u4 *>(p + l * 16), *reinterpret_cast<const u4 *>(p + kTile + l * 16)};
+            };
+            // A tile of K^T: rows of four dims of four tokens, read across.
+            auto across = [&](int t, int term) {
+                u4 r;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            v[e] = reinterpret_cast<const float *>(values + L::kValue)[(16 * (e / 4) + 4 * g + e % 4) * (NC * 16) + w * 16 + l % 16];
-        f4 beta[2], of_x[2], of_q[2], of_m[2], of_u[2];
-        Terms tk[2][KB], tq[2][KB], tt[2], tm[2], tu[TD];
+                for (int half = 0; half < 2; ++half) {
+                    typedef short s4 __attribute__((ext_vector_type(4)));
+                    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+                    const unsigned char *p = keys + L::kTerms + ((half * KB + split * KW + t / 2) * 2 + term) * kTile +
+                                             (m % 4 * 16 + 4 * g + m / 4) * 16 + t % 2 * 8;
+                    const u2 x = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)p));
+                    r[2 * half] = x[0];
+                    r[2 * half + 1] = x[1];
+                }
+                return r;
+            };
+            // A sum waits for the matrix instruction before it some time longer than
+            // that one keeps the others: as many sums as there are go on in turn.
+            auto step = [&](int which, const Terms &x, u4 hi, u4 lo, f4 &c) {
+                c = mfma(which == 0 ? x.lo : x.hi, which == 1 ? lo : hi, c);
+            };
+            auto of_rows = [&](uint32_t which, int half) { return *reinterpret_cast<const f4 *>(scalars + which + 16 * half + 4 * g); };
+            const float whole = scalars[kWhole], most = scalars[kMost];
+            const uint32_t wild = is_wild(c);
+            float v[8];  // tokens 16h + 4g + i at 4h + i
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            beta[half] = of_rows(kBeta, half);
+            for (int e = 0; e < 8; ++e)
+                v[e] = reinterpret_cast<const float *>(values + L::kValue)[(16 * (e / 4) + 4 * g + e % 4) * (NC * 16) + in_group * 16 + m];
+            f4 beta[2], of_x[2], of_u[2];
+            Terms tk[2][KW], tq[2][KW], tt[2], tu[TD];
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-                if constexpr (DELTA) tk[half][kb] = at(keys + 8 * kTile * KB + (half * KB + kb) * 2 * kTile);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        u4 sh[KB], sl[KB];
+            for (int half = 0; half < 2; ++half) {
+                beta[half] = of_rows(kBeta, half);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            float both[8];
+                for (int kb = 0; kb < KW; ++kb)
+                    if constexpr (DELTA) tk[half][kb] = at(keys + L::kTerms + (half * KB + split * KW + kb) * 2 * kTile);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            u4 sh[KW], sl[KW];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) both[e] = S[2 * kb + e / 4][e % 4];
-            terms(both, minus, sh[kb], sl[kb]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        // S^T k; meanwhile R's part that does not wait for it, all by 2^scale.
-        f4 x2[2][2] = {}, o2[2][2] = {}, x[2], o[2];  // blocks 0, 2, .. and 1, 3, ..
+            for (int kb = 0; kb < KW; ++kb) {
+                float both[8];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            of_x[half] = of_rows(kX, half);
-            if constexpr (DELTA) tt[half] = at(values + kScalars + kTile + half * 2 * kTile);
-        }
+                for (int e = 0; e < 8; ++e) both[e] = S[2 * kb + e / 4][e % 4];
+                terms(both, minus, sh[kb], sl[kb]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // S^T k; meanwhile R's part that does not wait for it, all by 2^scale.
+            constexpr int PAR = KW > 1 ? 2 : 1;  // sums of blocks 0, 2, .. and 1, 3, ..
+            f4 x2[2][PAR] = {}, o2[2][PAR] = {}, x[2], o[2];
 #pragma unroll
-        for (int kb = 0; kb < KB; kb += 2) {
-            if constexpr (DELTA) {
-#pragma unroll
-                for (int m = 0; m < 12; ++m)
-                    step(m / 4, tk[m % 2][kb + m / 2 % 2], sh[kb + m / 2 % 2], sl[kb + m / 2 % 2], x2[m % 2][m / 2 % 2]);
+            for (int half = 0; half < 2; ++half) {
+                of_x[half] = of_rows(kX, half);
+                if constexpr (DELTA) tt[half] = at(values + kScalars + kTile + half * 2 * kTile);
             }
 #pragma unroll
-            for (int m = 0; m < 4; ++m) tq[m % 2][kb + m / 2] = at(keys + (m % 2 * KB + kb + m / 2) * 2 * kTile);
-        }
-        float r[8];
-        {
-            const float by = ldexpf(1.f, scale);
+            for (int kb = 0; kb < KW; kb += PAR) {
+                if constexpr (DELTA) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) r[e] = v[e] * (DELTA ? beta[e / 4][e % 4] * by : by);
-        }
-        float odd = 0.f;
+                    for (int i = 0; i < 6 * PAR; ++i)
+                        step(i / (2 * PAR), tk[i % 2][kb + i / 2 % PAR], sh[kb + i / 2 % PAR], sl[kb + i / 2 % PAR], x2[i % 2][i / 2 % PAR]);
+                }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) odd = fmaf(v[e], 0.f, odd);
-        const float top = biggest();
-        if constexpr (DELTA) in_turn<6 * KB, 2, 1>();
-        __builtin_amdgcn_sched_barrier(0);
-        slow = __builtin_amdgcn_readfirstlane(wild) != 0 || __ballot(odd != 0.f) != 0;
-        if (slow) break;
-        // S^T q; meanwhile R and its terms, by 2^up more; the next state's scale:
-        // below 2^15 whatever the chunk adds.
+                for (int i = 0; i < 2 * PAR; ++i) tq[i % 2][kb + i / 2] = at(keys + (i % 2 * KB + split * KW + kb + i / 2) * 2 * kTile);
+            }
+            float r[8];
+            {
+                const float by = ldexpf(1.f, scale);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            tm[half] = at(values + half * 2 * kTile);
-            of_u[half] = of_rows(kU, half);
-            of_q[half] = of_rows(kQ, half);
-            of_m[half] = of_rows(kM, half);
-        }
+                for (int e = 0; e < 8; ++e) r[e] = v[e] * (DELTA ? beta[e / 4][e % 4] * by : by);
+            }
+            float odd = 0.f;
 #pragma unroll
-        for (int kb = 0; kb < KB; kb += 2) {
+            for (int e = 0; e < 8; ++e) odd = fmaf(v[e], 0.f, odd);
+            float top = biggest();
+            if constexpr (DELTA) in_turn<6 * KW, 2, 1>();
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int m = 0; m < 12; ++m)
-                step(m / 4, tq[m % 2][kb + m / 2 % 2], sh[kb + m / 2 % 2], sl[kb + m / 2 % 2], o2[m % 2][m / 2 % 2]);
+            for (int half = 0; half < 2; ++half) x[half] = PAR > 1 ? x2[half][0] + x2[half][PAR - 1] : x2[half][0];
+            const bool is_odd = !idle && __ballot(odd != 0.f) != 0;
+            if constexpr (SPLIT == 1) {
+                slow = __builtin_amdgcn_readfirstlane(wild) != 0 || is_odd;
+            } else {
+                // Both parts' sums.
+                if constexpr (DELTA) {
+                    *reinterpret_cast<f4 *>(told + l * 16) = x[0];
+                    *reinterpret_cast<f4 *>(told + kTile + l * 16) = x[1];
+                }
+                *reinterpret_cast<float *>(told + L::kX + L::kO + l * 4) = top;
+                if (l == 0) odd_waves[w] = is_odd;
+                lds_barrier();
+                if constexpr (DELTA) {
+                    x[0] += *reinterpret_cast<const f4 *>(heard + l * 16);
+                    x[1] += *reinterpret_cast<const f4 *>(heard + kTile + l * 16);
+                }
+                top = fmaxf(top, *reinterpret_cast<const float *>(heard + L::kX + L::kO + l * 4));
+                slow = __builtin_amdgcn_readfirstlane(wild | some_odd()) != 0;
+            }
+            if (slow) break;
+            // S^T q; meanwhile R and its terms, by 2^up more; the next state's scale:
+            // below 2^15 whatever the chunk adds.
 #pragma unroll
-            for (int t = 2 * kb; t < 2 * kb + 4; ++t) tu[t] = at(keys + 4 * kTile * KB + t * 2 * kTile);
-        }
+            for (int half = 0; half < 2; ++half) of_u[half] = of_rows(kU, half);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            x[half] = x2[half][0] + x2[half][1];
-            o[half] = o2[half][0] + o2[half][1];
-        }
-        if constexpr (DELTA) {
+            for (int kb = 0; kb < KW; kb += PAR) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) r[e] = fmaf(-of_x[e / 4][e % 4], x[e / 4][e % 4], r[e]);
-        }
-        float r_top = 0.f;
+                for (int i = 0; i < 6 * PAR; ++i)
+                    step(i / (2 * PAR), tq[i % 2][kb + i / 2 % PAR], sh[kb + i / 2 % PAR], sl[kb + i / 2 % PAR], o2[i % 2][i / 2 % PAR]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r_top = fmaxf(r_top, fabsf(r[e]));
-        r_top = column_max(r_top);
-        const int up = max(-113, min((DELTA ? 5 : 13) - exponent(r_top), 110));
-        int to = min(scale + 15 - exponent(fmaf(most, r_top, whole * top)), scale + 100);
-        to = max(-113, min(to, 110));
-        u4 uh, ul;
-        {
-            const float by = ldexpf(1.f, up);
+                for (int t = 2 * kb; t < 2 * kb + 2 * PAR; ++t) tu[t] = Terms{across(t, 0), across(t, 1)};
+            }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) r[e] *= by;
-        }
-        terms(r, minus, uh, ul);
-        in_turn<6 * KB, 3, 1>();
-        __builtin_amdgcn_sched_barrier(0);
-        // U, by 2^(scale + up + kSolve): below 2^15 while rows of T add up to 2^6.
-        float u[8];
-        if constexpr (DELTA) {
-            f4 y[2] = {};
+            for (int half = 0; half < 2; ++half) o[half] = PAR > 1 ? o2[half][0] + o2[half][PAR - 1] : o2[half][0];
+            if constexpr (DELTA) {
 #pragma unroll
-            for (int m = 0; m < 6; ++m) step(m / 2, tt[m % 2], uh, ul, y[m % 2]);
+                for (int e = 0; e < 8; ++e) r[e] = fmaf(-of_x[e / 4][e % 4], x[e / 4][e % 4], r[e]);
+            }
+            float r_top = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) u[e] = y[e / 4][e % 4];
-        } else {
+            for (int e = 0; e < 8; ++e) r_top = fmaxf(r_top, fabsf(r[e]));
+            r_top = column_max(r_top);
+            const int up = max(-113, min((DELTA ? 5 : 13) - exponent(r_top), 110));
+            int to = min(scale + 15 - exponent(fmaf(most, r_top, whole * top)), scale + 100);
+            to = max(-113, min(to, 110));
+            u4 uh, ul;
+            {
+                const float by = ldexpf(1.f, up);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) u[e] = r[e];
-        }
-        {
-            const float keep = ldexpf(whole, to - scale);
+                for (int e = 0; e < 8; ++e) r[e] *= by;
+            }
+            terms(r, minus, uh, ul);
+            in_turn<6 * KW, 3, 1>();
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (SPLIT > 1) *reinterpret_cast<f4 *>(told + L::kX + l * 16) = split ? o[0] : o[1];  // the other's tokens
+            // U, by 2^(scale + up + kSolve): below 2^15 while rows of T add up to 2^6.
+            float u[8];
+            if constexpr (DELTA) {
+                f4 y[2] = {};
 #pragma unroll
-            for (int t = 0; t < TD; ++t)
+                for (int i = 0; i < 6; ++i) step(i / 2, tt[i % 2], uh, ul, y[i % 2]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) S[t][i] *= keep;
-            const float by = ldexpf(1.f, to - scale - up - (DELTA ? kSolve : 0));
-            of_u[0] *= by;
-            of_u[1] *= by;
-        }
-        if constexpr (DELTA) in_turn<6, 6, 0>();
-        __builtin_amdgcn_sched_barrier(0);
-        u4 wh, wl;
-        {
-            float left[8];
+                for (int e = 0; e < 8; ++e) u[e] = y[e / 4][e % 4];
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) left[e] = u[e] * of_u[e / 4][e % 4];
-            terms(left, minus, wh, wl);
-            if constexpr (DELTA) terms(u, minus, uh, ul);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        // The next state, M U and the outputs.
+                for (int e = 0; e < 8; ++e) u[e] = r[e];
+            }
+            // M's rows of this wave's tokens: a half of them where two share a tile.
+            constexpr int HALVES = SPLIT > 1 ? 1 : 2;
+            Terms tm[HALVES];
+            f4 of_q[HALVES], of_m[HALVES];
 #pragma unroll
-        for (int m = 0; m < 3 * TD; ++m) step(m / TD, tu[m % TD], wh, wl, S[m % TD]);
-        f4 y[2] = {};
+            for (int half = 0; half < HALVES; ++half) {
+                const int which = SPLIT > 1 ? int(split) : half;
+                tm[half] = at(values + which * 2 * kTile);
+                of_q[half] = of_rows(kQ, which);
+                of_m[half] = of_rows(kM, which);
+            }
+            {
+                const float keep = ldexpf(whole, to - scale);
 #pragma unroll
-        for (int m = 0; m < 6; ++m) step(m / 2, tm[m % 2], uh, ul, y[m % 2]);
-        const auto rows = buffer_of(a.out + (size_t(first) + t0) * a.out_stride + size_t(h) * a.dv, ((n - 1) * a.out_stride + a.dv) * 4);
-        const float one = ldexpf(1.f, -scale), of_y = ldexpf(1.f, (DELTA ? -kSolve : 0) - up - scale);
+                for (int t = 0; t < TD; ++t)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float out = of_q[e / 4][e % 4] * (o[e / 4][e % 4] * one) + of_m[e / 4][e % 4] * (y[e / 4][e % 4] * of_y);
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(out), rows, int(out_at + (16 * (e / 4) + e % 4) * a.out_stride * 4), 0, 0);
-        }
-        scale = to;
+                    for (int i = 0; i < 4; ++i) S[t][i] *= keep;
+                const float by = ldexpf(1.f, to - scale - up - (DELTA ? kSolve : 0));
+                of_u[0] *= by;
+                of_u[1] *= by;
+            }
+            if constexpr (DELTA) in_turn<6, 6, 1>();
+            __builtin_amdgcn_sched_barrier(0);
+            u4 wh, wl;
+            {
+                float left[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) left[e] = u[e] * of_u[e / 4][e % 4];
+                terms(left, minus, wh, wl);
+                if constexpr (DELTA) terms(u, minus, uh, ul);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // The next state, M U and the outputs.
+            f4 y[HALVES] = {};
+#pragma unroll
+            for (int i = 0; i < 3 * HALVES; ++i) step(i / HALVES, tm[i % HALVES], uh, ul, y[i % HALVES]);
+#pragma unroll
+            for (int i = 0; i < 3 * TD; ++i) step(i / TD, tu[i % TD], wh, wl, S[i % TD]);
+            const float one = ldexpf(1.f, -scale), of_y = ldexpf(1.f, (DELTA ? -kSolve : 0) - up - scale);
+            if constexpr (SPLIT == 1) {
+                const auto rows = rows_of(c);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float out = of_q[e / 4][e % 4] * (o[e / 4][e % 4] * one) + of_m[e / 4][e % 4] * (y[e / 4][e % 4] * of_y);
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(out), rows,
+                                                          int(out_at + (16 * (e / 4) + e % 4) * a.out_stride * 4), 0, 0);
+                }
+            } else {
+                const f4 own = split ? o[1] : o[0];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    of_heard[i] = of_q[0][i] * one;
+                    waits[i] = of_heard[i] * own[i] + of_m[0][i] * (y[0][i] * of_y);
+                }
+                pending = true;
+            }
+            scale = to;
         } while (++c < c1);
         if (!slow) break;
-        rescale(0);
-        const uint32_t t0 = (c - begin) * kChunk;
-        tokens_of_chunk<TD>(a, size_t(first) + t0, min(kChunk, count - t0), h, col, S);
-        rescale(fitting(biggest()));
-        ++c;
+        tokens(c++);
     }
-    if (tile * 16 >= a.dv || (ends ? !a.keep || slot == seq::kNoSlot : pass.to == nullptr)) return;
+    if constexpr (SPLIT > 1) {
+        lds_barrier();
+        if (pending) finish(c1 - 1);
+    }
+    if (idle || (ends ? !a.keep || slot == seq::kNoSlot : pass.to == nullptr)) return;
     rescale(0);
     const auto r = buffer_of(ends ? pool : pass.to + size_t(h) * a.dk * a.dv, state_bytes);
     asm volatile("" : "+v"(state_at));  // or all of the addresses wait in registers for this
@@ -841,14 +977,14 @@ hipError_t go_prepare(const LinearArgs &a, const Pass &pass, hipStream_t stream)
     return hipGetLastError();
 }
 
-template <int KB, int NC, int NL, bool DELTA>
+template <int KB, int NC, int SPLIT, int NL, bool DELTA>
 hipError_t go_scan(const LinearArgs &a, const Pass &pass, hipStream_t stream) {
-    const auto kernel = linear_scan_kernel<KB, NC, NL, DELTA>;
-    constexpr uint32_t lds = ScanLds<KB, NC, DELTA>::kBytes;
-    const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
+    const auto kernel = linear_scan_kernel<KB, NC, SPLIT, NL, DELTA>;
+    using L = Scan<KB, NC, SPLIT, NL, DELTA>;
+    const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), L::kBytes);
     if (e != hipSuccess) return e;
     const uint32_t units = (a.seq.seqs * a.k_heads + 7) / 8 * 8;
-    kernel<<<units * (a.v_heads / a.k_heads) * pass.columns, (NC + NL) * 64, lds, stream>>>(a, pass);
+    kernel<<<units * (a.v_heads / a.k_heads) * pass.columns, L::kThreads, L::kBytes, stream>>>(a, pass);
     return hipGetLastError();
 }
 
@@ -856,9 +992,10 @@ template <int KB, bool DELTA>
 hipError_t go_pass(const LinearArgs &a, const LinearPlan &pl, const Pass &pass, hipStream_t stream) {
     const hipError_t e = go_prepare<KB, DELTA>(a, pass, stream);
     if (e != hipSuccess) return e;
-    switch (pl.columns) {
-        case 2: return go_scan<KB, 2, 4, DELTA>(a, pass, stream);
-        default: return go_scan<KB, 4, 4, DELTA>(a, pass, stream);
+    if constexpr (KB == 8) {
+        return go_scan<KB, 2, 1, 2, DELTA>(a, pass, stream);  // two states' worth of registers a wave
+    } else {
+        return pl.columns == 2 ? go_scan<KB, 2, 2, 4, DELTA>(a, pass, stream) : go_scan<KB, 4, 1, 4, DELTA>(a, pass, stream);
     }
 }
 
@@ -873,11 +1010,11 @@ LinearPlan plan_linear(const LinearArgs &a, const DeviceLimits &lim, size_t limi
     if (a.v_stride > 1u << 22 || a.out_stride > 1u << 22) return pl;
     const uint32_t tiles = (a.dv + 15) / 16;
     pl.blocks = a.dk <= 64 ? 2 : a.dk <= 128 ? 4 : 8;
-    pl.columns = columns ? columns : 2;
+    pl.columns = columns && pl.blocks < 8 ? columns : 2;
     pl.parts = uint32_t(std::min<uint64_t>(q.tokens, uint64_t(q.tokens) / kChunk + q.seqs));
-    pl.k_bytes = size_t(a.delta ? 12 : 8) * kTile * pl.blocks;
+    pl.k_bytes = size_t(8) * kTile * pl.blocks;
     pl.v_bytes = size_t(a.delta ? 9 : 5) * kTile;
-    if (columns == 0)
+    if (columns == 0 && pl.blocks < 8)
         while (pl.columns < 4 && uint64_t(std::min(q.seqs, pl.parts)) * a.v_heads * ((tiles + pl.columns - 1) / pl.columns) >
                                      2 * uint64_t(lim.num_cus))
             pl.columns *= 2;
