@@ -473,28 +473,23 @@ __device__ __forceinline__ void tokens_of_chunk(const LinearArgs &a, size_t toke
     }
 }
 
-// How a workgroup's waves share the work: NC 16-column tiles, of each SPLIT parts
-// of the key dimension, a wave each, and NL waves that load.
-template <int KB, int NC, int SPLIT, int NL, bool DELTA>
+// How a workgroup's waves share the work: NC have a 16-column tile each, NL load.
+template <int KB, int NC, int NL, bool DELTA>
 struct Scan {
-    static constexpr int kWorkers = NC * SPLIT, kThreads = (kWorkers + NL) * 64;
+    static constexpr int kThreads = (NC + NL) * 64;
     static constexpr uint32_t kTerms = 4 * kTile * KB;  // of Q, or of K
     static constexpr uint32_t kKey = 2 * kTerms, kValue = (DELTA ? 9 : 5) * kTile;
     static constexpr uint32_t kV = kChunk * NC * 16 * 4;  // the workgroup's columns of the values
     static constexpr uint32_t kStage = kKey + kValue + kV;
-    // What the waves of a tile tell each other: sums over their parts.
-    static constexpr uint32_t kX = 2 * kTile, kO = kTile, kTop = 256, kTold = kX + kO + kTop;
-    static constexpr uint32_t kShared = SPLIT > 1 ? kWorkers * kTold + kWorkers * 4 : 0;
-    static constexpr uint32_t kStages = 2 * kStage + kShared <= 160 * 1024 ? 2 : 1;
-    static constexpr uint32_t kBytes = kStages * kStage + kShared;
+    static constexpr uint32_t kBytes = 2 * kStage;
+    static_assert(kBytes <= 160 * 1024, "two stages fit LDS");
 };
 
-template <int KB, int NC, int SPLIT, int NL, bool DELTA>
-__global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1) void linear_scan_kernel(LinearArgs a, Pass pass) {
+template <int KB, int NC, int NL, bool DELTA>
+__global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_kernel(LinearArgs a, Pass pass) {
     extern __shared__ __align__(16) unsigned char lds[];
-    using L = Scan<KB, NC, SPLIT, NL, DELTA>;
-    constexpr int KW = KB / SPLIT, TD = 2 * KW;  // a wave's blocks and tiles of the key dimension
-    constexpr int kWorkers = L::kWorkers;
+    using L = Scan<KB, NC, NL, DELTA>;
+    constexpr int TD = 2 * KB;
     const uint32_t l = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), g = l / 16, m = l % 16;
 
     // Workgroups go to the eight dies in turn: all those of a key head to one,
@@ -512,33 +507,18 @@ __global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1
     if (c0 >= c1) return;
 
     const uint32_t lds0 = uint32_t(uintptr_t((__attribute__((address_space(3))) unsigned char *)lds));
-    auto stage_of = [&](uint32_t c) { return L::kStages == 2 ? (c - c0) % 2 * L::kStage : 0; };
-    // Whether a chunk is done token after token: the operands say so, or, where
-    // waves share a tile, one of them does (all then, as they meet at barriers).
-    unsigned char *shared = lds + L::kStages * L::kStage;
-    uint32_t *odd_waves = reinterpret_cast<uint32_t *>(shared + kWorkers * L::kTold);
-    auto is_wild = [&](uint32_t c) {
-        return reinterpret_cast<const uint32_t *>(lds + stage_of(c) + L::kKey + kScalars)[kWild];
-    };
-    auto some_odd = [&] {
-        uint32_t some = 0;
-#pragma unroll
-        for (int k = 0; k < kWorkers; ++k) some |= odd_waves[k];
-        return some;
-    };
-    if (w >= kWorkers) {
-        // A chunk ahead of the others: every first barrier says that a chunk is
-        // there and that the one before is no longer read.
+    auto stage_of = [&](uint32_t c) { return (c - c0) % 2 * L::kStage; };
+    if (w >= NC) {
+        // A chunk ahead of the others: every barrier says that a chunk is there
+        // and that the one before is no longer read.
         constexpr uint32_t kAt = NC * 16;  // columns of the workgroup
         const uint32_t col0 = in_unit % pass.columns * kAt + l % kAt;
         const uint32_t values_at = col0 < a.dv ? (l / kAt * a.v_stride + col0) * 4 : kOut;
-        const uint32_t own = w - kWorkers;
-        if (SPLIT > 1) lds_barrier();
+        const uint32_t own = w - NC;
         for (uint32_t c = c0; c < c1; ++c) {
             const uint32_t to = lds0 + stage_of(c), t0 = (c - begin) * kChunk, n = min(kChunk, count - t0);
             const u4 keys = rsrc_of(pass.of_key(a, c, kh), L::kKey), values = rsrc_of(pass.of_value(a, c, h), L::kValue);
             const u4 v = rsrc_of(a.v + (size_t(first) + t0) * a.v_stride + size_t(h) * a.dv, ((n - 1) * a.v_stride + a.dv) * 4);
-            if (L::kStages == 1 && c > c0) lds_barrier();
             uint32_t piece = own * 256, row = own * (64 / kAt) * a.v_stride * 4;
             asm volatile("" : "+s"(piece), "+s"(row));  // counted here, not kept in registers for every piece
 #pragma unroll
@@ -554,39 +534,22 @@ __global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1
                     dma16(values, l * 16, piece - L::kKey, to + piece);
                 }
             }
-            // With two stages the others are a chunk behind.
-            if (SPLIT > 1 && L::kStages == 2 && c > c0) {
-                lds_barrier();
-                if (is_wild(c - 1) | some_odd()) {
-                    lds_barrier();
-                    lds_barrier();
-                }
-            }
             wait_dma<0>();
             lds_barrier();
-            if (SPLIT > 1 && (L::kStages == 1 || c + 1 == c1)) {
-                lds_barrier();
-                if (is_wild(c) | some_odd()) {
-                    lds_barrier();
-                    lds_barrier();
-                }
-            }
         }
-        if (SPLIT > 1) lds_barrier();
         return;
     }
 
     const bool starts = c0 == begin, ends = c1 == end;
     bool read;
     const uint32_t slot = seq::slot_of(a.seq, s, read);
-    const uint32_t in_group = w / SPLIT, split = w % SPLIT, partner = w ^ (SPLIT - 1);
-    const uint32_t tile = in_unit % pass.columns * NC + in_group, col = tile * 16 + m, state_bytes = a.dk * a.dv * 4;
+    const uint32_t tile = in_unit % pass.columns * NC + w, col = tile * 16 + m, state_bytes = a.dk * a.dv * 4;
     const bool has = col < a.dv, idle = tile * 16 >= a.dv;
     float *pool = a.state + (size_t(slot == seq::kNoSlot ? 0 : slot) * a.v_heads + h) * a.dk * a.dv;
     const float *from = starts ? pool : pass.from + size_t(h) * a.dk * a.dv;
     // Of a buffer's rows these lanes have 4g + i of every 16; what is past the
     // head's dimensions or the sequence's tokens is past the buffer.
-    uint32_t state_at = has ? ((split * 16 * TD + 4 * g) * a.dv + col) * 4 : kOut;
+    uint32_t state_at = has ? (4 * g * a.dv + col) * 4 : kOut;
     const uint32_t out_at = has ? (4 * g * a.out_stride + col) * 4 : kOut;
     f4 S[TD];
     {
@@ -599,8 +562,6 @@ __global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1
     }
     float minus = -1.f;
     asm volatile("" : "+v"(minus));
-    unsigned char *told = shared + w * L::kTold;
-    const unsigned char *heard = shared + partner * L::kTold;
 
     // S is kept by 2^scale, a column's own.
     int scale = 0;
@@ -620,101 +581,32 @@ __global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1
         scale = to;
     };
     auto fitting = [](float top) { return max(-113, min(15 - exponent(top), 110)); };
-    {
-        float top = biggest();
-        if constexpr (SPLIT > 1) {
-            *reinterpret_cast<float *>(told + L::kX + L::kO + l * 4) = top;
-            lds_barrier();
-            top = fmaxf(top, *reinterpret_cast<const float *>(heard + L::kX + L::kO + l * 4));
-        }
-        rescale(fitting(top));
-    }
-
-    // Outputs of the chunk before that wait for the other part's sum over S.
-    float waits[4], of_heard[4];
-    auto rows_of = [&](uint32_t c) {
-        const uint32_t t0 = (c - begin) * kChunk, n = min(kChunk, count - t0);
-        return buffer_of(a.out + (size_t(first) + t0) * a.out_stride + size_t(h) * a.dv, ((n - 1) * a.out_stride + a.dv) * 4);
-    };
-    auto finish = [&](uint32_t c) {
-        const f4 o = *reinterpret_cast<const f4 *>(heard + L::kX + l * 16);
-        const auto rows = rows_of(c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(fmaf(of_heard[i], o[i], waits[i])), rows,
-                                                  int(out_at + (16 * split + i) * a.out_stride * 4), 0, 0);
-    };
-    auto enter = [&](uint32_t c) {  // the chunk's operands are there
-        if (L::kStages == 1 && c > c0) lds_barrier();
-        lds_barrier();
-    };
-    // Token after token: one wave of a tile has the whole state, which comes to
-    // it by way of the chunk's own place in LDS.
-    auto tokens = [&](uint32_t c) {
-        const uint32_t t0 = (c - begin) * kChunk, n = min(kChunk, count - t0);
-        rescale(0);
-        if constexpr (SPLIT == 1) {
-            tokens_of_chunk<TD>(a, size_t(first) + t0, n, h, col, S);
-            rescale(fitting(biggest()));
-        } else {
-            f4 *room = reinterpret_cast<f4 *>(lds + stage_of(c)) + in_group * (TD * 64) + l;
-            if (split == 1) {
-#pragma unroll
-                for (int t = 0; t < TD; ++t) room[t * 64] = S[t];
-            }
-            lds_barrier();
-            if (split == 0 && !idle) {
-                f4 all[SPLIT * TD];
-#pragma unroll
-                for (int t = 0; t < TD; ++t) {
-                    all[t] = S[t];
-                    all[TD + t] = room[t * 64];
-                }
-                tokens_of_chunk<SPLIT * TD>(a, size_t(first) + t0, n, h, col, all);
-                float top = 0.f;
-#pragma unroll
-                for (int t = 0; t < SPLIT * TD; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(all[t][i]));
-                *reinterpret_cast<float *>(told + L::kX + L::kO + l * 4) = column_max(top);
-#pragma unroll
-                for (int t = 0; t < TD; ++t) {
-                    S[t] = all[t];
-                    room[t * 64] = all[TD + t];
-                }
-            }
-            lds_barrier();
-            if (split == 1) {
-#pragma unroll
-                for (int t = 0; t < TD; ++t) S[t] = room[t * 64];
-            }
-            rescale(fitting(*reinterpret_cast<const float *>(split == 0 ? told + L::kX + L::kO + l * 4 : heard + L::kX + L::kO + l * 4)));
-        }
-    };
+    rescale(fitting(biggest()));
 
     uint32_t c = c0;
-    if (SPLIT == 1 && idle) {
-        for (; c < c1; ++c) enter(c);
+    if (idle) {
+        for (; c < c1; ++c) lds_barrier();
     }
-    bool pending = false;
     // Two loops, so that a chunk that is done token after token costs the others
     // no register moves where the paths would meet.
     while (c < c1) {
         bool slow = false;
         do {
-            enter(c);
-            if constexpr (SPLIT > 1)
-                if (pending) finish(c - 1);
-            pending = false;
-            const unsigned char *keys = lds + stage_of(c), *values = keys + L::kKey;
-            const float *scalars = reinterpret_cast<const float *>(values + kScalars);
+            lds_barrier();  // the chunk's operands are there
+            // This lane's places in the stage, each a register and constants from there.
+            const uint32_t stage = stage_of(c);
+            uint32_t own = stage + l * 16, rows_at = stage + L::kKey + kScalars + g * 16;
+            uint32_t across_at = stage + L::kTerms + (m % 4 * 16 + 4 * g + m / 4) * 16;
+            uint32_t v_at = stage + L::kKey + L::kValue + (4 * g * NC * 16 + w * 16 + m) * 4;
+            asm volatile("" : "+v"(own), "+v"(rows_at), "+v"(across_at), "+v"(v_at));
+            const float *scalars = reinterpret_cast<const float *>(lds + stage + L::kKey + kScalars);
             // LDS answers late: operands are asked for well before the matrix
             // instructions that take them, into registers that the last ones left.
             struct Terms {
                 u4 hi, lo;
             };
-            auto at = [&](const unsigned char *p) {
-                return Terms{*reinterpret_cast<const u4 *>(p + l * 16), *reinterpret_cast<const u4 *>(p + kTile + l * 16)};
+            auto at = [&](uint32_t p) {
+                return Terms{*reinterpret_cast<const u4 *>(lds + own + p), *reinterpret_cast<const u4 *>(lds + own + (p + kTile))};
             };
             // A tile of K^T: rows of four dims of four tokens, read across.
             auto across = [&](int t, int term) {
@@ -723,8 +615,7 @@ __global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1
                 for (int half = 0; half < 2; ++half) {
                     typedef short s4 __attribute__((ext_vector_type(4)));
                     typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-                    const unsigned char *p = keys + L::kTerms + ((half * KB + split * KW + t / 2) * 2 + term) * kTile +
-                                             (m % 4 * 16 + 4 * g + m / 4) * 16 + t % 2 * 8;
+                    const unsigned char *p = lds + across_at + (((half * KB + t / 2) * 2 + term) * kTile + t % 2 * 8);
                     const u2 x = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)p));
                     r[2 * half] = x[0];
                     r[2 * half + 1] = x[1];
@@ -736,26 +627,27 @@ __global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1
             auto step = [&](int which, const Terms &x, u4 hi, u4 lo, f4 &c) {
                 c = mfma(which == 0 ? x.lo : x.hi, which == 1 ? lo : hi, c);
             };
-            auto of_rows = [&](uint32_t which, int half) { return *reinterpret_cast<const f4 *>(scalars + which + 16 * half + 4 * g); };
+            auto of_rows = [&](uint32_t which, int half) { return *reinterpret_cast<const f4 *>(lds + rows_at + (which + 16 * half) * 4); };
             const float whole = scalars[kWhole], most = scalars[kMost];
-            const uint32_t wild = is_wild(c);
+            const uint32_t wild = reinterpret_cast<const uint32_t *>(scalars)[kWild];
+            const uint32_t t0 = (c - begin) * kChunk, n = min(kChunk, count - t0);
             float v[8];  // tokens 16h + 4g + i at 4h + i
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                v[e] = reinterpret_cast<const float *>(values + L::kValue)[(16 * (e / 4) + 4 * g + e % 4) * (NC * 16) + in_group * 16 + m];
+                v[e] = *reinterpret_cast<const float *>(lds + v_at + (16 * (e / 4) + e % 4) * (NC * 16) * 4);
             f4 beta[2], of_x[2], of_u[2];
-            Terms tk[2][KW], tq[2][KW], tt[2], tu[TD];
+            Terms tk[2][KB], tq[2][KB], tt[2], tu[TD];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 beta[half] = of_rows(kBeta, half);
 #pragma unroll
-                for (int kb = 0; kb < KW; ++kb)
-                    if constexpr (DELTA) tk[half][kb] = at(keys + L::kTerms + (half * KB + split * KW + kb) * 2 * kTile);
+                for (int kb = 0; kb < KB; ++kb)
+                    if constexpr (DELTA) tk[half][kb] = at(L::kTerms + (half * KB + kb) * 2 * kTile);
             }
             __builtin_amdgcn_sched_barrier(0);
-            u4 sh[KW], sl[KW];
+            u4 sh[KB], sl[KB];
 #pragma unroll
-            for (int kb = 0; kb < KW; ++kb) {
+            for (int kb = 0; kb < KB; ++kb) {
                 float both[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) both[e] = S[2 * kb + e / 4][e % 4];
@@ -763,22 +655,22 @@ __global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1
             }
             __builtin_amdgcn_sched_barrier(0);
             // S^T k; meanwhile R's part that does not wait for it, all by 2^scale.
-            constexpr int PAR = KW > 1 ? 2 : 1;  // sums of blocks 0, 2, .. and 1, 3, ..
+            constexpr int PAR = KB > 1 ? 2 : 1;  // sums of blocks 0, 2, .. and 1, 3, ..
             f4 x2[2][PAR] = {}, o2[2][PAR] = {}, x[2], o[2];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 of_x[half] = of_rows(kX, half);
-                if constexpr (DELTA) tt[half] = at(values + kScalars + kTile + half * 2 * kTile);
+                if constexpr (DELTA) tt[half] = at(L::kKey + kScalars + kTile + half * 2 * kTile);
             }
 #pragma unroll
-            for (int kb = 0; kb < KW; kb += PAR) {
+            for (int kb = 0; kb < KB; kb += PAR) {
                 if constexpr (DELTA) {
 #pragma unroll
                     for (int i = 0; i < 6 * PAR; ++i)
                         step(i / (2 * PAR), tk[i % 2][kb + i / 2 % PAR], sh[kb + i / 2 % PAR], sl[kb + i / 2 % PAR], x2[i % 2][i / 2 % PAR]);
                 }
 #pragma unroll
-                for (int i = 0; i < 2 * PAR; ++i) tq[i % 2][kb + i / 2] = at(keys + (i % 2 * KB + split * KW + kb + i / 2) * 2 * kTile);
+                for (int i = 0; i < 2 * PAR; ++i) tq[i % 2][kb + i / 2] = at((i % 2 * KB + kb + i / 2) * 2 * kTile);
             }
             float r[8];
             {
@@ -790,36 +682,18 @@ __global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1
 #pragma unroll
             for (int e = 0; e < 8; ++e) odd = fmaf(v[e], 0.f, odd);
             float top = biggest();
-            if constexpr (DELTA) in_turn<6 * KW, 2, 1>();
+            if constexpr (DELTA) in_turn<6 * KB, 2, 1>();
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int half = 0; half < 2; ++half) x[half] = PAR > 1 ? x2[half][0] + x2[half][PAR - 1] : x2[half][0];
-            const bool is_odd = !idle && __ballot(odd != 0.f) != 0;
-            if constexpr (SPLIT == 1) {
-                slow = __builtin_amdgcn_readfirstlane(wild) != 0 || is_odd;
-            } else {
-                // Both parts' sums.
-                if constexpr (DELTA) {
-                    *reinterpret_cast<f4 *>(told + l * 16) = x[0];
-                    *reinterpret_cast<f4 *>(told + kTile + l * 16) = x[1];
-                }
-                *reinterpret_cast<float *>(told + L::kX + L::kO + l * 4) = top;
-                if (l == 0) odd_waves[w] = is_odd;
-                lds_barrier();
-                if constexpr (DELTA) {
-                    x[0] += *reinterpret_cast<const f4 *>(heard + l * 16);
-                    x[1] += *reinterpret_cast<const f4 *>(heard + kTile + l * 16);
-                }
-                top = fmaxf(top, *reinterpret_cast<const float *>(heard + L::kX + L::kO + l * 4));
-                slow = __builtin_amdgcn_readfirstlane(wild | some_odd()) != 0;
-            }
+            slow = __builtin_amdgcn_readfirstlane(wild) != 0 || __ballot(odd != 0.f) != 0;
             if (slow) break;
             // S^T q; meanwhile R and its terms, by 2^up more; the next state's scale:
             // below 2^15 whatever the chunk adds.
 #pragma unroll
             for (int half = 0; half < 2; ++half) of_u[half] = of_rows(kU, half);
 #pragma unroll
-            for (int kb = 0; kb < KW; kb += PAR) {
+            for (int kb = 0; kb < KB; kb += PAR) {
 #pragma unroll
                 for (int i = 0; i < 6 * PAR; ++i)
                     step(i / (2 * PAR), tq[i % 2][kb + i / 2 % PAR], sh[kb + i / 2 % PAR], sl[kb + i / 2 % PAR], o2[i % 2][i / 2 % PAR]);
@@ -846,9 +720,8 @@ __global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1
                 for (int e = 0; e < 8; ++e) r[e] *= by;
             }
             terms(r, minus, uh, ul);
-            in_turn<6 * KW, 3, 1>();
+            in_turn<6 * KB, 3, 1>();
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (SPLIT > 1) *reinterpret_cast<f4 *>(told + L::kX + l * 16) = split ? o[0] : o[1];  // the other's tokens
             // U, by 2^(scale + up + kSolve): below 2^15 while rows of T add up to 2^6.
             float u[8];
             if constexpr (DELTA) {
@@ -861,16 +734,13 @@ __global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1
 #pragma unroll
                 for (int e = 0; e < 8; ++e) u[e] = r[e];
             }
-            // M's rows of this wave's tokens: a half of them where two share a tile.
-            constexpr int HALVES = SPLIT > 1 ? 1 : 2;
-            Terms tm[HALVES];
-            f4 of_q[HALVES], of_m[HALVES];
+            Terms tm[2];
+            f4 of_q[2], of_m[2];
 #pragma unroll
-            for (int half = 0; half < HALVES; ++half) {
-                const int which = SPLIT > 1 ? int(split) : half;
-                tm[half] = at(values + which * 2 * kTile);
-                of_q[half] = of_rows(kQ, which);
-                of_m[half] = of_rows(kM, which);
+            for (int half = 0; half < 2; ++half) {
+                tm[half] = at(L::kKey + half * 2 * kTile);
+                of_q[half] = of_rows(kQ, half);
+                of_m[half] = of_rows(kM, half);
             }
             {
                 const float keep = ldexpf(whole, to - scale);
@@ -894,37 +764,29 @@ __global__ __launch_bounds__((NC * SPLIT + NL) * 64, NC * SPLIT + NL > 4 ? 2 : 1
             }
             __builtin_amdgcn_sched_barrier(0);
             // The next state, M U and the outputs.
-            f4 y[HALVES] = {};
+            f4 y[2] = {};
 #pragma unroll
-            for (int i = 0; i < 3 * HALVES; ++i) step(i / HALVES, tm[i % HALVES], uh, ul, y[i % HALVES]);
+            for (int i = 0; i < 6; ++i) step(i / 2, tm[i % 2], uh, ul, y[i % 2]);
 #pragma unroll
             for (int i = 0; i < 3 * TD; ++i) step(i / TD, tu[i % TD], wh, wl, S[i % TD]);
             const float one = ldexpf(1.f, -scale), of_y = ldexpf(1.f, (DELTA ? -kSolve : 0) - up - scale);
-            if constexpr (SPLIT == 1) {
-                const auto rows = rows_of(c);
+            const auto rows = buffer_of(a.out + (size_t(first) + t0) * a.out_stride + size_t(h) * a.dv, ((n - 1) * a.out_stride + a.dv) * 4);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float out = of_q[e / 4][e % 4] * (o[e / 4][e % 4] * one) + of_m[e / 4][e % 4] * (y[e / 4][e % 4] * of_y);
-                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(out), rows,
-                                                          int(out_at + (16 * (e / 4) + e % 4) * a.out_stride * 4), 0, 0);
-                }
-            } else {
-                const f4 own = split ? o[1] : o[0];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    of_heard[i] = of_q[0][i] * one;
-                    waits[i] = of_heard[i] * own[i] + of_m[0][i] * (y[0][i] * of_y);
-                }
-                pending = true;
+            for (int e = 0; e < 8; ++e) {
+                const float out = of_q[e / 4][e % 4] * (o[e / 4][e % 4] * one) + of_m[e / 4][e % 4] * (y[e / 4][e % 4] * of_y);
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(out), rows,
+                                                      int(out_at + (16 * (e / 4) + e % 4) * a.out_stride * 4), 0, 0);
             }
             scale = to;
+#pragma unroll
+            for (int t = 0; t < TD; ++t) asm volatile("" : "+v"(S[t]));  // in the registers it came in
         } while (++c < c1);
         if (!slow) break;
-        tokens(c++);
-    }
-    if constexpr (SPLIT > 1) {
-        lds_barrier();
-        if (pending) finish(c1 - 1);
+        const uint32_t t0 = (c - begin) * kChunk;
+        rescale(0);
+        tokens_of_chunk<TD>(a, size_t(first) + t0, min(kChunk, count - t0), h, col, S);
+        rescale(fitting(biggest()));
+        ++c;
     }
     if (idle || (ends ? !a.keep || slot == seq::kNoSlot : pass.to == nullptr)) return;
     rescale(0);
@@ -977,10 +839,10 @@ hipError_t go_prepare(const LinearArgs &a, const Pass &pass, hipStream_t stream)
     return hipGetLastError();
 }
 
-template <int KB, int NC, int SPLIT, int NL, bool DELTA>
+template <int KB, int NC, int NL, bool DELTA>
 hipError_t go_scan(const LinearArgs &a, const Pass &pass, hipStream_t stream) {
-    const auto kernel = linear_scan_kernel<KB, NC, SPLIT, NL, DELTA>;
-    using L = Scan<KB, NC, SPLIT, NL, DELTA>;
+    const auto kernel = linear_scan_kernel<KB, NC, NL, DELTA>;
+    using L = Scan<KB, NC, NL, DELTA>;
     const hipError_t e = raise_lds_limit(reinterpret_cast<const void *>(kernel), L::kBytes);
     if (e != hipSuccess) return e;
     const uint32_t units = (a.seq.seqs * a.k_heads + 7) / 8 * 8;
@@ -993,9 +855,9 @@ hipError_t go_pass(const LinearArgs &a, const LinearPlan &pl, const Pass &pass, 
     const hipError_t e = go_prepare<KB, DELTA>(a, pass, stream);
     if (e != hipSuccess) return e;
     if constexpr (KB == 8) {
-        return go_scan<KB, 2, 1, 2, DELTA>(a, pass, stream);  // two states' worth of registers a wave
+        return go_scan<KB, 2, 2, DELTA>(a, pass, stream);  // two states' worth of registers a wave
     } else {
-        return pl.columns == 2 ? go_scan<KB, 2, 2, 4, DELTA>(a, pass, stream) : go_scan<KB, 4, 1, 4, DELTA>(a, pass, stream);
+        return pl.columns == 2 ? go_scan<KB, 2, 2, DELTA>(a, pass, stream) : go_scan<KB, 4, 4, DELTA>(a, pass, stream);
     }
 }
 
