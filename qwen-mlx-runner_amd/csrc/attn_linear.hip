@@ -14,6 +14,7 @@
 #include "kernels.hpp"
 #include "linear_common.hpp"
 #include "sequences.hpp"
+#include "wave_ops.hpp"
 
 namespace qmr {
 namespace {
@@ -23,19 +24,44 @@ using linear::log_decay;
 using linear::Quad;
 using linear::quad_at;
 using linear::sigmoid;
+using wave::f4;
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 
-// Token after token, a workgroup a sequence and value head. A thread has R rows
-// of four columns of the state in registers, CG threads a row. One sum over
-// the rows a token: k and q meet the old state together, since
+// v and another value, the sum of each over two halves of a wave: v's in the
+// lanes whose bit is clear, the other's where it is set.
+template <int LANES>
+__device__ __forceinline__ float both_halves(float v, float other) {
+    const uint32_t a = __float_as_uint(v), b = __float_as_uint(other);
+    if constexpr (LANES == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else {
+        const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+}
+
+// Token after token, a workgroup a sequence and value head: for single tokens
+// and a few. A thread has R rows of four columns of the state in registers; a
+// wave has 32 columns of 8R rows, eight lanes a row, and the waves are CB blocks
+// of columns by 8 / CB of rows. One sum over the rows a token, of 11 numbers a
+// lane: k and q meet the old state together, since
 //
-//   S_t^T q = e^g S_{t-1}^T q + (k . q) u,  u what the token adds along k.
-template <int CG, int R>
+//   S_t^T q = e^g S_{t-1}^T q + (k . q) u,  u what the token adds along k,
+//
+// and k.k, q.q and q.k give the lengths. In a wave the sum is halved and dealt at
+// once, 12 numbers to six to three a lane, so that 12 swaps and 12 adds do what
+// 33 exchanges would. Rows of q, k and v come to LDS two tokens ahead.
+template <int CB, int R>
 __global__ __launch_bounds__(kThreads) void attn_linear_tokens_kernel(LinearArgs a) {
-    __shared__ Quad sums[2][kWaves][2][CG];
-    __shared__ float dots[2][kWaves][3];
+    constexpr int RB = kWaves / CB, kKeys = R * 8 * RB, kValues = CB * 32;  // row blocks; dimensions there is room for
+    constexpr int kRow = 2 * kKeys + kValues, kEach = (kRow + kThreads - 1) / kThreads;
+    __shared__ __align__(16) float rows[3][kRow];          // q, k, v
+    __shared__ __align__(16) float sums[2][kWaves][8][12]; // of a wave's eight column groups
+    __shared__ float gates[3][2];
+    __shared__ float squares[2][CB];
     const uint32_t s = blockIdx.x / a.v_heads, h = blockIdx.x % a.v_heads;
     uint32_t first, count;
     seq::tokens_of(a.seq, s, first, count);
@@ -43,8 +69,9 @@ __global__ __launch_bounds__(kThreads) void attn_linear_tokens_kernel(LinearArgs
     bool read;
     const uint32_t slot = seq::slot_of(a.seq, s, read);
 
-    const uint32_t wave = threadIdx.x / 64, l = threadIdx.x % 64;
-    const uint32_t col = threadIdx.x % CG * 4, row = threadIdx.x / CG * R;
+    const uint32_t tid = threadIdx.x, wave = tid / 64, l = tid % 64;
+    const uint32_t cb = wave % CB, rb = wave / CB, group = l % 8;
+    const uint32_t col = cb * 32 + group * 4, row = rb * (8 * R) + l / 8 * R;
     const uint32_t dk = a.dk, dv = a.dv, kh = h / (a.v_heads / a.k_heads);
     const bool has = col < dv;
     float *state = a.state + (size_t(slot == seq::kNoSlot ? 0 : slot) * a.v_heads + h) * dk * dv;
@@ -52,80 +79,93 @@ __global__ __launch_bounds__(kThreads) void attn_linear_tokens_kernel(LinearArgs
 #pragma unroll
     for (int i = 0; i < R; ++i) S[i] = quad_at(state + size_t(row + i) * dv + col, read && has && row + i < dk);
 
-    const float *qp = a.q + size_t(first) * a.q_stride + size_t(kh) * dk + row;
-    const float *kp = a.k + size_t(first) * a.k_stride + size_t(kh) * dk + row;
-    const float *vp = a.v + size_t(first) * a.v_stride + size_t(h) * dv + col;
-    Quad q[R / 4], k[R / 4], v;
+    // What this thread brings of a token's rows, and of its decay and factor.
+    const float *from[kEach];
+    uint32_t step[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const uint32_t i = tid + e * kThreads;
+        const bool of_q = i < kKeys, of_k = !of_q && i < 2 * kKeys;
+        const uint32_t d = of_q ? i : of_k ? i - kKeys : i - 2 * kKeys;
+        const float *p = of_q   ? a.q + size_t(first) * a.q_stride + size_t(kh) * dk
+                         : of_k ? a.k + size_t(first) * a.k_stride + size_t(kh) * dk
+                                : a.v + size_t(first) * a.v_stride + size_t(h) * dv;
+        step[e] = of_q ? a.q_stride : of_k ? a.k_stride : a.v_stride;
+        from[e] = i < kRow && d < (of_q || of_k ? dk : dv) ? p + d : nullptr;
+    }
+    float next[kEach], next_gate = 0.f;
     auto load = [&](uint32_t t) {
 #pragma unroll
-        for (int i = 0; i < R / 4; ++i) {
-            q[i] = quad_at(qp + size_t(t) * a.q_stride + 4 * i, row + 4 * i < dk);
-            k[i] = quad_at(kp + size_t(t) * a.k_stride + 4 * i, row + 4 * i < dk);
-        }
-        v = quad_at(vp + size_t(t) * a.v_stride, has);
+        for (int e = 0; e < kEach; ++e) next[e] = from[e] ? from[e][size_t(t) * step[e]] : 0.f;
+        const size_t token = size_t(first) + t;
+        if (tid == 0) next_gate = log_decay(a, token, h);
+        if (tid == 64 && a.delta) next_gate = a.b[token * a.b_stride + h];
+    };
+    auto keep = [&](uint32_t t) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+            if (tid + e * kThreads < kRow) rows[t % 3][tid + e * kThreads] = next[e];
+        if (tid == 0) gates[t % 3][0] = expf(next_gate);
+        if (tid == 64) gates[t % 3][1] = a.delta ? sigmoid(next_gate) : 1.f;
     };
     load(0);
+    keep(0);
+    if (count > 1) load(1);
+    __syncthreads();
     for (uint32_t t = 0; t < count; ++t) {
-        Quad sk{}, sq{};
-        float kk = 0.f, qq = 0.f, qk = 0.f;
+        if (t + 1 < count) keep(t + 1);
+        if (t + 2 < count) load(t + 2);
+        const float *now = rows[t % 3];
+        float sum[12] = {};  // S^T k, S^T q, k.k, q.q, q.k
+        Quad k[R / 4];
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const float ki = k[i / 4].x[i % 4], qi = q[i / 4].x[i % 4];
-            kk = fmaf(ki, ki, kk);
-            qq = fmaf(qi, qi, qq);
-            qk = fmaf(qi, ki, qk);
+        for (int j = 0; j < R / 4; ++j) {
+            const Quad q = *reinterpret_cast<const Quad *>(now + row + 4 * j);
+            k[j] = *reinterpret_cast<const Quad *>(now + kKeys + row + 4 * j);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sk.x[j] = fmaf(S[i].x[j], ki, sk.x[j]);
-                sq.x[j] = fmaf(S[i].x[j], qi, sq.x[j]);
+            for (int i = 0; i < 4; ++i) {
+                const float ki = k[j].x[i], qi = q.x[i];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    sum[c] = fmaf(S[4 * j + i].x[c], ki, sum[c]);
+                    sum[4 + c] = fmaf(S[4 * j + i].x[c], qi, sum[4 + c]);
+                }
+                sum[8] = fmaf(ki, ki, sum[8]);
+                sum[9] = fmaf(qi, qi, sum[9]);
+                sum[10] = fmaf(qi, ki, sum[10]);
             }
         }
+        // Lanes with bit 5 have the last six, of those lanes with bit 4 the last three.
 #pragma unroll
-        for (int d = CG; d < 64; d *= 2) {
+        for (int i = 0; i < 6; ++i) sum[i] = both_halves<32>(sum[i], sum[6 + i]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sk.x[j] += __shfl_xor(sk.x[j], d);
-                sq.x[j] += __shfl_xor(sq.x[j], d);
-            }
-            kk += __shfl_xor(kk, d);
-            qq += __shfl_xor(qq, d);
-            qk += __shfl_xor(qk, d);
-        }
+        for (int i = 0; i < 3; ++i) sum[i] = both_halves<16>(sum[i], sum[3 + i]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            sum[i] += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(sum[i]), 0x128, 0xf, 0xf, true));  // row_ror:8
         const uint32_t at = t % 2;  // the other one may still be read
-        if (l < CG) {
-            sums[at][wave][0][l] = sk;
-            sums[at][wave][1][l] = sq;
+        if (!(l & 8)) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) sums[at][wave][group][l / 32 * 6 + l / 16 % 2 * 3 + i] = sum[i];
         }
-        if (l == 0) {
-            dots[at][wave][0] = kk;
-            dots[at][wave][1] = qq;
-            dots[at][wave][2] = qk;
-        }
-        const size_t token = size_t(first) + t;
-        const float decay = expf(log_decay(a, token, h));
-        const float beta = a.delta ? sigmoid(a.b[token * a.b_stride + h]) : 1.f;
         __syncthreads();
-        sk = Quad{};
-        sq = Quad{};
-        kk = qq = qk = 0.f;
+        f4 sk{}, sq{}, dots{};
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sk.x[j] += sums[at][w][0][l % CG].x[j];
-                sq.x[j] += sums[at][w][1][l % CG].x[j];
-            }
-            kk += dots[at][w][0];
-            qq += dots[at][w][1];
-            qk += dots[at][w][2];
+        for (int b = 0; b < RB; ++b) {
+            const f4 *p = reinterpret_cast<const f4 *>(sums[at][b * CB + cb][group]);
+            sk += p[0];
+            sq += p[1];
+            dots += p[2];
         }
-        const float fk = a.qk_eps > 0.f ? 1.f / sqrtf(kk + a.qk_eps) : 1.f;
-        const float fq = (a.qk_eps > 0.f ? 1.f / sqrtf(qq + a.qk_eps) : 1.f) * a.scale;
+        const float decay = gates[t % 3][0], beta = gates[t % 3][1];
+        const Quad v = *reinterpret_cast<const Quad *>(now + 2 * kKeys + col);
+        const float fk = a.qk_eps > 0.f ? 1.f / sqrtf(dots[0] + a.qk_eps) : 1.f;
+        const float fq = (a.qk_eps > 0.f ? 1.f / sqrtf(dots[1] + a.qk_eps) : 1.f) * a.scale;
         Quad u, o;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            u.x[j] = a.delta ? beta * (v.x[j] - decay * (sk.x[j] * fk)) : v.x[j];
-            o.x[j] = fq * (decay * sq.x[j] + qk * fk * u.x[j]);
+            u.x[j] = a.delta ? beta * (v.x[j] - decay * (sk[j] * fk)) : v.x[j];
+            o.x[j] = fq * (decay * sq[j] + dots[2] * fk * u.x[j]);
         }
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -133,23 +173,30 @@ __global__ __launch_bounds__(kThreads) void attn_linear_tokens_kernel(LinearArgs
 #pragma unroll
             for (int j = 0; j < 4; ++j) S[i].x[j] = fmaf(ki, u.x[j], decay * S[i].x[j]);
         }
-        if (t + 1 < count) load(t + 1);
-        if (wave == 0) {
-            if (a.out_eps > 0.f) {
-                float sum = 0.f;
+        if (a.out_eps > 0.f) {
+            float sum_sq = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sum += o.x[j] * o.x[j];  // columns past dv are zero
+            for (int j = 0; j < 4; ++j) sum_sq = fmaf(o.x[j], o.x[j], sum_sq);  // columns past dv are zero
 #pragma unroll
-                for (int d = 1; d < CG; d *= 2) sum += __shfl_xor(sum, d);
-                const float f = 1.f / sqrtf(sum / float(dv) + a.out_eps);
-                const Quad z = quad_at(a.z + token * a.z_stride + size_t(h) * dv + col, has);
-                const Quad n = quad_at(a.norm + col, has);
+            for (int d = 1; d < 8; d *= 2) sum_sq += __shfl_xor(sum_sq, d);
+            if constexpr (CB > 1) {
+                if (rb == 0 && l == 0) squares[at][cb] = sum_sq;
+                __syncthreads();
+                sum_sq = 0.f;
+#pragma unroll
+                for (int b = 0; b < CB; ++b) sum_sq += squares[at][b];
+            }
+            if (rb == 0 && l < 8 && has) {
+                const float f = 1.f / sqrtf(sum_sq / float(dv) + a.out_eps);
+                const size_t token = size_t(first) + t;
+                const Quad z = quad_at(a.z + token * a.z_stride + size_t(h) * dv + col, true);
+                const Quad n = quad_at(a.norm + col, true);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o.x[j] = o.x[j] * f * gate_of(z.x[j], n.x[j]);
             }
-            if (l < CG && has)
-                *reinterpret_cast<Quad *>(a.out + token * a.out_stride + size_t(h) * dv + col) = o;
         }
+        if (rb == 0 && l < 8 && has)
+            *reinterpret_cast<Quad *>(a.out + (size_t(first) + t) * a.out_stride + size_t(h) * dv + col) = o;
     }
     if (!a.keep || slot == seq::kNoSlot) return;
 #pragma unroll
@@ -157,19 +204,19 @@ __global__ __launch_bounds__(kThreads) void attn_linear_tokens_kernel(LinearArgs
         if (has && row + i < dk) *reinterpret_cast<Quad *>(state + size_t(row + i) * dv + col) = S[i];
 }
 
-template <int CG>
+template <int CB>
 void go_tokens(const LinearArgs &a, hipStream_t stream) {
-    const uint32_t blocks = a.seq.seqs * a.v_heads, rows = (a.dk + kThreads / CG - 1) / (kThreads / CG);
+    const uint32_t blocks = a.seq.seqs * a.v_heads, rows = (a.dk + 64 / CB - 1) / (64 / CB);  // of a thread
     if (rows <= 4) {
-        attn_linear_tokens_kernel<CG, 4><<<blocks, kThreads, 0, stream>>>(a);
-    } else if constexpr (CG >= 16) {
+        attn_linear_tokens_kernel<CB, 4><<<blocks, kThreads, 0, stream>>>(a);
+    } else if constexpr (CB >= 2) {
         if (rows <= 8) {
-            attn_linear_tokens_kernel<CG, 8><<<blocks, kThreads, 0, stream>>>(a);
-        } else if constexpr (CG >= 32) {
+            attn_linear_tokens_kernel<CB, 8><<<blocks, kThreads, 0, stream>>>(a);
+        } else if constexpr (CB >= 4) {
             if (rows <= 16) {
-                attn_linear_tokens_kernel<CG, 16><<<blocks, kThreads, 0, stream>>>(a);
-            } else if constexpr (CG >= 64) {
-                attn_linear_tokens_kernel<CG, 32><<<blocks, kThreads, 0, stream>>>(a);
+                attn_linear_tokens_kernel<CB, 16><<<blocks, kThreads, 0, stream>>>(a);
+            } else if constexpr (CB >= 8) {
+                attn_linear_tokens_kernel<CB, 32><<<blocks, kThreads, 0, stream>>>(a);
             }
         }
     }
@@ -180,13 +227,13 @@ void go_tokens(const LinearArgs &a, hipStream_t stream) {
 hipError_t launch_attn_linear(const LinearArgs &a, const LinearPlan &pl, void *workspace, hipStream_t stream) {
     if (pl.chunks) return launch_linear_chunks(a, pl, workspace, stream);
     if (a.dv <= 32) {
-        go_tokens<8>(a, stream);
+        go_tokens<1>(a, stream);
     } else if (a.dv <= 64) {
-        go_tokens<16>(a, stream);
+        go_tokens<2>(a, stream);
     } else if (a.dv <= 128) {
-        go_tokens<32>(a, stream);
+        go_tokens<4>(a, stream);
     } else {
-        go_tokens<64>(a, stream);
+        go_tokens<8>(a, stream);
     }
     return hipGetLastError();
 }

@@ -801,31 +801,39 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
 
 constexpr int kNorm = 256;
 
-// The RMS norm and gate of the outputs, where they are: `lanes` lanes a head's
-// row of a token. A workgroup has a chunk's tokens and `heads` heads.
-__global__ __launch_bounds__(kNorm) void linear_norm_kernel(LinearArgs a, uint32_t first_chunk, uint32_t lanes, uint32_t heads) {
+// The RMS norm and gate of the outputs, where they are: LANES lanes a head's row
+// of a token, a workgroup a chunk's tokens of one head, all of whose loads are
+// under way at once.
+template <int LANES>
+__global__ __launch_bounds__(kNorm) void linear_norm_kernel(LinearArgs a) {
+    constexpr int kSlots = kNorm / LANES, kEach = kSlots < 32 ? 32 / kSlots : 1;
     uint32_t s, part, first, count;
-    if (!seq::part_of(a.seq, first_chunk + blockIdx.x, kChunk, s, part)) return;
+    if (!seq::part_of(a.seq, blockIdx.x, kChunk, s, part)) return;
     seq::tokens_of(a.seq, s, first, count);
-    const uint32_t t0 = part * kChunk, n = min(kChunk, count - t0);
-    const uint32_t h0 = blockIdx.y * heads, own = min(heads, a.v_heads - h0);
-    const uint32_t lane = threadIdx.x % lanes, col = lane * 4;
+    const uint32_t t0 = part * kChunk, n = min(kChunk, count - t0), h = blockIdx.y;
+    const uint32_t col = threadIdx.x % LANES * 4, slot = threadIdx.x / LANES;
     const bool has = col < a.dv;
     const Quad norm = quad_at(a.norm + col, has);
-    for (uint32_t row = threadIdx.x / lanes; row < n * own; row += kNorm / lanes) {
-        const size_t token = size_t(first) + t0 + row / own;
-        const uint32_t h = h0 + row % own;
-        float *out = a.out + token * a.out_stride + size_t(h) * a.dv + col;
-        Quad o = quad_at(out, has);
-        const Quad z = quad_at(a.z + token * a.z_stride + size_t(h) * a.dv + col, has);
+    float *out = a.out + (size_t(first) + t0 + slot) * a.out_stride + size_t(h) * a.dv + col;
+    const float *gate = a.z + (size_t(first) + t0 + slot) * a.z_stride + size_t(h) * a.dv + col;
+    Quad o[kEach], z[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const bool there = has && slot + k * kSlots < n;
+        o[k] = quad_at(out + size_t(k) * kSlots * a.out_stride, there);
+        z[k] = quad_at(gate + size_t(k) * kSlots * a.z_stride, there);
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum = fmaf(o.x[i], o.x[i], sum);
-        for (uint32_t d = 1; d < lanes; d *= 2) sum += __shfl_xor(sum, d);
+        for (int i = 0; i < 4; ++i) sum = fmaf(o[k].x[i], o[k].x[i], sum);
+#pragma unroll
+        for (int d = 1; d < LANES; d *= 2) sum += __shfl_xor(sum, d);
         const float f = 1.f / sqrtf(sum / float(a.dv) + a.out_eps);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o.x[i] = o.x[i] * f * gate_of(z.x[i], norm.x[i]);
-        if (has) *reinterpret_cast<Quad *>(out) = o;
+        for (int i = 0; i < 4; ++i) o[k].x[i] = o[k].x[i] * f * gate_of(z[k].x[i], norm.x[i]);
+        if (has && slot + k * kSlots < n) *reinterpret_cast<Quad *>(out + size_t(k) * kSlots * a.out_stride) = o[k];
     }
 }
 
@@ -878,7 +886,7 @@ LinearPlan plan_linear(const LinearArgs &a, const DeviceLimits &lim, size_t limi
     pl.v_bytes = size_t(a.delta ? 9 : 5) * kTile;
     if (columns == 0 && pl.blocks < 8)
         while (pl.columns < 4 && uint64_t(std::min(q.seqs, pl.parts)) * a.v_heads * ((tiles + pl.columns - 1) / pl.columns) >
-                                     2 * uint64_t(lim.num_cus))
+                                     uint64_t(lim.num_cus))
             pl.columns *= 2;
     const size_t each = a.k_heads * pl.k_bytes + a.v_heads * pl.v_bytes;
     limit = std::min(limit, size_t(256) << 20);
@@ -920,10 +928,11 @@ hipError_t launch_linear_chunks(const LinearArgs &a, const LinearPlan &pl, void 
         }
     }
     if (e != hipSuccess || !(a.out_eps > 0.f)) return e;
-    uint32_t lanes = 2;
-    while (lanes * 4 < a.dv) lanes *= 2;
-    const uint32_t heads = 4;
-    linear_norm_kernel<<<dim3(pl.parts, (a.v_heads + heads - 1) / heads), kNorm, 0, stream>>>(a, 0, lanes, heads);
+    const dim3 grid(pl.parts, a.v_heads);
+    if (a.dv <= 32) linear_norm_kernel<8><<<grid, kNorm, 0, stream>>>(a);
+    else if (a.dv <= 64) linear_norm_kernel<16><<<grid, kNorm, 0, stream>>>(a);
+    else if (a.dv <= 128) linear_norm_kernel<32><<<grid, kNorm, 0, stream>>>(a);
+    else linear_norm_kernel<64><<<grid, kNorm, 0, stream>>>(a);
     return hipGetLastError();
 }
 

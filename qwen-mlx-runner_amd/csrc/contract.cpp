@@ -278,6 +278,7 @@ Layout linear_layout(const std::string &name, const uint32_t *p, size_t np) {
     const size_t kw = bytes({k_heads, dk}), vw = bytes({v_heads, dv});
     const bool gates = p[14] == 1, delta = p[15] == 1, normed = p[18] != 0;
     const size_t head = v_heads * 4;
+    ensure(v_heads <= 65535 && k_heads <= 65535, name + ": too many heads");
     threads({seqs, v_heads, 1024});
     threads({tokens + seqs, v_heads, 32});
     out.sizes = {rows(tokens, kw, p[6]),
