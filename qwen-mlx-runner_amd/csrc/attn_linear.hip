@@ -57,10 +57,10 @@ __device__ __forceinline__ float both_halves(float v, float other) {
 template <int CB, int R>
 __global__ __launch_bounds__(kThreads) void attn_linear_tokens_kernel(LinearArgs a) {
     constexpr int RB = kWaves / CB, kKeys = R * 8 * RB, kValues = CB * 32;  // row blocks; dimensions there is room for
-    constexpr int kRow = 2 * kKeys + kValues, kEach = (kRow + kThreads - 1) / kThreads;
-    __shared__ __align__(16) float rows[3][kRow];          // q, k, v
+    constexpr int kRow = 2 * (kKeys + kValues), kEach = (kRow + kThreads - 1) / kThreads;
+    __shared__ __align__(16) float rows[3][kRow];          // q, k, v, what z and the norm's weights make of an output
     __shared__ __align__(16) float sums[2][kWaves][8][12]; // of a wave's eight column groups
-    __shared__ float gates[3][2];
+    __shared__ float decays[2][64], betas[2][64];  // of 64 tokens at once, a lane a token
     __shared__ float squares[2][CB];
     const uint32_t s = blockIdx.x / a.v_heads, h = blockIdx.x % a.v_heads;
     uint32_t first, count;
@@ -79,40 +79,48 @@ __global__ __launch_bounds__(kThreads) void attn_linear_tokens_kernel(LinearArgs
 #pragma unroll
     for (int i = 0; i < R; ++i) S[i] = quad_at(state + size_t(row + i) * dv + col, read && has && row + i < dk);
 
-    // What this thread brings of a token's rows, and of its decay and factor.
+    // What this thread brings of a token's rows.
     const float *from[kEach];
+    float norm[kEach] = {};
     uint32_t step[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
         const uint32_t i = tid + e * kThreads;
-        const bool of_q = i < kKeys, of_k = !of_q && i < 2 * kKeys;
-        const uint32_t d = of_q ? i : of_k ? i - kKeys : i - 2 * kKeys;
+        const bool of_q = i < kKeys, of_k = !of_q && i < 2 * kKeys, of_z = i >= 2 * kKeys + kValues;
+        const uint32_t d = of_q ? i : of_k ? i - kKeys : i - 2 * kKeys - of_z * kValues;
         const float *p = of_q   ? a.q + size_t(first) * a.q_stride + size_t(kh) * dk
                          : of_k ? a.k + size_t(first) * a.k_stride + size_t(kh) * dk
+                         : of_z ? a.z + size_t(first) * a.z_stride + size_t(h) * dv
                                 : a.v + size_t(first) * a.v_stride + size_t(h) * dv;
-        step[e] = of_q ? a.q_stride : of_k ? a.k_stride : a.v_stride;
-        from[e] = i < kRow && d < (of_q || of_k ? dk : dv) ? p + d : nullptr;
+        step[e] = of_q ? a.q_stride : of_k ? a.k_stride : of_z ? a.z_stride : a.v_stride;
+        from[e] = i < kRow && d < (of_q || of_k ? dk : dv) && (!of_z || a.out_eps > 0.f) ? p + d : nullptr;
+        if (of_z && from[e]) norm[e] = a.norm[d];
     }
-    float next[kEach], next_gate = 0.f;
+    float next[kEach];
     auto load = [&](uint32_t t) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) next[e] = from[e] ? from[e][size_t(t) * step[e]] : 0.f;
-        const size_t token = size_t(first) + t;
-        if (tid == 0) next_gate = log_decay(a, token, h);
-        if (tid == 64 && a.delta) next_gate = a.b[token * a.b_stride + h];
     };
     auto keep = [&](uint32_t t) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e)
-            if (tid + e * kThreads < kRow) rows[t % 3][tid + e * kThreads] = next[e];
-        if (tid == 0) gates[t % 3][0] = expf(next_gate);
-        if (tid == 64) gates[t % 3][1] = a.delta ? sigmoid(next_gate) : 1.f;
+            if (const uint32_t i = tid + e * kThreads; i < kRow)
+                rows[t % 3][i] = i < 2 * kKeys + kValues ? next[e] : gate_of(next[e], norm[e]);
+    };
+    auto gates = [&](uint32_t t) {
+        const size_t token = size_t(first) + t + l;
+        const bool any = t + l < count;
+        if (wave == 0) decays[t / 64 % 2][l] = any ? expf(log_decay(a, token, h)) : 1.f;
+        if (wave == 1) betas[t / 64 % 2][l] = any && a.delta ? sigmoid(a.b[token * a.b_stride + h]) : 1.f;
     };
     load(0);
     keep(0);
+    gates(0);
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the state is here, and no wait for it below waits for the loads ahead
     if (count > 1) load(1);
-    __syncthreads();
+    wave::lds_barrier();
     for (uint32_t t = 0; t < count; ++t) {
+        if (t && t % 64 == 0) gates(t);
         if (t + 1 < count) keep(t + 1);
         if (t + 2 < count) load(t + 2);
         const float *now = rows[t % 3];
@@ -148,7 +156,7 @@ __global__ __launch_bounds__(kThreads) void attn_linear_tokens_kernel(LinearArgs
 #pragma unroll
             for (int i = 0; i < 3; ++i) sums[at][wave][group][l / 32 * 6 + l / 16 % 2 * 3 + i] = sum[i];
         }
-        __syncthreads();
+        wave::lds_barrier();
         f4 sk{}, sq{}, dots{};
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
@@ -157,10 +165,10 @@ __global__ __launch_bounds__(kThreads) void attn_linear_tokens_kernel(LinearArgs
             sq += p[1];
             dots += p[2];
         }
-        const float decay = gates[t % 3][0], beta = gates[t % 3][1];
+        const float decay = decays[t / 64 % 2][t % 64], beta = betas[t / 64 % 2][t % 64];
         const Quad v = *reinterpret_cast<const Quad *>(now + 2 * kKeys + col);
-        const float fk = a.qk_eps > 0.f ? 1.f / sqrtf(dots[0] + a.qk_eps) : 1.f;
-        const float fq = (a.qk_eps > 0.f ? 1.f / sqrtf(dots[1] + a.qk_eps) : 1.f) * a.scale;
+        const float fk = a.qk_eps > 0.f ? rsqrtf(dots[0] + a.qk_eps) : 1.f;
+        const float fq = (a.qk_eps > 0.f ? rsqrtf(dots[1] + a.qk_eps) : 1.f) * a.scale;
         Quad u, o;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -181,21 +189,17 @@ __global__ __launch_bounds__(kThreads) void attn_linear_tokens_kernel(LinearArgs
             for (int d = 1; d < 8; d *= 2) sum_sq += __shfl_xor(sum_sq, d);
             if constexpr (CB > 1) {
                 if (rb == 0 && l == 0) squares[at][cb] = sum_sq;
-                __syncthreads();
+                wave::lds_barrier();
                 sum_sq = 0.f;
 #pragma unroll
                 for (int b = 0; b < CB; ++b) sum_sq += squares[at][b];
             }
-            if (rb == 0 && l < 8 && has) {
-                const float f = 1.f / sqrtf(sum_sq / float(dv) + a.out_eps);
-                const size_t token = size_t(first) + t;
-                const Quad z = quad_at(a.z + token * a.z_stride + size_t(h) * dv + col, true);
-                const Quad n = quad_at(a.norm + col, true);
+            const Quad gate = *reinterpret_cast<const Quad *>(now + 2 * kKeys + kValues + col);
+            const float f = rsqrtf(sum_sq / float(dv) + a.out_eps);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o.x[j] = o.x[j] * f * gate_of(z.x[j], n.x[j]);
-            }
+            for (int j = 0; j < 4; ++j) o.x[j] = o.x[j] * f * gate.x[j];
         }
-        if (rb == 0 && l < 8 && has)
+        if (rb == 0 && l < 8 && has)  // the waves of the first rows write the outputs
             *reinterpret_cast<Quad *>(a.out + (size_t(first) + t) * a.out_stride + size_t(h) * dv + col) = o;
     }
     if (!a.keep || slot == seq::kNoSlot) return;

@@ -875,7 +875,12 @@ LinearPlan plan_linear(const LinearArgs &a, const DeviceLimits &lim, size_t limi
     LinearPlan pl;
     const Sequences &q = a.seq;
     const uint32_t longest = std::min(q.most, q.tokens);
-    if (form == 1 || (form == 0 && longest < 16)) return pl;
+    // Token after token up to eight. Both forms in us, 48 heads of 128 x 128: one
+    // sequence of 4, 8, 12 and 16 tokens 12/21, 17/21, 23/21 and 28/22; eight
+    // sequences of 8 and 12 29/38 and 38/39; 32 of 8 and 12 77/95 and 102/97. Eight
+    // heads of 64 x 64, one sequence of 8 and 12: 16/17 and 21/18; three of
+    // 256 x 192: 30/26 and 42/27.
+    if (form == 1 || (form == 0 && longest <= 8)) return pl;
     // Rows that a buffer's 32-bit offsets reach over a chunk.
     if (a.v_stride > 1u << 22 || a.out_stride > 1u << 22) return pl;
     const uint32_t tiles = (a.dv + 15) / 16;

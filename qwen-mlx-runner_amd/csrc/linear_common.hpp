@@ -21,13 +21,17 @@ __device__ __forceinline__ Quad quad_at(const float *p, bool there) {
     return there ? *reinterpret_cast<const Quad *>(p) : Quad{};
 }
 
-// The log of the decay of value head h at token t.
-__device__ __forceinline__ float log_decay(const LinearArgs &a, size_t t, uint32_t h) {
-    const float x = a.a[t * a.a_stride + h];
-    if (!a.gates) return x;
-    const float y = x + a.dt_bias[h];
+// The log of a decay, from its row's value and what the gates make of it.
+__device__ __forceinline__ float log_decay(bool gates, float x, float a_log, float dt_bias) {
+    if (!gates) return x;
+    const float y = x + dt_bias;
     // Past 20, log(1 + e^y) is y to 2^-33 of it.
-    return -expf(a.a_log[h]) * (y > 20.f ? y : log1pf(expf(y)));
+    return -expf(a_log) * (y > 20.f ? y : log1pf(expf(y)));
+}
+
+// That of value head h at token t.
+__device__ __forceinline__ float log_decay(const LinearArgs &a, size_t t, uint32_t h) {
+    return log_decay(a.gates, a.a[t * a.a_stride + h], a.gates ? a.a_log[h] : 0.f, a.gates ? a.dt_bias[h] : 0.f);
 }
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
