@@ -145,7 +145,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const float *p, uint
 // Which chunks a pass has, and where their operands are.
 struct Pass {
     unsigned char *operands;  // [chunk][k_heads * k_bytes + v_heads * v_bytes]
-    float *from, *to;         // a state [v_heads][dk][dv] that the last pass left, or this one leaves; the last one leaves none
+    float *from, *to;         // a state [v_heads][dk][dv] and its scales that the last pass left, or this one leaves; the last one leaves none
     uint32_t first, last;
     uint32_t k_bytes, v_bytes;
     uint32_t columns;         // workgroups of a head
@@ -581,7 +581,11 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
         scale = to;
     };
     auto fitting = [](float top) { return max(-113, min(15 - exponent(top), 110)); };
-    rescale(fitting(biggest()));
+    // A state that the last pass left is kept as it was there, its columns'
+    // scales behind it: no result depends on where passes end.
+    const size_t scale_at = size_t(a.v_heads) * a.dk * a.dv + size_t(h) * a.dv + col;
+    if (!starts && has) scale = __float_as_int(pass.from[scale_at]);
+    rescale(starts ? fitting(biggest()) : scale);
 
     uint32_t c = c0;
     if (idle) {
@@ -789,7 +793,8 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
         ++c;
     }
     if (idle || (ends ? !a.keep || slot == seq::kNoSlot : pass.to == nullptr)) return;
-    rescale(0);
+    if (!ends && has && g == 0) pass.to[scale_at] = __int_as_float(scale);
+    rescale(ends ? 0 : scale);
     const auto r = buffer_of(ends ? pool : pass.to + size_t(h) * a.dk * a.dv, state_bytes);
     asm volatile("" : "+v"(state_at));  // or all of the addresses wait in registers for this
 #pragma unroll
@@ -883,6 +888,7 @@ LinearPlan plan_linear(const LinearArgs &a, const DeviceLimits &lim, size_t limi
     if (form == 1 || (form == 0 && longest <= 8)) return pl;
     // Rows that a buffer's 32-bit offsets reach over a chunk.
     if (a.v_stride > 1u << 22 || a.out_stride > 1u << 22) return pl;
+    if (columns != 2 && columns != 4) columns = 0;
     const uint32_t tiles = (a.dv + 15) / 16;
     pl.blocks = a.dk <= 64 ? 2 : a.dk <= 128 ? 4 : 8;
     pl.columns = columns && pl.blocks < 8 ? columns : 2;
@@ -897,7 +903,7 @@ LinearPlan plan_linear(const LinearArgs &a, const DeviceLimits &lim, size_t limi
     limit = std::min(limit, size_t(256) << 20);
     pl.per_pass = pl.parts;
     if (each * pl.parts > limit) {
-        pl.carry_bytes = (size_t(a.v_heads) * a.dk * a.dv * 4 + 255) / 256 * 256;
+        pl.carry_bytes = (size_t(a.v_heads) * (a.dk + 1) * a.dv * 4 + 255) / 256 * 256;
         if (limit < 2 * pl.carry_bytes + each) return LinearPlan{};
         pl.per_pass = uint32_t((limit - 2 * pl.carry_bytes) / each);
     }
