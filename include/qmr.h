@@ -122,7 +122,7 @@ int qmr_command_begin(qmr_device *device, qmr_command **out);
  * `name` is a reference kernel name (matvec_affine, matvec_affine_bf16,
  * matmul_affine, matmul_affine_bf16, embed_affine, embed_affine_bf16,
  * matvec_f16, matmul_f16, embed_f16, copy_f32) or one of this library's additions
- * (matmul_affine_wide[_bf16], rope_axes, attn_paged_bf16, .., see below). `offsets` may be NULL (all zero) or
+ * (matmul_affine_wide[_bf16], rope_axes, attn_paged_bf16, attn_linear, .., see below). `offsets` may be NULL (all zero) or
  * hold one 4-byte-aligned byte offset per buffer. `params`, `threads` and
  * `group_size` follow dispatch_layout (src/gpu.rs:1041-1294). */
 int qmr_encode(qmr_command *command, const char *name, qmr_buffer *const *buffers,
@@ -134,21 +134,25 @@ int qmr_encode(qmr_command *command, const char *name, qmr_buffer *const *buffer
  * it calls no hipMalloc, hipFree or allocating library routine. The
  * workspace its kernels need (the row-band kernel's split sums, the split-K
  * kernel's partial sums and counters, the wide block's activation images,
- * attention's results of key ranges) comes from a static scratch array of QMR_STATIC_SCRATCH_BYTES that each GPU
+ * attention's results of key ranges, linear attention's chunks, a draw's
+ * candidates) comes from a static scratch array of QMR_STATIC_SCRATCH_BYTES that each GPU
  * holds from library load until the process ends; a launch needing more is
  * rejected with QMR_ERR_INVALID before anything is enqueued. (Of the wide
  * blocks these are Q4 ones of group 64 and more than eight RHS over whole 256
  * columns, codes, scales and biases 16-byte aligned; the others run in
  * passes over fewer RHS, or as blocks of four, that fit the scratch, and do
  * so in qmr_encode too. attn_paged is planned with as many key ranges as fit:
- * its bits are qmr_encode's wherever both plans agree, as for single tokens.) Workspace that
+ * its bits are qmr_encode's wherever both plans agree, as for single tokens.
+ * attn_linear takes the chunks of long prompts in as many passes as the
+ * scratch asks for, with qmr_encode's bits.) Workspace that
  * must start at zero (split sums tagged with a fixed epoch, arrival counters)
  * is cleared by a fill kernel inside the call when earlier launches may have
  * left it non-zero: the split-K kernel and the row-band kernel's GEMV and
  * block forms (plain or residual) clear every slot and counter they take, so
  * after the first fill the region stays zero from call to call and needs no
  * fill until a wide block, a group 32 block of three or four RHS on the wide
- * kernel, the row-band MLP form, attn_paged or a failed command has used it. All calls on one GPU share its scratch: calls whose launches
+ * kernel, the row-band MLP form, attn_paged, attn_linear's chunks,
+ * sample_logits or a failed command has used it. All calls on one GPU share its scratch: calls whose launches
  * overlap in time (other streams, other device handles on the same GPU)
  * race. */
 #define QMR_STATIC_SCRATCH_BYTES (8u << 20)
@@ -273,6 +277,63 @@ int qmr_supported_bf16_quantization(uint32_t bits, size_t group);
  *     a BF16 cache queries and weights keep 24 bits. With an F16 cache they keep
  *     22, but a query's element is off by 2^-39 of its row's largest and a weight
  *     by 2^-36 of its row's where that is more.
+ *   "conv_causal"
+ *     The short convolution of each channel over its sequence, in front of
+ *     linear attention: y_t = f(bias + sum_j w[j] x_{t-width+1+j}), f silu or
+ *     nothing. Buffers x, w FP32 [channels][width], bias [channels], starts u32
+ *     [seqs+1], slots u32 [seqs], state FP32 [pool][width-1][channels], y;
+ *     params seqs, tokens, channels, width (2..4), x stride, y stride, silu,
+ *     bias (0: none is read), pool, keep. Sequence s has the tokens
+ *     starts[s]..starts[s+1]-1 (to the last of `tokens` at most; rows in no
+ *     sequence stay as they were). The rows in front of its first token are
+ *     those of its slot, oldest first; with keep = 1 the last width-1 rows, old
+ *     ones included, replace them. Low 31 bits of slots[s] name the slot; bit 31
+ *     set: the sequence starts here, its state is zeros and is not read. A slot
+ *     that is not below `pool`, or that an earlier sequence of the call names,
+ *     is none: zeros in front, and nothing is kept. A sequence without tokens
+ *     leaves its slot as it was. y may be rows beside x's in one buffer.
+ *   "attn_linear"
+ *     Linear attention with decaying states, for single tokens as for whole
+ *     prompts. Of value head h with a state S of dk x dv, and the queries and
+ *     keys of key head h / (v heads / k heads):
+ *       S_t = e^g S_{t-1} + k (beta (v - (e^g S_{t-1})^T k))^T  with delta = 1,
+ *       S_t = e^g S_{t-1} + k v^T                               with delta = 0,
+ *       o_t = scale S_t^T q_t;
+ *     beta = 1 / (1 + e^-b); g = a (0 or below) with gates = 0, with gates = 1
+ *     -e^a_log log(1 + e^(a + dt_bias)). Buffers q, k, v, a, b (FP32 rows, which
+ *     may be columns of one buffer), a_log, dt_bias FP32 [v heads], z (rows),
+ *     norm FP32 [dv], starts u32 [seqs+1], slots u32 [seqs], state FP32
+ *     [pool][v heads][dk][dv], out; params seqs, tokens, k heads, v heads, dk,
+ *     dv, strides of q, k, v, a, b, z and out, most, gates, delta, scale, qk eps
+ *     and out eps as FP32 bits, pool, keep. With a stride of 0 (and gates = 0)
+ *     all tokens have one row of a. b is read with delta = 1 alone, a_log and
+ *     dt_bias with gates = 1. qk eps > 0 divides each query and key by
+ *     sqrt(sum x^2 + eps) first; out eps > 0 makes an output
+ *     o / sqrt(mean o^2 + eps) * norm * z / (1 + e^-z), over its head, and else z
+ *     and norm are not read. Sequences, slots and keep as in conv_causal; of a
+ *     sequence the first `most` tokens count, those behind them stay as they
+ *     were, and the launch is planned for sequences that long. dk and dv
+ *     multiples of 8, at most 256; v heads a multiple of k heads, at most 65535.
+ *     out may be rows beside an input's in one buffer. Results are near FP32
+ *     arithmetic's. With delta = 1 that supposes keys at most about 1 long, as
+ *     qk eps makes them: longer ones can make the state grow without bound, in
+ *     which case a prompt's results come token after token, and slowly.
+ *   "sample_logits"
+ *     A token of each row of logits: the greatest, or one drawn from what
+ *     temperature, top-k, top-p and min-p leave. Buffers logits (FP32 rows),
+ *     temperature, top_k (u32), top_p, min_p, uniform [rows each], tokens u32
+ *     [rows], probs FP32 [rows]; params rows, vocab (at most 2^24), stride.
+ *     Tokens stand in the order of their logits, the lower index first where two
+ *     are equal; w_i = e^((x_i - max) / temperature). Kept are the first top_k
+ *     (0: all), of these the first whose weights reach top_p of those
+ *     top_k's sum (1 and above: all; the first at least), of these the ones with
+ *     w_i >= min_p. The token is the first, by index, at which the sum of
+ *     kept weights passes uniform (0 to 1) times all of it, and probs its share
+ *     of that sum. temperature 0 (or below, or not a number): the greatest, with
+ *     probability 1. NaN and -inf are never kept; a row that has no more than
+ *     those gives token 0xFFFFFFFF and probability 0. Of +inf each weighs the
+ *     same and all else nothing. Weights add up as whole numbers, 2^-38 of the
+ *     greatest or finer, so that a result depends on no order and calls repeat.
  *   "matvec_affine_f16meta", "matmul_affine_f16meta", "embed_affine_f16meta"
  *     As the FP32-metadata names, with scales/biases stored as IEEE binary16
  *     (the dtype MLX checkpoints ship). The reference expands F16 metadata
@@ -322,6 +383,9 @@ int qmr_supported_bf16_quantization(uint32_t bits, size_t group);
  *   rr = -7: attn_paged on the kernel of tiles of 16 or 128 query rows with
  *            ks = rows*1000 + key ranges (zero fields leave them to its
  *            planner); any other rr leaves attention to its planner.
+ *   rr = -8: attn_linear with ks = form*100 + columns (form 1 token after
+ *            token, 2 chunks; 2 or 4 tiles of 16 columns a workgroup; zero
+ *            fields leave them to its planner).
  * Shapes a forced kernel does not support fall back to the next one; pairs
  * that are not compiled fall back to the planner. */
 int qmr_set_gemv_plan(qmr_device *device, int rr, int ks);
@@ -348,8 +412,8 @@ int qmr_set_read_plan(qmr_device *device, uint32_t workgroups, uint32_t unroll, 
 int qmr_set_band_wait_fault(qmr_device *device, int enabled);
 /* Bytes of device workspace this handle has allocated for its kernels (the
  * row-band split sums, the split-K partial sums and counters, the wide
- * block's activation images, attention's results of key ranges);
- * qmr_encode_static allocates none. */
+ * block's activation images, attention's results of key ranges, linear
+ * attention's chunks, a draw's candidates); qmr_encode_static allocates none. */
 size_t qmr_device_workspace_bytes(const qmr_device *device);
 /* Reference pipeline label selected by the last successful qmr_encode. */
 const char *qmr_last_kernel(const qmr_device *device);
