@@ -50,6 +50,7 @@ constexpr uint32_t kPerNat = 16;         // bins of a temperature: 511 of them r
 constexpr uint32_t kCandidates = 8192;   // of a row, at most
 constexpr uint32_t kSliceStep = 4096;
 constexpr uint32_t kNone = 0xffffffffu;
+constexpr int kSteps = 64;  // of an octave, in the table of powers
 
 // Ordered as the logits are; NaN and -infinity are 0. Both zeros are one logit.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -75,21 +76,31 @@ __host__ __device__ constexpr uint32_t shift_of(uint32_t n) {
     return 62 - bits;
 }
 
+// A row's, read before anything is waited for.
+struct Settings {
+    float temperature, min_p, top_p;
+    uint32_t top_k;
+    __device__ Settings(const SampleArgs &a, uint32_t row)
+        : temperature(a.temperature[row]), min_p(a.min_p[row]), top_p(a.top_p[row]), top_k(a.top_k[row]) {}
+};
+
 // A row's weights and bins, from its largest and smallest logit.
 struct Weights {
     uint32_t top;
     float max, half_max, per_bin;  // bins: half the distance from the largest, times per_bin
-    double temperature, per_octave;  // per_octave: log2(e) / temperature
+    double temperature, per_step;  // per_step: kSteps log2(e) / temperature
+    const double *powers;          // 2^(i / kSteps)
     int shift;
     float min_p;
 
-    __device__ Weights(const SampleArgs &a, uint32_t row, uint32_t top_, uint32_t least)
-        : top(top_), max(logit_of(top_)), temperature(a.temperature[row]), shift(shift_of(a.vocab)), min_p(a.min_p[row]) {
-        per_octave = 1.4426950408889634 / temperature;
+    __device__ Weights(const SampleArgs &a, const Settings &set, uint32_t top_, uint32_t least, const double *powers_)
+        : top(top_), max(logit_of(top_)), temperature(set.temperature), powers(powers_), shift(shift_of(a.vocab)),
+          min_p(set.min_p) {
+        per_step = 1.4426950408889634 * kSteps / temperature;
         half_max = 0.5f * max;
         const float width = half_max - 0.5f * logit_of(least);
         // Narrow rows take all bins but the last, which then is empty.
-        per_bin = fminf(fmaxf(2.f * kPerNat / a.temperature[row], width > 0.f ? float(kBins - 2) / width : 0.f), 1e38f);
+        per_bin = fminf(fmaxf(2.f * kPerNat / set.temperature, width > 0.f ? float(kBins - 2) / width : 0.f), 1e38f);
     }
     __device__ bool greedy() const { return !(temperature > 0); }
     __device__ double plain(uint32_t key) const {
@@ -97,27 +108,22 @@ struct Weights {
         if (max == INFINITY) return 0.0;
         return exp((double(logit_of(key)) - double(max)) / temperature);
     }
-    // 2^t = 2^n 2^f, |f| <= 1/2, from the exponential's series: the term after the
-    // last is below 2^-52. Added to 2^52 the weight is rounded to a whole number
-    // and stands in the mantissa's low bits.
+    // 2^t = 2^(n / 64) e^y, |y| <= ln 2 / 128, from a table and the exponential's
+    // series: the term after the last is below 2^-54. Added to 2^52 the weight is
+    // rounded to a whole number and stands in the mantissa's low bits.
     __device__ u64 whole(uint32_t key) const {
-        const double t = (double(logit_of(key)) - double(max)) * per_octave;
-        if (!(t > -64.0)) return key == top ? u64(1) << shift : 0;  // also where both are infinite
-        const double n = rint(t), y = (t - n) * 0.6931471805599453;
-        double e = 1.0 / 479001600;
-        e = fma(e, y, 1.0 / 39916800);
-        e = fma(e, y, 1.0 / 3628800);
-        e = fma(e, y, 1.0 / 362880);
-        e = fma(e, y, 1.0 / 40320);
-        e = fma(e, y, 1.0 / 5040);
-        e = fma(e, y, 1.0 / 720);
-        e = fma(e, y, 1.0 / 120);
+        const double t = (double(logit_of(key)) - double(max)) * per_step;
+        if (!(t > -64.0 * kSteps)) return key == top ? u64(1) << shift : 0;  // also where both are infinite
+        const double n = rint(t), y = (t - n) * (0.6931471805599453 / kSteps);
+        const int steps = int(n);
+        double e = 1.0 / 120;
         e = fma(e, y, 1.0 / 24);
         e = fma(e, y, 1.0 / 6);
         e = fma(e, y, 0.5);
         e = fma(e, y, 1.0);
         e = fma(e, y, 1.0);
-        return u64(__double_as_longlong(ldexp(e, int(n) + shift) + 0x1p52)) & ((u64(1) << 52) - 1);
+        e *= powers[steps & (kSteps - 1)];
+        return u64(__double_as_longlong(ldexp(e, (steps >> 6) + shift) + 0x1p52)) & ((u64(1) << 52) - 1);
     }
     __device__ bool likely(uint32_t key) const { return key == top || !(min_p > 0.f) || plain(key) >= double(min_p); }
     // Never smaller for a smaller logit, whatever rounds.
@@ -128,38 +134,73 @@ struct Weights {
     }
 };
 
-template <typename T>
-__device__ __forceinline__ T block_sum(T v, T *room) {
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+// For whole workgroups, which wait before they look at it.
+__device__ __forceinline__ void fill_powers(double *powers) {
+    if (threadIdx.x < kSteps) powers[threadIdx.x] = exp2(double(threadIdx.x) / kSteps);
+}
+
+// The value of the lane that CTRL names in the rows of ROWS, 0 where there is
+// none: steps of scans that stay in registers. Through LDS the four launches of
+// a row of 248320 took 34.7 us, so 31.9: they have some 30 such scans.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 from_lane(u64 v) {
+    const uint32_t low = __builtin_amdgcn_update_dpp(0, int(uint32_t(v)), CTRL, ROWS, 0xf, false);
+    const uint32_t high = __builtin_amdgcn_update_dpp(0, int(uint32_t(v >> 32)), CTRL, ROWS, 0xf, false);
+    return u64(high) << 32 | low;
+}
+
+// Each lane's join of all lanes up to it; 0 changes nothing.
+template <typename Join>
+__device__ __forceinline__ u64 wave_scan(u64 v, Join join) {
+    v = join(v, from_lane<0x111, 0xf>(v));  // row_shr:1
+    v = join(v, from_lane<0x112, 0xf>(v));
+    v = join(v, from_lane<0x114, 0xf>(v));
+    v = join(v, from_lane<0x118, 0xf>(v));
+    v = join(v, from_lane<0x142, 0xa>(v));  // row_bcast:15
+    return join(v, from_lane<0x143, 0xc>(v));  // row_bcast:31
+}
+
+struct Add {
+    __device__ u64 operator()(u64 a, u64 b) const { return a + b; }
+};
+struct Max {
+    __device__ u64 operator()(u64 a, u64 b) const { return a > b ? a : b; }
+};
+
+// Of both values, the join over the workgroup.
+template <typename Join>
+__device__ __forceinline__ void block_all(u64 &a, u64 &b, u64 *room, Join join) {
+    a = wave_scan(a, join);
+    b = wave_scan(b, join);
     __syncthreads();
-    if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = v;
+    if (threadIdx.x % 64 == 63) room[threadIdx.x / 64] = a, room[kWaves + threadIdx.x / 64] = b;
     __syncthreads();
-    v = 0;
-    for (int w = 0; w < kWaves; ++w) v += room[w];
+    a = room[0], b = room[kWaves];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) a = join(a, room[w]), b = join(b, room[kWaves + w]);
+}
+
+__device__ __forceinline__ u64 block_sum(u64 v, u64 *room) {
+    u64 none = 0;
+    block_all(v, none, room, Add{});
     return v;
 }
 
-template <typename T>
-__device__ __forceinline__ T block_max(T v, T *room) {
-    for (int d = 1; d < 64; d *= 2) v = max(v, T(__shfl_xor(v, d)));
+// Of both values, the sums up to and with each thread's.
+__device__ __forceinline__ void block_scan(u64 &a, u64 &b, u64 *room) {
+    a = wave_scan(a, Add{});
+    b = wave_scan(b, Add{});
     __syncthreads();
-    if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = v;
+    if (threadIdx.x % 64 == 63) room[threadIdx.x / 64] = a, room[kWaves + threadIdx.x / 64] = b;
     __syncthreads();
-    for (int w = 0; w < kWaves; ++w) v = max(v, room[w]);
-    return v;
+    const int wave = threadIdx.x / 64;
+#pragma unroll
+    for (int w = 0; w < kWaves - 1; ++w) a += w < wave ? room[w] : 0, b += w < wave ? room[kWaves + w] : 0;
 }
 
-// The sums up to and with each thread's v.
-template <typename T>
-__device__ __forceinline__ T block_scan(T v, T *room) {
-    for (int d = 1; d < 64; d *= 2) {
-        const T before = __shfl_up(v, d);
-        if (int(threadIdx.x % 64) >= d) v += before;
-    }
-    __syncthreads();
-    if (threadIdx.x % 64 == 63) room[threadIdx.x / 64] = v;
-    __syncthreads();
-    for (int w = 0; w < int(threadIdx.x / 64); ++w) v += room[w];
+__device__ __forceinline__ u64 block_scan(u64 v, u64 *room) {
+    u64 none = 0;
+    block_scan(v, none, room);
     return v;
 }
 
@@ -189,17 +230,17 @@ struct Work {
 // A row's largest and smallest key from its slices'.
 __device__ __forceinline__ void extremes(const Work &w, uint32_t row, u64 &best, uint32_t &least, u64 *room) {
     best = 0;
-    uint32_t low = 0;  // upside down
+    u64 low = 0;  // upside down
     for (uint32_t i = threadIdx.x; i < w.slices; i += kThreads) {
         best = max(best, w.best[size_t(row) * w.slices + i]);
-        low = max(low, ~w.least[size_t(row) * w.slices + i]);
+        low = max(low, u64(~w.least[size_t(row) * w.slices + i]));
     }
-    best = block_max(best, room);
-    least = ~uint32_t(block_max(u64(low), room));
+    block_all(best, low, room, Max{});
+    least = ~uint32_t(low);
 }
 
 __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, Work w) {
-    __shared__ u64 room[kWaves];
+    __shared__ u64 room[2 * kWaves];
     const uint32_t row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
     const float *x = a.logits + size_t(row) * a.stride;
     for (uint32_t i = slice * kThreads + tid; i < kBins; i += w.slices * kThreads) {
@@ -207,21 +248,19 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, Work
         w.weight[size_t(row) * kBins + i] = 0;
     }
     if (slice == 0 && tid == 0) w.found[row] = 0;
-    u64 best = 0;
-    uint32_t low = 0;
+    u64 best = 0, low = 0;
     const uint32_t end = min((slice + 1) * w.slice, a.vocab);
 #pragma unroll 8
     for (uint32_t i = slice * w.slice + tid; i < end; i += kThreads) {
         const uint32_t key = key_of(x[i]);
         if (key == 0) continue;
         best = max(best, place_of(key, i));
-        low = max(low, ~key);
+        low = max(low, u64(~key));
     }
-    best = block_max(best, room);
-    low = uint32_t(block_max(u64(low), room));
+    block_all(best, low, room, Max{});
     if (tid == 0) {
         w.best[size_t(row) * w.slices + slice] = best;
-        w.least[size_t(row) * w.slices + slice] = ~low;
+        w.least[size_t(row) * w.slices + slice] = ~uint32_t(low);
     }
 }
 
@@ -236,17 +275,20 @@ struct Ahead {
 };
 
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Work w) {
-    __shared__ u64 room[kWaves], weight[kBins];
+    __shared__ u64 room[2 * kWaves], weight[kBins];
+    __shared__ double powers[kSteps];
     __shared__ uint32_t count[kBins];
     const uint32_t row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
     const float *x = a.logits + size_t(row) * a.stride;
     const uint32_t begin = slice * w.slice + tid, end = min((slice + 1) * w.slice, a.vocab);
     Ahead ahead;
     ahead.load(x, begin, end);  // on their way while the slices' largest is found
+    const Settings set(a, row);
+    fill_powers(powers);
     u64 best;
     uint32_t least;
     extremes(w, row, best, least, room);
-    const Weights of(a, row, key_at(best), least);
+    const Weights of(a, set, key_at(best), least, powers);
     if (best == 0 || of.greedy()) return;
     weight[tid] = 0;
     count[tid] = 0;
@@ -273,12 +315,12 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Wor
     }
 }
 
-__device__ Bounds bounds_of(const SampleArgs &a, const Work &w, uint32_t row, const Weights &of, u64 *room, u64 *found) {
-    const uint32_t tid = threadIdx.x, k = a.top_k[row];
-    const float p = a.top_p[row];
-    const uint32_t n = w.count[size_t(row) * kBins + tid];
-    const u64 sum = w.weight[size_t(row) * kBins + tid];
-    const u64 tokens = block_scan(u64(n), room), weight = block_scan(sum, room);
+// n, sum: tokens and weight of this thread's bin.
+__device__ Bounds bounds_of(const Settings &set, const Weights &of, uint32_t n, u64 sum, u64 *room, u64 *found) {
+    const uint32_t tid = threadIdx.x, k = set.top_k;
+    const float p = set.top_p;
+    u64 tokens = n, weight = sum;
+    block_scan(tokens, weight, room);
     Bounds b;
     if (tid < 4) found[tid] = kNone;
     __syncthreads();
@@ -340,21 +382,23 @@ __device__ Bounds bounds_of(const SampleArgs &a, const Work &w, uint32_t row, co
 
 __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a, Work w) {
     constexpr uint32_t kRoom = 2048;
-    __shared__ u64 room[kWaves], found[4], places[kRoom];
+    __shared__ u64 room[2 * kWaves], found[4], places[kRoom];
     __shared__ uint32_t here, first;
     const uint32_t row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
     const float *x = a.logits + size_t(row) * a.stride;
     const uint32_t begin = slice * w.slice + tid, end = min((slice + 1) * w.slice, a.vocab);
     Ahead ahead;
     ahead.load(x, begin, end);
-    const u64 own = w.of_slice[(size_t(row) * w.slices + slice) * kBins + tid];
+    const Settings set(a, row);
+    const u64 own = w.of_slice[(size_t(row) * w.slices + slice) * kBins + tid], sum = w.weight[size_t(row) * kBins + tid];
+    const uint32_t count = w.count[size_t(row) * kBins + tid];
     u64 best;
     uint32_t least;
     extremes(w, row, best, least, room);
-    const Weights of(a, row, key_at(best), least);
+    const Weights of(a, set, key_at(best), least, nullptr);  // bins alone
     if (best == 0 || of.greedy()) return;
     if (tid == 0) here = 0;
-    const Bounds b = bounds_of(a, w, row, of, room, found);
+    const Bounds b = bounds_of(set, of, count, sum, room, found);
     const u64 sure = block_sum(tid < b.first ? own : u64(0), room);
     if (tid == 0) w.sure[size_t(row) * w.slices + slice] = sure;
     if (slice == 0 && tid == 0) w.bounds[row] = b;
@@ -391,7 +435,7 @@ struct PickLds {
     u64 amounts[256];
     u64 some[256];       // a place of each bin
     uint32_t counts[256];
-    u64 room[kWaves];
+    u64 room[2 * kWaves];
     u64 found[4];
 };
 
@@ -407,8 +451,8 @@ __device__ u64 border_of(PickLds &lds, Each each, In in, Amount amount, Inside i
     each([&](u64 place) {
         if (in(place)) top = max(top, place), rest = max(rest, ~place);
     });
-    top = block_max(top, lds.room);
-    rest = ~block_max(rest, lds.room);
+    block_all(top, rest, lds.room, Max{});
+    rest = ~rest;
     if (top == 0) return 0;
     if (top == rest) return top;
     // The window's bits, and those above it.
@@ -446,7 +490,7 @@ __device__ u64 border_of(PickLds &lds, Each each, In in, Amount amount, Inside i
     }
 }
 
-// Draws from what tokens begin..end-1 keep: weight(i) of token i, 0 if it is not
+// Draws from what tokens begin..end-1 keep: weight(i), 0 if it is not
 // kept; `before` of the weight stands before them, and `target` falls into them.
 template <typename Weight>
 __device__ void draw(const SampleArgs &a, uint32_t row, PickLds &lds, uint32_t begin, uint32_t end, Weight weight, u64 before, u64 target,
@@ -491,26 +535,35 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a, Wor
     u64 *places = reinterpret_cast<u64 *>(dynamic);            // [kCandidates]
     u64 *of_slices = places + (whole ? a.vocab : kCandidates);  // [slices]
     __shared__ PickLds lds;
+    __shared__ double powers[kSteps];
     const uint32_t row = blockIdx.x, tid = threadIdx.x;
     const float *x = a.logits + size_t(row) * a.stride;
+    const Settings set(a, row);
+    Bounds b{};  // not there for rows that return below
+    uint32_t found = 0;
+    if (!whole) {
+        b = w.bounds[row];
+        found = w.found[row];
+    }
+    fill_powers(powers);
     u64 best = 0;
     uint32_t least = 0, n = 0;
     if (whole) {
         n = a.vocab;
-        uint32_t low = 0;
+        u64 low = 0;
         for (uint32_t i = tid; i < n; i += kThreads) {
             const uint32_t key = key_of(x[i]);
             const u64 place = key ? place_of(key, i) : 0;
             places[i] = place;
             best = max(best, place);
-            if (key) low = max(low, ~key);
+            if (key) low = max(low, u64(~key));
         }
-        best = block_max(best, lds.room);
-        least = ~uint32_t(block_max(u64(low), lds.room));
+        block_all(best, low, lds.room, Max{});
+        least = ~uint32_t(low);
     } else {
         extremes(w, row, best, least, lds.room);
     }
-    const Weights of(a, row, key_at(best), least);
+    const Weights of(a, set, key_at(best), least, powers);
     if (best == 0 || of.greedy()) {
         if (tid == 0) {
             a.tokens[row] = best ? index_at(best) : kNone;
@@ -518,11 +571,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a, Wor
         }
         return;
     }
-    Bounds b{};
-    if (!whole) {
-        b = w.bounds[row];
-        n = b.first < kBins ? w.found[row] : 0;
-    }
+    if (!whole) n = b.first < kBins ? found : 0;
     const bool listed = whole || n <= kCandidates;
     if (!whole && listed) {
         for (uint32_t i = tid; i < n; i += kThreads) places[i] = w.candidates[size_t(row) * kCandidates + i];
@@ -542,8 +591,8 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a, Wor
     const bool bins = listed && !whole;  // the places are those of some bins
 
     // Top k.
-    const uint32_t k = a.top_k[row];
-    const float p = a.top_p[row];
+    const uint32_t k = set.top_k;
+    const float p = set.top_p;
     u64 k_border = 0, kept_by_k = 0;
     if (bins ? b.k_bin != kNone : k > 0 && k < a.vocab) {
         const u64 rank = bins ? b.k_rank : k;
