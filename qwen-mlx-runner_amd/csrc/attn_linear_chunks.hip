@@ -13,11 +13,15 @@
 //
 // Three launches. linear_prepare_kernel has a workgroup a chunk and key head:
 // everything that does not depend on the state, all chunks at once, left in the
-// workspace as the operands that the matrix instructions take. linear_scan_kernel
+// workspace as the operands that the matrix instructions take (4100 tokens of 16
+// key and 48 value heads of 128: 51 us, 68 MB read and 122 MB written, 3.7 TB/s,
+// bound by memory and the splits' vector work alike). linear_scan_kernel
 // goes through a sequence's chunks: a workgroup has some 16-column tiles of a
 // value head's state, a wave one, in its accumulators; the next chunk's operands
-// come to LDS meanwhile. linear_norm_kernel norms the outputs, whose rows the
-// workgroups of a head share.
+// come to LDS meanwhile (bound by a chunk's chain of products and splits: 1.67 us
+// a chunk, 216 us for those tokens, of which 84 matrix instructions are a third).
+// linear_norm_kernel norms the outputs, whose rows the workgroups of a head share
+// (49 us for those: 302 MB at 6.2 TB/s, much of it from the last-level cache).
 //
 // Columns of the state do not meet until the output norm, so a wave needs
 // nothing of another one, and S, R and U need not leave its registers: a product
@@ -895,6 +899,10 @@ LinearPlan plan_linear(const LinearArgs &a, const DeviceLimits &lim, size_t limi
     pl.parts = uint32_t(std::min<uint64_t>(q.tokens, uint64_t(q.tokens) / kChunk + q.seqs));
     pl.k_bytes = size_t(8) * kTile * pl.blocks;
     pl.v_bytes = size_t(a.delta ? 9 : 5) * kTile;
+    // Four tiles a workgroup read a chunk's operands half as often, two are twice
+    // as many workgroups: as long as those have a CU each. 48 heads of 128 x 128,
+    // 512 tokens a sequence, two tiles / four in us: one sequence 59/61, two 96/74,
+    // four 144/125, 16 572/449; 64 heads of 64 x 64: 47/49, 54/56, 76/70, 280/265.
     if (columns == 0 && pl.blocks < 8)
         while (pl.columns < 4 && uint64_t(std::min(q.seqs, pl.parts)) * a.v_heads * ((tiles + pl.columns - 1) / pl.columns) >
                                      uint64_t(lim.num_cus))

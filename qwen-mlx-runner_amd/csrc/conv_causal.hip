@@ -7,7 +7,9 @@
 // width - 1 inputs that it had; the last ones of state and new tokens together
 // are its next state.
 //
-// Memory bounds it: every input is read once and every output written once.
+// Memory bounds it: every input is read once and every output written once
+// (10240 channels, 12000 tokens: 209 us, 4.7 TB/s, a large copy's rate; one token:
+// 3.9 us, a launch and two loads one after the other).
 // A thread has four channels of `span` successive tokens of one sequence and
 // keeps the window in registers, so that of its inputs only the width - 1
 // before its first are read again. Spans begin where their sequence begins
@@ -122,7 +124,10 @@ hipError_t launch_conv_causal(const ConvArgs &a, const DeviceLimits &lim, hipStr
     const Sequences &q = a.seq;
     const uint32_t v = a.channels % 4 == 0 ? 4 : 1;
     const uint32_t columns = (a.channels / v + kThreads - 1) / kThreads;
-    // The longest span of which there are still eight waves for every CU.
+    // The longest span of which there are still eight waves for every CU. With
+    // two and with 32 in place of eight, 10240 channels in us: 200 tokens 9.4 and
+    // 6.6 (6.6), 600 17.7 and 12.5 (13.4), 1400 23.3 and 23.0 (21.5), 6000 109 and
+    // 104 (108).
     uint32_t span = 32;
     while (span > 4 && uint64_t(q.tokens / span + 1) * columns < uint64_t(lim.num_cus) * 8) span /= 2;
     const uint32_t parts = uint32_t(std::min<uint64_t>(q.tokens, uint64_t(q.tokens) / span + q.seqs));

@@ -32,6 +32,11 @@
 // A row that fits sample_pick's LDS needs that launch alone. One that has too
 // many tokens in its bins (many equal logits) is worked on by sample_pick
 // alone, which reads it once a digit of the borders.
+//
+// One row of 248320 takes 4.4, 7.6, 7.1 and 11.9 us: launches, and each kernel's
+// chain of loads, scans and barriers. 48 rows take 14, 27, 23 and 29: reading them
+// (48 MB, 3.4 TB/s at first, then from the caches), the weights' 15 operations of
+// 64 bits and LDS sums in the second, a workgroup a row in the last.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -665,7 +670,9 @@ size_t row_bytes(uint32_t slices) {
 }  // namespace
 
 // Slices of at least 4096 logits, eight a thread, and more where there are rows
-// enough to fill the chip four times over.
+// enough to fill the chip four times over. A row of 248320 in slices of 2048 and
+// 1024 took 36 and 39 us where it took 35 (bins are added up across slices); 48
+// rows that may fill it twice and eight times 118 and 94 us for 94.
 SamplePlan plan_sample(const SampleArgs &a, const DeviceLimits &lim, size_t limit) {
     SamplePlan pl;
     pl.whole = a.vocab <= kCandidates;
