@@ -66,8 +66,8 @@ class Block:
         xb = self.gpu.upload_f32(x)
         cmd = self.gpu.begin()
         self._product(cmd, self.in_w, xb, self.rows, step.tokens)
-        layer.convolve(cmd, step, slots, self.rows, self.filter_buffer, self.filter_buffer, self.states, self.qkv, keep)
-        layer.attend(cmd, step, slots, self.rows, self.qkv, self.weights, self.states, self.heads_out, keep)
+        layer.convolve(cmd, step, slots, self.rows, self.filter_buffer, self.filter_buffer, self.states, self.qkv)
+        layer.attend(cmd, step, slots, self.rows, self.qkv, self.weights, self.states, self.heads_out)
         self._product(cmd, self.out_w, self.heads_out, self.y, step.tokens)
         for s, end in enumerate(step.starts[1:]):
             self._product(cmd, self.head, self.y, self.logits, 1, int(end) - 1, s)

@@ -305,7 +305,7 @@ int qmr_supported_bf16_quantization(uint32_t bits, size_t group);
  *     norm FP32 [dv], starts u32 [seqs+1], slots u32 [seqs], state FP32
  *     [pool][v heads][dk][dv], out; params seqs, tokens, k heads, v heads, dk,
  *     dv, strides of q, k, v, a, b, z and out, most, gates, delta, scale, qk eps
- *     and out eps as FP32 bits, pool, keep. With a stride of 0 (and gates = 0)
+ *     and out eps as FP32 bits, pool, keep. With a stride of 0
  *     all tokens have one row of a. b is read with delta = 1 alone, a_log and
  *     dt_bias with gates = 1. qk eps > 0 divides each query and key by
  *     sqrt(sum x^2 + eps) first; out eps > 0 makes an output
@@ -327,13 +327,14 @@ int qmr_supported_bf16_quantization(uint32_t bits, size_t group);
  *     are equal; w_i = e^((x_i - max) / temperature). Kept are the first top_k
  *     (0: all), of these the first whose weights reach top_p of those
  *     top_k's sum (1 and above: all; the first at least), of these the ones with
- *     w_i >= min_p. The token is the first, by index, at which the sum of
- *     kept weights passes uniform (0 to 1) times all of it, and probs its share
- *     of that sum. temperature 0 (or below, or not a number): the greatest, with
- *     probability 1. NaN and -inf are never kept; a row that has no more than
- *     those gives token 0xFFFFFFFF and probability 0. Of +inf each weighs the
- *     same and all else nothing. Weights add up as whole numbers, 2^-38 of the
- *     greatest or finer, so that a result depends on no order and calls repeat.
+ *     w_i >= min_p (the greatest always). The token is the first, by index, at
+ *     which the sum of kept weights passes uniform (0 to 1) times all of it, and
+ *     probs its share of that sum. temperature 0 (or below, or not a number): the
+ *     greatest, with probability 1. NaN and -inf are never kept; a row that has no
+ *     more than those gives token 0xFFFFFFFF and probability 0. Of +inf each
+ *     weighs the same and all else nothing. Weights add up as whole numbers, 2^-38
+ *     of the greatest or finer, so that a result depends on no order and calls
+ *     repeat.
  *   "matvec_affine_f16meta", "matmul_affine_f16meta", "embed_affine_f16meta"
  *     As the FP32-metadata names, with scales/biases stored as IEEE binary16
  *     (the dtype MLX checkpoints ship). The reference expands F16 metadata

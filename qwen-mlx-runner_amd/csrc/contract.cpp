@@ -258,6 +258,7 @@ Layout linear_layout(const std::string &name, const uint32_t *p, size_t np) {
         ensure(p[8] < 1u << 31, name + ": too many slots");
         const size_t span = (channels + 3) / 4;
         threads({tokens + seqs, span});
+        threads({tokens / 4 + seqs, 64});  // a wave for every four tokens begun of a sequence, at most
         ensure(span <= size_t(65535) * 16, name + ": too many channels");
         out.sizes = {rows(tokens, channels, p[4]), bytes({channels, width, 4}), p[7] ? bytes({channels, 4}) : 0, starts,
                      slots, bytes({p[8], width - 1, channels, 4}), rows(tokens, channels, p[5])};
@@ -279,7 +280,7 @@ Layout linear_layout(const std::string &name, const uint32_t *p, size_t np) {
     const bool gates = p[14] == 1, delta = p[15] == 1, normed = p[18] != 0;
     const size_t head = v_heads * 4;
     ensure(v_heads <= 65535 && k_heads <= 65535, name + ": too many heads");
-    threads({seqs, v_heads, 1024});
+    threads({seqs + 8, v_heads, 2048});  // of a state, at most; sequences' key heads are dealt to eight dies
     threads({tokens + seqs, v_heads, 32});
     out.sizes = {rows(tokens, kw, p[6]),
                  rows(tokens, kw, p[7]),

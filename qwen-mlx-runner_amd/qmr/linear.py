@@ -11,8 +11,8 @@ dispatches over a step; `Draws` holds what a row of logits is drawn with:
     draws.sample(cmd, logits, vocab, tokens, probs)
 
 A sequence has one state, of its last token: what a token did to it is not
-undone. Tokens that may be taken back (to verify) run with keep=False, and the
-accepted ones again with keep=True. include/qmr.h says what the operators
+undone. Tokens that may be taken back (to verify) go in a step with keep=False,
+and the accepted ones again in one with keep=True. include/qmr.h says what the operators
 compute.
 """
 from __future__ import annotations
@@ -32,9 +32,11 @@ NO_TOKEN = 0xFFFFFFFF
 @dataclass
 class Step:
     """New tokens of some sequences: tokens starts[s]..starts[s+1]-1 are those
-    of the sequence whose states are in slot words[s]."""
+    of the sequence whose states are in slot words[s], where what they make of
+    them is kept or not."""
     starts: np.ndarray
     words: np.ndarray
+    keep: bool = True
     buffers: tuple[Buffer, ...] = ()
 
     @property
@@ -81,14 +83,14 @@ class Slots:
 
     def step(self, new: Sequence[tuple[int, int]], keep: bool = True) -> Step:
         """`count` more tokens of each sequence (sequence, count). A sequence's
-        first tokens find zeros, whatever the slot's last owner left; keep=False
-        says that the step's dispatches will not keep what they make of them."""
+        first tokens find zeros, whatever the slot's last owner left. A step that
+        keeps is to be run by every layer, once."""
         if not new or len({seq for seq, _ in new}) != len(new) or any(count < 0 for _, count in new):
             raise ValueError("a step names each sequence once, with its number of tokens")
         words = [self._held[seq] | (FRESH if seq in self._fresh else 0) for seq, _ in new]
         if keep:
             self._fresh -= {seq for seq, count in new if count > 0}
-        return Step(np.cumsum([0, *(count for _, count in new)], dtype=np.uint32), np.array(words, np.uint32))
+        return Step(np.cumsum([0, *(count for _, count in new)], dtype=np.uint32), np.array(words, np.uint32), keep)
 
 
 class Weights(NamedTuple):
@@ -137,32 +139,33 @@ class Layer:
         return States(gpu.alloc_f32(slots.slots * (self.width - 1) * self.channels),
                       gpu.alloc_f32(slots.slots * self.v_heads * self.dk * self.dv))
 
-    def convolve_params(self, step: Step, slots: Slots, keep: bool = True) -> list[int]:
+    def convolve_params(self, step: Step, slots: Slots) -> list[int]:
         return [len(step.words), step.tokens, self.channels, self.width, self.row, self.channels, 1, int(self.bias),
-                slots.slots, int(keep)]
+                slots.slots, int(step.keep)]
 
     def convolve(self, cmd: Command, step: Step, slots: Slots, rows: Buffer, filters: Buffer, bias: Buffer,
-                 states: States, qkv: Buffer, keep: bool = True) -> None:
+                 states: States, qkv: Buffer) -> None:
         """qkv [tokens][channels] from the product's rows [tokens][row]; `bias`
         is read if the layer has one, and may be any buffer if not."""
         encode(cmd, "conv_causal", [rows, filters, bias, *step.buffers, states.inputs, qkv],
-               self.convolve_params(step, slots, keep))
+               self.convolve_params(step, slots))
 
-    def attend_params(self, step: Step, slots: Slots, keep: bool = True) -> list[int]:
+    def attend_params(self, step: Step, slots: Slots) -> list[int]:
         scale = self.dk ** -0.5 if self.scale is None else self.scale
         c, r = self.channels, self.row
         return [len(step.words), step.tokens, self.k_heads, self.v_heads, self.dk, self.dv, c, c, c, r, r, r, self.out_width,
-                step.most, 1, 1, f32_bits(scale), f32_bits(self.qk_eps), f32_bits(self.out_eps), slots.slots, int(keep)]
+                step.most, 1, 1, f32_bits(scale), f32_bits(self.qk_eps), f32_bits(self.out_eps), slots.slots,
+                int(step.keep)]
 
     def attend(self, cmd: Command, step: Step, slots: Slots, rows: Buffer, qkv: Buffer, weights: Weights,
-               states: States, out: Buffer, keep: bool = True) -> None:
+               states: States, out: Buffer) -> None:
         """out [tokens][v_heads * dv] from the convolution's rows and the product's."""
         k = 4 * self.k_heads * self.dk
         z = 4 * self.channels
         b = z + 4 * self.out_width
         encode(cmd, "attn_linear",
                [qkv, qkv, qkv, rows, rows, weights.a_log, weights.dt_bias, rows, weights.norm, *step.buffers, states.heads, out],
-               self.attend_params(step, slots, keep), [0, k, 2 * k, b + 4 * self.v_heads, b, 0, 0, z, 0, 0, 0, 0, 0])
+               self.attend_params(step, slots), [0, k, 2 * k, b + 4 * self.v_heads, b, 0, 0, z, 0, 0, 0, 0, 0])
 
 
 class Draws:

@@ -107,3 +107,21 @@ def test_static_entry(gpu):
     s = Sample(logits(12, 32001), *zip(*SETTINGS))
     a, b = s.run(gpu), s.run(gpu, static=True)
     assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("setting", [dict(k=50, p=0.9), dict(p=0.7), dict(min_p=0.02), dict(), dict(temperature=0.0)])
+def test_the_largest_vocabulary(gpu, setting):
+    """2^24 logits: weights are whole numbers of 2^-38 of the greatest, off by
+    half of one each."""
+    case = Sample(2 * np.random.default_rng(1).standard_normal((2, 1 << 24), np.float32), **{"temperature": 0.8, **setting})
+    tokens, probs = case.run(gpu)
+    for r, row in enumerate(case.logits):
+        kept, share = distribution(row, case.temperature[r], case.k[r], case.p[r], case.min_p[r])
+        # Off by 2^-39 each, of the greatest one's share; borders by as much.
+        slip = len(kept) * 2.0 ** -39 * share.max() + 2.0 ** -30
+        at = np.searchsorted(kept, tokens[r])
+        assert kept[at] == tokens[r]
+        up_to = np.cumsum(share)
+        assert up_to[at] - share[at] - slip <= case.u[r] <= up_to[at] + slip, r
+        # An FP32 number is off by up to 2^-24 of itself: 0.13468765 by 3.6e-9.
+        assert abs(probs[r] - share[at]) <= slip + 2.0 ** -24 * share[at]

@@ -58,7 +58,10 @@ def test_words_fit_the_layouts():
     assert layer.channels == 512 and layer.row == 512 + 384 + 12 and layer.out_width == 384
     sizes, _ = qmr.dispatch_layout("conv_causal", layer.convolve_params(step, slots))
     assert sizes == [4 * (10 * 908 + 512), 4 * 512 * 3, 4 * 512, 12, 8, 4 * 4 * 2 * 512, 4 * 11 * 512]
-    sizes, _ = qmr.dispatch_layout("attn_linear", layer.attend_params(step, slots, keep=False))
+    sizes, _ = qmr.dispatch_layout("attn_linear", layer.attend_params(step, slots))
     assert sizes[3:9] == [4 * (10 * 908 + 6)] * 2 + [24, 24, 4 * (10 * 908 + 384), 256]
     assert sizes[9:] == [12, 8, 4 * 4 * 6 * 32 * 64, 4 * 11 * 384]
-    assert layer.attend_params(step, slots, keep=False)[-1] == 0 and layer.attend_params(step, slots)[13] == 9
+    assert layer.attend_params(step, slots)[13] == 9
+    assert layer.attend_params(step, slots)[-1] == layer.convolve_params(step, slots)[-1] == 1
+    step = slots.step([(a, 3)], keep=False)
+    assert layer.attend_params(step, slots)[-1] == layer.convolve_params(step, slots)[-1] == 0

@@ -38,7 +38,7 @@ NAN, INF = f32_word(float("nan")), f32_word(float("inf"))
     (dict(width=1), "taps"), (dict(width=5), "taps"), (dict(xs=29), "stride"), (dict(ys=29), "stride"),
     (dict(silu=2), "switches"), (dict(bias=2), "switches"), (dict(keep=2), "switches"), (dict(pool=1 << 31), "slots"),
     (dict(channels=1 << 23, xs=1 << 23, ys=1 << 23), "channels"),
-    (dict(tokens=1 << 31, channels=64, xs=64, ys=64), "overflow")])
+    (dict(tokens=1 << 31, channels=64, xs=64, ys=64), "overflow"), (dict(seqs=1 << 27), "overflow")])
 def test_conv_refusals(change, match):
     with pytest.raises(qmr.QmrError, match=match):
         layout("conv_causal", **change)
@@ -53,7 +53,8 @@ def test_conv_refusals(change, match):
     (dict(delta=2), "switches"), (dict(keep=2), "switches"), (dict(scale=0), "scale"), (dict(scale=NAN), "scale"),
     (dict(scale=INF), "scale"), (dict(qk=NAN), "epsilons"), (dict(qk=0x80000000), "epsilons"), (dict(out=INF), "epsilons"),
     (dict(out=f32_word(-1.0)), "epsilons"), (dict(pool=1 << 31), "slots"), (dict(seqs=1 << 20), "overflow"),
-    (dict(tokens=1 << 26), "overflow")])
+    (dict(tokens=1 << 26), "overflow"), (dict(seqs=1 << 19), "overflow"),
+    (dict(hk=1, hv=65536, dk=8, dv=8, qs=8, ks=8, vs=1 << 19, sa=65536, sb=65536, sz=1 << 19, so=1 << 19), "too many heads")])
 def test_linear_refusals(change, match):
     with pytest.raises(qmr.QmrError, match=match):
         layout("attn_linear", **change)
