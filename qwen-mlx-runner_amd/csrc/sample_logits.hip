@@ -27,14 +27,15 @@
 //   sample_gather  from the row's bins, those that a border may fall into; the
 //                  tokens in them, and each slice's weight above them
 //   sample_pick    a workgroup a row: the borders among those tokens, the slice
-//                  that the number falls into, and the token there
+//                  that the number falls into, and the token there (one of
+//                  them, without a look at slices, if there are few)
 //
 // A row that fits sample_pick's LDS needs that launch alone. One that has too
 // many tokens in its bins (many equal logits) is worked on by sample_pick
 // alone, which reads it once a digit of the borders.
 //
-// One row of 248320 takes 4.4, 7.6, 7.1 and 11.9 us: launches, and each kernel's
-// chain of loads, scans and barriers. 48 rows take 14, 27, 23 and 29: reading them
+// One row of 248320 takes 4.4, 7.7, 6.6 and 5.5 us: launches, and each kernel's
+// chain of loads, scans and barriers. 48 rows take 14, 28, 23 and 30: reading them
 // (48 MB, 3.4 TB/s at first, then from the caches), the weights' 15 operations of
 // 64 bits and LDS sums in the second, a workgroup a row in the last.
 #include <hip/hip_runtime.h>
@@ -54,6 +55,7 @@ constexpr uint32_t kBins = kThreads;     // a thread a bin; the last: weights th
 constexpr uint32_t kPerNat = 16;         // bins of a temperature: 511 of them reach below 2^-45
 constexpr uint32_t kCandidates = 8192;   // of a row, at most
 constexpr uint32_t kSliceStep = 4096;
+constexpr uint32_t kFew = 64;            // candidates that a wave has in its lanes
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr int kSteps = 64;  // of an octave, in the table of powers
 
@@ -376,6 +378,12 @@ __device__ Bounds bounds_of(const Settings &set, const Weights &of, uint32_t n, 
         b.last = min(b.last, at + 1);
     }
     if (b.first == kNone) b.first = kBins;  // no border: all is kept
+    // Few tokens down to the last border: they are all candidates.
+    if (tid == 0) found[1] = kNone;
+    __syncthreads();
+    if (tid == b.last) found[1] = tokens;
+    __syncthreads();
+    if (found[1] <= kFew) b.first = 0;
     if (tid == 0) found[0] = 0;
     __syncthreads();
     if (b.first > 0 && tid == min(b.first, kBins) - 1) found[0] = weight;
@@ -495,6 +503,30 @@ __device__ u64 border_of(PickLds &lds, Each each, In in, Amount amount, Inside i
     }
 }
 
+__device__ __forceinline__ u64 target_of(const SampleArgs &a, uint32_t row, u64 total) {
+    const double u = fmin(fmax(double(a.uniform[row]), 0.0), 1.0);
+    return min(u64(u * double(total)), total - 1);
+}
+
+__device__ __forceinline__ u64 lane_of(u64 v, uint32_t l) {
+    return u64(__builtin_amdgcn_readlane(uint32_t(v >> 32), l)) << 32 | uint32_t(__builtin_amdgcn_readlane(uint32_t(v), l));
+}
+
+// border_of for places of a wave's first n lanes, `in` and amount theirs: each
+// lane adds up what stands before it.
+template <typename Inside>
+__device__ __forceinline__ u64 border_of_few(uint32_t n, u64 place, bool in, u64 amount, Inside inside, u64 above) {
+    const u64 own = in ? place : 0, weight = in ? amount : 0;
+    u64 before = above, top = 0;
+    for (uint32_t j = 0; j < n; ++j) {
+        const u64 other = lane_of(own, j);
+        before += other > place ? lane_of(weight, j) : 0;
+        top = max(top, other);
+    }
+    const u64 last = lane_of(wave_scan(in && inside(before) ? ~place : 0, Max{}), 63);
+    return last ? ~last : top;
+}
+
 // Draws from what tokens begin..end-1 keep: weight(i), 0 if it is not
 // kept; `before` of the weight stands before them, and `target` falls into them.
 template <typename Weight>
@@ -527,11 +559,6 @@ __device__ void draw(const SampleArgs &a, uint32_t row, PickLds &lds, uint32_t b
         if (before > target) return;
         __syncthreads();
     }
-}
-
-__device__ __forceinline__ u64 target_of(const SampleArgs &a, uint32_t row, u64 total) {
-    const double u = fmin(fmax(double(a.uniform[row]), 0.0), 1.0);
-    return min(u64(u * double(total)), total - 1);
 }
 
 // `whole`: rows that fit the candidates' LDS, with no launch before this one.
@@ -578,7 +605,11 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a, Wor
     }
     if (!whole) n = b.first < kBins ? found : 0;
     const bool listed = whole || n <= kCandidates;
-    if (!whole && listed) {
+    // Few candidates (top k, or a narrow row): every wave has them in its lanes,
+    // and no border takes a barrier. Three of a row of 248320, none above them: this
+    // launch takes 5.5 us, where it took 10.7.
+    const bool few = !whole && n <= kFew;
+    if (!whole && listed && !few) {
         for (uint32_t i = tid; i < n; i += kThreads) places[i] = w.candidates[size_t(row) * kCandidates + i];
     }
     __syncthreads();
@@ -595,19 +626,47 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a, Wor
     };
     const bool bins = listed && !whole;  // the places are those of some bins
 
-    // Top k.
     const uint32_t k = set.top_k;
     const float p = set.top_p;
-    u64 k_border = 0, kept_by_k = 0;
-    if (bins ? b.k_bin != kNone : k > 0 && k < a.vocab) {
+    u64 k_border = 0, p_border = 0, kept_by_k = 0, few_place = 0, few_weight = 0;
+    if (few) {
+        const uint32_t l = tid % 64;
+        const u64 place = l < n ? w.candidates[size_t(row) * kCandidates + l] : 0;
+        const uint32_t key = key_at(place), bin = place ? of.bin(key) : kNone;
+        const u64 amount = place ? of.whole(key) : 0;
+        if (b.k_bin != kNone) {
+            k_border = border_of_few(n, place, bin == b.k_bin, 1, [&](u64 before) { return before < b.k_rank; }, 0);
+            kept_by_k = lane_of(wave_scan(bin == b.k_bin && place >= k_border ? amount : 0, Add{}), 63);
+        }
+        if (p < 1.f) {
+            const double target = fmax(double(p), 0.0) * double(kept_by_k + b.above_k);
+            p_border = border_of_few(n, place, place >= k_border && bin <= b.last, amount,
+                                     [&](u64 before) { return double(before) < target; }, b.above);
+        }
+        const bool kept = place && place >= max(k_border, p_border) && bin >= b.first && bin <= b.last && of.likely(key);
+        few_place = place;
+        few_weight = kept ? amount : 0;
+        if (b.first == 0) {  // no other token is kept
+            const u64 total = lane_of(wave_scan(few_weight, Add{}), 63), target = target_of(a, row, total);
+            u64 before = 0;
+            for (uint32_t j = 0; j < n; ++j)
+                before += index_at(lane_of(few_place, j)) < index_at(place) ? lane_of(few_weight, j) : 0;
+            if (tid < 64 && kept && before <= target && before + few_weight > target) {
+                a.tokens[row] = index_at(place);
+                a.probs[row] = float(double(few_weight) / double(total));
+            }
+            return;
+        }
+    }
+    // Top k.
+    if (!few && (bins ? b.k_bin != kNone : k > 0 && k < a.vocab)) {
         const u64 rank = bins ? b.k_rank : k;
         k_border = border_of(
             lds, each, [&](u64 place) { return !bins || of.bin(key_at(place)) == b.k_bin; }, [](uint32_t) { return u64(1); },
             [&](u64 before) { return before < rank; }, 0);
     }
     // Top p, of what top k keeps.
-    u64 p_border = 0;
-    if (p < 1.f) {
+    if (!few && p < 1.f) {
         u64 sum = 0;
         if (!bins || b.k_bin != kNone)
             each([&](u64 place) {
@@ -636,10 +695,15 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a, Wor
     // The slice that the number falls into.
     for (uint32_t s = tid; s < w.slices; s += kThreads) of_slices[s] = w.sure[size_t(row) * w.slices + s];
     __syncthreads();
-    each([&](u64 place) {
-        const uint32_t key = key_at(place), bin = of.bin(key);
-        if (place >= border && bin >= b.first && bin <= b.last && of.likely(key)) atomicAdd(&of_slices[index_at(place) / w.slice], of.whole(key));
-    });
+    if (few) {
+        if (tid < 64 && few_weight) atomicAdd(&of_slices[index_at(few_place) / w.slice], few_weight);
+    } else {
+        each([&](u64 place) {
+            const uint32_t key = key_at(place), bin = of.bin(key);
+            if (place >= border && bin >= b.first && bin <= b.last && of.likely(key))
+                atomicAdd(&of_slices[index_at(place) / w.slice], of.whole(key));
+        });
+    }
     __syncthreads();
     u64 sum = 0;
     for (uint32_t s = tid; s < w.slices; s += kThreads) sum += of_slices[s];
@@ -671,7 +735,7 @@ size_t row_bytes(uint32_t slices) {
 
 // Slices of at least 4096 logits, eight a thread, and more where there are rows
 // enough to fill the chip four times over. A row of 248320 in slices of 2048 and
-// 1024 took 36 and 39 us where it took 35 (bins are added up across slices); 48
+// 1024 took 36 and 39 us where it took 35 (its bins are added up across slices); 48
 // rows that may fill it twice and eight times 118 and 94 us for 94.
 SamplePlan plan_sample(const SampleArgs &a, const DeviceLimits &lim, size_t limit) {
     SamplePlan pl;

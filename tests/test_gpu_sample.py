@@ -125,3 +125,18 @@ def test_the_largest_vocabulary(gpu, setting):
         assert up_to[at] - share[at] - slip <= case.u[r] <= up_to[at] + slip, r
         # An FP32 number is off by up to 2^-24 of itself: 0.13468765 by 3.6e-9.
         assert abs(probs[r] - share[at]) <= slip + 2.0 ** -24 * share[at]
+
+
+@pytest.mark.parametrize("live", [1, 2, 40, 63, 64, 65, 66, 130])
+@pytest.mark.parametrize("setting", [dict(k=1), dict(k=64), dict(k=65), dict(p=0.5), dict(p=0.999), dict(min_p=0.3), dict(),
+                                     dict(k=30, p=0.9, min_p=0.01)])
+def test_few_tokens_stand_out(gpu, live, setting):
+    """Some tokens above a floor that weighs next to nothing, many of them alike,
+    and numbers at both ends and between."""
+    rng = np.random.default_rng(live)
+    rows = rng.standard_normal((12, 20000)).astype(np.float32) - 60
+    for r, row in enumerate(rows):
+        at = rng.permutation(20000)[:live]
+        row[at] = rng.choice([0.0, 1.0, 1.5], live) if r % 2 else rng.uniform(-3, 3, live)
+    case = Sample(rows, **setting, u=[0, 1, 0.5, *rng.random(9)])
+    case.check(gpu)
