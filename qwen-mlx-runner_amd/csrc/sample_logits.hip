@@ -450,6 +450,7 @@ struct PickLds {
     uint32_t counts[256];
     u64 room[2 * kWaves];
     u64 found[4];
+    u64 inside[4], there[4];  // of the bins, a bit each
 };
 
 // The last place, from the first one down, before which `inside(sum)` holds,
@@ -475,7 +476,6 @@ __device__ u64 border_of(PickLds &lds, Each each, In in, Amount amount, Inside i
     for (;;) {
         __syncthreads();
         if (tid < 256) lds.amounts[tid] = 0, lds.some[tid] = 0, lds.counts[tid] = 0;
-        if (tid < 2) lds.found[tid] = 0;
         __syncthreads();
         each([&](u64 place) {
             if (!in(place) || place >> low >> width != prefix) return;
@@ -487,16 +487,22 @@ __device__ u64 border_of(PickLds &lds, Each each, In in, Amount amount, Inside i
         __syncthreads();
         const u64 sum = tid < 256 ? lds.amounts[tid] : 0, before = above + block_scan(sum, lds.room) - sum;
         // inside() holds up to some of the bins, of which the last is taken.
-        if (tid < 256 && lds.counts[tid] != 0) {
-            if (inside(before)) atomicMax(&lds.found[0], u64(tid) + 1);
-            atomicMax(&lds.found[1], 256 - u64(tid));
+        if (tid < 256) {
+            const bool there = lds.counts[tid] != 0;
+            const u64 all = __ballot(there), some = __ballot(there && inside(before));
+            if (tid % 64 == 0) lds.there[tid / 64] = all, lds.inside[tid / 64] = some;
+            lds.amounts[tid] = before;
         }
         __syncthreads();
-        const uint32_t at = lds.found[0] ? uint32_t(lds.found[0]) - 1 : 256 - uint32_t(lds.found[1]);
-        if (tid == at) lds.found[2] = before;
-        __syncthreads();
+        uint32_t at = 0;
+#pragma unroll
+        for (int w = 3; w >= 0; --w)
+            if (lds.there[w]) at = 64 * w + __ffsll(lds.there[w]) - 1;  // the first, if it holds for none
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            if (lds.inside[w]) at = 64 * w + 63 - __clzll(lds.inside[w]);
         if (lds.counts[at] == 1) return lds.some[at];
-        above = lds.found[2];
+        above = lds.amounts[at];
         prefix = prefix << width | (255 - at);
         width = min(8, low);
         low -= width;
