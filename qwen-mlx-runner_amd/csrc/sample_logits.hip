@@ -34,9 +34,9 @@
 // many tokens in its bins (many equal logits) is worked on by sample_pick
 // alone, which reads it once a digit of the borders.
 //
-// One row of 248320 takes 4.4, 7.7, 6.6 and 5.5 us: launches, and each kernel's
-// chain of loads, scans and barriers. 48 rows take 14, 28, 23 and 30: reading them
-// (48 MB, 3.4 TB/s at first, then from the caches), the weights' 15 operations of
+// One row of 248320 takes 3.6, 7.4, 7.0 and 5.6 us: launches, and each kernel's
+// chain of loads, scans and barriers. 48 rows take 13, 26, 22 and 25: reading them
+// (48 MB, 3.6 TB/s at first, then from the caches), the weights' 15 operations of
 // 64 bits and LDS sums in the second, a workgroup a row in the last.
 #include <hip/hip_runtime.h>
 
@@ -246,6 +246,35 @@ __device__ __forceinline__ void extremes(const Work &w, uint32_t row, u64 &best,
     least = ~uint32_t(low);
 }
 
+// Eight logits of a thread, two runs of four (which need not lie on more than 4
+// bytes) that are a workgroup's width apart; -infinity past the end. (By single
+// ones the three launches that read 48 rows took 14, 28 and 23 us, so 13, 26, 22.)
+constexpr uint32_t kAhead = 8;
+struct Four {
+    float x[4];
+};
+struct Ahead {
+    float x[kAhead];
+    static __device__ __forceinline__ uint32_t first() { return threadIdx.x * 4; }
+    static __device__ __forceinline__ uint32_t at(uint32_t i, uint32_t j) { return i + j / 4 * (4 * kThreads) + j % 4; }
+    __device__ __forceinline__ void load(const float *p, uint32_t i, uint32_t end) {
+#pragma unroll
+        for (uint32_t r = 0; r < kAhead; r += 4) {
+            const uint32_t k = at(i, r);
+            Four v{{-INFINITY, -INFINITY, -INFINITY, -INFINITY}};
+            if (k + 4 <= end) {
+                v = *reinterpret_cast<const Four *>(p + k);
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    if (k + j < end) v.x[j] = p[k + j];
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) x[r + j] = v.x[j];
+        }
+    }
+};
+
 __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, Work w) {
     __shared__ u64 room[2 * kWaves];
     const uint32_t row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
@@ -257,12 +286,19 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, Work
     if (slice == 0 && tid == 0) w.found[row] = 0;
     u64 best = 0, low = 0;
     const uint32_t end = min((slice + 1) * w.slice, a.vocab);
-#pragma unroll 8
-    for (uint32_t i = slice * w.slice + tid; i < end; i += kThreads) {
-        const uint32_t key = key_of(x[i]);
-        if (key == 0) continue;
-        best = max(best, place_of(key, i));
-        low = max(low, u64(~key));
+    Ahead ahead;
+    const uint32_t begin = slice * w.slice + Ahead::first();
+    ahead.load(x, begin, end);
+    for (uint32_t i = begin; i < end; i += kAhead * kThreads) {
+        const Ahead now = ahead;
+        ahead.load(x, i + kAhead * kThreads, end);
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            const uint32_t key = key_of(now.x[j]);
+            if (key == 0) continue;
+            best = max(best, place_of(key, Ahead::at(i, j)));
+            low = max(low, u64(~key));
+        }
     }
     block_all(best, low, room, Max{});
     if (tid == 0) {
@@ -271,23 +307,13 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a, Work
     }
 }
 
-// Eight logits of a thread, a workgroup's width apart; -infinity past the end.
-constexpr int kAhead = 8;
-struct Ahead {
-    float x[kAhead];
-    __device__ __forceinline__ void load(const float *p, uint32_t i, uint32_t end) {
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) x[j] = i + j * kThreads < end ? p[i + j * kThreads] : -INFINITY;
-    }
-};
-
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Work w) {
     __shared__ u64 room[2 * kWaves], weight[kBins];
     __shared__ double powers[kSteps];
     __shared__ uint32_t count[kBins];
     const uint32_t row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
     const float *x = a.logits + size_t(row) * a.stride;
-    const uint32_t begin = slice * w.slice + tid, end = min((slice + 1) * w.slice, a.vocab);
+    const uint32_t begin = slice * w.slice + Ahead::first(), end = min((slice + 1) * w.slice, a.vocab);
     Ahead ahead;
     ahead.load(x, begin, end);  // on their way while the slices' largest is found
     const Settings set(a, row);
@@ -304,7 +330,7 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Wor
         const Ahead now = ahead;
         ahead.load(x, i + kAhead * kThreads, end);
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
+        for (uint32_t j = 0; j < kAhead; ++j) {
             const uint32_t key = key_of(now.x[j]);
             const uint32_t bin = key ? of.bin(key) : kBins - 1;
             if (bin == kBins - 1) continue;
@@ -399,7 +425,7 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a, W
     __shared__ uint32_t here, first;
     const uint32_t row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
     const float *x = a.logits + size_t(row) * a.stride;
-    const uint32_t begin = slice * w.slice + tid, end = min((slice + 1) * w.slice, a.vocab);
+    const uint32_t begin = slice * w.slice + Ahead::first(), end = min((slice + 1) * w.slice, a.vocab);
     Ahead ahead;
     ahead.load(x, begin, end);
     const Settings set(a, row);
@@ -420,12 +446,12 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a, W
         const Ahead now = ahead;
         ahead.load(x, i + kAhead * kThreads, end);
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
+        for (uint32_t j = 0; j < kAhead; ++j) {
             const uint32_t key = key_of(now.x[j]);
             const uint32_t bin = key ? of.bin(key) : kBins - 1;
             if (bin == kBins - 1 || ((bin < b.first || bin > b.last) && bin != b.k_bin)) continue;
             const uint32_t at = atomicAdd(&here, 1u);
-            const u64 place = place_of(key, i + j * kThreads);
+            const u64 place = place_of(key, Ahead::at(i, j));
             if (at < kRoom) {
                 places[at] = place;
             } else {
@@ -613,7 +639,7 @@ __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs a, Wor
     const bool listed = whole || n <= kCandidates;
     // Few candidates (top k, or a narrow row): every wave has them in its lanes,
     // and no border takes a barrier. Three of a row of 248320, none above them: this
-    // launch takes 5.5 us, where it took 10.7.
+    // launch takes 5.6 us, where it took 10.7.
     const bool few = !whole && n <= kFew;
     if (!whole && listed && !few) {
         for (uint32_t i = tid; i < n; i += kThreads) places[i] = w.candidates[size_t(row) * kCandidates + i];
