@@ -35,7 +35,9 @@
 // terms, 2^-22 of it, is left out); sums are FP32. One FP32 matrix instruction
 // would take 5.3 times as long as those three. Rows of q and k are scaled by
 // powers of two to 2^3..2^4, a column of S, R and U to at most 2^15, so that the
-// terms stay among the normal f16 numbers as far as they matter.
+// terms stay among the normal f16 numbers as far as they matter: an element of R
+// and U is off by 2^-30 of the largest of its column and chunk where that is more
+// than its own 22 bits, and one of S by 2^-35 of its column's.
 //
 // The chunk's algebra has products of tokens with later ones, by zero: a value
 // that is not finite would reach tokens before it. A chunk that has some, or
@@ -584,7 +586,8 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
             for (int i = 0; i < 4; ++i) S[t][i] = ldexpf(S[t][i], to - scale);
         scale = to;
     };
-    auto fitting = [](float top) { return max(-113, min(15 - exponent(top), 110)); };
+    // A column of zeros has room for values of any size.
+    auto fitting = [](float top) { return top > 0.f ? max(-113, min(15 - exponent(top), 110)) : 0; };
     // A state that the last pass left is kept as it was there, its columns'
     // scales behind it: no result depends on where passes end.
     const size_t scale_at = size_t(a.v_heads) * a.dk * a.dv + size_t(h) * a.dv + col;
@@ -686,9 +689,11 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
 #pragma unroll
                 for (int e = 0; e < 8; ++e) r[e] = v[e] * (DELTA ? beta[e / 4][e % 4] * by : by);
             }
+            // Values that are not finite, or so far above the state that they leave the
+            // exponents that `up` can take back (2^116).
             float odd = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) odd = fmaf(v[e], 0.f, odd);
+            for (int e = 0; e < 8; ++e) odd = fmaf(r[e] * 0x1p12f, 0.f, odd);
             float top = biggest();
             if constexpr (DELTA) in_turn<6 * KB, 2, 1>();
             __builtin_amdgcn_sched_barrier(0);

@@ -111,11 +111,13 @@ class Linear:
         assert (after[:shift] == PAD).all()
         return out.read(), after[shift:].reshape(self.state.shape)
 
-    def want(self, roundings):
+    def want(self, roundings, floor=0.0):
         """(out, its bound, states, their bound) in 64 bits. Of a column of the
         state the error's length grows by `roundings` of what a token leaves
         there, and shrinks by its decay: the step is a contraction, since keys
-        are at most 1 long and beta below 1."""
+        are at most 1 long and beta below 1. A token's part may also be off by
+        `floor` of the largest value of its column among the 32 tokens (from the
+        sequence's first on) that it is one of."""
         hk, hv, dk, dv = self.k_heads, self.v_heads, self.dk, self.dv
         d = np.float64
         out = np.full((self.tokens, hv * dv), PAD)
@@ -144,7 +146,9 @@ class Linear:
                 u = beta * (v - np.einsum("hij,hi->hj", S, k)) if self.delta else v
                 S = S + k[:, :, None] * u[:, None, :]
                 length = np.linalg.norm(k, axis=-1)[:, None]
-                E = decay[:, 0] * E + roundings * ULP * (size + length * (np.abs(u) + np.abs(v))) + 2 * slip * size
+                at = first + (t - first) // 32 * 32
+                largest = np.abs(self.v[at:min(at + 32, first + n)]).max(0).reshape(hv, dv).astype(d)
+                E = decay[:, 0] * E + floor * length * largest + roundings * ULP * (size + length * (np.abs(u) + np.abs(v))) + 2 * slip * size
                 o = np.einsum("hij,hi->hj", S, q)
                 off = np.linalg.norm(q, axis=-1)[:, None] * (E + roundings * ULP * np.linalg.norm(S, axis=1))
                 if self.out_eps:

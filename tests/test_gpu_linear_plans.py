@@ -216,3 +216,26 @@ def test_attention_and_draws_share_a_workspace(gpu):
                 assert np.array_equal(tokens, drawn[0]) and np.array_equal(probs, drawn[1])
     finally:
         other.close()
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("sizes", [(1e8, 1e8, 1e8), (1e20, 1.0, 1e-20), (1e-30, 1e10, 1e-30), (1.0, 1e36, 1.0),
+                                   (0.0, 1e3, 1e-3), (1e-38, 0.0, 1e30)])
+def test_values_far_larger_than_the_state(gpu, planned, sizes, delta):
+    """From a state of zeros, values whose size changes from chunk to chunk and
+    within one."""
+    case = Linear([110, 40], 1, 2, 32, 32, out_eps=0.0, delta=delta)
+    case.state[:] = 0
+    for i, size in enumerate(sizes):
+        case.v[37 * i:37 * (i + 1)] *= np.float32(size)
+        case.v[110 + 13 * i:110 + 13 * (i + 1)] *= np.float32(size)
+    for plan in (200, 100):
+        planned(-8, plan)
+        got, after = case.run(gpu)
+        # R and U are two f16 terms, scaled to a largest of 2^5 to 2^6 in a column and
+        # chunk: the second is off by 2^-25, so 2^-30 of that largest. Twice, over rows
+        # of T at most 8 long.
+        want, bound, states, state_bound = case.want(CHUNKS, 2.0 ** -30 * 2 * 8 if plan == 200 else 0.0)
+        # Numbers below FP32's normal ones are off by its least step in each term.
+        assert (np.abs(got - want) <= bound + 1e-36).all(), plan
+        assert (np.abs(after - states) <= state_bound + 1e-36).all(), plan
