@@ -37,7 +37,7 @@
 // powers of two to 2^3..2^4, a column of S, R and U to at most 2^15, so that the
 // terms stay among the normal f16 numbers as far as they matter: an element of R
 // and U is off by 2^-30 of the largest of its column and chunk where that is more
-// than its own 22 bits, and one of S by 2^-35 of its column's.
+// than its own 22 bits, and one of S by 2^-30 of its column's.
 //
 // The chunk's algebra has products of tokens with later ones, by zero: a value
 // that is not finite would reach tokens before it. A chunk that has some, or
