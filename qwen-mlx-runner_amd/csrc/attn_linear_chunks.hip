@@ -170,22 +170,24 @@ template <int KB>
 struct PrepareLds {
     static constexpr uint32_t kPitch = 36;                      // floats of a row of 32
     static constexpr uint32_t kSquare = 32 * kPitch * 4;
-    static constexpr uint32_t kGram = 0;                        // q k, k k
-    static constexpr uint32_t kRows = 2 * kSquare;              // [4][32] FP32 of rows
-    static constexpr uint32_t kRest = kRows + 4 * 32 * 4;       // terms of q and k, then each wave's own
+    static constexpr uint32_t kRows = 0;                        // [4][32] FP32 of rows
+    static constexpr uint32_t kRest = kRows + 4 * 32 * 4;       // terms of q and k, then what follows
     static constexpr uint32_t kTerms = 4 * kTile * KB;          // of q, or of k
-    static constexpr uint32_t kA = 0, kT = kSquare, kG = 2 * kSquare, kWave = kG + 32 * 8 + 32 * 4;
-    static constexpr uint32_t kBytes = kRest + (2 * kTerms > 4 * kWave ? 2 * kTerms : 4 * kWave);
+    static constexpr uint32_t kGram = kRest;                    // q k, k k
+    static constexpr uint32_t kWaves = kGram + 2 * kSquare;     // each wave's own
+    static constexpr uint32_t kG = kSquare, kWave = kG + 32 * 8 + 32 * 4;
+    static constexpr uint32_t kEnd = kWaves + 4 * kWave;
+    static constexpr uint32_t kBytes = kRest + 2 * kTerms > kEnd ? kRest + 2 * kTerms : kEnd;
 };
 
 __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-// T = (I + A)^-1 for A [32][pitch] below its diagonal, a wave's: two blocks of
+// T = (I + A)^-1 in the place of A [32][pitch], a wave's: two blocks of
 // 16 on the diagonal, a lane a column, then T21 = -T22 (A21 T11) in FP32
 // matrix instructions. (A lane a column of all 32 takes 496 products in place
 // of 120, and each row waits for the one before it.)
 template <uint32_t PITCH>
-__device__ __forceinline__ void invert(const float *A, float *T) {
+__device__ __forceinline__ void invert(float *A) {
     const uint32_t l = threadIdx.x % 64, g = l / 16, m = l % 16, at = l / 16 % 2 * 16;
     float x[16];
 #pragma unroll
@@ -199,6 +201,7 @@ __device__ __forceinline__ void invert(const float *A, float *T) {
         }
         x[i] = even + odd;
     }
+    float *T = A;
     if (l < 32) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) T[(at + i) * PITCH + at + m] = x[i];
@@ -292,9 +295,9 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
     __syncthreads();
 
     // Products of rows: tiles (0, 0), (1, 0), (1, 1).
+    const uint32_t rt = w > 0, ct = w == 2;
+    f4 qk{}, kk{};
     if (w < 3) {
-        const uint32_t rt = w > 0, ct = w == 2;
-        f4 qk{}, kk{};
         auto term = [&](uint32_t r, uint32_t tile, uint32_t kb, uint32_t hl) {
             return *reinterpret_cast<const u4 *>(rest + r * L::kTerms + ((tile * KB + kb) * 2 + hl) * kTile + l * 16);
         };
@@ -304,6 +307,9 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
             qk = mfma3(term(0, rt, kb, 0), term(0, rt, kb, 1), bh, bl, qk);
             if constexpr (DELTA) kk = mfma3(term(1, rt, kb, 0), term(1, rt, kb, 1), bh, bl, kk);
         }
+    }
+    __syncthreads();  // the terms give way to the products
+    if (w < 3) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             gram[(rt * 16 + 4 * g + i) * L::kPitch + ct * 16 + m] = qk[i];
@@ -314,8 +320,8 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
 
     // A wave a value head of this key head. Lanes have a token each (twice), and
     // then of rows m and 16 + m the columns 4g.. and 16 + 4g.., as operands do.
-    unsigned char *own = rest + w * L::kWave;
-    float *A = reinterpret_cast<float *>(own + L::kA), *T = reinterpret_cast<float *>(own + L::kT);
+    unsigned char *own = lds + L::kWaves + w * L::kWave;
+    float *A = reinterpret_cast<float *>(own);  // then T
     double *Gs = reinterpret_cast<double *>(own + L::kG);
     float *by_row = reinterpret_cast<float *>(own + L::kG + 32 * 8);
     const uint32_t group = a.v_heads / a.k_heads, j = l % 32;
@@ -380,7 +386,7 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
         float rows_of_t = 1.f;
         if constexpr (DELTA) {
             wave_lds_sync();
-            invert<L::kPitch>(A, T);
+            invert<L::kPitch>(A);
             rows_of_t = 0.f;
 #pragma unroll
             for (uint32_t half = 0; half < 2; ++half) {
@@ -388,7 +394,7 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
                 float x[8], sum = 0.f;
 #pragma unroll
                 for (uint32_t c = 0; c < 2; ++c) {
-                    const f4 t = c <= half ? *reinterpret_cast<const f4 *>(T + i * L::kPitch + 16 * c + 4 * g) : f4{};
+                    const f4 t = c <= half ? *reinterpret_cast<const f4 *>(A + i * L::kPitch + 16 * c + 4 * g) : f4{};
 #pragma unroll
                     for (uint32_t q = 0; q < 4; ++q) {
                         bad |= !(fabsf(t[q]) < 2.f);
