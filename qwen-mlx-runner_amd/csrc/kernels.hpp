@@ -372,7 +372,7 @@ struct LinearPlan {
     size_t workspace = 0;
 };
 // `form` (tuning hook): 1 token after token, 2 chunks where they are possible, 0
-// the planner's choice; `columns` 2, 4 or 8, or 0.
+// the planner's choice; `columns` 2 or 4, or 0.
 LinearPlan plan_linear(const LinearArgs &a, const DeviceLimits &lim, size_t workspace_limit, uint32_t form = 0,
                        uint32_t columns = 0);
 hipError_t launch_attn_linear(const LinearArgs &a, const LinearPlan &pl, void *workspace, hipStream_t stream);

@@ -140,3 +140,14 @@ def test_few_tokens_stand_out(gpu, live, setting):
         row[at] = rng.choice([0.0, 1.0, 1.5], live) if r % 2 else rng.uniform(-3, 3, live)
     case = Sample(rows, **setting, u=[0, 1, 0.5, *rng.random(9)])
     case.check(gpu)
+
+
+def test_more_rows_than_the_workspace_holds(gpu):
+    """Rows of 9000 take 84 KB each: 900 go in two turns, through the scratch in
+    ten."""
+    rng = np.random.default_rng(8)
+    case = Sample(2 * rng.standard_normal((900, 9000)), rng.choice([0.0, 0.7, 1.2], 900), k=rng.choice([0, 1, 40], 900),
+                  p=rng.choice([0.5, 0.9, 1.0], 900), min_p=rng.choice([0.0, 0.1], 900))
+    tokens, probs = case.check(gpu)
+    got, shares = case.run(gpu, static=True)
+    assert np.array_equal(tokens, got) and np.array_equal(probs, shares)
