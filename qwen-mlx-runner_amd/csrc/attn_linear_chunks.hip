@@ -767,9 +767,11 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
                 for (int t = 0; t < TD; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) S[t][i] *= keep;
-                const float by = ldexpf(1.f, to - scale - up - (DELTA ? kSolve : 0));
-                of_u[0] *= by;
-                of_u[1] *= by;
+                // Each by itself: where keys are zero and the state has shrunk, the
+                // power of two alone may be past FP32's.
+                const int by = to - scale - up - (DELTA ? kSolve : 0);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) of_u[e / 4][e % 4] = ldexpf(of_u[e / 4][e % 4], by);
             }
             if constexpr (DELTA) in_turn<6, 6, 1>();
             __builtin_amdgcn_sched_barrier(0);

@@ -1,0 +1,49 @@
+"""attn_linear's chunks where sizes within one differ by many powers of two."""
+import numpy as np
+import pytest
+
+from linear_cases import Linear
+
+pytestmark = pytest.mark.gpu
+
+# Roundings of one token at dk = 32, relative to the lengths of what they act
+# on. A product of two-term operands is off by 6 (2^-23 each, and as much for the
+# product left out) and adds up as many terms as its depth. S^T q, S^T k and M
+# have dk of them, T R and M U 32, T's own rows 32 twice, gates and norms 40:
+# 3 (6 + 32) + 2 (6 + 32) + 64 + 40.
+ROUNDINGS = 294
+# What is below FP32's normal numbers is off by its least step in each term.
+LEAST = 1e-36
+
+
+def plain(counts, delta, dv=32, **how):
+    """A case without norms, of keys at most about 1 long."""
+    return Linear(counts, 1, 2, 32, dv, gates=False, delta=delta, qk_eps=0.0, out_eps=0.0, **how)
+
+
+def right(got, want, bound):
+    assert np.isfinite(got).all()
+    off = np.abs(got.astype(np.float64) - want)
+    assert (off <= bound + LEAST).all(), float((off / (bound + LEAST)).max())
+
+
+def check(gpu, case):
+    out, after = case.run(gpu)
+    want, bound, states, state_bound = case.want(ROUNDINGS)
+    right(out, want, bound)
+    right(after, states, state_bound)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("size", [1e8, 1e10, 1e20])
+@pytest.mark.parametrize("counts", [[32], [64], [20, 33]])
+def test_large_values_of_zero_keys_beside_a_state_that_decays(gpu, delta, size, counts):
+    """Keys of zero take nothing on, whatever their values: the state is what
+    its decays leave, e^-70 of it."""
+    case = plain(counts, delta)
+    for first, n in zip(case.starts, counts):
+        rows = slice(int(first), int(first) + min(n, 32))
+        case.k[rows] = 0
+        case.v[rows] *= np.float32(size)
+        case.a[rows] = -70.0 / min(n, 32)
+    check(gpu, case)
