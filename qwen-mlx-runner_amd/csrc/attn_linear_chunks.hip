@@ -730,7 +730,10 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
             for (int e = 0; e < 8; ++e) r_top = fmaxf(r_top, fabsf(r[e]));
             r_top = column_max(r_top);
             const int up = max(-113, min((DELTA ? 5 : 13) - exponent(r_top), 110));
-            int to = min(scale + 15 - exponent(fmaf(most, r_top, whole * top)), scale + 100);
+            // In 64 bits: the product of long keys' part and large values may be past
+            // FP32's range where the sum they bound is not.
+            const double next = fma(double(most), double(r_top), double(whole) * double(top));
+            int to = min(scale + 15 - __builtin_amdgcn_frexp_exp(next), scale + 100);
             to = max(-113, min(to, 110));
             u4 uh, ul;
             {

@@ -47,3 +47,19 @@ def test_large_values_of_zero_keys_beside_a_state_that_decays(gpu, delta, size, 
         case.v[rows] *= np.float32(size)
         case.a[rows] = -70.0 / min(n, 32)
     check(gpu, case)
+
+
+@pytest.mark.parametrize("size", [200.0, 5000.0, 1e9, 1e18])
+@pytest.mark.parametrize("zeros", [0, 256, 300])
+def test_long_keys_behind_values_of_zero(gpu, size, zeros):
+    """Columns whose values and states are zero for some chunks, then of size 1
+    to 60, along keys that are long: sums stay far from FP32's largest number."""
+    case = plain([400], False)
+    rng = np.random.default_rng(zeros)
+    case.k *= np.float32(size)
+    case.v[:] = rng.choice([-1, 1], case.v.shape) * rng.uniform(1, 60, case.v.shape)
+    case.v[:zeros, ::2] = 0
+    case.state[..., ::2] = 0
+    if size == 1e18:
+        case.v *= np.float32(1e16)
+    check(gpu, case)
