@@ -733,7 +733,7 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
             // In 64 bits: the product of long keys' part and large values may be past
             // FP32's range where the sum they bound is not.
             const double next = fma(double(most), double(r_top), double(whole) * double(top));
-            int to = min(scale + 15 - __builtin_amdgcn_frexp_exp(next), scale + 100);
+            int to = next > 0.0 ? min(scale + 15 - __builtin_amdgcn_frexp_exp(next), scale + 100) : 0;  // as fitting()
             to = max(-113, min(to, 110));
             u4 uh, ul;
             {

@@ -63,3 +63,21 @@ def test_long_keys_behind_values_of_zero(gpu, size, zeros):
     if size == 1e18:
         case.v *= np.float32(1e16)
     check(gpu, case)
+
+
+def test_columns_of_zeros_keep_their_room(gpu):
+    """Nine chunks of values of zero, from a state of zeros, leave a column as it
+    was: what follows has the bits that it has alone."""
+    for delta in (True, False):
+        both = plain([288 + 70], delta, slots=[0], pool=1)
+        both.state[:] = 0
+        both.v[:288] = 0
+        both.v[288:] *= np.float32(1000)
+        alone = plain([70], delta, slots=[0], pool=1)
+        for name in ("q", "k", "v", "a", "b", "z"):
+            setattr(alone, name, getattr(both, name)[288:])
+        alone.state = both.state
+        out, after = both.run(gpu)
+        want, state = alone.run(gpu)
+        assert np.array_equal(out[288:], want) and np.array_equal(after, state)
+        assert not out[:288].any()
