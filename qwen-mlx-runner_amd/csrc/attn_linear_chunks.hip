@@ -592,13 +592,21 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
             for (int i = 0; i < 4; ++i) S[t][i] = ldexpf(S[t][i], to - scale);
         scale = to;
     };
-    // A column of zeros has room for values of any size.
-    auto fitting = [](float top) { return top > 0.f ? max(-113, min(15 - exponent(top), 110)) : 0; };
+    // A column of zeros has room for values of any size; one with an infinity is
+    // kept as it is.
+    auto fitting = [](float top) { return top > 0.f && top < INFINITY ? max(-113, min(15 - exponent(top), 110)) : 0; };
     // A state that the last pass left is kept as it was there, its columns'
     // scales behind it: no result depends on where passes end.
     const size_t scale_at = size_t(a.v_heads) * a.dk * a.dv + size_t(h) * a.dv + col;
     if (!starts && has) scale = __float_as_int(pass.from[scale_at]);
-    rescale(starts ? fitting(biggest()) : scale);
+    // An infinity fits no scale: with one in its state a wave goes token after token.
+    uint32_t infinite;  // whether there is one
+    auto fit = [&](bool anew) {
+        const float top = biggest();
+        infinite = __ballot(top == INFINITY) != 0;
+        rescale(anew ? fitting(top) : scale);
+    };
+    fit(starts);
 
     uint32_t c = c0;
     if (idle) {
@@ -700,12 +708,12 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
             float odd = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) odd = fmaf(r[e] * 0x1p12f, 0.f, odd);
-            float top = biggest();
+            const float top = biggest();
             if constexpr (DELTA) in_turn<6 * KB, 2, 1>();
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int half = 0; half < 2; ++half) x[half] = PAR > 1 ? x2[half][0] + x2[half][PAR - 1] : x2[half][0];
-            slow = __builtin_amdgcn_readfirstlane(wild) != 0 || __ballot(odd != 0.f) != 0;
+            slow = (__builtin_amdgcn_readfirstlane(wild) | infinite) != 0 || __ballot(odd != 0.f) != 0;
             if (slow) break;
             // S^T q; meanwhile R and its terms, by 2^up more; the next state's scale:
             // below 2^15 whatever the chunk adds.
@@ -809,7 +817,7 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
         const uint32_t t0 = (c - begin) * kChunk;
         rescale(0);
         tokens_of_chunk<TD>(a, size_t(first) + t0, min(kChunk, count - t0), h, col, S);
-        rescale(fitting(biggest()));
+        fit(true);
         ++c;
     }
     if (idle || (ends ? !a.keep || slot == seq::kNoSlot : pass.to == nullptr)) return;

@@ -81,3 +81,21 @@ def test_columns_of_zeros_keep_their_room(gpu):
         want, state = alone.run(gpu)
         assert np.array_equal(out[288:], want) and np.array_equal(after, state)
         assert not out[:288].any()
+
+
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("counts", [[1], [40], [300]])
+def test_an_element_of_a_state_that_is_not_finite_stays_alone(gpu, value, counts):
+    """Without the delta rule no element of a state meets another: outputs of its
+    column are not finite, the rest of it is what it would be."""
+    case = plain(counts, False, slots=[0], pool=1)
+    want, bound, states, state_bound = case.want(ROUNDINGS)
+    case.state[0, 1, 3, 5] = value
+    out, after = case.run(gpu)
+    other = np.ones(out.shape[1], bool)
+    other[32 + 5] = False
+    right(out[:, other], want[:, other], bound[:, other])
+    assert not np.isfinite(out[:, 32 + 5]).any()
+    assert not np.isfinite(after[0, 1, 3, 5])
+    after[0, 1, 3, 5] = states[0, 1, 3, 5]
+    right(after, states, state_bound)
