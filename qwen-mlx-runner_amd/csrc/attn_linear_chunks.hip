@@ -37,7 +37,8 @@
 // powers of two to 2^3..2^4, a column of S, R and U to at most 2^15, so that the
 // terms stay among the normal f16 numbers as far as they matter: an element of R
 // and U is off by 2^-30 of the largest of its column and chunk where that is more
-// than its own 22 bits, and one of S by 2^-30 of its column's.
+// than its own 22 bits, one of S by 2^-30 of its column's, and one of M by 2^-29
+// of scale |q_i| |k|, k the longest key up to i as far as it is not yet forgotten.
 //
 // The chunk's algebra has products of tokens with later ones, by zero: a value
 // that is not finite would reach tokens before it. A chunk that has some, or
@@ -77,7 +78,7 @@ constexpr uint32_t kChunk = 32;
 constexpr uint32_t kTile = 1024;         // bytes of one f16 operand of 16 x 32
 constexpr uint32_t kOut = 0x80000000u;   // buffer offset past every range
 constexpr float kForget = -1000.f;       // e^-1000 is 0 in FP32 whatever it meets
-constexpr int kScore = 2;                // M's entries are products of scaled rows by 2^-kScore
+constexpr int kScore = 2;                // M's entries are products of scaled rows by 2^-kScore, and a row's own power
 constexpr int kSolve = 4;                // T's entries are by 2^kSolve
 
 // A chunk's operands. Of a key head: Q [2 tiles of 16 tokens][blocks][2 terms],
@@ -175,7 +176,7 @@ struct PrepareLds {
     static constexpr uint32_t kTerms = 4 * kTile * KB;          // of q, or of k
     static constexpr uint32_t kGram = kRest;                    // q k, k k
     static constexpr uint32_t kWaves = kGram + 2 * kSquare;     // each wave's own
-    static constexpr uint32_t kG = kSquare, kWave = kG + 32 * 8 + 32 * 4;
+    static constexpr uint32_t kG = kSquare, kWave = kG + 32 * 8 + 2 * 32 * 4;
     static constexpr uint32_t kEnd = kWaves + 4 * kWave;
     static constexpr uint32_t kBytes = kRest + 2 * kTerms > kEnd ? kRest + 2 * kTerms : kEnd;
 };
@@ -324,13 +325,18 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
     float *A = reinterpret_cast<float *>(own);  // then T
     double *Gs = reinterpret_cast<double *>(own + L::kG);
     float *by_row = reinterpret_cast<float *>(own + L::kG + 32 * 8);
+    int *long_row = reinterpret_cast<int *>(by_row + 32);
     const uint32_t group = a.v_heads / a.k_heads, j = l % 32;
     const float ck = rows[j], cq = rows[32 + j];
     const bool bad_rows = rows[64 + j] + rows[96 + j] > 0.f;
-    float top = ck;
+    // Up to its token, a row's longest key as an exponent.
+    const float length = ck > 0.f ? float(exponent(ck)) : -INFINITY;
+    float longest = length;
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    const float of_top = top > 0.f ? 1.f / top : 0.f;
+    for (int d = 1; d < 32; d *= 2) {
+        const float before = __shfl_up(longest, d, 32);
+        if (j >= uint32_t(d)) longest = fmaxf(longest, before);
+    }
     f4 cks[2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) cks[half] = *reinterpret_cast<const f4 *>(rows + 16 * half + 4 * g);
@@ -347,8 +353,20 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
             if (j >= uint32_t(d)) G += before;
         }
         const double all = __shfl(G, 31, 32);
+        // M's rows are by 2^-p: no key up to theirs, decayed as far as they see it,
+        // is longer than 2^p. A later key has no part in it, nor one that is forgotten,
+        // down to 2^-96 of the longest (where e^(G_i - G_j) leaves FP32's normal numbers).
+        const float nats = float(G) * 1.4426950408889634f;
+        float seen = length - nats;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const float before = __shfl_up(seen, d, 32);
+            if (j >= uint32_t(d)) seen = fmaxf(seen, before);
+        }
+        const int p = longest > -INFINITY ? int(fmaxf(ceilf(seen + nats), longest - 96.f)) : 0;
         Gs[j] = G;
         by_row[j] = beta * ck;
+        long_row[j] = p;
         wave_lds_sync();
         unsigned char *to = pass.of_value(a, chunk, h);
         bool bad = bad_rows;
@@ -357,6 +375,7 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
             const uint32_t i = 16 * half + m;
             const double Gi = Gs[i];
             const float of_row = by_row[i];
+            const int p_row = long_row[i];
             float M[8];
 #pragma unroll
             for (uint32_t c = 0; c < 2; ++c) {  // columns
@@ -371,7 +390,7 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
 #pragma unroll
                     for (uint32_t q = 0; q < 4; ++q) {
                         const float e = i >= j0 + q ? expf(float(Gi - Gs[j0 + q])) : 0.f;
-                        M[4 * c + q] = i >= j0 + q ? ldexpf(qk[q], -kScore) * (cks[c][q] * of_top) * e : 0.f;
+                        M[4 * c + q] = i >= j0 + q ? qk[q] * ldexpf(cks[c][q], -kScore - p_row) * e : 0.f;
                         below[q] = i > j0 + q ? of_row * cks[c][q] * kk[q] * e : 0.f;
                         bad |= !(fabsf(M[4 * c + q]) < 60000.f);
                     }
@@ -414,7 +433,7 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
         }
         const float grown = expf(float(G)), left = expf(float(all - G)), whole = expf(float(all));
         const float of_q = a.scale * grown * cq, of_x = beta * grown * ck, of_u = left * ck;
-        const float of_m = ldexpf(a.scale * cq * top, kScore);
+        const float of_m = ldexpf(a.scale * cq, kScore + p);
         bad |= !(fabsf(of_q) < INFINITY) || !(fabsf(of_x) < INFINITY) || !(of_u < INFINITY) || !(fabsf(of_m) < INFINITY) ||
                !(whole < INFINITY);
         float most = of_u;

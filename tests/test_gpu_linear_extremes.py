@@ -83,6 +83,29 @@ def test_columns_of_zeros_keep_their_room(gpu):
         assert not out[:288].any()
 
 
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 20, 2.0 ** 30])
+def test_a_long_key_takes_nothing_from_tokens_before_it(gpu, delta, size):
+    case = plain([32, 61], delta)
+    case.state[:] = 0
+    case.k[31] *= np.float32(size)
+    case.k[32 + 60] *= np.float32(size)
+    out, _ = case.run(gpu)
+    want, bound, _, _ = case.want(ROUNDINGS)
+    before = np.ones(93, bool)
+    before[[31, 92]] = False
+    right(out[before], want[before], bound[before])
+
+
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 20, 2.0 ** 30])
+def test_a_long_key_that_is_forgotten_takes_nothing_from_tokens_behind(gpu, size):
+    case = plain([32, 61], False)
+    for at in (3, 32 + 40):
+        case.k[at] *= np.float32(size)
+        case.a[at + 1] = -40.0
+    check(gpu, case)
+
+
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
 @pytest.mark.parametrize("counts", [[1], [40], [300]])
 def test_an_element_of_a_state_that_is_not_finite_stays_alone(gpu, value, counts):
