@@ -315,7 +315,8 @@ int qmr_supported_bf16_quantization(uint32_t bits, size_t group);
  *     were, and the launch is planned for sequences that long. dk and dv
  *     multiples of 8, at most 256; v heads a multiple of k heads, at most 65535.
  *     out may be rows beside an input's in one buffer. Results are near FP32
- *     arithmetic's; past eight tokens a value counts to 2^-30 of the largest of its
+ *     arithmetic's; past eight tokens a value (with delta = 1 less what the state has
+ *     for its key) counts to 2^-30 of the largest of its
  *     column among the 32 tokens that it goes with, an element of a state to 2^-30 of
  *     its column's, and a key to 2^-29 of the longest one in front of it among those
  *     32, decayed as far as it is. With delta = 1 that supposes keys at most about 1 long, as

@@ -43,7 +43,8 @@
 // The chunk's algebra has products of tokens with later ones, by zero: a value
 // that is not finite would reach tokens before it. A chunk that has some, or
 // whose T is not small (keys longer than 1, where the recurrence itself is not
-// stable), is done token after token by the same waves.
+// stable), or, with the delta rule, that has a key longer than kLongest, is done
+// token after token by the same waves.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -89,6 +90,10 @@ enum Scalar : uint32_t { kBeta = 0, kX = 32, kQ = 64, kM = 96, kU = 128, kWhole 
 __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
+
+// Under the delta rule R has S^T k: a key of this length takes as much from the
+// other tokens' part in R as a value that many times the state.
+constexpr float kLongest = 16.f;
 
 // Two terms of each side.
 __device__ __forceinline__ f4 mfma3(u4 ah, u4 al, u4 bh, u4 bl, f4 c) {
@@ -270,7 +275,8 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
             const float f = a.qk_eps > 0.f ? 1.f / sqrtf(sum + a.qk_eps) : 1.f;
             if (seg == 0) {
                 rows[32 * (1 - r) + i] = top > 0.f ? ldexpf(f, -p) : 0.f;
-                rows[64 + 32 * r + i] = sum < INFINITY ? 0.f : 1.f;
+                // (finite, and with the delta rule keys of up to kLongest)
+                rows[64 + 32 * r + i] = sum * f * f < (DELTA && r == 1 ? kLongest * kLongest : INFINITY) ? 0.f : 1.f;
             }
             const float by = ldexpf(1.f, p);
 #pragma unroll

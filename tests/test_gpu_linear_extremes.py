@@ -106,6 +106,22 @@ def test_a_long_key_that_is_forgotten_takes_nothing_from_tokens_behind(gpu, size
     check(gpu, case)
 
 
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("size", [1e18, 1e35])
+def test_a_key_past_all_bounds_reaches_no_token_before_it(gpu, delta, size):
+    """Its own direction is no other key's, so that nothing but the state, along
+    it, grows; what it leaves behind it may be infinite."""
+    case = plain([32, 40], delta)
+    case.k[:, 7] = 0
+    for at in (31, 32 + 20):
+        case.k[at] = 0
+        case.k[at, 7] = size
+    out, _ = case.run(gpu)
+    want, bound, _, _ = case.want(ROUNDINGS)
+    before = np.r_[0:31, 32:52]
+    right(out[before], want[before], bound[before])
+
+
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
 @pytest.mark.parametrize("counts", [[1], [40], [300]])
 def test_an_element_of_a_state_that_is_not_finite_stays_alone(gpu, value, counts):
