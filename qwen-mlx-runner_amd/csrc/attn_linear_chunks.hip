@@ -81,6 +81,7 @@ constexpr uint32_t kOut = 0x80000000u;   // buffer offset past every range
 constexpr float kForget = -1000.f;       // e^-1000 is 0 in FP32 whatever it meets
 constexpr int kScore = 2;                // M's entries are products of scaled rows by 2^-kScore, and a row's own power
 constexpr int kSolve = 4;                // T's entries are by 2^kSolve
+constexpr int kRoom = 16;                // products with S and U, of scaled rows, are by 2^-kRoom: S and U may be near FP32's largest
 
 // A chunk's operands. Of a key head: Q [2 tiles of 16 tokens][blocks][2 terms],
 // and K. Of a value head: M [2][2 terms], scalars, T as M (delta rule).
@@ -438,8 +439,8 @@ __global__ __launch_bounds__(kPrepare) void linear_prepare_kernel(LinearArgs a, 
             for (int d = 1; d < 16; d *= 2) rows_of_t = fmaxf(rows_of_t, __shfl_xor(rows_of_t, d));
         }
         const float grown = expf(float(G)), left = expf(float(all - G)), whole = expf(float(all));
-        const float of_q = a.scale * grown * cq, of_x = beta * grown * ck, of_u = left * ck;
-        const float of_m = ldexpf(a.scale * cq, kScore + p);
+        const float of_q = ldexpf(a.scale * grown * cq, kRoom), of_x = beta * grown * ck, of_u = left * ck;
+        const float of_m = ldexpf(a.scale * cq, kScore + p + kRoom);
         bad |= !(fabsf(of_q) < INFINITY) || !(fabsf(of_x) < INFINITY) || !(of_u < INFINITY) || !(fabsf(of_m) < INFINITY) ||
                !(whole < INFINITY);
         float most = of_u;
@@ -826,7 +827,7 @@ __global__ __launch_bounds__((NC + NL) * 64, KB < 8 ? 2 : 1) void linear_scan_ke
             for (int i = 0; i < 6; ++i) step(i / 2, tm[i % 2], uh, ul, y[i % 2]);
 #pragma unroll
             for (int i = 0; i < 3 * TD; ++i) step(i / TD, tu[i % TD], wh, wl, S[i % TD]);
-            const float one = ldexpf(1.f, -scale), of_y = ldexpf(1.f, (DELTA ? -kSolve : 0) - up - scale);
+            const float one = ldexpf(1.f, -scale - kRoom), of_y = ldexpf(1.f, (DELTA ? -kSolve : 0) - up - scale - kRoom);
             const auto rows = buffer_of(a.out + (size_t(first) + t0) * a.out_stride + size_t(h) * a.dv, ((n - 1) * a.out_stride + a.dv) * 4);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {

@@ -138,3 +138,18 @@ def test_an_element_of_a_state_that_is_not_finite_stays_alone(gpu, value, counts
     assert not np.isfinite(after[0, 1, 3, 5])
     after[0, 1, 3, 5] = states[0, 1, 3, 5]
     right(after, states, state_bound)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("n", [4, 100])
+def test_states_near_the_largest_number(gpu, delta, n):
+    """Sums of scaled rows stay below it where results do. (Columns this large have
+    the least scale there is, so that bits may differ from a smaller one's.)"""
+    case = plain([n], delta)
+    case.v /= np.float32(8)
+    case.state /= np.float32(8)
+    out, after = case.run(gpu)
+    assert max(np.abs(out).max(), np.abs(after).max()) < 2
+    two = np.float32(2.0 ** 126)
+    case.v, case.state = case.v * two, case.state * two
+    check(gpu, case)
