@@ -153,3 +153,17 @@ def test_states_near_the_largest_number(gpu, delta, n):
     two = np.float32(2.0 ** 126)
     case.v, case.state = case.v * two, case.state * two
     check(gpu, case)
+
+
+@pytest.mark.parametrize("length", [1.5, 40.0, 3e5])
+def test_long_keys_without_the_delta_rule(gpu, length):
+    """Every token and the states: nothing grows but by the keys' lengths."""
+    case = plain([70, 9, 200], False)
+    case.k *= np.float32(length)
+    check(gpu, case)
+
+
+@pytest.mark.parametrize("most", [1, 9, 32, 64, 80])
+@pytest.mark.parametrize("delta", [True, False])
+def test_states_of_the_first_tokens_of_a_sequence(gpu, most, delta):
+    check(gpu, plain([100, 2, 70, 33], delta, most=most))
