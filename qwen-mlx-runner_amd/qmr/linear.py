@@ -12,11 +12,14 @@ dispatches over a step; `Draws` holds what a row of logits is drawn with:
 
 A sequence has one state, of its last token: what a token did to it is not
 undone. Tokens that may be taken back (to verify) go in a step with keep=False,
-and the accepted ones again in one with keep=True. include/qmr.h says what the operators
-compute.
+and the accepted ones again in one with keep=True. A step that not every layer ran,
+since a call was refused or its command failed, is given to `Slots.undo` (a
+layer's own two calls do that when they are refused). include/qmr.h says what the
+operators compute.
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Sequence
 
@@ -33,11 +36,13 @@ NO_TOKEN = 0xFFFFFFFF
 class Step:
     """New tokens of some sequences: tokens starts[s]..starts[s+1]-1 are those
     of the sequence whose states are in slot words[s], where what they make of
-    them is kept or not."""
+    them is kept or not. `begun` are the sequences that have their first tokens
+    kept by it."""
     starts: np.ndarray
     words: np.ndarray
     keep: bool = True
     buffers: tuple[Buffer, ...] = ()
+    begun: frozenset[int] = frozenset()
 
     @property
     def tokens(self) -> int:
@@ -62,6 +67,7 @@ class Slots:
         self._free = list(range(slots - 1, -1, -1))
         self._held: dict[int, int] = {}
         self._fresh: set[int] = set()
+        self._begun: dict[int, Step] = {}  # sequences whose one kept step so far this is
         self._next = 0
 
     @property
@@ -80,6 +86,7 @@ class Slots:
     def close(self, seq: int) -> None:
         self._free.append(self._held.pop(seq))
         self._fresh.discard(seq)
+        self._begun.pop(seq, None)
 
     def step(self, new: Sequence[tuple[int, int]], keep: bool = True) -> Step:
         """`count` more tokens of each sequence (sequence, count). A sequence's
@@ -88,9 +95,34 @@ class Slots:
         if not new or len({seq for seq, _ in new}) != len(new) or any(count < 0 for _, count in new):
             raise ValueError("a step names each sequence once, with its number of tokens")
         words = [self._held[seq] | (FRESH if seq in self._fresh else 0) for seq, _ in new]
-        if keep:
-            self._fresh -= {seq for seq, count in new if count > 0}
-        return Step(np.cumsum([0, *(count for _, count in new)], dtype=np.uint32), np.array(words, np.uint32), keep)
+        kept = {seq for seq, count in new if keep and count > 0}
+        step = Step(np.cumsum([0, *(count for _, count in new)], dtype=np.uint32), np.array(words, np.uint32), keep,
+                    begun=frozenset(kept & self._fresh))
+        self._fresh -= kept
+        for seq in kept:
+            self._begun.pop(seq, None)
+        self._begun.update(dict.fromkeys(step.begun, step))
+        return step
+
+    def undo(self, step: Step) -> None:
+        """Takes back a step that not every layer ran: the sequences whose first
+        tokens it has start from zeros again, whatever it left in their slots. The
+        states of its other sequences are as far as each layer ran, which nothing
+        brings back."""
+        again = {seq for seq in step.begun if self._begun.get(seq) is step}
+        self._fresh |= again
+        for seq in again:
+            del self._begun[seq]
+
+
+@contextmanager
+def _undone(slots: Slots, step: Step):
+    """Takes the step back if what is inside is refused."""
+    try:
+        yield
+    except BaseException:
+        slots.undo(step)
+        raise
 
 
 class Weights(NamedTuple):
@@ -147,8 +179,9 @@ class Layer:
                  states: States, qkv: Buffer) -> None:
         """qkv [tokens][channels] from the product's rows [tokens][row]; `bias`
         is read if the layer has one, and may be any buffer if not."""
-        encode(cmd, "conv_causal", [rows, filters, bias, *step.buffers, states.inputs, qkv],
-               self.convolve_params(step, slots))
+        with _undone(slots, step):
+            encode(cmd, "conv_causal", [rows, filters, bias, *step.buffers, states.inputs, qkv],
+                   self.convolve_params(step, slots))
 
     def attend_params(self, step: Step, slots: Slots) -> list[int]:
         scale = self.dk ** -0.5 if self.scale is None else self.scale
@@ -163,9 +196,10 @@ class Layer:
         k = 4 * self.k_heads * self.dk
         z = 4 * self.channels
         b = z + 4 * self.out_width
-        encode(cmd, "attn_linear",
-               [qkv, qkv, qkv, rows, rows, weights.a_log, weights.dt_bias, rows, weights.norm, *step.buffers, states.heads, out],
-               self.attend_params(step, slots), [0, k, 2 * k, b + 4 * self.v_heads, b, 0, 0, z, 0, 0, 0, 0, 0])
+        with _undone(slots, step):
+            encode(cmd, "attn_linear",
+                   [qkv, qkv, qkv, rows, rows, weights.a_log, weights.dt_bias, rows, weights.norm, *step.buffers, states.heads, out],
+                   self.attend_params(step, slots), [0, k, 2 * k, b + 4 * self.v_heads, b, 0, 0, z, 0, 0, 0, 0, 0])
 
 
 class Draws:
