@@ -14,7 +14,7 @@
 // Weights are whole numbers, w_i * 2^shift rounded, the shift such that a row's
 // sum stays below 2^62: sums are exact in any order, so a token does not depend
 // on how the row was split, and a weight is off by 2^-45 at most at 248320
-// tokens. They are worked out in 64 bits: with weights of 32, one draw in a
+// tokens (2^-46 where there are fewer). They are worked out in 64 bits: with weights of 32, one draw in a
 // hundred of a broad row would fall on the other side of a border.
 //
 // Nothing is sorted. A token's place is one number, its logit's bits above its
@@ -52,7 +52,7 @@ using u64 = unsigned long long;
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr uint32_t kBins = kThreads;     // a thread a bin; the last: weights that round to nothing
-constexpr uint32_t kPerNat = 16;         // bins of a temperature: 511 of them reach below 2^-45
+constexpr uint32_t kPerNat = 16;         // bins of a temperature: 511 of them reach below 2^-46
 constexpr uint32_t kCandidates = 8192;   // of a row, at most
 constexpr uint32_t kSliceStep = 4096;
 constexpr uint32_t kFew = 64;            // candidates that a wave has in its lanes
@@ -76,11 +76,12 @@ __device__ __forceinline__ uint32_t key_at(u64 place) { return uint32_t(place >>
 __device__ __forceinline__ uint32_t index_at(u64 place) { return ~uint32_t(place); }
 
 // n weights of at most 2^shift add up to 2^62 at most; a weight and 2^52 are a
-// double's whole number.
+// double's whole number. Rows in bins: 2^45 at most, so that a weight of the last
+// bin, below 2^-46 of the greatest, is nothing wherever it is worked out.
 __host__ __device__ constexpr uint32_t shift_of(uint32_t n) {
     uint32_t bits = 12;
     while ((uint64_t(1) << bits) < n) ++bits;
-    return 62 - bits;
+    return n > kCandidates && bits < 17 ? 45 : 62 - bits;
 }
 
 // A row's, read before anything is waited for.
