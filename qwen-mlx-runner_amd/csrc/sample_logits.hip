@@ -398,11 +398,15 @@ __device__ Bounds bounds_of(const Settings &set, const Weights &of, uint32_t n, 
         __syncthreads();
     }
     if (of.min_p > 0.f) {
-        // Where the weight min_p stands, give or take a bin for what rounds.
-        const double z = of.temperature * -log(double(fminf(of.min_p, 1.f))) * 0.5 * double(of.per_bin);
-        const uint32_t at = z < double(kBins) ? uint32_t(z) : kBins;
-        b.first = min(b.first, at > 0 ? at - 1 : 0);
-        b.last = min(b.last, at + 1);
+        // Where the weight min_p stands, give or take what the weights round to in 64
+        // bits (at a temperature far above the logits that is many bins) and a bin for
+        // what else rounds.
+        const double nats = -log(double(fminf(of.min_p, 1.f))), off = 1e-14 * (1 + nats);
+        const double bins = 0.5 * of.temperature * double(of.per_bin);
+        auto bin_at = [&](double n) { return n > 0 ? n * bins < double(kBins) ? uint32_t(n * bins) : kBins : 0u; };
+        const uint32_t from = bin_at(nats - off);
+        b.first = min(b.first, from > 0 ? from - 1 : 0);
+        b.last = min(b.last, bin_at(nats + off) + 1);
     }
     if (b.first == kNone) b.first = kBins;  // no border: all is kept
     // Few tokens down to the last border: they are all candidates.

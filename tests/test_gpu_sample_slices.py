@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from sample_cases import Sample
+from sample_cases import Sample, distribution
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +25,15 @@ def test_weights_next_to_nothing_count_alike_in_every_slice(gpu, vocab, far):
     for i in range(0, len(u), 7):
         got, share = Sample(row, u=u[i:i + 1]).run(gpu)
         assert got[0] == tokens[i] and share[0] == probs[i]
+
+
+@pytest.mark.parametrize("vocab", [5000, 20000])
+@pytest.mark.parametrize("temperature", [1e12, 1e15, 1e18, 1e30, np.inf])
+@pytest.mark.parametrize("min_p", [0.5, np.nextafter(np.float32(1), np.float32(0)), 1.0])
+def test_temperatures_far_above_the_logits(gpu, vocab, temperature, min_p):
+    """Weights all but equal, of which min_p keeps those that reach it in 64 bits."""
+    rng = np.random.default_rng(vocab)
+    case = Sample(3 * rng.standard_normal((6, vocab)), temperature, min_p=min_p, u=[0, 1, 0.25, *rng.random(3)])
+    tokens, _ = case.check(gpu)
+    if temperature == 1e18:
+        assert len(distribution(case.logits[0], 1e18, 0, 1.0, min_p)[0]) == vocab and tokens[0] == 0
