@@ -144,7 +144,10 @@ int qmr_encode(qmr_command *command, const char *name, qmr_buffer *const *buffer
  * so in qmr_encode too. attn_paged is planned with as many key ranges as fit:
  * its bits are qmr_encode's wherever both plans agree, as for single tokens.
  * attn_linear takes the chunks of long prompts in as many passes as the
- * scratch asks for, with qmr_encode's bits.) Workspace that
+ * scratch asks for, with qmr_encode's bits, if it holds two states of all value
+ * heads and a chunk's operands beside them: 48 heads of 128 x 128 it does, 64 it
+ * does not, and then chunks that do not fit at once go token after token, 1.3 us
+ * each, with other last bits.) Workspace that
  * must start at zero (split sums tagged with a fixed epoch, arrival counters)
  * is cleared by a fill kernel inside the call when earlier launches may have
  * left it non-zero: the split-K kernel and the row-band kernel's GEMV and
@@ -314,7 +317,11 @@ int qmr_supported_bf16_quantization(uint32_t bits, size_t group);
  *     sequence the first `most` tokens count, those behind them stay as they
  *     were, and the launch is planned for sequences that long. dk and dv
  *     multiples of 8, at most 256; v heads a multiple of k heads, at most 65535.
- *     out may be rows beside an input's in one buffer. Results are near FP32
+ *     out may be rows beside an input's in one buffer. All sequences of a call go
+ *     token after token, or, if one may have more than eight, all in chunks of 32: a
+ *     token's last bits depend on which, and single tokens beside a prompt go faster
+ *     in a call of their own (48 heads of 128 x 128: 256 tokens and 31 single ones 100
+ *     us, in two calls of one command 72). Results are near FP32
  *     arithmetic's; past eight tokens a value (with delta = 1 less what the state has
  *     for its key) counts to 2^-30 of the largest of its
  *     column among the 32 tokens that it goes with, an element of a state to 2^-30 of

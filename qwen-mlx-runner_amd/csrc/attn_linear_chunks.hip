@@ -14,12 +14,12 @@
 // Three launches. linear_prepare_kernel has a workgroup a chunk and key head:
 // everything that does not depend on the state, all chunks at once, left in the
 // workspace as the operands that the matrix instructions take (4100 tokens of 16
-// key and 48 value heads of 128: 51 us, 68 MB read and 122 MB written, 3.7 TB/s,
+// key and 48 value heads of 128: 53 us, 68 MB read and 122 MB written, 3.6 TB/s,
 // bound by memory and the splits' vector work alike). linear_scan_kernel
 // goes through a sequence's chunks: a workgroup has some 16-column tiles of a
 // value head's state, a wave one, in its accumulators; the next chunk's operands
-// come to LDS meanwhile (bound by a chunk's chain of products and splits: 1.67 us
-// a chunk, 216 us for those tokens, of which 84 matrix instructions are a third).
+// come to LDS meanwhile (bound by a chunk's chain of products and splits: 1.7 us
+// a chunk, 219 us for those tokens, of which 84 matrix instructions are a third).
 // linear_norm_kernel norms the outputs, whose rows the workgroups of a head share
 // (49 us for those: 302 MB at 6.2 TB/s, much of it from the last-level cache).
 //
@@ -934,11 +934,12 @@ LinearPlan plan_linear(const LinearArgs &a, const DeviceLimits &lim, size_t limi
     LinearPlan pl;
     const Sequences &q = a.seq;
     const uint32_t longest = std::min(q.most, q.tokens);
-    // Token after token up to eight. Both forms in us, 48 heads of 128 x 128: one
-    // sequence of 4, 8, 12 and 16 tokens 12/21, 17/21, 23/21 and 28/22; eight
-    // sequences of 8 and 12 29/38 and 38/39; 32 of 8 and 12 77/95 and 102/97. Eight
-    // heads of 64 x 64, one sequence of 8 and 12: 16/17 and 21/18; three of
-    // 256 x 192: 30/26 and 42/27.
+    // Token after token up to eight, whatever the dimensions. Both forms in us, 48
+    // heads of 128 x 128: one sequence of 4, 8, 12 and 16 tokens 12/21, 17/21, 23/21
+    // and 28/22; eight sequences of 8 and 12 29/38 and 38/39; 32 of 8 and 12 77/95 and
+    // 102/97. Eight heads of 64 x 64, one sequence of 8 and 12: 16/17 and 21/18. Three
+    // heads of 256 x 192 would do with fewer (8 and 12: 30/26 and 42/27); a rule for
+    // them alone would save those 4 us.
     if (form == 1 || (form == 0 && longest <= 8)) return pl;
     // Rows that a buffer's 32-bit offsets reach over a chunk.
     if (a.v_stride > 1u << 22 || a.out_stride > 1u << 22) return pl;

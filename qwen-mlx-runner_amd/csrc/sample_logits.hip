@@ -31,8 +31,10 @@
 //                  them, without a look at slices, if there are few)
 //
 // A row that fits sample_pick's LDS needs that launch alone. One that has too
-// many tokens in its bins (many equal logits) is worked on by sample_pick
-// alone, which reads it once a digit of the borders.
+// many tokens in its bins (many equal logits, or a temperature so far above most
+// of them that they share a few bins, beside an outlier that widens those) is
+// worked on by sample_pick alone, which reads it once a digit of the borders: 0.9
+// to 1.7 ms for 248320 logits with top k or top p, where 35 to 44 us are usual.
 //
 // One row of 248320 takes 3.6, 7.4, 7.0 and 5.6 us: launches, and each kernel's
 // chain of loads, scans and barriers. 48 rows take 13, 26, 22 and 25: reading them

@@ -10,7 +10,8 @@ dispatches over a step; `Draws` holds what a row of logits is drawn with:
     layer.attend(cmd, step, slots, rows, qkv, weights, states, out)
     draws.sample(cmd, logits, vocab, tokens, probs)
 
-A sequence has one state, of its last token: what a token did to it is not
+Single tokens go faster in a step of their own than beside a prompt's, in the same
+command. A sequence has one state, of its last token: what a token did to it is not
 undone. Tokens that may be taken back (to verify) go in a step with keep=False,
 and the accepted ones again in one with keep=True. A step that not every layer ran,
 since a call was refused or its command failed, is given to `Slots.undo` (a
