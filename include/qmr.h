@@ -135,29 +135,29 @@ int qmr_encode(qmr_command *command, const char *name, qmr_buffer *const *buffer
  * workspace its kernels need (the row-band kernel's split sums, the split-K
  * kernel's partial sums and counters, the wide block's activation images,
  * attention's results of key ranges, linear attention's chunks, a draw's
- * candidates) comes from a static scratch array of QMR_STATIC_SCRATCH_BYTES that each GPU
- * holds from library load until the process ends; a launch needing more is
- * rejected with QMR_ERR_INVALID before anything is enqueued. (Of the wide
- * blocks these are Q4 ones of group 64 and more than eight RHS over whole 256
- * columns, codes, scales and biases 16-byte aligned; the others run in
- * passes over fewer RHS, or as blocks of four, that fit the scratch, and do
- * so in qmr_encode too. attn_paged is planned with as many key ranges as fit:
- * its bits are qmr_encode's wherever both plans agree, as for single tokens.
- * attn_linear takes the chunks of long prompts in as many passes as the
- * scratch asks for, with qmr_encode's bits, if it holds two states of all value
- * heads and a chunk's operands beside them: 48 heads of 128 x 128 it does, 64 it
- * does not, and then chunks that do not fit at once go token after token, 1.3 us
- * each, with other last bits.) Workspace that
- * must start at zero (split sums tagged with a fixed epoch, arrival counters)
- * is cleared by a fill kernel inside the call when earlier launches may have
- * left it non-zero: the split-K kernel and the row-band kernel's GEMV and
- * block forms (plain or residual) clear every slot and counter they take, so
- * after the first fill the region stays zero from call to call and needs no
- * fill until a wide block, a group 32 block of three or four RHS on the wide
+ * candidates) comes from a static scratch array of QMR_STATIC_SCRATCH_BYTES
+ * that each GPU holds from library load until the process ends; a launch
+ * needing more is rejected with QMR_ERR_INVALID before anything is enqueued.
+ * (Of the wide blocks these are Q4 ones of group 64 and more than eight RHS
+ * over whole 256 columns, codes, scales and biases 16-byte aligned; the others
+ * run in passes over fewer RHS, or as blocks of four, that fit the scratch,
+ * and do so in qmr_encode too. attn_paged is planned with as many key ranges
+ * as fit: its bits are qmr_encode's wherever both plans agree, as for single
+ * tokens. attn_linear takes the chunks of long prompts in as many passes as
+ * the scratch asks for, with qmr_encode's bits, if it holds two states of all
+ * value heads and a chunk's operands beside them: 48 heads of 128 x 128 it
+ * does, 64 it does not, and then a call with more chunks than fit at once goes
+ * token after token, 1.3 us each, with other last bits.) Workspace that must
+ * start at zero (split sums tagged with a fixed epoch, arrival counters) is
+ * cleared by a fill kernel inside the call when earlier launches may have left
+ * it non-zero: the split-K kernel and the row-band kernel's GEMV and block
+ * forms (plain or residual) clear every slot and counter they take, so after
+ * the first fill the region stays zero from call to call and needs no fill
+ * until a wide block, a group 32 block of three or four RHS on the wide
  * kernel, the row-band MLP form, attn_paged, attn_linear's chunks,
- * sample_logits or a failed command has used it. All calls on one GPU share its scratch: calls whose launches
- * overlap in time (other streams, other device handles on the same GPU)
- * race. */
+ * sample_logits or a failed command has used it. All calls on one GPU share
+ * its scratch: calls whose launches overlap in time (other streams, other
+ * device handles on the same GPU) race. */
 #define QMR_STATIC_SCRATCH_BYTES (8u << 20)
 int qmr_encode_static(qmr_command *command, const char *name, qmr_buffer *const *buffers,
                       const size_t *offsets, size_t nbuffers, const uint32_t *params,
@@ -318,17 +318,18 @@ int qmr_supported_bf16_quantization(uint32_t bits, size_t group);
  *     were, and the launch is planned for sequences that long. dk and dv
  *     multiples of 8, at most 256; v heads a multiple of k heads, at most 65535.
  *     out may be rows beside an input's in one buffer. All sequences of a call go
- *     token after token, or, if one may have more than eight, all in chunks of 32: a
- *     token's last bits depend on which, and single tokens beside a prompt go faster
- *     in a call of their own (48 heads of 128 x 128: 256 tokens and 31 single ones 100
- *     us, in two calls of one command 72). Results are near FP32
- *     arithmetic's; past eight tokens a value (with delta = 1 less what the state has
- *     for its key) counts to 2^-30 of the largest of its
- *     column among the 32 tokens that it goes with, an element of a state to 2^-30 of
- *     its column's, and a key to 2^-29 of the longest one in front of it among those
- *     32, decayed as far as it is. With delta = 1 that supposes keys at most about 1 long, as
+ *     token after token, or, if one may have more than eight, all in chunks of 32:
+ *     a token's last bits depend on which, and single tokens beside a prompt go
+ *     faster in a call of their own (48 heads of 128 x 128: 256 tokens and 31
+ *     single ones 100 us, in two calls of one command 72). Results are near FP32
+ *     arithmetic's; past eight tokens a value (with delta = 1 less what the state
+ *     has for its key) counts to 2^-30 of the largest of its column among the 32
+ *     tokens that it goes with, an element of a state to 2^-30 of its column's,
+ *     and a key to 2^-29 of the longest one in front of it among those 32, decayed
+ *     as far as it is. With delta = 1 that supposes keys at most about 1 long, as
  *     qk eps makes them: longer ones can make the state grow without bound, in
- *     which case a prompt's results come token after token, and slowly.
+ *     which case, as with any key longer than 16, a prompt's results come token
+ *     after token, and slowly.
  *   "sample_logits"
  *     A token of each row of logits: the greatest, or one drawn from what
  *     temperature, top-k, top-p and min-p leave. Buffers logits (FP32 rows),
